@@ -471,6 +471,128 @@ int kmoe_argmax(kmoe_ctx *ctx, const float *logits_dev, int64_t n, uint32_t *out
  * graph-captured steps). */
 int kmoe_pos_advance(kmoe_ctx *ctx, int32_t *pos_dev, int32_t by);
 
+/* ---- Paged key-value cache: many sequences at once ----
+ * No counterpart in the reference, whose engine holds one sequence
+ * (Transformer::forward(&mut self), transformer.rs:228-232, :278); the
+ * per-row arithmetic is that of rope, the cache store and attention there
+ * (transformer.rs:342-358, :406-418, :591-631).
+ *
+ * A cache is a buffer of n_pages pages per layer; a page holds `page`
+ * consecutive positions of every kv head, K and V. A sequence's positions
+ * p * page .. p * page + page - 1 lie on the page that column p of its row of a
+ * page table names, so sequences grow page by page, share pages and leave
+ * none behind. The bytes inside a page are the library's own order (the
+ * attention kernels' operand order): kmoe_paged_kv_store and its RoPE form
+ * write them, kmoe_paged_kv_read gives rows back, kmoe_pages_copy moves whole
+ * pages. Cache types: KMOE_F16 (rounded to nearest even, as kmoe_kv_store) and
+ * KMOE_Q8_0 (34 bytes per 32 dims: int8 quants and one f16 scale, the f16
+ * nearest to max|x| / 127; quants are x / scale to the nearest, ties to even. A
+ * group whose scale would pass f16's range saturates at 127 * 65504; one with a
+ * NaN or an infinity reads as NaN).
+ *
+ * Rows of a call belong to the sequences of a batch: sequence b holds rows
+ * row_start[b] .. row_start[b+1] - 1, and they are its last ones: with n of
+ * them, row i sits at position seq_len[b] - n + i (seq_len counts the new rows
+ * too). So one call takes decoding sequences (one row), prompt chunks (many)
+ * and sequences that sit a step out (none). Rows behind the last sequence are
+ * not touched. The three arrays are device memory, read when the kernels run: a
+ * captured call may be replayed with other lengths, tables and row counts up to
+ * s_rows. What they hold is checked on the device: rows are kept inside
+ * 0 .. s_rows - 1, and a position without a page (column past table_cols, id
+ * outside 0 .. n_pages - 1, as a trimmed page's -1) is neither written nor
+ * seen; kmoe_paged_kv_read gives zeros for it. Two rows of one call must not
+ * share a position of a page, and a page that is written must belong to one
+ * sequence only. */
+typedef struct {
+  int32_t type;            /* KMOE_F16 or KMOE_Q8_0 */
+  int32_t n_kv, head_dim;  /* kv heads (1 .. 4096); head_dim 64 or 128 */
+  int32_t page;            /* positions per page: 32, 64, 128 or 256 */
+  int64_t n_pages;         /* pages in the buffer, at most 2^31 - 1 */
+} kmoe_paged_desc;
+typedef struct {
+  int32_t n_seq;                 /* 1 .. KMOE_PAGED_MAX_SEQ */
+  int32_t table_cols;            /* pages per row of the table */
+  int64_t s_rows;                /* rows of the call's q, k, v and outputs, at most 2^22 */
+  const int32_t *row_start_dev;  /* [n_seq + 1] ascending, or NULL: one row per sequence (s_rows == n_seq) */
+  const int32_t *seq_len_dev;    /* [n_seq] */
+  const int32_t *table_dev;      /* [n_seq, table_cols] */
+} kmoe_paged_batch;
+#define KMOE_PAGED_MAX_SEQ 4096
+/* Bytes of one page of one layer: n_kv * page * head_dim * 4 (f16), * 34 / 16 (Q8_0). */
+int kmoe_paged_page_bytes(const kmoe_paged_desc *desc, uint64_t *bytes);
+/* k, v rows [s_rows] of n_kv * head_dim floats, k_stride and v_stride floats
+ * apart (so parts of a q/k/v projection's rows are taken as they lie), into
+ * the pages (16-byte aligned). */
+int kmoe_paged_kv_store(kmoe_ctx *ctx, const kmoe_paged_desc *desc, void *pages_dev, const kmoe_paged_batch *batch,
+                        const float *k_dev, int64_t k_stride, const float *v_dev, int64_t v_stride);
+/* RoPE of q and k at the rows' positions, then the store: q rotated into q_out
+ * [s_rows, n_head * head_dim] (q_out must not overlap the inputs), k rotated
+ * and stored with v. Angles and arithmetic of kmoe_rope_kv_store (the angle is
+ * the f32 product of position and inv_freq[i]). A row whose position has no
+ * page still gets its q. */
+int kmoe_paged_rope_kv_store(kmoe_ctx *ctx, const kmoe_paged_desc *desc, void *pages_dev,
+                             const kmoe_paged_batch *batch, const float *q_dev, int64_t q_stride,
+                             const float *k_dev, int64_t k_stride, const float *v_dev, int64_t v_stride,
+                             int32_t n_head, int32_t rope_dim, const float *inv_freq_dev, int32_t neox,
+                             float *q_out_dev);
+/* The batch's rows read back: k, v [s_rows, n_kv * head_dim] f16 (KMOE_F16: the
+ * bits that were stored; KMOE_Q8_0: quant * scale, rounded to nearest even). */
+int kmoe_paged_kv_read(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *pages_dev,
+                       const kmoe_paged_batch *batch, uint16_t *k_dev, uint16_t *v_dev);
+/* Causal GQA attention of the batch's rows q [s_rows, n_head, head_dim] (after
+ * RoPE) over their sequences' pages: out [s_rows, n_head * head_dim]. A row at
+ * position i sees the positions p <= i; with window > 0 only those with
+ * p > i - window or p < n_sink (the first n_sink positions stay visible; window
+ * 0: all, n_sink unused). Pages that no row sees are not read. A row that sees
+ * nothing gives zeros. Sums and softmax statistics are f32; a row's last bits
+ * depend on the batch it is in (how the positions are shared out), a call's on
+ * nothing else. n_head / n_kv <= 16 heads per kv head. */
+int kmoe_paged_attention(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *pages_dev,
+                         const kmoe_paged_batch *batch, const float *q_dev, int32_t n_head, int64_t window,
+                         int64_t n_sink, float *out_dev);
+/* Pages src[i] onto dst[i], i < n, in each of n_layer buffers layer_stride
+ * bytes apart (16-byte aligned; desc->n_pages pages each). src and dst are
+ * host arrays, read before the call returns (the copies are asynchronous and
+ * may be captured). A page must not be copied onto twice, nor be both copied
+ * from and onto: KMOE_E_INVALID. */
+int kmoe_pages_copy(kmoe_ctx *ctx, const kmoe_paged_desc *desc, void *pages_dev, int64_t n_layer,
+                    int64_t layer_stride, const int32_t *src, const int32_t *dst, int64_t n);
+
+/* ---- Who holds which page (host memory only; no context, no GPU) ----
+ * Sequences are named by the caller. Pages are counted by holders: forks share
+ * them, the last holder's drop frees them. Not thread-safe. A call that fails
+ * changes nothing. KMOE_E_BUDGET: no free page; KMOE_E_NOT_LOADED: no such
+ * sequence. The device side is the caller's: copies that a call asks for are
+ * made with kmoe_pages_copy before the next store, and page tables are given
+ * to the kernels as kmoe_pages_table writes them. */
+typedef struct kmoe_pages kmoe_pages;
+int kmoe_pages_create(int64_t n_pages, int32_t page, kmoe_pages **out);
+int kmoe_pages_destroy(kmoe_pages *p);
+const char *kmoe_pages_last_error(const kmoe_pages *p);
+/* n more positions for seq (begun where it does not exist). Where they begin on
+ * a page that other sequences hold too, seq gets a page of its own in its
+ * place: *copies = 1 and *src must be copied onto *dst. Otherwise *copies = 0. */
+int kmoe_pages_append(kmoe_pages *p, uint32_t seq, int64_t n, int32_t *src, int32_t *dst, int32_t *copies);
+/* A new sequence `to` of the first n positions of `from`, on the same pages. */
+int kmoe_pages_fork(kmoe_pages *p, uint32_t from, uint32_t to, int64_t n);
+/* Back to the first n positions; pages past them are given up. */
+int kmoe_pages_truncate(kmoe_pages *p, uint32_t seq, int64_t n);
+/* Gives up the pages that no later row of seq sees under kmoe_paged_attention's
+ * window and n_sink (their table entries become -1); *freed (may be NULL)
+ * counts those that are free now. Truncating or forking seq to where a trimmed
+ * position would be seen again is refused. */
+int kmoe_pages_trim(kmoe_pages *p, uint32_t seq, int64_t window, int64_t n_sink, int64_t *freed);
+int kmoe_pages_drop(kmoe_pages *p, uint32_t seq);
+int kmoe_pages_length(const kmoe_pages *p, uint32_t seq, int64_t *n);
+/* Rows of the page table [n_seq, table_cols] for seqs (-1 past a sequence's
+ * pages) and their lengths, host memory. */
+int kmoe_pages_table(kmoe_pages *p, const uint32_t *seqs, int32_t n_seq, int32_t table_cols, int32_t *table,
+                     int32_t *seq_len);
+/* Moves the used pages to the front, the highest first, at most cap of them:
+ * writes *n pairs to copy and changes every table accordingly. */
+int kmoe_pages_compact(kmoe_pages *p, int32_t *src, int32_t *dst, int64_t cap, int64_t *n);
+int kmoe_pages_usage(const kmoe_pages *p, int64_t *used, int64_t *total);
+
 /* ---- Measured figures for the planner's cost model ----
  * kestrel's planner prices a GPU tier with Bandwidths.vram / .pcie and a
  * fixed per-layer overhead (crates/kestrel-planner/src/cost.rs:26-83, :102,

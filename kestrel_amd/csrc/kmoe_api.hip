@@ -12,11 +12,13 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
 #include "../../include/kmoe.h"
 #include "kmoe_launch.h"
+#include "kmoe_paged.h"
 
 namespace kmoe {
 thread_local LaunchTiming g_timing;
@@ -2457,6 +2459,153 @@ int kmoe_pos_advance(kmoe_ctx *c, int32_t *pos_dev, int32_t by) {
   if (!pos_dev) return fail(c, KMOE_E_INVALID, "null pointer");
   DeviceGuard g(c->device);
   LAUNCH(c, "pos_advance", launch_pos_advance(c->stream, pos_dev, by));
+  return KMOE_OK;
+}
+
+// ---------------------------------------------------------------- paged cache
+
+int kmoe_paged_page_bytes(const kmoe_paged_desc *d, uint64_t *bytes) {
+  if (!d || !bytes || !paged_type_ok(d->type) || d->n_kv <= 0 || d->n_kv > 4096 ||
+      (d->head_dim != 64 && d->head_dim != 128) ||
+      (d->page != 32 && d->page != 64 && d->page != 128 && d->page != 256))
+    return KMOE_E_INVALID;
+  *bytes = (uint64_t)d->n_kv * (uint64_t)paged_block_bytes(d->type, d->page, d->head_dim);
+  return KMOE_OK;
+}
+
+constexpr int64_t kPagedMaxRows = (int64_t)1 << 22;  // (a work-group of 256 per row stays a valid grid)
+
+static int check_paged_desc(kmoe_ctx *c, const kmoe_paged_desc *d) {
+  if (!d) return fail(c, KMOE_E_INVALID, "null pointer");
+  if (!paged_type_ok(d->type)) return fail(c, KMOE_E_UNSUPPORTED, "ggml type %d is no cache type (F16=1, Q8_0=8)", d->type);
+  if (d->head_dim != 64 && d->head_dim != 128)
+    return fail(c, KMOE_E_UNSUPPORTED, "head_dim %d (kernels: 64 or 128)", d->head_dim);
+  if (d->page != 32 && d->page != 64 && d->page != 128 && d->page != 256)
+    return fail(c, KMOE_E_UNSUPPORTED, "%d positions per page (kernels: 32, 64, 128 or 256)", d->page);
+  if (d->n_kv <= 0 || d->n_kv > 4096) return fail(c, KMOE_E_INVALID, "%d kv heads (1 .. 4096)", d->n_kv);
+  if (d->n_pages <= 0 || d->n_pages > INT32_MAX) return fail(c, KMOE_E_INVALID, "%lld pages", (long long)d->n_pages);
+  return KMOE_OK;
+}
+
+// Checks of the entry points that take a batch; *a is the kernels' view, with
+// s_rows 0 where there is nothing to do.
+static int check_paged(kmoe_ctx *c, const kmoe_paged_desc *d, const void *pages, const kmoe_paged_batch *b,
+                       PagedArgs *a) {
+  int rc = check_paged_desc(c, d);
+  if (rc) return rc;
+  if (!b) return fail(c, KMOE_E_INVALID, "null pointer");
+  if (b->n_seq < 0 || b->n_seq > KMOE_PAGED_MAX_SEQ)
+    return fail(c, KMOE_E_INVALID, "%d sequences (at most %d)", b->n_seq, KMOE_PAGED_MAX_SEQ);
+  if (b->s_rows < 0 || b->s_rows > kPagedMaxRows || b->table_cols < 0) return fail(c, KMOE_E_INVALID, "negative or too large size");
+  if (!b->row_start_dev && b->s_rows != b->n_seq)
+    return fail(c, KMOE_E_INVALID, "%lld rows of %d sequences need row_start", (long long)b->s_rows, b->n_seq);
+  *a = PagedArgs{d->type, d->n_kv,          d->head_dim,     d->page,     d->n_pages, (uint8_t *)pages,
+                 b->n_seq, b->table_cols, b->n_seq ? b->s_rows : 0, b->row_start_dev, b->seq_len_dev, b->table_dev};
+  if (a->s_rows == 0) return KMOE_OK;
+  if (!pages || !b->seq_len_dev || (b->table_cols > 0 && !b->table_dev)) return fail(c, KMOE_E_INVALID, "null pointer");
+  if ((uintptr_t)pages & 15) return fail(c, KMOE_E_INVALID, "pages not 16-byte aligned");
+  return KMOE_OK;
+}
+
+int kmoe_paged_kv_store(kmoe_ctx *c, const kmoe_paged_desc *d, void *pages, const kmoe_paged_batch *b, const float *k,
+                        int64_t k_stride, const float *v, int64_t v_stride) {
+  if (!c) return KMOE_E_INVALID;
+  PagedArgs a;
+  int rc = check_paged(c, d, pages, b, &a);
+  if (rc) return rc;
+  const int64_t w = (int64_t)a.n_kv * a.hd;
+  if (k_stride < w || v_stride < w) return fail(c, KMOE_E_INVALID, "rows of %lld floats closer together", (long long)w);
+  if (a.s_rows == 0) return KMOE_OK;
+  if (!k || !v) return fail(c, KMOE_E_INVALID, "null pointer");
+  DeviceGuard g(c->device);
+  LAUNCH(c, "paged_store",
+         launch_paged_store(c->stream, a, nullptr, 0, k, k_stride, v, v_stride, 0, 0, nullptr, 0, nullptr));
+  return KMOE_OK;
+}
+
+int kmoe_paged_rope_kv_store(kmoe_ctx *c, const kmoe_paged_desc *d, void *pages, const kmoe_paged_batch *b,
+                             const float *q, int64_t q_stride, const float *k, int64_t k_stride, const float *v,
+                             int64_t v_stride, int32_t n_head, int32_t rope_dim, const float *inv_freq, int32_t neox,
+                             float *q_out) {
+  if (!c) return KMOE_E_INVALID;
+  PagedArgs a;
+  int rc = check_paged(c, d, pages, b, &a);
+  if (rc) return rc;
+  if (n_head <= 0 || n_head > 65536 || rope_dim <= 0 || rope_dim > a.hd || rope_dim % 2)
+    return fail(c, KMOE_E_INVALID, "rope: need heads and 0 < rope_dim <= head_dim, rope_dim even");
+  const int64_t w = (int64_t)a.n_kv * a.hd;
+  if (k_stride < w || v_stride < w || q_stride < (int64_t)n_head * a.hd)
+    return fail(c, KMOE_E_INVALID, "rows closer together than their width");
+  if (a.s_rows == 0) return KMOE_OK;
+  if (!q || !k || !v || !inv_freq || !q_out) return fail(c, KMOE_E_INVALID, "null pointer");
+  DeviceGuard g(c->device);
+  LAUNCH(c, "paged_store",
+         launch_paged_store(c->stream, a, q, q_stride, k, k_stride, v, v_stride, n_head, rope_dim, inv_freq, neox,
+                            q_out));
+  return KMOE_OK;
+}
+
+int kmoe_paged_kv_read(kmoe_ctx *c, const kmoe_paged_desc *d, const void *pages, const kmoe_paged_batch *b,
+                       uint16_t *k, uint16_t *v) {
+  if (!c) return KMOE_E_INVALID;
+  PagedArgs a;
+  int rc = check_paged(c, d, pages, b, &a);
+  if (rc) return rc;
+  if (a.s_rows == 0) return KMOE_OK;
+  if (!k || !v) return fail(c, KMOE_E_INVALID, "null pointer");
+  DeviceGuard g(c->device);
+  LAUNCH(c, "paged_read", launch_paged_read(c->stream, a, k, v));
+  return KMOE_OK;
+}
+
+int kmoe_paged_attention(kmoe_ctx *c, const kmoe_paged_desc *d, const void *pages, const kmoe_paged_batch *b,
+                         const float *q, int32_t n_head, int64_t window, int64_t n_sink, float *out) {
+  if (!c) return KMOE_E_INVALID;
+  PagedArgs a;
+  int rc = check_paged(c, d, pages, b, &a);
+  if (rc) return rc;
+  if (n_head <= 0 || n_head % a.n_kv) return fail(c, KMOE_E_INVALID, "attention: need n_head %% n_kv == 0");
+  if (n_head / a.n_kv > 16)
+    return fail(c, KMOE_E_UNSUPPORTED, "%d query heads per kv head (kernels: <= 16)", n_head / a.n_kv);
+  if (window < 0 || n_sink < 0) return fail(c, KMOE_E_INVALID, "negative window or n_sink");
+  if (a.s_rows == 0) return KMOE_OK;
+  if (!q || !out) return fail(c, KMOE_E_INVALID, "null pointer");
+  DeviceGuard g(c->device);
+  LAUNCH(c, "paged_attention", launch_paged_attention(c->stream, a, q, n_head, window, n_sink, out));
+  return KMOE_OK;
+}
+
+int kmoe_pages_copy(kmoe_ctx *c, const kmoe_paged_desc *d, void *pages, int64_t n_layer, int64_t layer_stride,
+                    const int32_t *src, const int32_t *dst, int64_t n) {
+  if (!c) return KMOE_E_INVALID;
+  int rc = check_paged_desc(c, d);
+  if (rc) return rc;
+  const int64_t pb = (int64_t)d->n_kv * paged_block_bytes(d->type, d->page, d->head_dim);
+  if (n < 0 || n_layer < 0 || n_layer > 65535) return fail(c, KMOE_E_INVALID, "negative or too large size");
+  if (n_layer > 1 && (layer_stride < d->n_pages * pb || layer_stride % 16))
+    return fail(c, KMOE_E_INVALID, "layers %lld bytes apart, pages need %lld", (long long)layer_stride,
+                (long long)(d->n_pages * pb));
+  if (n == 0 || n_layer == 0) return KMOE_OK;
+  if (!pages || !src || !dst) return fail(c, KMOE_E_INVALID, "null pointer");
+  if ((uintptr_t)pages & 15) return fail(c, KMOE_E_INVALID, "pages not 16-byte aligned");
+  try {
+    std::vector<std::pair<int32_t, uint8_t>> seen;  // (page, 1: copied onto)
+    seen.reserve(2 * (size_t)n);
+    for (int64_t i = 0; i < n; ++i) {
+      if (src[i] < 0 || src[i] >= d->n_pages || dst[i] < 0 || dst[i] >= d->n_pages)
+        return fail(c, KMOE_E_INVALID, "page %d -> %d of %lld", src[i], dst[i], (long long)d->n_pages);
+      seen.emplace_back(src[i], 0);
+      seen.emplace_back(dst[i], 1);
+    }
+    std::sort(seen.begin(), seen.end());
+    for (size_t i = 1; i < seen.size(); ++i)
+      if (seen[i].first == seen[i - 1].first && seen[i].second)
+        return fail(c, KMOE_E_INVALID, "page %d is copied onto and named again", seen[i].first);
+  } catch (const std::bad_alloc &) {
+    return fail(c, KMOE_E_BUDGET, "out of host memory");
+  }
+  DeviceGuard g(c->device);
+  LAUNCH(c, "pages_copy", launch_pages_copy(c->stream, (uint8_t *)pages, n_layer, layer_stride, pb, src, dst, n));
   return KMOE_OK;
 }
 

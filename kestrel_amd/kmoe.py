@@ -105,6 +105,24 @@ SIGNATURES = {
     "kmoe_add_rows": (C.c_int, [_P, _P, _P, _i64, _i64]),
     "kmoe_argmax": (C.c_int, [_P, _P, _i64, _P, _P, _i32]),
     "kmoe_pos_advance": (C.c_int, [_P, _P, _i32]),
+    "kmoe_paged_page_bytes": (C.c_int, [_P, C.POINTER(_u64)]),
+    "kmoe_paged_kv_store": (C.c_int, [_P, _P, _P, _P, _P, _i64, _P, _i64]),
+    "kmoe_paged_rope_kv_store": (C.c_int, [_P, _P, _P, _P, _P, _i64, _P, _i64, _P, _i64, _i32, _i32, _P, _i32, _P]),
+    "kmoe_paged_kv_read": (C.c_int, [_P, _P, _P, _P, _P, _P]),
+    "kmoe_paged_attention": (C.c_int, [_P, _P, _P, _P, _P, _i32, _i64, _i64, _P]),
+    "kmoe_pages_copy": (C.c_int, [_P, _P, _P, _i64, _i64, _P, _P, _i64]),
+    "kmoe_pages_create": (C.c_int, [_i64, _i32, C.POINTER(_P)]),
+    "kmoe_pages_destroy": (C.c_int, [_P]),
+    "kmoe_pages_last_error": (C.c_char_p, [_P]),
+    "kmoe_pages_append": (C.c_int, [_P, _u32, _i64, C.POINTER(_i32), C.POINTER(_i32), C.POINTER(_i32)]),
+    "kmoe_pages_fork": (C.c_int, [_P, _u32, _u32, _i64]),
+    "kmoe_pages_truncate": (C.c_int, [_P, _u32, _i64]),
+    "kmoe_pages_trim": (C.c_int, [_P, _u32, _i64, _i64, C.POINTER(_i64)]),
+    "kmoe_pages_drop": (C.c_int, [_P, _u32]),
+    "kmoe_pages_length": (C.c_int, [_P, _u32, C.POINTER(_i64)]),
+    "kmoe_pages_table": (C.c_int, [_P, _P, _i32, _i32, _P, _P]),
+    "kmoe_pages_compact": (C.c_int, [_P, _P, _P, _i64, C.POINTER(_i64)]),
+    "kmoe_pages_usage": (C.c_int, [_P, C.POINTER(_i64), C.POINTER(_i64)]),
     "kmoe_measure": (C.c_int, [_P, _P]),
     "kmoe_profile_enable": (C.c_int, [_P, C.c_int]),
     "kmoe_profile_read": (C.c_int, [_P, C.c_char_p, C.POINTER(C.c_double), C.POINTER(_i64)]),
@@ -125,6 +143,40 @@ class MoeDesc(C.Structure):
         ("up_type", _i32),
         ("down_type", _i32),
     ]
+
+
+class PagedDesc(C.Structure):
+    """kmoe_paged_desc (include/kmoe.h)."""
+
+    _fields_ = [("type", _i32), ("n_kv", _i32), ("head_dim", _i32), ("page", _i32), ("n_pages", _i64)]
+
+
+class PagedBatch(C.Structure):
+    """kmoe_paged_batch (include/kmoe.h), with the tensors it points into."""
+
+    _fields_ = [("n_seq", _i32), ("table_cols", _i32), ("s_rows", _i64), ("row_start", _P), ("seq_len", _P),
+                ("table", _P)]
+
+
+@dataclass(frozen=True)
+class PagedKV:
+    """Shape of a paged key-value cache: type F16 or Q8_0, kv heads, head_dim 64
+    or 128, positions per page (32, 64, 128 or 256)."""
+
+    type: int
+    n_kv: int
+    head_dim: int
+    page: int
+
+    @property
+    def page_bytes(self) -> int:
+        """Bytes of one page of one layer."""
+        e = 2 * self.n_kv * self.page * self.head_dim
+        return 2 * e if self.type == F16 else e // 32 * 34
+
+    def desc(self, pages, n_layer: int = 1) -> PagedDesc:
+        return PagedDesc(self.type, self.n_kv, self.head_dim, self.page,
+                         pages.numel() * pages.element_size() // (n_layer * self.page_bytes))
 
 
 class KmoeError(RuntimeError):
@@ -318,6 +370,94 @@ class Context:
                                                   head_dim, pos0, _ptr(pos_dev), n_ctx, _ptr(attn), t, _ptr(w),
                                                   w.numel() * w.element_size(), rows, _ptr(out)))
         return out
+
+    # ------------------------------------------------- paged key-value cache
+    def _need(self, name: str, t, dtype, rows: int, width: int, strided: bool = False):
+        """A [rows, width] device tensor of dtype, contiguous (strided: its rows may lie apart)."""
+        if t.dtype != dtype or t.device.type != "cuda" or t.device.index != self.device:
+            raise ValueError(f"{name}: need {dtype} on cuda:{self.device}, got {t.dtype} on {t.device}")
+        if t.numel() != rows * width:
+            raise ValueError(f"{name}: need [{rows}, {width}], got {list(t.shape)}")
+        if strided and t.dim() == 2 and rows and t.shape[0] == rows and t.stride(1) == 1:
+            return max(t.stride(0), width)
+        if not t.is_contiguous():
+            raise ValueError(f"{name}: rows are not contiguous")
+        return width
+
+    def paged_batch(self, table, seq_len, row_start=None, s_rows=None) -> PagedBatch:
+        """kmoe_paged_batch: table [n_seq, columns], seq_len [n_seq] and row_start [n_seq + 1] (or None: one
+        row per sequence), int32 on the device; the struct keeps them alive. A call reads what they hold when
+        its kernels run."""
+        i32, n = self.torch.int32, seq_len.numel()
+        self._need("seq_len", seq_len, i32, 1, n)
+        self._need("table", table, i32, n, table.numel() // n if n else 0)
+        if row_start is not None:
+            self._need("row_start", row_start, i32, 1, n + 1)
+            if s_rows is None:
+                raise ValueError("s_rows: the rows of a batch with row_start")
+        b = PagedBatch(n, table.numel() // n if n else 0, n if s_rows is None else s_rows, _ptr(row_start) or None,
+                       _ptr(seq_len), _ptr(table))
+        b.keep = (table, seq_len, row_start)
+        return b
+
+    def paged_kv_store(self, kv: PagedKV, pages, batch: PagedBatch, k, v):
+        """k, v [S, n_kv*head_dim] f32 (rows may be strided) into the pages."""
+        w, f = kv.n_kv * kv.head_dim, self.torch.float32
+        ks = self._need("k", k, f, batch.s_rows, w, True)
+        vs = self._need("v", v, f, batch.s_rows, w, True)
+        self.check(self.lib.kmoe_paged_kv_store(self.h, C.byref(kv.desc(pages)), _ptr(pages), C.byref(batch), _ptr(k),
+                                                ks, _ptr(v), vs))
+
+    def paged_rope_kv_store(self, kv: PagedKV, pages, batch: PagedBatch, q, k, v, n_head: int, rope_dim: int,
+                            inv_freq, neox: bool, q_out=None):
+        """RoPE of q (into q_out, returned) and k at the rows' positions, then the store; q, k and v may be
+        column ranges of one tensor."""
+        w, f = kv.n_kv * kv.head_dim, self.torch.float32
+        qs = self._need("q", q, f, batch.s_rows, n_head * kv.head_dim, True)
+        ks = self._need("k", k, f, batch.s_rows, w, True)
+        vs = self._need("v", v, f, batch.s_rows, w, True)
+        self._need("inv_freq", inv_freq, f, 1, rope_dim // 2)
+        if q_out is None:
+            q_out = self._empty((batch.s_rows, n_head * kv.head_dim), f)
+        else:
+            self._need("q_out", q_out, f, batch.s_rows, n_head * kv.head_dim)
+        self.check(self.lib.kmoe_paged_rope_kv_store(self.h, C.byref(kv.desc(pages)), _ptr(pages), C.byref(batch),
+                                                     _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, n_head, rope_dim,
+                                                     _ptr(inv_freq), int(neox), _ptr(q_out)))
+        return q_out
+
+    def paged_kv_read(self, kv: PagedKV, pages, batch: PagedBatch):
+        """The batch's rows read back: (k, v) f16 [S, n_kv*head_dim]."""
+        shape = (batch.s_rows, kv.n_kv * kv.head_dim)
+        k, v = self._empty(shape, self.torch.float16), self._empty(shape, self.torch.float16)
+        self.check(self.lib.kmoe_paged_kv_read(self.h, C.byref(kv.desc(pages)), _ptr(pages), C.byref(batch), _ptr(k),
+                                               _ptr(v)))
+        return k, v
+
+    def paged_attention(self, kv: PagedKV, pages, batch: PagedBatch, q, n_head: int, window: int = 0, n_sink: int = 0,
+                        out=None):
+        """Causal attention of the batch's rows q [S, n_head*head_dim] over their sequences' pages; with a
+        window a row sees its last `window` positions and the first n_sink."""
+        shape, f = (batch.s_rows, n_head * kv.head_dim), self.torch.float32
+        self._need("q", q, f, *shape)
+        if out is None:
+            out = self._empty(shape, f)
+        else:
+            self._need("out", out, f, *shape)
+        self.check(self.lib.kmoe_paged_attention(self.h, C.byref(kv.desc(pages)), _ptr(pages), C.byref(batch), _ptr(q),
+                                                 n_head, window, n_sink, _ptr(out)))
+        return out
+
+    def pages_copy(self, kv: PagedKV, pages, src, dst, n_layer: int = 1):
+        """Pages src[i] onto dst[i] (host sequences) in each of the n_layer equal parts of pages."""
+        s, d = (np.ascontiguousarray(a, dtype=np.int32).reshape(-1) for a in (src, dst))
+        if s.size != d.size:
+            raise ValueError(f"{s.size} source pages, {d.size} destinations")
+        if not pages.is_contiguous():
+            raise ValueError("pages: not contiguous")
+        self.check(self.lib.kmoe_pages_copy(self.h, C.byref(kv.desc(pages, n_layer)), _ptr(pages), n_layer,
+                                            pages.numel() * pages.element_size() // max(1, n_layer), s.ctypes.data,
+                                            d.ctypes.data, s.size))
 
     def swiglu(self, g, u, out=None):
         out = self.torch.empty_like(g) if out is None else out
@@ -570,6 +710,83 @@ class Context:
         ms, n = C.c_double(), _i64()
         self.check(self.lib.kmoe_profile_read(self.h, kernel.encode(), C.byref(ms), C.byref(n)))
         return ms.value, n.value
+
+
+class Pages:
+    """kmoe_pages: who holds which page of a paged cache (host only, no GPU)."""
+
+    def __init__(self, n_pages: int, page: int):
+        self.lib = load_library()
+        h = _P()
+        rc = self.lib.kmoe_pages_create(n_pages, page, C.byref(h))
+        if rc != 0:
+            raise KmoeError(rc, "kmoe_pages_create failed")
+        self.h, self.page, self.n_pages = h, page, n_pages
+
+    def close(self):
+        if getattr(self, "h", None):
+            self.lib.kmoe_pages_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def check(self, rc: int):
+        if rc != 0:
+            raise KmoeError(rc, self.lib.kmoe_pages_last_error(self.h).decode())
+
+    def append(self, seq: int, n: int):
+        """n more positions for seq (begun where there is none); the (src, dst) page to copy, or None."""
+        s, d, c = _i32(), _i32(), _i32()
+        self.check(self.lib.kmoe_pages_append(self.h, seq, n, C.byref(s), C.byref(d), C.byref(c)))
+        return (s.value, d.value) if c.value else None
+
+    def fork(self, src: int, dst: int, n: int):
+        """A new sequence dst of the first n positions of src, on the same pages."""
+        self.check(self.lib.kmoe_pages_fork(self.h, src, dst, n))
+
+    def truncate(self, seq: int, n: int):
+        self.check(self.lib.kmoe_pages_truncate(self.h, seq, n))
+
+    def trim(self, seq: int, window: int, n_sink: int = 0) -> int:
+        """Gives up the pages that no later row of seq sees; how many are free by it."""
+        n = _i64()
+        self.check(self.lib.kmoe_pages_trim(self.h, seq, window, n_sink, C.byref(n)))
+        return n.value
+
+    def drop(self, seq: int):
+        self.check(self.lib.kmoe_pages_drop(self.h, seq))
+
+    def length(self, seq: int) -> int:
+        n = _i64()
+        rc = self.lib.kmoe_pages_length(self.h, seq, C.byref(n))
+        if rc != 0:
+            raise KmoeError(rc, f"no sequence {seq}")
+        return n.value
+
+    def table(self, seqs, table_cols: int):
+        """(page table [n, table_cols], lengths [n]) of seqs, int32 on the host."""
+        ids = np.ascontiguousarray(seqs, dtype=np.uint32).reshape(-1)
+        t, n = np.empty((ids.size, table_cols), np.int32), np.empty(ids.size, np.int32)
+        self.check(self.lib.kmoe_pages_table(self.h, ids.ctypes.data, ids.size, table_cols, t.ctypes.data,
+                                             n.ctypes.data))
+        return t, n
+
+    def compact(self, most: int | None = None):
+        """Moves used pages to the front (at most `most`): (src, dst) pages to copy."""
+        cap = self.n_pages if most is None else most
+        s, d, n = np.empty(max(cap, 0), np.int32), np.empty(max(cap, 0), np.int32), _i64()
+        self.check(self.lib.kmoe_pages_compact(self.h, s.ctypes.data, d.ctypes.data, cap, C.byref(n)))
+        return s[:n.value], d[:n.value]
+
+    def usage(self):
+        """(used pages, all pages)."""
+        u, t = _i64(), _i64()
+        self.check(self.lib.kmoe_pages_usage(self.h, C.byref(u), C.byref(t)))
+        return u.value, t.value
 
 
 @dataclass
