@@ -181,7 +181,8 @@ struct kmoe_ctx {
   hipStream_t stream = nullptr;
   std::string err;
   int regime = KMOE_REGIME_AVX2;
-  uint32_t *counters = nullptr;  // device, kCounterWords completion counters, zero between calls
+  // device, zero between calls: kCounterWords completion counters, then the paged attention's
+  uint32_t *counters = nullptr;
   uint64_t vram_limit = 0;
   uint64_t vram_reserved = 0;
   std::map<uint32_t, Layer> layers;
@@ -212,6 +213,12 @@ struct kmoe_ctx {
   hipStream_t pws_stream = nullptr;  // of the last use outside a capture
   hipEvent_t pws_event = nullptr;
   std::vector<void *> pws_retired;
+  // partials of the paged attention's split units: one size, allocated at the
+  // first call and kept
+  float *gws = nullptr;
+  bool gws_used = false, gws_wait = false;
+  hipStream_t gws_stream = nullptr;  // of the last use outside a capture
+  hipEvent_t gws_event = nullptr;
   // last moe_ffn routing (pointers into ws) and its sizes
   uint32_t *last_idx = nullptr, *last_perm = nullptr, *last_off = nullptr;
   float *last_w = nullptr;
@@ -666,8 +673,44 @@ uint8_t *pieces(kmoe_ctx *c, size_t need) {
   return c->pws;
 }
 
+// The paged attention's partials: allocated once (in a capture too) and never
+// moved, so graphs that hold them stay valid. A call on another stream than the
+// last one waits for that one's use, as with the pieces.
+int paged_ws(kmoe_ctx *c, float **p) {
+  const bool cap = capturing(c->stream);
+  if (!c->gws) {
+    void *d = nullptr;
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    if (cap) (void)hipThreadExchangeStreamCaptureMode(&mode);
+    const int rc = dev_alloc(c, paged_part_floats() * sizeof(float), &d, "paged attention partials");
+    if (cap) (void)hipThreadExchangeStreamCaptureMode(&mode);
+    if (rc) return rc;
+    c->gws = (float *)d;
+  }
+  *p = c->gws;
+  if (cap) return KMOE_OK;
+  if (c->gws_wait) HIP_OK(c, hipStreamWaitEvent(c->stream, c->gws_event, 0));
+  c->gws_wait = false;
+  c->gws_used = true;
+  c->gws_stream = c->stream;
+  return KMOE_OK;
+}
+
+void leave_paged(kmoe_ctx *c, hipStream_t next) {
+  if (!c->gws_used || next == c->gws_stream || capturing(c->gws_stream) || capturing(next)) return;
+  DeviceGuard g(c->device);
+  if ((!c->gws_event && hipEventCreateWithFlags(&c->gws_event, hipEventDisableTiming) != hipSuccess) ||
+      hipEventRecord(c->gws_event, c->gws_stream) != hipSuccess) {
+    (void)hipGetLastError();  // no such stream any more
+    return;
+  }
+  c->gws_wait = true;
+  c->gws_used = false;
+}
+
 // The stream is about to change: the last use of the pieces is marked on its own.
 void leave_stream(kmoe_ctx *c, hipStream_t next) {
+  leave_paged(c, next);
   if (!c->pws_used || next == c->pws_stream || capturing(c->pws_stream) || capturing(next)) return;
   DeviceGuard g(c->device);
   if ((!c->pws_event && hipEventCreateWithFlags(&c->pws_event, hipEventDisableTiming) != hipSuccess) ||
@@ -787,8 +830,8 @@ int kmoe_create(int device, kmoe_ctx **out) {
   }
   c->stream = c->own;
   // completion counters of multi-work-group kernels; zero between calls
-  if (hipMalloc((void **)&c->counters, kCounterWords * 4) != hipSuccess ||
-      hipMemset(c->counters, 0, kCounterWords * 4) != hipSuccess) {
+  const size_t cw = ((size_t)kCounterWords + paged_counters()) * 4;
+  if (hipMalloc((void **)&c->counters, cw) != hipSuccess || hipMemset(c->counters, 0, cw) != hipSuccess) {
     (void)hipStreamDestroy(c->own);
     delete c;
     return KMOE_E_HIP;
@@ -832,6 +875,8 @@ int kmoe_destroy(kmoe_ctx *c) {
   if (c->pws) (void)hipFree(c->pws);
   for (void *p : c->pws_retired) (void)hipFree(p);
   if (c->pws_event) (void)hipEventDestroy(c->pws_event);
+  if (c->gws) (void)hipFree(c->gws);
+  if (c->gws_event) (void)hipEventDestroy(c->gws_event);
   if (c->counters) (void)hipFree(c->counters);
   if (c->own) (void)hipStreamDestroy(c->own);
   delete c;
@@ -2571,7 +2616,11 @@ int kmoe_paged_attention(kmoe_ctx *c, const kmoe_paged_desc *d, const void *page
   if (a.s_rows == 0) return KMOE_OK;
   if (!q || !out) return fail(c, KMOE_E_INVALID, "null pointer");
   DeviceGuard g(c->device);
-  LAUNCH(c, "paged_attention", launch_paged_attention(c->stream, a, q, n_head, window, n_sink, out));
+  float *part = nullptr;
+  rc = paged_ws(c, &part);
+  if (rc) return rc;
+  LAUNCH(c, "paged_attention", launch_paged_attention(c->stream, a, q, n_head, window, n_sink, out, part,
+                                                      c->counters + kCounterWords));
   return KMOE_OK;
 }
 

@@ -114,7 +114,11 @@ hipError_t launch_paged_store(hipStream_t st, const PagedArgs &a, const float *q
 hipError_t launch_paged_read(hipStream_t st, const PagedArgs &a, uint16_t *k, uint16_t *v);
 hipError_t launch_pages_copy(hipStream_t st, uint8_t *pages, int64_t n_layer, int64_t layer_stride,
                              int64_t page_bytes, const int32_t *src, const int32_t *dst, int64_t n);
+// part: paged_part_floats() floats, counters: paged_counters() words, zero
+// between calls; both of this call alone until it has run.
+size_t paged_part_floats();
+int paged_counters();
 hipError_t launch_paged_attention(hipStream_t st, const PagedArgs &a, const float *q, int n_head, int64_t window,
-                                  int64_t n_sink, float *out);
+                                  int64_t n_sink, float *out, float *part, uint32_t *counters);
 
 }  // namespace kmoe
