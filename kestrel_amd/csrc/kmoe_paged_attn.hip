@@ -234,282 +234,307 @@ __device__ __forceinline__ Span span_of(int64_t pos_lo, int64_t pos_hi, int64_t 
   return Span{n, t_lo, n + t_hi - t_lo};
 }
 
-// How a call's work is shared out. A unit is one kv head of one column tile (16 C
-// columns: the sequence's rows by the heads of the group, row-major); its
-// positions are cut into chunks of `tpc` tiles, and an item is one chunk. Every
-// work-group forms the same plan from the lengths, so the shares follow what a
-// captured call finds when it is replayed.
-struct Plan {
-  int tpc, items;
+// How a call's work is shared out. A column tile is 16 C columns: the sequence's
+// rows by the heads of the group, row-major. A unit is one kv head of two column
+// tiles of a sequence, the i-th from the front and the i-th from the back: with a
+// causal mask the tiles that the two see together are about the same for every
+// i. All units' tiles of 32 positions, a unit's rounded up to fours (one per
+// wave) and with kUnitCost for what a unit costs besides, lie in one line, and
+// every work-group takes an equal stretch of it: segments of column tiles, at most
+// two of them split with its neighbours. Every work-group forms the plan from the
+// lengths, so the shares follow what a captured call finds when it is replayed.
+constexpr int kUnitCost = 4;
+constexpr int kMinShare = 8;  // tiles
+
+struct SeqPlan {
+  int n_ct, per;  // column tiles; tiles of the line per unit
+  __device__ __forceinline__ int pairs() const { return (n_ct + 1) >> 1; }
 };
-// Most tiles that a column tile of the sequence can see.
-__device__ __forceinline__ int seq_tiles(const PagedArgs &a, int64_t n, int64_t len, int rows_per, int window, int sink) {
-  if (n == 0) return 0;
-  const int all = span_of(0, len - 1, (int64_t)a.table_cols * a.page, 0, 0).vt;
-  if (window == 0) return all;
-  const int64_t w = (int64_t)(sink + kTile - 1) / kTile + ((int64_t)window + rows_per + kTile - 2) / kTile + 1;
-  return w < all ? (int)w : all;
+__device__ __forceinline__ int round4(int x) { return (x + 3) & ~3; }
+template <int COLS>
+__device__ __forceinline__ SeqPlan seq_plan(int64_t n, int64_t len, int group, int64_t cap, int window, int sink) {
+  SeqPlan r{(int)((n * group + COLS - 1) / COLS), 0};
+  if (r.n_ct == 0) return r;
+  const int all = span_of(0, len - 1, cap, 0, 0).vt;  // of the last row without a window
+  // most of a column tile, and most of two that are paired: their last rows lie
+  // (n_ct - 1) COLS / group + COLS / group positions after the first row together
+  int one = all;
+  const int64_t rows_per = (COLS + group - 1) / group + 1, base = len - n > 0 ? len - n : 0;
+  int64_t two = (2 * base + (int64_t)(r.n_ct + 1) * COLS / group + 3 + kTile - 1) / kTile + 2;
+  two = two < 2 * (int64_t)all ? two : 2 * (int64_t)all;
+  if (window) {
+    const int64_t w = (int64_t)(sink + kTile - 1) / kTile + ((int64_t)window + rows_per + kTile - 2) / kTile + 1;
+    one = w < one ? (int)w : one;
+    two = two < 2 * w ? two : 2 * w;
+  }
+  // (each rounded up to fours, and a column tile that sees nothing takes a place too)
+  r.per = kUnitCost + (r.n_ct == 1 ? round4(one > 0 ? one : 1) : round4((int)two) + 8);
+  return r;
 }
 
-// Exclusive scan of two counts over the work-group's threads.
-__device__ __forceinline__ void scan2(int64_t &x, int64_t &y, int64_t &tx, int64_t &ty, int64_t (*red)[2]) {
+// Exclusive scan over the work-group's threads, and the total.
+__device__ __forceinline__ int64_t scan(int64_t x, int64_t &total, int64_t *red) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t ix = x, iy = y;
+  int64_t ix = x;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int64_t ux = __shfl_up(ix, d), uy = __shfl_up(iy, d);
-    if (lane >= d) {
-      ix += ux;
-      iy += uy;
-    }
+    const int64_t ux = __shfl_up(ix, d);
+    if (lane >= d) ix += ux;
   }
-  __syncthreads();
-  if (lane == 63) {
-    red[wave][0] = ix;
-    red[wave][1] = iy;
-  }
+  if (lane == 63) red[wave] = ix;
   __syncthreads();
   x = ix - x;
-  y = iy - y;
-  tx = ty = 0;
+  total = 0;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    if (w < wave) {
-      x += red[w][0];
-      y += red[w][1];
-    }
-    tx += red[w][0];
-    ty += red[w][1];
+    if (w < wave) x += red[w];
+    total += red[w];
   }
+  return x;
 }
 
-// start[b], slot[b] (b <= n_seq): items and partial slots before sequence b.
-template <int C>
-__device__ Plan make_plan(const PagedArgs &a, int group, int window, int sink, int target, int *start, int *slot,
-                          int64_t (*red)[2]) {
+// start[b] (b <= n_seq): the line's tiles before sequence b.
+template <int COLS>
+__device__ void make_plan(const PagedArgs &a, int group, int64_t cap, int window, int sink, int64_t *start, int64_t *red) {
   const int per = (a.n_seq + 255) / 256, b0 = threadIdx.x * per;
-  const int rows_per = (16 * C + group - 1) / group + 1;
-  int64_t tiles = 0, units = 0, tt, tu;
-  for (int b = b0; b < b0 + per && b < a.n_seq; ++b) {
+  auto space = [&](int b) -> int64_t {
     int64_t r0, n;
     paged_rows(a, b, r0, n);
-    const int64_t u = (n * group + 16 * C - 1) / (16 * C) * a.n_kv;
-    units += u;
-    tiles += u * seq_tiles(a, n, a.seq_len[b], rows_per, window, sink);
-  }
-  scan2(tiles, units, tt, tu, red);
-  // chunks that give the launch's work-groups one item each where the units leave room for that
-  const int64_t room = tu < target / 2 ? target - tu : target / 2;
-  int64_t tpc = (tt + room - 1) / room;
-  tpc = (tpc + 3) / 4 * 4;
-  if (tpc < 4) tpc = 4;
-  if (tpc > (int64_t)1 << 26) tpc = (int64_t)1 << 26;
-  int64_t items = 0, slots = 0, ti, ts;
-  for (int pass = 0; pass < 2; ++pass) {
-    int64_t i = items, s = slots;
+    const SeqPlan s = seq_plan<COLS>(n, a.seq_len[b], group, cap, window, sink);
+    return (int64_t)s.pairs() * a.n_kv * s.per;
+  };
+  int64_t sum = 0, total;
+  for (int b = b0; b < b0 + per && b < a.n_seq; ++b) sum += space(b);
+  int64_t at = scan(sum, total, red);
+  if (per == 1) {
+    if (b0 < a.n_seq) start[b0] = at;
+  } else {
     for (int b = b0; b < b0 + per && b < a.n_seq; ++b) {
-      int64_t r0, n;
-      paged_rows(a, b, r0, n);
-      const int64_t u = (n * group + 16 * C - 1) / (16 * C) * a.n_kv;
-      const int vt = seq_tiles(a, n, a.seq_len[b], rows_per, window, sink);
-      const int64_t nch = vt > tpc ? (vt + tpc - 1) / tpc : 1;
-      if (pass) {
-        start[b] = (int)i;
-        slot[b] = (int)s;
-      }
-      i += u * nch;
-      s += nch > 1 ? u * nch : 0;
-    }
-    if (!pass) {
-      items = i;
-      slots = s;
-      scan2(items, slots, ti, ts, red);
+      start[b] = at;
+      at += space(b);
     }
   }
-  if (threadIdx.x == 0) start[a.n_seq] = (int)ti;
+  if (threadIdx.x == 0) start[a.n_seq] = total;
   __syncthreads();
-  // (more items than rows and positions allow: row_start is not ascending, nothing is done)
-  return Plan{__builtin_amdgcn_readfirstlane((int)tpc), __builtin_amdgcn_readfirstlane(ti < (1 << 30) ? (int)ti : 0)};
 }
 
-// Work-group: four waves, one item at a time; wave w takes the chunk's tiles w,
-// w + 4, ... (32 positions each) with its own running softmax, and the waves are
-// merged through LDS.
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
+                   (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32);
+}
+
+// Work-group: four waves, one segment of a column tile at a time; wave w takes
+// its tiles w, w + 4, ... (32 positions each) with its own running softmax, and
+// the waves are merged through LDS.
 //
 // Per tile and wave, v_mfma_f32_16x16x32_f16 throughout:
 //   scores S^T[position, column] = K . q^T: A = K tiles as they lie in the page,
 //     B = q, scaled by a power of two per column to [2^14, 2^15) and split into
-//     two f16 pieces, in registers. Lane (kg, column) ends with positions 4 kg ..
-//     4 kg + 3 of each 16.
+//     two f16 pieces (LDS). Lane (kg, column) ends with positions 4 kg .. 4 kg + 3
+//     of each 16.
 //   O^T[dim, column] += V^T . P: A = V tiles as they lie in the page, B = the
 //     weights of the lane's own eight positions, times 2^14, as two f16 pieces,
 //     straight from the score registers.
 // K and V (Q8_0: the quants) are exact in f16 and all sums are f32. Q8_0: a score
 // is summed 32 dims at a time, one K step, and scaled by the position's scale of
-// those; V's scales go into the weights before they are split, over the tile's
-// largest (a power of two), once per 32 dims.
-// Scores and the running maximum are in units of log2 e.
-#ifndef KMOE_OCC1
-#define KMOE_OCC1 2
-#endif
+// those; V's scales go into the weights before they are split, over a power of
+// two that no scale so far has passed, per 32 dims.
+// The running maximum is in units of log2 e.
 template <int T, int HD, int C>
-__global__ void __launch_bounds__(256, KMOE_OCC1)
-    k_paged_attn(PagedArgs a, const float *__restrict__ q, int nh, int window, int sink, int target,
-                 float *__restrict__ part, float *__restrict__ part_ml, uint32_t *counters, float *__restrict__ out) {
+__global__ void __launch_bounds__(256, 2)
+    k_paged_attn(PagedArgs a, const float *__restrict__ q, int nh, int window, int sink, float *__restrict__ part,
+                 float *__restrict__ part_ml, uint32_t *counters, float *__restrict__ out) {
   constexpr int NT = HD / 32, NU = HD / 16, COLS = 16 * C, OROW = HD + 4;
-  extern __shared__ int plan_lds[];  // [2][n_seq + 1]
-  __shared__ __attribute__((aligned(16))) float o_lds[4][COLS][OROW];
-  __shared__ float m_lds[4][COLS], l_lds[4][COLS];
-  __shared__ int64_t red[4][2];
+  extern __shared__ int64_t start[];  // [n_seq + 1]
+  __shared__ union {
+    u32x4 q[C][NT][2][64];
+    float o[4][COLS][OROW];
+    float f[4 * COLS * OROW];
+  } L;
+  __shared__ float fs_lds[COLS], m_lds[4][COLS], l_lds[4][COLS];
+  __shared__ f32x4 grp[256];
+  __shared__ int64_t red[4];
   __shared__ uint32_t bad_cols, arrived;
-  int *start = plan_lds, *slot = plan_lds + a.n_seq + 1;
   const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, kg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = nh / a.n_kv;
   const int64_t bb = paged_block_bytes(T, a.page, HD);
   const int64_t cap = (int64_t)a.table_cols * a.page;
   const int pshift = __builtin_ctz(a.page);
-  const Plan plan = make_plan<C>(a, group, window, sink, target, start, slot, red);
+  make_plan<COLS>(a, group, cap, window, sink, start, red);
 
-  for (int item = blockIdx.x; item < plan.items; item += gridDim.x) {
-    // the item's sequence: the last one that starts at or before it
-    int b = 0;
+  // this work-group's stretch of the line; neighbours in it share an XCD's L2
+  const int64_t total = uniform64(start[a.n_seq]);
+  const int rank = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+  int64_t share = (total + gridDim.x - 1) / gridDim.x;
+  share = share < kMinShare ? kMinShare : (share + 3) & ~(int64_t)3;
+  const int64_t x0 = rank * share, x1 = x0 + share < total ? x0 + share : total;
+  int b = 0;
+  if (x0 < x1)  // the last sequence that starts at or before x0
     for (int hi = a.n_seq; hi - b > 1;) {
       const int mid = (b + hi) >> 1;
-      if (start[mid] <= item) b = mid;
+      if (start[mid] <= x0) b = mid;
       else hi = mid;
     }
-    b = __builtin_amdgcn_readfirstlane(b);
-    int64_t r0v, nv_;
-    paged_rows(a, b, r0v, nv_);
-    const int64_t r0 = __builtin_amdgcn_readfirstlane((int)r0v), n = __builtin_amdgcn_readfirstlane((int)nv_);
+  b = __builtin_amdgcn_readfirstlane(b);
+
+  for (int64_t x = x0; x < x1;) {
+    while (uniform64(start[b + 1]) <= x) ++b;
+    const int64_t sb = uniform64(start[b]);
+    int64_t r0v, rnv;
+    paged_rows(a, b, r0v, rnv);
+    const int64_t r0 = __builtin_amdgcn_readfirstlane((int)r0v), n = __builtin_amdgcn_readfirstlane((int)rnv);
     const int64_t len = __builtin_amdgcn_readfirstlane(a.seq_len[b]);
-    const int local = __builtin_amdgcn_readfirstlane(item - start[b]);
-    const int n_ct = (int)((n * group + COLS - 1) / COLS);
-    const int nch = __builtin_amdgcn_readfirstlane(start[b + 1] - start[b]) / (n_ct * a.n_kv);
-    const int g = local % a.n_kv, ch = local / a.n_kv % nch;
-    const int ct = n_ct - 1 - local / a.n_kv / nch;  // the later rows, which see more, first
-    const int64_t c0 = (int64_t)ct * COLS;           // first column
+    const SeqPlan pl_ = seq_plan<COLS>(n, len, group, cap, window, sink);
+    const int64_t unit = (x - sb) / pl_.per;
+    const int off = (int)(x - sb - unit * pl_.per);
+    const int g = (int)(unit / pl_.pairs()), pair = (int)(unit - (int64_t)g * pl_.pairs());
+    auto span = [&](int ct) {
+      const int64_t c = (int64_t)ct * COLS, e = c + COLS < n * group ? c + COLS : n * group;
+      return span_of(len - n + c / group, len - n + (e - 1) / group, cap, window, sink);
+    };
+    const int ct_a = pl_.n_ct - 1 - pair;
+    const Span sp_a = span(ct_a);
+    const int len_a = round4(sp_a.vt > 0 ? sp_a.vt : 1);
+    const bool second = off >= len_a;
+    const int ct = second ? pair : ct_a;
+    const Span sp = second ? span(ct) : sp_a;
+    const int extent = second && ct == ct_a ? 0 : sp.vt > 0 ? sp.vt : 1;  // (a middle column tile has no partner)
+    const int at = second ? off - len_a : off;
+    if (at >= extent) {  // what is left of the first part's fours, or of the unit
+      x += (second ? pl_.per : len_a) - off;
+      continue;
+    }
+    const int64_t X = x - at;  // where the column tile lies in the line
+    const int v_end = (int)(x1 - X < extent ? x1 - X : extent);
+    const int64_t w_first = X / share, n_seg = (X + extent - 1) / share - w_first + 1;
+    x = X + v_end;
+
+    const int64_t c0 = (int64_t)ct * COLS;  // first column
     const int nv = (int)(n * group - c0 < COLS ? n * group - c0 : COLS);
-    const int64_t i_lo = c0 / group, i_hi = (c0 + nv - 1) / group;
-    const int64_t pos_lo = len - n + i_lo, pos_hi = len - n + i_hi;
-    const Span sp = span_of(pos_lo, pos_hi, cap, window, sink);
-    const int n_act = (sp.vt + plan.tpc - 1) / plan.tpc;
-    if (ch >= n_act && !(ch == 0 && n_act == 0)) continue;
-    const int v_end = (ch + 1) * plan.tpc < sp.vt ? (ch + 1) * plan.tpc : sp.vt;
-    const int hi_pos = (int)(pos_hi + 1 < cap ? pos_hi + 1 : cap);  // positions of the item end here
+    const int64_t pos_lo = len - n + c0 / group, pos_hi = len - n + (c0 + nv - 1) / group;
+    const int hi_pos = (int)(pos_hi + 1 < cap ? pos_hi + 1 : cap);  // the columns' positions end here
     const int lo_pos = window && pos_lo - window + 1 > 0 ? (int)(pos_lo - window + 1) : 0;
-
-    // columns: position, first position of the window, q in two pieces
-    int pos_c[C], lo_c[C];
-    float fs[C];
-    h8 qh[C][NT], ql[C][NT];
-#pragma unroll
-    for (int j = 0; j < C; ++j) {
-      const int cc = 16 * j + c16, cv = cc < nv ? cc : nv - 1;
-      const int64_t i = (c0 + cv) / group;
-      const int h = (int)((c0 + cv) - i * group);
-      const int64_t p = len - n + i;
-      pos_c[j] = cc < nv ? (int)(p < cap ? p : cap - 1) : -1;
-      lo_c[j] = window && p - window + 1 > 0 ? (int)(p - window + 1) : 0;
-      const float *qp = q + ((r0 + i) * nh + (int64_t)g * group + h) * HD + 8 * kg;
-      f32x4a4 x[NT][2];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        x[t][0] = *(const f32x4a4 *)(qp + 32 * t);
-        x[t][1] = *(const f32x4a4 *)(qp + 32 * t + 4);
-      }
-      float amax = 0.0f;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[t][e >> 2][e & 3]));
-      amax = quad_max(amax);
-      int sh = 15 - ((int)(__float_as_uint(amax) >> 23) - 126);
-      sh = sh < 100 ? sh : 100;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        u32x4 hi, lo;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t y, z;
-          split2(ldexpf(x[t][e >> 1][2 * (e & 1)], sh), ldexpf(x[t][e >> 1][2 * (e & 1) + 1], sh), y, z);
-          hi[e] = y;
-          lo[e] = z;
-        }
-        qh[j][t] = __builtin_bit_cast(h8, hi);
-        ql[j][t] = __builtin_bit_cast(h8, lo);
-      }
-      fs[j] = ldexpf((float)(1.4426950408889634 / (HD == 64 ? 8.0 : 11.313708498984761)), -sh);
-    }
-
-    f32x4 O[C][NU];
-    float m[C], l[C];
-#pragma unroll
-    for (int j = 0; j < C; ++j) {
-      m[j] = -INFINITY;
-      l[j] = 0.0f;
-#pragma unroll
-      for (int u = 0; u < NU; ++u) O[j][u] = f32x4{0};
-    }
+    const int v_last = v_end < sp.vt ? v_end : sp.vt;
 
     const_i32 row = (const_i32)(uintptr_t)(a.table + (int64_t)b * a.table_cols);
-    // the block of a tile, and whether its page exists (page 0 stands in for one that does not)
-    auto page_of = [&](int v) -> int { return v < v_end ? row[sp.tile(v) >> (pshift - 5)] : -1; };
+    auto page_of = [&](int v) -> int { return v < v_last ? row[sp.tile(v) >> (pshift - 5)] : -1; };
+    // the block of a tile's page (page 0 stands in for one that does not exist)
     auto block = [&](int id) { return a.pages + ((int64_t)id * a.n_kv + g) * bb; };
     Frags<T, HD> fr;
-    int v = ch * plan.tpc + wave;
+    int v = at + wave;
     int id = page_of(v), id_next = page_of(v + 4);
     bool ok = id >= 0 && id < a.n_pages;
-    if (v < v_end) {
+    if (v < v_last) {
       const int pp = (sp.tile(v) * kTile) & (a.page - 1);
       const uint8_t *p = block(ok ? id : 0);
       fr.load_k(p, a.page, pp, lane);
       fr.load_v(p, a.page, pp, lane);
     }
-    for (; v < v_end; v += 4) {
+
+    // columns: position, first position of the window; q in two pieces, wave j column tile j of 16
+    int pos_c[C], lo_c[C];
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const int cc = 16 * j + c16, cv = cc < nv ? cc : nv - 1;
+      const int64_t i = (c0 + cv) / group;
+      const int64_t p = len - n + i;
+      pos_c[j] = cc < nv ? (int)(p < cap ? p : cap - 1) : -1;
+      lo_c[j] = window && p - window + 1 > 0 ? (int)(p - window + 1) : 0;
+      if (wave == j) {
+        const int h = (int)((c0 + cv) - i * group);
+        const float *qp = q + ((r0 + i) * nh + (int64_t)g * group + h) * HD + 8 * kg;
+        f32x4a4 y[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          y[t][0] = *(const f32x4a4 *)(qp + 32 * t);
+          y[t][1] = *(const f32x4a4 *)(qp + 32 * t + 4);
+        }
+        float amax = 0.0f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(y[t][e >> 2][e & 3]));
+        amax = quad_max(amax);
+        int sh = 15 - ((int)(__float_as_uint(amax) >> 23) - 126);
+        sh = sh < 100 ? sh : 100;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          u32x4 hi, lo;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t u, w;
+            split2(ldexpf(y[t][e >> 1][2 * (e & 1)], sh), ldexpf(y[t][e >> 1][2 * (e & 1) + 1], sh), u, w);
+            hi[e] = u;
+            lo[e] = w;
+          }
+          L.q[j][t][0][lane] = hi;
+          L.q[j][t][1][lane] = lo;
+        }
+        if (kg == 0) fs_lds[cc] = ldexpf((float)(1.4426950408889634 / (HD == 64 ? 8.0 : 11.313708498984761)), -sh);
+      }
+    }
+    lds_barrier();
+    float fs[C];
+    f32x4 O[C][NU];
+    float m[C], l[C], up[T == kPgQ8 ? NT : 1], back[T == kPgQ8 ? NT : 1];
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      fs[j] = fs_lds[16 * j + c16];
+      m[j] = -INFINITY;
+      l[j] = 0.0f;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) O[j][u] = f32x4{0};
+    }
+    if constexpr (T == kPgQ8) {
+#pragma unroll
+      for (int u = 0; u < NT; ++u) up[u] = 0x1p30f, back[u] = 0x1p-16f;
+    }
+
+    for (; v < v_last; v += 4) {
       const int p0 = sp.tile(v) * kTile;
-      const bool more = v + 4 < v_end;
+      const bool more = v + 4 < v_last;
       const bool ok_next = id_next >= 0 && id_next < a.n_pages;
       const int pp_next = more ? (sp.tile(v + 4) * kTile) & (a.page - 1) : 0;
       const uint8_t *p_next = block(ok_next ? id_next : 0);
       id_next = page_of(v + 8);
-      // scores
+      int lq = lane;
+      asm volatile("" : "+v"(lq));  // q's pieces are read here, not held in registers over the loop
+      // scores, in q's scale
       f32x4 S[C][2];
-      if constexpr (T == kPgF16) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < 2; ++s) {
+        if constexpr (T == kPgF16) {
 #pragma unroll
           for (int j = 0; j < C; ++j) {
             f32x4 lo = f32x4{0}, hi = f32x4{0};
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-              const h8 x = __builtin_bit_cast(h8, fr.k[s][t]);
-              lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ql[j][t], lo, 0, 0, 0);
-              hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qh[j][t], hi, 0, 0, 0);
+              const h8 k = __builtin_bit_cast(h8, fr.k[s][t]);
+              lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, __builtin_bit_cast(h8, L.q[j][t][1][lq]), lo, 0, 0, 0);
+              hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, __builtin_bit_cast(h8, L.q[j][t][0][lq]), hi, 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) S[j][s][i] = fmaf(lo[i], kLo, hi[i]) * fs[j];
+            for (int i = 0; i < 4; ++i) S[j][s][i] = fmaf(lo[i], kLo, hi[i]);
           }
-      } else {
+        } else {
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+          for (int j = 0; j < C; ++j) S[j][s] = f32x4{0};
 #pragma unroll
-          for (int j = 0; j < C; ++j) {
-            f32x4 sum = f32x4{0};
+          for (int t = 0; t < NT; ++t) {
+            const h8 k = i8_h8(fr.k[s][t >> 1][2 * (t & 1)], fr.k[s][t >> 1][2 * (t & 1) + 1]);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              const h8 x = i8_h8(fr.k[s][t >> 1][2 * (t & 1)], fr.k[s][t >> 1][2 * (t & 1) + 1]);
-              f32x4 lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ql[j][t], f32x4{0}, 0, 0, 0);
-              f32x4 hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qh[j][t], f32x4{0}, 0, 0, 0);
+            for (int j = 0; j < C; ++j) {
+              const f32x4 lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, __builtin_bit_cast(h8, L.q[j][t][1][lq]), f32x4{0}, 0, 0, 0);
+              const f32x4 hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, __builtin_bit_cast(h8, L.q[j][t][0][lq]), f32x4{0}, 0, 0, 0);
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                sum[i] = fmaf(fmaf(lo[i], kLo, hi[i]), half_of(fr.ks[s][t >> 1], 4 * (t & 1) + i), sum[i]);
+                S[j][s][i] = fmaf(fmaf(lo[i], kLo, hi[i]), half_of(fr.ks[s][t >> 1], 4 * (t & 1) + i), S[j][s][i]);
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) S[j][s][i] = sum[i] * fs[j];
           }
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);
       if (more) fr.load_k(p_next, a.page, pp_next, lane);
       // what some row does not see
       if (!ok || p0 + kTile > pos_lo + 1 || (window && p0 < (int)(pos_hi - window + 1) && p0 + kTile > sink)) {
@@ -526,14 +551,32 @@ __global__ void __launch_bounds__(256, KMOE_OCC1)
           }
         fr.keep_v(keep);
       }
+      if constexpr (T == kPgQ8) {  // V's largest scales so far
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          h2 d = {(_Float16)0.0f, (_Float16)0.0f};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d = __builtin_elementwise_max(d, __builtin_bit_cast(h2, fr.vs[u][i]));
+          const float dm = fmaxf((float)d.x, (float)d.y);
+          if (__builtin_amdgcn_ballot_w64(dm > back[u])) {
+            const int ex = (int)(__float_as_uint(quad_max(dm)) >> 23) - 126;  // largest in [2^(ex - 1), 2^ex)
+            const float r = ldexpf(back[u], -ex);  // O is kept over 2^14 * 2^-ex
+            back[u] = ldexpf(1.0f, ex);
+            up[u] = ldexpf(1.0f, 14 - ex);
+#pragma unroll
+            for (int j = 0; j < C; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) O[j][2 * u][i] *= r, O[j][2 * u + 1][i] *= r;
+          }
+        }
+      }
       // running softmax, and the weights' pieces
-      u32x4 ph[C], pl[C];
       float e8[C][8];
 #pragma unroll
       for (int j = 0; j < C; ++j) {
         float mx = fmaxf(fmaxf(S[j][0][0], S[j][0][1]), fmaxf(S[j][0][2], S[j][0][3]));
         mx = fmaxf(mx, fmaxf(fmaxf(S[j][1][0], S[j][1][1]), fmaxf(S[j][1][2], S[j][1][3])));
-        mx = fmaxf(m[j], quad_max(mx));
+        mx = fmaxf(m[j], quad_max(mx) * fs[j]);
         if (__builtin_amdgcn_ballot_w64(mx > m[j])) {
           const float f = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[j] - mx);
           m[j] = mx;
@@ -547,75 +590,69 @@ __global__ void __launch_bounds__(256, KMOE_OCC1)
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          e8[j][i] = __builtin_amdgcn_exp2f(S[j][i >> 2][i & 3] - mb);
+          e8[j][i] = __builtin_amdgcn_exp2f(fmaf(S[j][i >> 2][i & 3], fs[j], -mb));
           sum += e8[j][i];
         }
         l[j] += sum;
-        if constexpr (T == kPgF16) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t x, y;
-            split2(e8[j][2 * i] * 0x1p14f, e8[j][2 * i + 1] * 0x1p14f, x, y);
-            ph[j][i] = x;
-            pl[j][i] = y;
-          }
-        }
       }
       // weighted V
       if constexpr (T == kPgF16) {
+        u32x4 ph[C], pl[C];
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t y, z;
+            split2(e8[j][2 * i] * 0x1p14f, e8[j][2 * i + 1] * 0x1p14f, y, z);
+            ph[j][i] = y;
+            pl[j][i] = z;
+          }
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-          const h8 x = __builtin_bit_cast(h8, fr.v[u]);
+          const h8 y = __builtin_bit_cast(h8, fr.v[u]);
 #pragma unroll
           for (int j = 0; j < C; ++j) {
-            f32x4 t = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, __builtin_bit_cast(h8, pl[j]), f32x4{0}, 0, 0, 0);
+            const f32x4 t = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, __builtin_bit_cast(h8, pl[j]), f32x4{0}, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) t[i] *= kLo;
-            t = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, __builtin_bit_cast(h8, ph[j]), t, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) O[j][u][i] += t[i];
+            for (int i = 0; i < 4; ++i) O[j][u][i] = fmaf(t[i], kLo, O[j][u][i]);
+            O[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, __builtin_bit_cast(h8, ph[j]), O[j][u], 0, 0, 0);
           }
         }
       } else {
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
-          // the tile's largest scale of these dims, as a power of two
-          float dm = 0.0f;
+          const h8 y0 = i8_h8(fr.v[u][0], fr.v[u][1]), y1 = i8_h8(fr.v[u][2], fr.v[u][3]);
+          float sc[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) dm = fmaxf(dm, half_of(fr.vs[u], i));
-          dm = quad_max(dm);
-          int ex = (int)(__float_as_uint(dm) >> 23) - 126;  // dm in [2^(ex - 1), 2^ex)
-          ex = dm > 0.0f ? ex : 0;
-          const float up = ldexpf(1.0f, 14 - ex), back = ldexpf(1.0f, ex);
-          const h8 x0 = i8_h8(fr.v[u][0], fr.v[u][1]), x1 = i8_h8(fr.v[u][2], fr.v[u][3]);
+          for (int i = 0; i < 8; ++i) sc[i] = half_of(fr.vs[u], i) * up[u];
 #pragma unroll
           for (int j = 0; j < C; ++j) {
             u32x4 wh, wl;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              uint32_t x, y;
-              split2(e8[j][2 * i] * (half_of(fr.vs[u], 2 * i) * up), e8[j][2 * i + 1] * (half_of(fr.vs[u], 2 * i + 1) * up), x, y);
-              wh[i] = x;
-              wl[i] = y;
+              uint32_t y, z;
+              split2(e8[j][2 * i] * sc[2 * i], e8[j][2 * i + 1] * sc[2 * i + 1], y, z);
+              wh[i] = y;
+              wl[i] = z;
             }
 #pragma unroll
             for (int d = 0; d < 2; ++d) {
-              const h8 x = d ? x1 : x0;
-              f32x4 t = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, __builtin_bit_cast(h8, wl), f32x4{0}, 0, 0, 0);
+              const h8 y = d ? y1 : y0;
+              const f32x4 t = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, __builtin_bit_cast(h8, wl), f32x4{0}, 0, 0, 0);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) t[i] *= kLo;
-              t = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, __builtin_bit_cast(h8, wh), t, 0, 0, 0);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) O[j][2 * u + d][i] = fmaf(t[i], back, O[j][2 * u + d][i]);
+              for (int i = 0; i < 4; ++i) O[j][2 * u + d][i] = fmaf(t[i], kLo, O[j][2 * u + d][i]);
+              O[j][2 * u + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, __builtin_bit_cast(h8, wh), O[j][2 * u + d], 0, 0, 0);
             }
           }
         }
       }
       ok = ok_next;
+      __builtin_amdgcn_sched_barrier(0);
       if (more) fr.load_v(p_next, a.page, pp_next, lane);
     }
 
     // the four waves' sums, O times 2^14
+    lds_barrier();  // every wave is done with q
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const float ls = quad_sum(l[j]);
@@ -624,91 +661,121 @@ __global__ void __launch_bounds__(256, KMOE_OCC1)
         l_lds[wave][16 * j + c16] = ls;
       }
 #pragma unroll
-      for (int u = 0; u < NU; ++u) *(f32x4 *)&o_lds[wave][16 * j + c16][16 * u + 4 * kg] = O[j][u];
+      for (int u = 0; u < NU; ++u) {
+        f32x4 y = O[j][u];
+        if constexpr (T == kPgQ8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] *= back[u >> 1];
+        *(f32x4 *)&L.o[wave][16 * j + c16][16 * u + 4 * kg] = y;
+      }
     }
     if (tid == 0) bad_cols = 0;
     lds_barrier();
-    const bool whole = n_act <= 1;
-    const int unit_slot = slot[b] + ((n_ct - 1 - ct) * nch) * a.n_kv + g;  // of chunk 0; chunk i is i * n_kv further
-    const int64_t my_slot = unit_slot + (int64_t)ch * a.n_kv;
-    auto out_at = [&](int c) {
+    const bool whole = n_seg == 1;
+    const int64_t my_slot = 2 * (int64_t)rank + (X >= x0);
+    auto finish = [&](int c, int d, const f32x4 &y, float M, float Lsum) {
+      const float inv = M == -INFINITY ? 0.0f : 0x1p-14f / Lsum;  // nothing seen: zeros
       const int64_t i = (c0 + c) / group;
-      return out + ((r0 + i) * nh + (int64_t)g * group + (c0 + c - i * group)) * HD;
+      bool fin = true;
+      f32x4a4 r;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        r[k] = y[k] * inv;
+        fin = fin && fabsf(r[k]) < INFINITY;
+      }
+      *(f32x4a4 *)(out + ((r0 + i) * nh + (int64_t)g * group + (c0 + c - i * group)) * HD + d) = r;
+      if (!fin || (M == -INFINITY && len - n + i >= 0)) atomicOr(&bad_cols, 1u << c);
     };
     for (int e = tid; e < nv * (HD / 4); e += 256) {
       const int c = e / (HD / 4), d = e % (HD / 4) * 4;
       const float M = fmaxf(fmaxf(m_lds[0][c], m_lds[1][c]), fmaxf(m_lds[2][c], m_lds[3][c]));
       const float Mb = M == -INFINITY ? 0.0f : M;
-      f32x4 x = f32x4{0};
-      float L = 0.0f;
+      f32x4 y = f32x4{0};
+      float Ls = 0.0f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const float f = __builtin_amdgcn_exp2f(m_lds[w][c] - Mb);
-        L = fmaf(l_lds[w][c], f, L);
-        const f32x4 y = *(const f32x4 *)&o_lds[w][c][d];
+        Ls = fmaf(l_lds[w][c], f, Ls);
+        const f32x4 z = *(const f32x4 *)&L.o[w][c][d];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = fmaf(y[i], f, x[i]);
+        for (int i = 0; i < 4; ++i) y[i] = fmaf(z[i], f, y[i]);
       }
       if (whole) {
-        const float inv = M == -INFINITY ? 0.0f : 0x1p-14f / L;  // no position seen: zeros
-        float *op = out_at(c) + d;
-        bool fin = true;
-        f32x4a4 y;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          y[i] = x[i] * inv;
-          fin = fin && fabsf(y[i]) < INFINITY;
-        }
-        *(f32x4a4 *)op = y;
-        if (!fin || (M == -INFINITY && len - n + (c0 + c) / group >= 0)) atomicOr(&bad_cols, 1u << c);
+        finish(c, d, y, M, Ls);
       } else {
         float *op = part + (my_slot * COLS + c) * HD + d;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) st_agent(op + i, x[i]);
+        for (int i = 0; i < 4; ++i) st_agent(op + i, y[i]);
         if (d == 0) {
           st_agent(part_ml + (my_slot * COLS + c) * 2, M);
-          st_agent(part_ml + (my_slot * COLS + c) * 2 + 1, L);
+          st_agent(part_ml + (my_slot * COLS + c) * 2 + 1, Ls);
         }
       }
     }
     if (!whole) {
-      // hand over; the unit's last work-group to arrive joins its chunks, in their order
+      // hand over; the last work-group to arrive joins the segments, in their order
       vm_wait();
       __syncthreads();
-      if (tid == 0) {
-        arrived = add_release(counters + unit_slot, 1u);
-        if (arrived == (uint32_t)(n_act - 1)) acquire_agent();
+      if (tid == 0) arrived = add_release(counters + w_first, 1u);
+      __syncthreads();
+      if (arrived != (uint32_t)(n_seg - 1)) continue;
+      acquire_agent();
+      auto slot = [&](int i) { return 2 * (w_first + i) + (i == 0); };
+      // each column's maximum, its segments' factors (LDS) and its sum: wave w columns w, w + 4, ...
+      const int ns = (int)n_seg;
+      for (int c = wave; c < nv; c += 4) {
+        float M = -INFINITY, Ls = 0.0f;
+        for (int i = lane; i < ns; i += 64) M = fmaxf(M, part_ml[(slot(i) * COLS + c) * 2]);
+        M = group_max<64>(M);
+        const float Mb = M == -INFINITY ? 0.0f : M;
+        for (int i = lane; i < ns; i += 64) {
+          const float f = __builtin_amdgcn_exp2f(part_ml[(slot(i) * COLS + c) * 2] - Mb);
+          Ls = fmaf(part_ml[(slot(i) * COLS + c) * 2 + 1], f, Ls);
+          L.f[i * COLS + c] = f;
+        }
+        Ls = group_sum<64>(Ls);
+        if (lane == 0) {
+          m_lds[0][c] = M;
+          l_lds[0][c] = Ls;
+        }
       }
       __syncthreads();
-      if (arrived != (uint32_t)(n_act - 1)) continue;
-      acquire_agent();
-      for (int e = tid; e < nv * (HD / 4); e += 256) {
+      // four dims per thread, the segments shared out among the threads that are left
+      const int need = nv * (HD / 4), gs = need <= 128 ? 256 / need : 1;
+      for (int e0 = 0; e0 < need; e0 += 256) {
+        const int e = gs > 1 ? tid % need : e0 + tid, w = gs > 1 ? tid / need : 0;
         const int c = e / (HD / 4), d = e % (HD / 4) * 4;
-        float M = -INFINITY;
-        for (int i = 0; i < n_act; ++i) M = fmaxf(M, ld_agent(part_ml + ((unit_slot + (int64_t)i * a.n_kv) * COLS + c) * 2));
-        const float Mb = M == -INFINITY ? 0.0f : M;
-        f32x4 x = f32x4{0};
-        float L = 0.0f;
-        for (int i = 0; i < n_act; ++i) {
-          const int64_t at = (unit_slot + (int64_t)i * a.n_kv) * COLS + c;
-          const float f = __builtin_amdgcn_exp2f(ld_agent(part_ml + at * 2) - Mb);
-          L = fmaf(ld_agent(part_ml + at * 2 + 1), f, L);
+        f32x4 y = f32x4{0};
+        if (e < need && w < gs) {
+          int i = w;
+          for (; i + 7 * gs < ns; i += 8 * gs) {
+            f32x4 z[8];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) x[k] = fmaf(ld_agent(part + at * HD + d + k), f, x[k]);
-        }
-        const float inv = M == -INFINITY ? 0.0f : 0x1p-14f / L;
-        float *op = out_at(c) + d;
-        bool fin = true;
-        f32x4a4 y;
+            for (int k = 0; k < 8; ++k) z[k] = *(const f32x4 *)(part + (slot(i + k * gs) * COLS + c) * HD + d);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          y[k] = x[k] * inv;
-          fin = fin && fabsf(y[k]) < INFINITY;
+            for (int k = 0; k < 8; ++k) {
+              const float f = L.f[(i + k * gs) * COLS + c];
+#pragma unroll
+              for (int t = 0; t < 4; ++t) y[t] = fmaf(z[k][t], f, y[t]);
+            }
+          }
+          for (; i < ns; i += gs) {
+            const f32x4 z = *(const f32x4 *)(part + (slot(i) * COLS + c) * HD + d);
+            const float f = L.f[i * COLS + c];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) y[t] = fmaf(z[t], f, y[t]);
+          }
         }
-        *(f32x4a4 *)op = y;
-        if (!fin || (M == -INFINITY && len - n + (c0 + c) / group >= 0)) atomicOr(&bad_cols, 1u << c);
+        if (gs > 1) {
+          grp[tid] = y;
+          __syncthreads();
+          for (int k = 1; w == 0 && k < gs; ++k)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) y[t] += grp[tid + k * need][t];
+        }
+        if (e < need && w == 0) finish(c, d, y, m_lds[0][c], l_lds[0][c]);
       }
-      if (tid == 0) st_agent(counters + unit_slot, 0u);  // zero again for the next call
+      if (tid == 0) st_agent(counters + w_first, 0u);  // zero again for the next call
     }
     __syncthreads();
     // an infinity or NaN among what a tile's columns see together spreads in the
@@ -729,35 +796,31 @@ __global__ void __launch_bounds__(256, KMOE_OCC1)
 
 }  // namespace
 
-// Work-groups of a launch (resident at once on the whole chip) and the most items
-// they are given: one each where the units leave room.
-constexpr int kPagedTarget[2] = {512, 512};
+// Work-groups of a launch: as many as are resident at once on the whole chip.
+constexpr int kPagedGrid = 512;
 
-size_t paged_part_floats() {
-  size_t m = 0;
-  for (int c = 0; c < 2; ++c) m = std::max(m, (size_t)2 * kPagedTarget[c] * 16 * (c + 1) * (128 + 2));
-  return m;
-}
-int paged_counters() { return 2 * kPagedTarget[0]; }
+size_t paged_part_floats() { return (size_t)2 * kPagedGrid * 32 * (128 + 2); }
+int paged_counters() { return kPagedGrid; }
 
 hipError_t launch_paged_attention(hipStream_t st, const PagedArgs &a, const float *q, int n_head, int64_t window,
                                   int64_t n_sink, float *out, float *part, uint32_t *counters) {
   const int group = n_head / a.n_kv;
   const int w = window >= INT32_MAX ? 0 : (int)window, sink = (int)(n_sink < (1 << 30) ? n_sink : (1 << 30));
-  // 16 columns per item where sequences have about one row
+  // 16 columns per tile where sequences have about one row
   const bool one = a.s_rows * group <= (int64_t)24 * a.n_seq;
-  const int cols = one ? 16 : 32, target = kPagedTarget[one ? 0 : 1];
+  const int cols = one ? 16 : 32;
+  // no more work-groups than the longest sequences that the table allows would fill
   const int64_t units = (a.s_rows * group / cols + a.n_seq) * a.n_kv;
-  const int64_t chunks = ((int64_t)a.table_cols * a.page / kTile + 3) / 4;  // most of a unit
-  const unsigned grid = (unsigned)std::min<int64_t>(target, units * std::max<int64_t>(1, std::min<int64_t>(chunks, target)));
-  const size_t lds = (size_t)2 * (a.n_seq + 1) * 4;
-  float *ml = part + (size_t)2 * target * cols * a.hd;
+  const int64_t most = units * (((int64_t)a.table_cols * a.page / kTile + kUnitCost + 3) / kMinShare + 1);
+  const unsigned grid = (unsigned)std::min<int64_t>(kPagedGrid, (most + 7) / 8 * 8);
+  const size_t lds = (size_t)(a.n_seq + 1) * 8;
+  float *ml = part + (size_t)2 * kPagedGrid * cols * a.hd;
 #define KMOE_PAGED(T, H, C) \
-  KMOE_LAUNCH((k_paged_attn<T, H, C>), dim3(grid), dim3(256), lds, st, a, q, n_head, w, sink, target, part, ml, counters, out)
-#define KMOE_PAGED_C(T, H)     \
-  do {                         \
+  KMOE_LAUNCH((k_paged_attn<T, H, C>), dim3(grid), dim3(256), lds, st, a, q, n_head, w, sink, part, ml, counters, out)
+#define KMOE_PAGED_C(T, H)        \
+  do {                            \
     if (one) KMOE_PAGED(T, H, 1); \
-    else KMOE_PAGED(T, H, 2);  \
+    else KMOE_PAGED(T, H, 2);     \
   } while (0)
   if (a.type == kPgF16) {
     if (a.hd == 64) KMOE_PAGED_C(kPgF16, 64);
