@@ -277,11 +277,26 @@ def test_one_sequence(ctx, t, nh, nkv, hd, page, n):
     _close(_attend(c, q, nh), ref, tol)
 
 
+@pytest.mark.parametrize("t,hd", [(F16, 64), (Q8_0, 64), (F16, 128)])
+def test_one_head_over_a_long_context(ctx, t, hd):
+    """A single kv head split over every work-group of the launch."""
+    nh, n = 3, 300007
+    c = Cache(ctx, t, 1, hd, 256, [n], 5)
+    q = np.random.default_rng(n).standard_normal((1, nh, hd)).astype(np.float32)
+    ref, tol, _ = _reference(c, q, None, nh)
+    _close(_attend(c, q, nh), ref, tol)
+    rows = [9]
+    q = np.random.default_rng(n).standard_normal((9, nh, hd)).astype(np.float32)
+    ref, tol, _ = _reference(c, q, rows, nh)
+    _close(_attend(c, q, nh, rows), ref, tol)
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("nh,nkv,hd,page,lens,rows", [
     (4, 2, 128, 64, [100], [100]), (8, 2, 64, 32, [333], [150]), (2, 2, 128, 128, [77, 200, 5], [77, 1, 5]),
     (16, 1, 64, 64, [40, 3, 90], [9, 3, 0]), (6, 2, 64, 32, [700, 33, 64, 1], [2, 17, 64, 1]), (3, 1, 128, 256, [600], [31]),
-    (4, 4, 64, 32, [1, 1, 1], [1, 0, 1]), (16, 16, 128, 64, [65], [65]), (14, 2, 64, 64, [2100], [5])])
+    (4, 4, 64, 32, [1, 1, 1], [1, 0, 1]), (16, 16, 128, 64, [65], [65]), (14, 2, 64, 64, [2100], [5]),
+    (5, 1, 64, 32, [129, 700], [129, 300]), (16, 1, 128, 128, [1500], [257]), (1, 1, 128, 64, [513], [513])])
 def test_chunks_and_mixed_batches(ctx, t, nh, nkv, hd, page, lens, rows):
     c = Cache(ctx, t, nkv, hd, page, lens, sum(lens))
     q = np.random.default_rng(1).standard_normal((sum(rows), nh, hd)).astype(np.float32)
