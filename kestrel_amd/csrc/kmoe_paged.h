@@ -84,20 +84,6 @@ __device__ __forceinline__ void paged_rows(const PagedArgs &a, int b, int64_t &r
   n = hi > lo ? hi - lo : 0;
 }
 
-// The sequence of row r: the last b with row_start[b] <= r, or -1 past the last
-// sequence (and before the first).
-__device__ __forceinline__ int paged_seq_of(const PagedArgs &a, int64_t r) {
-  if (!a.row_start) return r < a.n_seq ? (int)r : -1;
-  if (r >= a.row_start[a.n_seq] || r < a.row_start[0]) return -1;
-  int lo = 0, hi = a.n_seq;  // row_start[lo] <= r < row_start[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.row_start[mid] <= r) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
 // Block of kv head g in the page of sequence b's position p, or null where the
 // table has none.
 __device__ __forceinline__ uint8_t *paged_block(const PagedArgs &a, int64_t block_bytes, int b, int64_t p, int g) {

@@ -175,8 +175,7 @@ class PagedKV:
         return 2 * e if self.type == F16 else e // 32 * 34
 
     def desc(self, pages, n_layer: int = 1) -> PagedDesc:
-        return PagedDesc(self.type, self.n_kv, self.head_dim, self.page,
-                         pages.numel() * pages.element_size() // (n_layer * self.page_bytes))
+        return PagedDesc(self.type, self.n_kv, self.head_dim, self.page, pages.nbytes // (n_layer * self.page_bytes))
 
 
 class KmoeError(RuntimeError):
@@ -223,6 +222,7 @@ class Context:
         self.torch = torch
         self.lib = load_library()
         self.device = device
+        self._dev = torch.device("cuda", device)
         self._descs = {}  # layer -> (n_expert, part lengths)
         h = _P()
         rc = self.lib.kmoe_create(device, C.byref(h))
@@ -273,7 +273,7 @@ class Context:
 
     # ------------------------------------------------------------ kernel seam
     def _empty(self, shape, dtype):
-        return self.torch.empty(shape, dtype=dtype, device=f"cuda:{self.device}")
+        return self.torch.empty(shape, dtype=dtype, device=self._dev)
 
     def matmul(self, t: int, w, rows: int, cols: int, x):
         """quant::matmul (quant.rs:229): x [S, cols] f32 -> [S, rows] f32."""
@@ -372,14 +372,17 @@ class Context:
         return out
 
     # ------------------------------------------------- paged key-value cache
-    def _need(self, name: str, t, dtype, rows: int, width: int, strided: bool = False):
-        """A [rows, width] device tensor of dtype, contiguous (strided: its rows may lie apart)."""
-        if t.dtype != dtype or t.device.type != "cuda" or t.device.index != self.device:
+    def _need(self, name: str, t, dtype, rows: int, width: int, strided: bool = False) -> int:
+        """Checks a [rows, width] device tensor of dtype, contiguous (strided: its rows may lie apart); the floats
+        from row to row."""
+        if t.dtype is not dtype or t.get_device() != self.device:
             raise ValueError(f"{name}: need {dtype} on cuda:{self.device}, got {t.dtype} on {t.device}")
+        if strided and t.dim() == 2 and t.shape == (rows, width):
+            r, c = t.stride()
+            if (c == 1 or width == 1) and (r >= width or rows <= 1):
+                return max(r, width)
         if t.numel() != rows * width:
             raise ValueError(f"{name}: need [{rows}, {width}], got {list(t.shape)}")
-        if strided and t.dim() == 2 and rows and t.shape[0] == rows and t.stride(1) == 1:
-            return max(t.stride(0), width)
         if not t.is_contiguous():
             raise ValueError(f"{name}: rows are not contiguous")
         return width
@@ -450,13 +453,13 @@ class Context:
 
     def pages_copy(self, kv: PagedKV, pages, src, dst, n_layer: int = 1):
         """Pages src[i] onto dst[i] (host sequences) in each of the n_layer equal parts of pages."""
-        s, d = (np.ascontiguousarray(a, dtype=np.int32).reshape(-1) for a in (src, dst))
+        s, d = np.array(src, np.int32, ndmin=1), np.array(dst, np.int32, ndmin=1)
         if s.size != d.size:
             raise ValueError(f"{s.size} source pages, {d.size} destinations")
         if not pages.is_contiguous():
             raise ValueError("pages: not contiguous")
         self.check(self.lib.kmoe_pages_copy(self.h, C.byref(kv.desc(pages, n_layer)), _ptr(pages), n_layer,
-                                            pages.numel() * pages.element_size() // max(1, n_layer), s.ctypes.data,
+                                            pages.nbytes // max(1, n_layer), s.ctypes.data,
                                             d.ctypes.data, s.size))
 
     def swiglu(self, g, u, out=None):
