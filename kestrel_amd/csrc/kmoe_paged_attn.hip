@@ -409,10 +409,10 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
       // XCD's whole L2, and with a work-group per slot of the chip it took 45 us
       // per launch (one row at 131000 positions 118 -> 96 us, 48 rows under a
       // window of 1024 68 -> 32).
-      vm_wait();
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       const int tj = here(tid);
-            if (tj == 0) arrived = __hip_atomic_fetch_add(counters + w_first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (tj == 0) arrived = __hip_atomic_fetch_add(counters + w_first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       __syncthreads();
       if (arrived != (uint32_t)(n_seg - 1)) continue;
       auto slot = [&](int i) { return (int64_t)2 * (w_first + i) + (i == 0); };
