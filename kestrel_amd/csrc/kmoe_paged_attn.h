@@ -122,26 +122,33 @@ __device__ __forceinline__ f32x4 ld4_agent(const float *p) {
   const f32x2 a = ld2_agent(p), b = ld2_agent(p + 2);
   return f32x4{a.x, a.y, b.x, b.y};
 }
-constexpr float kLo = 0x1p-12f;
 constexpr int kTile = 32;  // positions per step of a wave
 // The running maximum is moved only by scores that pass it by more than this (in
 // units of log2 e): the weights are then at most 2^kLag, and O is seldom scaled.
 constexpr float kLag = 4.0f;
-constexpr float kUp = 0x1p10f;  // weights times kUp stay below 2^14 in f16
+constexpr float kUp = 0x1p11f;  // weights times kUp stay below 2^15 in f16
 
-// A pair of f32 as two dwords of f16 pairs: hi, the nearest f16, and lo, the
-// nearest f16 of 2^12 times what hi leaves: x = hi + lo * 2^-12 to 2^-23 of x for
-// |x| in 2^-14..2^15 and to 2^-37 below that.
-__device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
+// A pair of f32 times a power of two as two dwords of f16 pairs: hi, the nearest
+// f16, and lo, the nearest f16 of `lo_up` (a power of two) times what hi leaves:
+// hi + lo / lo_up is off by 2^-23 of the product at most, and by 2^-25 / lo_up where
+// that is less than it (the matrix cores take f16 subnormals as they are).
+__device__ __forceinline__ void split2(float a, float b, float up, float lo_up, uint32_t &hi, uint32_t &lo) {
   // (f32 values from here on: a product before the call may otherwise be rounded
   // to f16 in one step for hi and in two for lo, and the two then disagree)
   asm("" : "+v"(a), "+v"(b));
-  hi = __builtin_bit_cast(uint32_t, (h2){(_Float16)a, (_Float16)b});
-  asm("" : "+v"(hi));  // one packed conversion; lo reads its halves
+  hi = __builtin_bit_cast(uint32_t, (h2){(_Float16)(a * up), (_Float16)(b * up)});
+  asm("" : "+v"(hi));  // lo reads its halves
   const h2 h = __builtin_bit_cast(h2, hi);
-  lo = __builtin_bit_cast(uint32_t, (h2){(_Float16)fmaf((float)h.x, -1.0f / kLo, a * (1.0f / kLo)),
-                                         (_Float16)fmaf((float)h.y, -1.0f / kLo, b * (1.0f / kLo))});
+  lo = __builtin_bit_cast(uint32_t, (h2){(_Float16)fmaf((float)h.x, -lo_up, a * (up * lo_up)),
+                                         (_Float16)fmaf((float)h.y, -lo_up, b * (up * lo_up))});
 }
+// lo_up of q and of the weights, per page type. F16: 2^12, a second sum for the
+// products with lo, joined tile by tile: errors beside 2^-23 of 2^-48 of the largest
+// weight (1) and 2^-52 of q's largest element. Q8_0: 1, one sum for both pieces:
+// 2^-36 and 2^-40, below what the quants leave (half a step in 127) unless a
+// position has less than 2^-28 of the largest weight (4096 rows, 32 heads of 128:
+// 590 -> 510 us; F16 would win a twentieth).
+constexpr float lo_up(int t) { return t == kPgF16 ? 0x1p12f : 1.0f; }
 
 // Largest of the four lanes l, l ^ 16, l ^ 32, l ^ 48 (a column's share of one
 // score tile), and their sum.
@@ -304,13 +311,24 @@ __device__ __forceinline__ int64_t uniform64(int64_t x) {
 // (h0 + c) % group of the sequence's rows.
 struct Seg {
   int b, g, n, len, pos0;  // pos0: the position of row 0
-  int64_t r0;
+  int r0;
   int nv, i0, h0;
   Span sp;
   int at, v_last;
   int w_first, n_seg;  // the stretches that the column tile lies in
-  bool first;          // it starts in this one
+  int first;           // it starts in this one
 };
+
+// Of a segment that every lane reads at one place.
+__device__ __forceinline__ Seg uniform(const Seg &x) {
+  constexpr int W = sizeof(Seg) / 4;
+  struct Words {
+    int w[W];
+  } r = __builtin_bit_cast(Words, x);
+#pragma unroll
+  for (int i = 0; i < W; ++i) r.w[i] = __builtin_amdgcn_readfirstlane(r.w[i]);
+  return __builtin_bit_cast(Seg, r);
+}
 
 template <class SH>
 struct Cursor {
@@ -348,11 +366,16 @@ struct Cursor {
     while (x < x1) {
       while (uniform64(start[b + 1]) <= x) ++b;
       const int64_t sb = uniform64(start[b]);
-      int64_t r0v, rnv;
-      paged_rows(a, b, r0v, rnv);
       s.b = b;
-      s.r0 = __builtin_amdgcn_readfirstlane((int)r0v);
-      s.n = __builtin_amdgcn_readfirstlane((int)rnv);
+      if (a.row_start) {
+        const const_i32 rs = (const_i32)(uintptr_t)a.row_start + b;
+        s.r0 = rs[0] < 0 ? 0 : rs[0];
+        const int hi = rs[1] < (int)a.s_rows ? rs[1] : (int)a.s_rows;
+        s.n = hi > (int)s.r0 ? hi - (int)s.r0 : 0;
+      } else {
+        s.r0 = b;
+        s.n = b < a.s_rows ? 1 : 0;
+      }
       s.len = __builtin_amdgcn_readfirstlane(lens[b]);
       s.pos0 = s.len - s.n;
       const int n_cols = s.n * group;

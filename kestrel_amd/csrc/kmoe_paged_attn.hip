@@ -89,10 +89,9 @@ constexpr int paged_occ(int hd, int c) { return hd == 64 ? (c == 1 ? 4 : 3) : (c
 //   O^T[dim, column] += V^T . P: A = V tiles as they lie in the page, B = the
 //     weights of the lane's own eight positions, times kUp, as two f16 pieces,
 //     straight from the score registers.
-// K and V (Q8_0: the quants) are exact in f16 and all sums are f32. Q8_0: a score
+// K (Q8_0: its quants) and V are exact in f16 and all sums are f32. Q8_0: a score
 // is summed 32 dims at a time, one K step, and scaled by the position's scale of
-// those; V's scales go into the weights before they are split, over a power of
-// two that no scale so far has passed, per 32 dims.
+// those; a value, eight bits times eleven, is the sum of two f16 exactly.
 // The running maximum is in units of log2 e.
 template <int T, int HD, int C>
 __global__ void __launch_bounds__(256, paged_occ(HD, C))
@@ -117,7 +116,19 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
   Cursor<Shares<COLS, 4, 8, 8>> cur(a, nh, window, sink, start, (int32_t *)(start + a.n_seq + 1), red);
   const int64_t cap = cur.cap;
 
-  for (Seg s_; cur.next(s_);) {
+  // wave 3 finds the next segment while this one's first loads are on their way
+  __shared__ Seg segs[2];
+  auto find = [&](int i) {
+    if (wave != 3) return;
+    Seg s;
+    if (!cur.next(s)) s.b = -1;
+    if (lane == 0) segs[i] = s;
+  };
+  find(0);
+  lds_barrier();
+  for (int turn = 0;; turn ^= 1) {
+    const Seg s_ = uniform(segs[turn]);
+    if (s_.b < 0) break;
     const int b = s_.b, g = s_.g, nv = s_.nv, pos0 = s_.pos0, v_last = s_.v_last, n_seg = s_.n_seg, w_first = s_.w_first;
     const int64_t r0 = s_.r0;
     const Span sp = s_.sp;
@@ -152,6 +163,8 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
       fr.load_v(p, a.page, pp, lane);
     }
     __builtin_amdgcn_sched_barrier(0);
+    find(turn ^ 1);
+    __builtin_amdgcn_sched_barrier(0);
     {
       float amax = 0.0f;
 #pragma unroll
@@ -167,7 +180,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           uint32_t u, w;
-          split2(ldexpf(y[t][e >> 1][2 * (e & 1)], sh), ldexpf(y[t][e >> 1][2 * (e & 1) + 1], sh), u, w);
+          split2(ldexpf(y[t][e >> 1][2 * (e & 1)], sh), ldexpf(y[t][e >> 1][2 * (e & 1) + 1], sh), 1.0f, lo_up(T), u, w);
           hi[e] = u;
           lo[e] = w;
         }
@@ -233,7 +246,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
 #pragma unroll
           for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) S[j][s][i] = fmaf(lo[j][s][i], kLo, hi[j][s][i]);
+            for (int i = 0; i < 4; ++i) S[j][s][i] = fmaf(lo[j][s][i], 1.0f / lo_up(T), hi[j][s][i]);
       } else {
 #pragma unroll
         for (int j = 0; j < C; ++j) S[j][0] = S[j][1] = f32x4{0};
@@ -245,11 +258,10 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
 #pragma unroll
             for (int j = 0; j < C; ++j) {
               const h8 ql = __builtin_bit_cast(h8, L.q[j][t][1][lq]), qh = __builtin_bit_cast(h8, L.q[j][t][0][lq]);
-              const f32x4 lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql, f32x4{0}, 0, 0, 0);
-              const f32x4 hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh, f32x4{0}, 0, 0, 0);
+              f32x4 x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql, f32x4{0}, 0, 0, 0);
+              x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh, x, 0, 0, 0);
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                S[j][s][i] = fmaf(fmaf(lo[i], kLo, hi[i]), half_of(fr.ks[s][t >> 1], 4 * (t & 1) + i), S[j][s][i]);
+              for (int i = 0; i < 4; ++i) S[j][s][i] = fmaf(x[i], half_of(fr.ks[s][t >> 1], 4 * (t & 1) + i), S[j][s][i]);
             }
           }
           __builtin_amdgcn_sched_barrier(0);  // (few registers rather than many products at once)
@@ -301,7 +313,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           uint32_t x, z;
-          split2(e8[2 * i] * kUp, e8[2 * i + 1] * kUp, x, z);
+          split2(e8[2 * i], e8[2 * i + 1], kUp, lo_up(T), x, z);
           ph[j][i] = x;
           pl[j][i] = z;
         }
@@ -315,7 +327,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
           for (int j = 0; j < C; ++j) {
             const f32x4 t = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, __builtin_bit_cast(h8, pl[j]), f32x4{0}, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) O[j][u][i] = fmaf(t[i], kLo, O[j][u][i]);
+            for (int i = 0; i < 4; ++i) O[j][u][i] = fmaf(t[i], 1.0f / lo_up(T), O[j][u][i]);
             O[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, __builtin_bit_cast(h8, ph[j]), O[j][u], 0, 0, 0);
           }
         }
@@ -324,15 +336,16 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
         for (int u = 0; u < NU; ++u) {
           const h8 x = i8_h8(here(fr.v[u >> 1][2 * (u & 1)]), here(fr.v[u >> 1][2 * (u & 1) + 1]));
           const h8 d = __builtin_bit_cast(h8, fr.vs[u >> 1]);
-          const h8 vh = x * d, vl = __builtin_elementwise_fma(x, d, -vh) * (_Float16)(1.0f / kLo);
+          const h8 vh = x * d, vl = __builtin_elementwise_fma(x, d, -vh);  // exact: eight bits by eleven
 #pragma unroll
-          for (int j = 0; j < C; ++j) {
-            f32x4 t = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, __builtin_bit_cast(h8, pl[j]), f32x4{0}, 0, 0, 0);
-            t = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, __builtin_bit_cast(h8, ph[j]), t, 0, 0, 0);
+          for (int j = 0; j < C; ++j)
+            O[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, __builtin_bit_cast(h8, ph[j]), O[j][u], 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) O[j][u][i] = fmaf(t[i], kLo, O[j][u][i]);
+          for (int j = 0; j < C; ++j)
+            O[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, __builtin_bit_cast(h8, pl[j]), O[j][u], 0, 0, 0);
+#pragma unroll
+          for (int j = 0; j < C; ++j)
             O[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, __builtin_bit_cast(h8, ph[j]), O[j][u], 0, 0, 0);
-          }
           if (u & 1) __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -432,50 +445,64 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
         m_lds[0][jc] = Mc;
         l_lds[0][jc] = Ls;
       }
-      // four dims per thread, the segments shared out among the threads that are
-      // left; their factors lie in LDS, kF segments at a time
+      // four dims of R elements per thread, the segments shared out among the threads
+      // that are left; eight loads on their way at a time. The segments' factors lie
+      // in LDS, kF segments at a time.
       constexpr int kF = 4 * OROW;
-      const int need = nv * (HD / 4), gs = need <= 128 ? 256 / need : 1;
-      for (int e0 = 0; e0 < need; e0 += 256) {
-        const int e = gs > 1 ? tj % need : e0 + tj, w = gs > 1 ? tj / need : 0;
-        const int c = e / (HD / 4), d = e % (HD / 4) * 4;
-        f32x4 y = f32x4{0};
+      const int need = nv * (HD / 4);
+      auto join = [&](auto r_, int gs) {
+        constexpr int R = decltype(r_)::value, U = 8 / R;
+        const int e = gs > 1 ? tj % need : tj, w = gs > 1 ? tj / need : 0;
+        const float *op[R];
+        int cs[R];
+        f32x4 y[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int er = e + 256 * r < need ? e + 256 * r : need - 1;
+          cs[r] = er / (HD / 4);
+          op[r] = part + (int64_t)er * 4;
+          y[r] = f32x4{0};
+        }
         for (int i0 = 0; i0 < ns; i0 += kF) {
           const int i1 = i0 + kF < ns ? i0 + kF : ns;
           __syncthreads();
           for (int i = i0 + jp; i < i1; i += JP)
             L.f[(i - i0) * COLS + jc] = __builtin_amdgcn_exp2f(ld_agent(part_ml + (slot(i) * COLS + jc) * 2) - Mb);
           __syncthreads();
-          if (e < need && w < gs) {
-            int i = i0 + w;
-            for (; i + 7 * gs < i1; i += 8 * gs) {
-              f32x4 z[8];
+          if (w >= gs) continue;
+          auto add = [&](auto u_, int i) {
+            constexpr int N = decltype(u_)::value;
+            f32x4 z[N][R];
 #pragma unroll
-              for (int k = 0; k < 8; ++k) z[k] = ld4_agent(part + (slot(i + k * gs) * COLS + c) * HD + d);
+            for (int k = 0; k < N; ++k)
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const float f = L.f[(i - i0 + k * gs) * COLS + c];
+              for (int r = 0; r < R; ++r) z[k][r] = ld4_agent(op[r] + slot(i + k * gs) * (COLS * HD));
 #pragma unroll
-                for (int t = 0; t < 4; ++t) y[t] = fmaf(z[k][t], f, y[t]);
+            for (int k = 0; k < N; ++k)
+#pragma unroll
+              for (int r = 0; r < R; ++r) {
+                const float f = L.f[(i - i0 + k * gs) * COLS + cs[r]];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) y[r][t] = fmaf(z[k][r][t], f, y[r][t]);
               }
-            }
-            for (; i < i1; i += gs) {
-              const f32x4 z = ld4_agent(part + (slot(i) * COLS + c) * HD + d);
-              const float f = L.f[(i - i0) * COLS + c];
-#pragma unroll
-              for (int t = 0; t < 4; ++t) y[t] = fmaf(z[t], f, y[t]);
-            }
-          }
+          };
+          int i = i0 + w;
+          for (; i + (U - 1) * gs < i1; i += U * gs) add(std::integral_constant<int, U>(), i);
+          for (; i < i1; i += gs) add(std::integral_constant<int, 1>(), i);
         }
         if (gs > 1) {
-          grp[tj] = y;
+          grp[tj] = y[0];
           __syncthreads();
           for (int k = 1; w == 0 && k < gs; ++k)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) y[t] += grp[tj + k * need][t];
+            for (int t = 0; t < 4; ++t) y[0][t] += grp[tj + k * need][t];
         }
-        if (e < need && w == 0) finish(c, d, y, m_lds[0][c], l_lds[0][c]);
-      }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (e + 256 * r < need && w == 0) finish(cs[r], (e + 256 * r) % (HD / 4) * 4, y[r], m_lds[0][cs[r]], l_lds[0][cs[r]]);
+      };
+      if (need <= 128) join(std::integral_constant<int, 1>(), 256 / need);
+      else join(std::integral_constant<int, COLS * HD / 1024>(), 1);
       if (tj == 0) st_agent(counters + w_first, 0u);  // zero again for the next call
     }
     lds_barrier();

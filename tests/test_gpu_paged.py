@@ -461,6 +461,37 @@ def test_small_weights_and_elements_keep_their_bits(ctx, kind, hd, rows):
             assert np.linalg.norm(got[s, h] - ref[s, h]) <= (3e-6 if kind == "sink" else 1.5e-6) * np.linalg.norm(ref[s, h])
 
 
+# Q8_0: a weight is off by up to 2^-36 of the largest besides its own 2^-23, an element of q by 2^-40 of the row's
+# largest
+@pytest.mark.parametrize("kind", ["sink", "outlier"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows", [None, [37]])
+def test_q8_small_weights_and_elements(ctx, kind, hd, rows):
+    rng = np.random.default_rng(hd + 1)
+    nh, nkv, n = 4, 2, 160
+    r = 1 if rows is None else rows[0]
+    c = Cache(ctx, Q8_0, nkv, hd, 32, [n], 4)
+    q = rng.standard_normal((r, nh, hd)).astype(np.float32)
+    k, v = (rng.standard_normal((n, nkv, hd)).astype(np.float32) for _ in range(2))
+    if kind == "sink":
+        q[:, :, 0] = 8.0
+        k[:, :, 0] = 0.0
+        k[0] = 0.0
+        k[0, :, 0] = 10 * np.sqrt(hd) / 8.0
+        v[0] = 0.0
+    else:
+        q[:, :, 3] = 2.0 ** 16
+        k[:, :, 3] = 0.0
+    ctx.paged_kv_store(c.kv, c.pages, c.batch([n]), _dev(k.reshape(n, -1)), _dev(v.reshape(n, -1)))
+    c.hk, c.hv = [_held(Q8_0, k)], [_held(Q8_0, v)]  # (the rows that paged_kv_read gives are rounded to f16)
+    ref, tol, S = _reference(c, q, rows, nh)
+    got = _attend(c, q, nh, rows).reshape(S, nh, hd)
+    # sink: n weights, the largest 1, values up to 5. outlier: a score is off by that much of hd elements with |k| up
+    # to 5, and so, in units of the weights (1 together), is each weight, with values up to 5
+    more = n * 2.0 ** -36 * 5 if kind == "sink" else 2.0 ** 16 * 2.0 ** -40 * hd * 5 / np.sqrt(hd) * 5
+    assert (np.abs(got - ref) <= tol + more).all()
+
+
 @pytest.mark.parametrize("t", TYPES)
 def test_scores_of_any_size(ctx, t):
     """Rows of very different size, from almost even weights to a single position's."""
