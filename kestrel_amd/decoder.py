@@ -21,13 +21,14 @@ Layers with routed experts go through kmoe_moe_ffn and its HBM expert tier;
 the rest through the decoder ops of include/kmoe.h. A single-token decode
 step reads its position from a device counter, so it is captured once as a
 HIP graph and replayed for every later token (greedy decoding keeps the
-sampled token on the device too).
+sampled token on the device too). PagedDecoder runs many sequences together
+over a paged key-value cache.
 """
 from __future__ import annotations
 
 import numpy as np
 
-from .kmoe import BLOCK, F32, Context, bytes_for
+from .kmoe import BLOCK, F16, F32, Q8_0, Context, KmoeError, PagedKV, Pages, bytes_for
 
 
 def _nbytes(t: int, dims) -> int:
@@ -112,15 +113,19 @@ class Decoder:
                 else:
                     L["gate"], L["up"] = raw(p + "ffn_gate.weight"), raw(p + "ffn_up.weight")
                 L["down"] = raw(p + "ffn_down.weight")
-            L["kc"] = torch.zeros((self.n_ctx, kvw), dtype=torch.int16, device=dev)
-            L["vc"] = torch.zeros((self.n_ctx, kvw), dtype=torch.int16, device=dev)
             self.layers.append(L)
+        self._make_cache()
         self.cached = 0
         self.pos_dev = torch.zeros(1, dtype=torch.int32, device=dev)
         self.token_dev = torch.zeros(1, dtype=torch.int32, device=dev)
         self.graph = None
         self._graph_gen = None  # the context's workspace generation the graph was captured at
         self._graph_bufs = None
+
+    def _make_cache(self):
+        for L in self.layers:
+            for n in ("kc", "vc"):
+                L[n] = self.torch.zeros((self.n_ctx, self.nkv * self.hd), dtype=self.torch.int16, device=self.dev)
 
     def _moe_layer(self, l: int, lid: int, tensors: dict) -> int:
         ctx, hp, p = self.ctx, self.hp, f"blk.{l}."
@@ -198,6 +203,11 @@ class Decoder:
         ty, dims, t = L["wo"]
         o = ctx.attention_matmul(qr, L["kc"], L["vc"], nh, nkv, hd, pos0, self.n_ctx, ty, t,
                                  int(np.prod(dims[1:])), pos_dev)
+        return self._ffn(L, x, o, S)
+
+    def _ffn(self, L, x, o, S):
+        """The FFN of the attention's output o added to x."""
+        ctx = self.ctx
         if "moe" in L:
             # x += o, the norm of x, then the routed experts (one token: the
             # router kernel takes the norm)
@@ -305,4 +315,250 @@ class Decoder:
         self.graph = None
 
 
-__all__ = ["Decoder", "BLOCK"]
+class PagedDecoder(Decoder):
+    """A Decoder for many sequences at once over one paged key-value cache of
+    n_pages pages, F16 or Q8_0: every call takes new tokens of any of them,
+    prompts and single tokens together. Sequences are numbered by the caller and
+    begin with their first tokens; forks share pages until one of them writes.
+    With a window a row sees the last `window` positions and the first n_sink,
+    and pages that no later row sees are free again after a call. head_dim 64 or
+    128; a sequence has at most hp["n_ctx"] positions, a call at most 4096
+    sequences, and hp["n_batch"] rows at a time go through the layers."""
+
+    def __init__(self, ctx: Context, hp: dict, tensors: dict, n_pages: int, page: int = 64, kv_type: int = F16,
+                 window: int = 0, n_sink: int = 0, layer_base: int = 1000):
+        if hp["head_dim"] not in (64, 128):
+            raise ValueError(f"head_dim {hp['head_dim']}: the paged cache has heads of 64 or 128")
+        if kv_type not in (F16, Q8_0):
+            raise ValueError("kv_type: F16 or Q8_0")
+        if window < 0 or n_sink < 0 or (n_sink and not window):
+            raise ValueError("window and n_sink: not negative, and n_sink with a window only")
+        if page not in (32, 64, 128, 256):
+            raise ValueError(f"page {page}: 32, 64, 128 or 256 positions")
+        self.account = Pages(n_pages, page)
+        self.kv = PagedKV(kv_type, hp["n_head_kv"], hp["head_dim"], page)
+        self.n_pages, self.window, self.n_sink = n_pages, window, n_sink
+        super().__init__(ctx, hp, tensors, layer_base)
+        self.cols = -(-self.n_ctx // page)
+        self._graph_n = 0
+
+    def _make_cache(self):
+        self.pages = self.torch.zeros((self.n_layer, self.n_pages, self.kv.page_bytes), dtype=self.torch.uint8,
+                                      device=self.dev)
+
+    # ---------------------------------------------------------- sequences
+    def length(self, seq: int) -> int:
+        """Positions of seq in the cache; 0 where there is no such sequence."""
+        try:
+            return self.account.length(seq)
+        except KmoeError:
+            return 0
+
+    def fork(self, src: int, dst: int, n: int | None = None):
+        """A new sequence dst of the first n positions of src (all of them by default)."""
+        self.account.fork(src, dst, self.account.length(src) if n is None else n)
+
+    def truncate(self, seq: int, n: int):
+        self.account.truncate(seq, n)
+
+    def drop(self, seq: int):
+        self.account.drop(seq)
+
+    def compact(self, most: int | None = None) -> int:
+        """Moves used pages to the front of the cache, at most `most`; how many were moved."""
+        src, dst = self.account.compact(most)
+        self._copy(list(zip(src.tolist(), dst.tolist())))
+        return len(src)
+
+    def _copy(self, pairs):
+        if pairs:
+            self.ctx.pages_copy(self.kv, self.pages, [s for s, _ in pairs], [d for _, d in pairs], self.n_layer)
+
+    def _reserve(self, want: dict) -> dict:
+        """Positions for new tokens, all of them or none; returns the lengths before (None: a new sequence)."""
+        if not want or len(want) > 4096:
+            raise ValueError(f"{len(want)} sequences: a call takes 1 to 4096")
+        had = {}
+        for s, n in want.items():
+            try:
+                had[s] = self.account.length(s)
+            except KmoeError:
+                had[s] = None
+            if (had[s] or 0) + n > self.n_ctx:
+                raise ValueError(f"context full: sequence {s} needs {(had[s] or 0) + n}, n_ctx {self.n_ctx}")
+        copies, done = [], {}
+        try:
+            for s, n in want.items():
+                c = self.account.append(s, n)
+                done[s] = had[s]
+                if c:
+                    copies.append(c)
+        except KmoeError:
+            self._copy(copies)  # (a page of one's own stays, and has to hold what the shared one does)
+            self._back(done)
+            raise
+        self._copy(copies)
+        return had
+
+    def _back(self, had: dict):
+        for s, n in had.items():
+            if n is None:
+                self.account.drop(s)
+            else:
+                self.account.truncate(s, n)
+
+    def _trim(self, seqs):
+        if self.window:
+            for s in seqs:
+                self.account.trim(s, self.window, self.n_sink)
+
+    # -------------------------------------------------------------- steps
+    def _paged_layer(self, L, pages, batch, x, f_prev):
+        """_layer for the rows of a batch; `pages`: the layer's."""
+        ctx, nh, nkv, hd, S = self.ctx, self.nh, self.nkv, self.hd, batch.s_rows
+        kvw, nq = nkv * hd, nh * hd
+        if "wqkv" in L:
+            ty, dims, t = L["wqkv"]
+            qkv = ctx.norm_matmul(x, L["attn_norm"], self.eps, ty, t, dims[1], dims[0], y=f_prev)
+            q, k, v = qkv[:, :nq], qkv[:, nq:nq + kvw], qkv[:, nq + kvw:]
+            if any(n in L for n in ("bq", "bk", "bv", "q_norm", "k_norm")):
+                q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+        else:
+            h = ctx.rmsnorm(x, L["attn_norm"], self.eps, y=f_prev)
+            q, k, v = self._mm(L["wq"], h), self._mm(L["wk"], h), self._mm(L["wv"], h)
+        for n, y in (("q", q), ("k", k), ("v", v)):
+            if "b" + n in L:
+                ctx.add_rows(y, L["b" + n])
+        if "q_norm" in L:
+            ctx.rmsnorm(q, L["q_norm"], self.eps, out=q)
+        if "k_norm" in L:
+            ctx.rmsnorm(k, L["k_norm"], self.eps, out=k)
+        qr = ctx.paged_rope_kv_store(self.kv, pages, batch, q, k, v, nh, self.rd, self.inv_freq, self.neox)
+        o = ctx.paged_attention(self.kv, pages, batch, qr, nh, self.window, self.n_sink)
+        return self._ffn(L, x, self._mm(L["wo"], o), S)
+
+    def _rows(self, x, batch):
+        """All layers over the batch's rows: (x, f), whose sum is the residual stream."""
+        f = None
+        for L, pages in zip(self.layers, self.pages):
+            f = self._paged_layer(L, pages, batch, x, f)
+        return x, f
+
+    def _logits(self, x, f):
+        ty, dims, t = self.head
+        return self.ctx.norm_matmul(x, self.out_norm, self.eps, ty, t, dims[1], dims[0], y=f)
+
+    def _batch(self, seqs, ends, counts):
+        """The batch of counts[i] rows of seqs[i] that end at its position ends[i]."""
+        cols = -(-max(self.account.length(s) for s in seqs) // self.kv.page)
+        table, _ = self.account.table(seqs, cols)
+        starts = np.concatenate([[0], np.cumsum(counts)])
+        n = len(seqs)
+        d = self.torch.from_numpy(np.concatenate([ends, starts, table.reshape(-1)]).astype(np.int32)).to(self.dev)
+        rs = None if max(counts) == 1 else d[n:2 * n + 1]
+        return self.ctx.paged_batch(d[2 * n + 1:].view(n, cols), d[:n], rs, int(starts[-1]))
+
+    def forward(self, rows: dict):
+        """Feeds rows {sequence: its next tokens}; returns the logits of each one's last token [len(rows), n_vocab],
+        in the order of rows. A call that fails leaves the sequences as they were."""
+        rows = {int(s): [int(t) for t in ts] for s, ts in rows.items()}
+        for s, ts in rows.items():
+            if not ts or min(ts) < 0 or max(ts) >= self.n_vocab:
+                raise ValueError(f"sequence {s}: need at least one token, each below {self.n_vocab}")
+        had = self._reserve({s: len(ts) for s, ts in rows.items()})
+        try:
+            pieces = [(s, i, min(i + self.n_batch, len(ts))) for s, ts in rows.items()
+                      for i in range(0, len(ts), self.n_batch)]
+            logits = []
+            while pieces:
+                part, room = [], self.n_batch
+                while pieces and room:
+                    s, i, j = pieces.pop(0)
+                    m = min(room, j - i)
+                    if i + m < j:
+                        pieces.insert(0, (s, i + m, j))
+                    part.append((s, i, i + m))
+                    room -= m
+                    if len(part) > 1 and part[-2][0] == s:  # (two pieces of one sequence are one)
+                        part[-2:] = [(s, part[-2][1], i + m)]
+                ty, dims, t = self.embed
+                x = self.ctx.get_rows(ty, t, dims[1], dims[0], [tk for s, i, j in part for tk in rows[s][i:j]])
+                counts = [j - i for _, i, j in part]
+                x, f = self._rows(x, self._batch([p[0] for p in part], [(had[s] or 0) + j for s, _, j in part], counts))
+                last = [e - 1 for e, (s, _, j) in zip(np.cumsum(counts).tolist(), part) if j == len(rows[s])]
+                if last:
+                    if len(last) < len(x):
+                        x, f = (self.ctx.get_rows(F32, y, len(y), self.d, last) for y in (x, f))
+                    logits.append(self._logits(x, f))
+        except BaseException:
+            self._back(had)
+            raise
+        self._trim(rows)
+        return logits[0] if len(logits) == 1 else self.torch.cat(logits)
+
+    # ------------------------------------------------------ greedy decode
+    def _decode_rows(self, b):
+        ty, dims, t = self.embed
+        x = self.ctx.get_rows(ty, t, dims[1], dims[0], b["tok"], out=b["x"])
+        b["logits"] = self._logits(*self._rows(x, b["batch"]))
+        for i in range(len(b["logits"])):
+            self.ctx.argmax(b["logits"][i], out=b["tok"][i:i + 1], pos_dev=b["len"][i:i + 1], advance=1)
+
+    def decode_greedy(self, first: dict, n: int, use_graph: bool = True):
+        """Greedy decoding of several sequences together: feeds first {sequence: token}, then each one's argmax,
+        n steps; returns the sampled ids [n, len(first)]. With use_graph a step is captured once per number of
+        sequences and replayed: lengths, tokens and page tables are read on the device."""
+        torch, seqs = self.torch, [int(s) for s in first]
+        if n < 1:
+            raise ValueError("n: at least one step")
+        if any(not 0 <= int(t) < self.n_vocab for t in first.values()):
+            raise ValueError(f"a token is not below {self.n_vocab}")
+        had = self._reserve({s: n for s in seqs})
+        try:
+            b = self._graph_bufs
+            if b is None or self._graph_n != len(seqs):
+                i32 = dict(dtype=torch.int32, device=self.dev)
+                b = {"x": torch.empty((len(seqs), self.d), dtype=torch.float32, device=self.dev),
+                     "tok": torch.empty(len(seqs), **i32), "len": torch.empty(len(seqs), **i32),
+                     "table": torch.empty((len(seqs), self.cols), **i32)}
+                b["batch"] = self.ctx.paged_batch(b["table"], b["len"])
+                self._graph_bufs, self._graph_n, self.graph = b, len(seqs), None
+            at = torch.tensor([(had[s] or 0) + 1 for s in seqs], dtype=torch.int32)
+            tok = torch.tensor([int(t) for t in first.values()], dtype=torch.int32)
+            b["table"].copy_(torch.from_numpy(self.account.table(seqs, self.cols)[0]))
+            b["len"].copy_(at)
+            b["tok"].copy_(tok)
+            out = torch.empty((n, len(seqs)), dtype=torch.int32, device=self.dev)
+            if use_graph and (self.graph is None or self.ctx.workspace_generation() != self._graph_gen):
+                self._decode_rows(b)  # grows every workspace first
+                b["len"].copy_(at)
+                b["tok"].copy_(tok)
+                torch.cuda.synchronize()
+                g = torch.cuda.CUDAGraph()
+                try:
+                    with torch.cuda.graph(g):
+                        self.ctx.set_stream(torch.cuda.current_stream())  # the capturing stream
+                        self._decode_rows(b)
+                finally:
+                    self.ctx.set_stream(torch.cuda.current_stream())
+                self.graph, self._graph_gen = g, self.ctx.workspace_generation()
+                torch.cuda.synchronize()
+            for i in range(n):
+                if use_graph:
+                    self.graph.replay()
+                else:
+                    self._decode_rows(b)
+                out[i].copy_(b["tok"])
+        except BaseException:
+            self._back(had)
+            raise
+        self._trim(seqs)
+        return out
+
+    def close(self):
+        super().close()
+        self.pages = None
+        self.account.close()
+
+
+__all__ = ["Decoder", "PagedDecoder", "BLOCK"]
