@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
   const int group = nh / a.n_kv, magic = 65536 / group + 1;  // x / group = x * magic >> 16 for x < 4096
   const int64_t bb = paged_block_bytes(T, a.page, HD);
   const int pshift = __builtin_ctz(a.page);
-  Cursor<Shares<COLS, 4, 8, 8>> cur(a, nh, window, sink, start, (int32_t *)(start + a.n_seq + 1), red);
+  Cursor<Shares<COLS, 4, 8, 8, 24>> cur(a, nh, window, sink, start, (int32_t *)(start + a.n_seq + 1), red);
   const int64_t cap = cur.cap;
 
   // wave 3 finds the next segment while this one's first loads are on their way
