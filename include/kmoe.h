@@ -546,7 +546,19 @@ int kmoe_paged_kv_read(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *p
  * 0: all, n_sink unused). Pages that no row sees are not read. A row that sees
  * nothing gives zeros. Sums and softmax statistics are f32; a row's last bits
  * depend on the batch it is in (how the positions are shared out), a call's on
- * nothing else. n_head / n_kv <= 16 heads per kv head. */
+ * nothing else. n_head / n_kv <= 16 heads per kv head. The matrix cores take q,
+ * the weights and Q8_0 values as two f16 pieces each: F16 pages as f32 arithmetic,
+ * Q8_0 pages with weights off by up to 2^-36 of a row's largest and q's elements by
+ * 2^-40 of its largest. Rows whose result is not finite, or whose scores are all
+ * -inf, are formed again in plain f32, so that an infinity or NaN at a position
+ * reaches the rows that see it only (slower; so are Q8_0 rows that see a value
+ * past f16's range).
+ * Work-groups that share a row join their sums in a workspace of the context (17
+ * MB, counted against the VRAM budget; KMOE_E_BUDGET where the first call finds no
+ * room). It is allocated once, also inside a capture, and never moves, so graphs
+ * stay valid; calls on several streams of one context are ordered by the library,
+ * but replays of graphs that hold such calls of one context must not overlap with
+ * each other or with a call. */
 int kmoe_paged_attention(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *pages_dev,
                          const kmoe_paged_batch *batch, const float *q_dev, int32_t n_head, int64_t window,
                          int64_t n_sink, float *out_dev);

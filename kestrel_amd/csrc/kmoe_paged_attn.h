@@ -1,6 +1,6 @@
-// kmoe_paged_attn.h — device code shared by the paged attention's kernels: the
-// plain form of one row, exact splits for the f16 matrix cores, and how a call's
-// work is shared out (internal).
+// kmoe_paged_attn.h — device code of the paged attention's kernel: the plain form
+// of one row, splits for the f16 matrix cores, and how a call's work is shared out
+// (internal).
 #pragma once
 
 #include "kmoe_device.h"
@@ -122,6 +122,7 @@ __device__ __forceinline__ f32x4 ld4_agent(const float *p) {
   const f32x2 a = ld2_agent(p), b = ld2_agent(p + 2);
   return f32x4{a.x, a.y, b.x, b.y};
 }
+
 constexpr int kTile = 32;  // positions per step of a wave
 // The running maximum is moved only by scores that pass it by more than this (in
 // units of log2 e): the weights are then at most 2^kLag, and O is seldom scaled.
@@ -277,7 +278,7 @@ __device__ void make_plan(const PagedArgs &a, int group, int64_t cap, int window
   auto space = [&](int b) -> int64_t {
     int64_t r0, n;
     paged_rows(a, b, r0, n);
-    const int32_t len = a.seq_len[b];
+    const int32_t len = a.seq_len[b] > 0 ? a.seq_len[b] : 0;  // (a length below the rows leaves them nothing)
     lens[b] = len;
     const SeqPlan s = seq_plan<SH>(n, len, group, cap, window, sink);
     return (int64_t)s.pairs() * a.n_kv * s.per;

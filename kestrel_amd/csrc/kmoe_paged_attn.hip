@@ -1,5 +1,16 @@
-// kmoe_paged_attn.hip — attention over the paged key-value cache, few rows per
-// sequence: decode steps.
+// kmoe_paged_attn.hip — attention over the paged key-value cache: decode steps,
+// prompt chunks and both in one launch.
+//
+// What bounds it, with times at the sizes of the comments below (F16 pages of 64
+// positions, heads of 128 unless said): one row per sequence reads every K and V
+// once for all heads of a group, 64 rows at 100 .. 8192 positions 88 us = 5.6 TB/s
+// of pages, one row at 131000 positions (8 kv heads) 95 us; with Q8_0 pages (half
+// the bytes) the vector units, which make f16 of the quants: 64 us for 286 MB.
+// Prompts are bound by the vector and matrix units together, which overlap little
+// with two waves a SIMD (4096 rows, 32 heads over 8: 395 us, 700 Tflop/s of f16
+// products: matrix units busy 32 % of the time, vector units 44 %; K and V all from
+// one page: a tenth less time), short calls by latencies: 37 positions 9.6 us, of
+// which 4 are the launch, 3 the plan and 1 the first loads.
 #include <algorithm>
 #include <type_traits>
 
@@ -10,7 +21,7 @@ namespace kmoe {
 
 namespace {
 
-// 16 bytes per lane; the lines are used whole by one load and by nobody else.
+// 16 bytes per lane, each line whole by one load.
 __device__ __forceinline__ u32x4 load16(const uint8_t *p) { return __builtin_nontemporal_load((const u32x4 *)p); }
 
 // A wave's share of 32 positions of K and of V, as loaded.
@@ -77,6 +88,9 @@ struct Frags<kPgQ8, HD> {
 // Work-groups of a CU that the registers let reside.
 constexpr int paged_occ(int hd, int c) { return hd == 64 ? (c == 1 ? 4 : 3) : (c == 1 ? 3 : 2); }
 
+template <int COLS>
+using Work = Shares<COLS, 4, 8, 8, 24>;
+
 // Work-group: four waves, one segment of a column tile at a time; wave w takes
 // its tiles w, w + 4, ... (32 positions each) with its own running softmax, and
 // the waves are merged through LDS.
@@ -113,10 +127,11 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
   const int group = nh / a.n_kv, magic = 65536 / group + 1;  // x / group = x * magic >> 16 for x < 4096
   const int64_t bb = paged_block_bytes(T, a.page, HD);
   const int pshift = __builtin_ctz(a.page);
-  Cursor<Shares<COLS, 4, 8, 8, 24>> cur(a, nh, window, sink, start, (int32_t *)(start + a.n_seq + 1), red);
+  Cursor<Work<COLS>> cur(a, nh, window, sink, start, (int32_t *)(start + a.n_seq + 1), red);
   const int64_t cap = cur.cap;
 
-  // wave 3 finds the next segment while this one's first loads are on their way
+  // wave 3 finds the next segment while this one's first loads are on their way (all
+  // waves at once, each segment on its turn: 200 rows, Q8_0, 64 -> 58 us)
   __shared__ Seg segs[2];
   auto find = [&](int i) {
     if (wave != 3) return;
@@ -438,9 +453,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
         float *op = part + (my_slot * COLS + c) * HD + d;
         st2_agent(op, f32x2{y[0], y[1]});
         st2_agent(op + 2, f32x2{y[2], y[3]});
-        if (d == 0) {
-          st2_agent(part_ml + (my_slot * COLS + c) * 2, f32x2{M, Ls});
-        }
+        if (d == 0) st2_agent(part_ml + (my_slot * COLS + c) * 2, f32x2{M, Ls});
       }
     }
     if (!whole) {
@@ -554,7 +567,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
 
 // Work-groups of a launch: as many as are resident at once on 256 CUs. (Twice as
 // many, for an evener end: one row at 131000 positions 96 -> 106 us, 64 rows at
-// 2000 95 -> 102, a prompt of 1777 rows 73 -> 104: more units are split.)
+// 2000 95 -> 102: more units are split.)
 constexpr int paged_grid(int hd, int c) { return 256 * paged_occ(hd, c); }
 
 size_t paged_part_floats() {
@@ -570,13 +583,13 @@ hipError_t launch_paged_attention(hipStream_t st, const PagedArgs &a, const floa
   const int group = n_head / a.n_kv;
   const int w = window >= INT32_MAX ? 0 : (int)window, sink = (int)(n_sink < (1 << 30) ? n_sink : (1 << 30));
   // 16 columns per tile where sequences have few rows: at 32 columns each 36 us with
-  // 16, 26 with 32 (16 sequences of 2000 positions, Q8_0, heads of 64); decode steps
+  // 16, 23 with 32 (16 sequences of 2000 positions, Q8_0, heads of 64); decode steps
   // of 8 heads would leave three quarters of 32 idle
   const bool one = a.s_rows * group <= (int64_t)24 * a.n_seq;
   const int cols = one ? 16 : 32, full = paged_grid(a.hd, one ? 1 : 2);
   // no more work-groups than the longest sequences that the table allows would fill
   const int64_t units = (a.s_rows * group / cols + a.n_seq) * a.n_kv;
-  const int64_t most = units * (((int64_t)a.table_cols * a.page / kTile + 8 + 3) / 8 + 1);
+  const int64_t most = units * (((int64_t)a.table_cols * a.page / kTile + Work<16>::cost) / Work<16>::least + 2);
   const unsigned grid = (unsigned)std::min<int64_t>(full, (most + 7) / 8 * 8);
   const size_t lds = (size_t)(a.n_seq + 1) * 8 + (size_t)a.n_seq * 4;
   float *ml = part + (size_t)2 * full * cols * a.hd;
