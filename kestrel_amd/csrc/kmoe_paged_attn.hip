@@ -235,8 +235,6 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
       const bool ok = exists(id);
       const int pp_next = more ? (sp.tile(v + 4) * kTile) & (a.page - 1) : 0;
       const uint8_t *p_next = more ? block(exists(id_next) ? id_next : 0) : nullptr;
-      id = id_next;
-      id_next = page_of(v + 8);
       const int lq = here(lane);  // (q's pieces are read at each tile)
       // (Q8_0: the wave at its products goes first, the others have the quants and
       // the softmax to do: 4096 rows 490 -> 480 us; F16 388 -> 400)
@@ -302,6 +300,11 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (T == kPgQ8) __builtin_amdgcn_s_setprio(0);
       if constexpr (more) fr.load_k(p_next, a.page, pp_next, lane);
+      // (here, as scalar loads and LDS reads are waited for together: at the tile's
+      // start the first products waited for the page table)
+      id = id_next;
+      id_next = page_of(v + 8);
+      __builtin_amdgcn_sched_barrier(0);
       // what some row does not see
       if (!ok || p0 + kTile > pos_lo + 1 || (window && p0 < (int)(pos_hi - window + 1) && p0 + kTile > sink)) {
         uint32_t keep = 0;
