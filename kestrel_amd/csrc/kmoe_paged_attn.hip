@@ -21,26 +21,33 @@ namespace kmoe {
 
 namespace {
 
-// 16 bytes per lane, each line whole by one load.
-__device__ __forceinline__ u32x4 load16(const uint8_t *p) { return __builtin_nontemporal_load((const u32x4 *)p); }
+// 16 bytes per lane, each line whole by one load. ONCE: by one work-group only, past
+// the caches' order of use (decode steps, 64 rows at 2000 positions 100 -> 90 us).
+// Column tiles of many rows read the same pages (with it two chunks of 512 rows and
+// seven single rows, Q8_0, 250 -> 281 us; 4096 rows 382 -> 405).
+template <bool ONCE>
+__device__ __forceinline__ u32x4 load16(const uint8_t *p) {
+  if constexpr (ONCE) return __builtin_nontemporal_load((const u32x4 *)p);
+  return *(const u32x4 *)p;
+}
 
 // A wave's share of 32 positions of K and of V, as loaded.
-template <int T, int HD>
+template <int T, int HD, bool ONCE>
 struct Frags;
-template <int HD>
-struct Frags<kPgF16, HD> {
+template <int HD, bool ONCE>
+struct Frags<kPgF16, HD, ONCE> {
   u32x4 k[2][HD / 32], v[HD / 16];
   __device__ __forceinline__ void load_k(const uint8_t *blk, int pg, int pp, int lane) {
     const uint8_t *p = blk + (pp >> 5) * (64 * HD) + lane * 16;
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int t = 0; t < HD / 32; ++t) k[s][t] = load16(p + (s * (HD / 32) + t) * 1024);
+      for (int t = 0; t < HD / 32; ++t) k[s][t] = load16<ONCE>(p + (s * (HD / 32) + t) * 1024);
   }
   __device__ __forceinline__ void load_v(const uint8_t *blk, int pg, int pp, int lane) {
     const uint8_t *p = blk + pg * HD * 2 + (pp >> 5) * (64 * HD) + lane * 16;
 #pragma unroll
-    for (int u = 0; u < HD / 16; ++u) v[u] = load16(p + u * 1024);
+    for (int u = 0; u < HD / 16; ++u) v[u] = load16<ONCE>(p + u * 1024);
   }
   // V elements of the lane's positions that are in `m` only (bit j: position j of its eight)
   __device__ __forceinline__ void keep_v(uint32_t m) {
@@ -51,8 +58,8 @@ struct Frags<kPgF16, HD> {
     for (int u = 0; u < HD / 16; ++u) v[u] &= b;
   }
 };
-template <int HD>
-struct Frags<kPgQ8, HD> {
+template <int HD, bool ONCE>
+struct Frags<kPgQ8, HD, ONCE> {
   u32x4 k[2][HD / 64], ks[2][HD / 64], v[HD / 32], vs[HD / 32];
   __device__ __forceinline__ void load_k(const uint8_t *blk, int pg, int pp, int lane) {
     const uint8_t *p = blk + (pp >> 5) * (32 * HD) + lane * 16;
@@ -61,7 +68,7 @@ struct Frags<kPgQ8, HD> {
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int t = 0; t < HD / 64; ++t) {
-        k[s][t] = load16(p + (s * (HD / 64) + t) * 1024);
+        k[s][t] = load16<ONCE>(p + (s * (HD / 64) + t) * 1024);
         ks[s][t] = *(const u32x4 *)(d + s * HD + t * 16);
       }
   }
@@ -71,7 +78,7 @@ struct Frags<kPgQ8, HD> {
     const uint8_t *d = h + pg * HD + (pp >> 5) * (2 * HD) + (lane >> 4) * (HD / 2);
 #pragma unroll
     for (int u = 0; u < HD / 32; ++u) {
-      v[u] = load16(p + u * 1024);
+      v[u] = load16<ONCE>(p + u * 1024);
       vs[u] = *(const u32x4 *)(d + u * 16);
     }
   }
@@ -168,7 +175,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
     // the block of a tile's page (page 0 stands in for one that does not exist)
     auto block = [&](int id) { return a.pages + ((int64_t)id * a.n_kv + g) * bb; };
     auto exists = [&](int id) { return id >= 0 && id < a.n_pages; };
-    Frags<T, HD> fr;
+    Frags<T, HD, C == 1> fr;
     int v = s_.at + wave;
     int id = page_of(v), id_next = page_of(v + 4);  // pages of the wave's tile and of its next one
     if (v < v_last) {
