@@ -8,8 +8,8 @@
 // the bytes) the vector units, which make f16 of the quants: 64 us for 286 MB.
 // Prompts are bound by the vector and matrix units together, which overlap little
 // with two waves a SIMD (4096 rows, 32 heads over 8: 400 us, 690 Tflop/s of f16
-// products: matrix units busy 32 % of the time, vector units 44 %; K and V all from
-// one page: a tenth less time), short calls by latencies: 37 positions 8.6 us, of
+// products, at 2.05 GHz; a wave's next scores beside its own softmax, in whatever
+// order, gained nothing), short calls by latencies: 37 positions 8.6 us, of
 // which 4 are the launch, 2 the plan and 1 the first loads.
 #include <algorithm>
 #include <type_traits>
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
       const uint8_t *p_next = more ? block(exists(id_next) ? id_next : 0) : nullptr;
       const int lq = here(lane);  // (q's pieces are read at each tile)
       // (Q8_0: the wave at its products goes first, the others have the quants and
-      // the softmax to do: 4096 rows 490 -> 480 us; F16 388 -> 400)
+      // the softmax to do: 4096 rows 470 -> 458 us; with F16 pages the same)
       if constexpr (T == kPgQ8) __builtin_amdgcn_s_setprio(1);
       // scores, in q's scale
       f32x4 S[C][2];
