@@ -540,7 +540,8 @@ int kmoe_paged_rope_kv_store(kmoe_ctx *ctx, const kmoe_paged_desc *desc, void *p
 int kmoe_paged_kv_read(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *pages_dev,
                        const kmoe_paged_batch *batch, uint16_t *k_dev, uint16_t *v_dev);
 /* Causal GQA attention of the batch's rows q [s_rows, n_head, head_dim] (after
- * RoPE) over their sequences' pages: out [s_rows, n_head * head_dim]. A row at
+ * RoPE) over their sequences' pages: out [s_rows, n_head * head_dim], which must
+ * not overlap q. A row at
  * position i sees the positions p <= i; with window > 0 only those with
  * p > i - window or p < n_sink (the first n_sink positions stay visible; window
  * 0: all, n_sink unused). Pages that no row sees are not read. A row that sees

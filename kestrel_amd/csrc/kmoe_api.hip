@@ -2615,6 +2615,9 @@ int kmoe_paged_attention(kmoe_ctx *c, const kmoe_paged_desc *d, const void *page
   if (window < 0 || n_sink < 0) return fail(c, KMOE_E_INVALID, "negative window or n_sink");
   if (a.s_rows == 0) return KMOE_OK;
   if (!q || !out) return fail(c, KMOE_E_INVALID, "null pointer");
+  const uintptr_t bytes = (uintptr_t)a.s_rows * n_head * a.hd * sizeof(float);
+  if ((uintptr_t)q < (uintptr_t)out + bytes && (uintptr_t)out < (uintptr_t)q + bytes)
+    return fail(c, KMOE_E_INVALID, "out overlaps q");
   DeviceGuard g(c->device);
   float *part = nullptr;
   rc = paged_ws(c, &part);

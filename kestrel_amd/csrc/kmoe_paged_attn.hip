@@ -7,7 +7,7 @@
 // of pages, one row at 131000 positions (8 kv heads) 95 us; with Q8_0 pages (half
 // the bytes) the vector units, which make f16 of the quants: 64 us for 286 MB.
 // Prompts are bound by the vector and matrix units together, which overlap little
-// with two waves a SIMD (4096 rows, 32 heads over 8: 400 us, 690 Tflop/s of f16
+// with two waves a SIMD (4096 rows, 32 heads over 8: 375 us, 730 Tflop/s of f16
 // products, at 2.05 GHz; a wave's next scores beside its own softmax, in whatever
 // order, gained nothing), short calls by latencies: 37 positions 8.6 us, of
 // which 4 are the launch, 2 the plan and 1 the first loads.

@@ -387,6 +387,11 @@ class Context:
             raise ValueError(f"{name}: rows are not contiguous")
         return width
 
+    def _pages(self, kv: PagedKV, pages, n_layer: int = 1):
+        if pages.get_device() != self.device or not pages.is_contiguous():
+            raise ValueError(f"pages: need contiguous memory on cuda:{self.device}")
+        return C.byref(kv.desc(pages, n_layer))
+
     def paged_batch(self, table, seq_len, row_start=None, s_rows=None) -> PagedBatch:
         """kmoe_paged_batch: table [n_seq, columns], seq_len [n_seq] and row_start [n_seq + 1] (or None: one
         row per sequence), int32 on the device; the struct keeps them alive. A call reads what they hold when
@@ -408,7 +413,7 @@ class Context:
         w, f = kv.n_kv * kv.head_dim, self.torch.float32
         ks = self._need("k", k, f, batch.s_rows, w, True)
         vs = self._need("v", v, f, batch.s_rows, w, True)
-        self.check(self.lib.kmoe_paged_kv_store(self.h, C.byref(kv.desc(pages)), _ptr(pages), C.byref(batch), _ptr(k),
+        self.check(self.lib.kmoe_paged_kv_store(self.h, self._pages(kv, pages), _ptr(pages), C.byref(batch), _ptr(k),
                                                 ks, _ptr(v), vs))
 
     def paged_rope_kv_store(self, kv: PagedKV, pages, batch: PagedBatch, q, k, v, n_head: int, rope_dim: int,
@@ -424,7 +429,7 @@ class Context:
             q_out = self._empty((batch.s_rows, n_head * kv.head_dim), f)
         else:
             self._need("q_out", q_out, f, batch.s_rows, n_head * kv.head_dim)
-        self.check(self.lib.kmoe_paged_rope_kv_store(self.h, C.byref(kv.desc(pages)), _ptr(pages), C.byref(batch),
+        self.check(self.lib.kmoe_paged_rope_kv_store(self.h, self._pages(kv, pages), _ptr(pages), C.byref(batch),
                                                      _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, n_head, rope_dim,
                                                      _ptr(inv_freq), int(neox), _ptr(q_out)))
         return q_out
@@ -433,7 +438,7 @@ class Context:
         """The batch's rows read back: (k, v) f16 [S, n_kv*head_dim]."""
         shape = (batch.s_rows, kv.n_kv * kv.head_dim)
         k, v = self._empty(shape, self.torch.float16), self._empty(shape, self.torch.float16)
-        self.check(self.lib.kmoe_paged_kv_read(self.h, C.byref(kv.desc(pages)), _ptr(pages), C.byref(batch), _ptr(k),
+        self.check(self.lib.kmoe_paged_kv_read(self.h, self._pages(kv, pages), _ptr(pages), C.byref(batch), _ptr(k),
                                                _ptr(v)))
         return k, v
 
@@ -447,7 +452,7 @@ class Context:
             out = self._empty(shape, f)
         else:
             self._need("out", out, f, *shape)
-        self.check(self.lib.kmoe_paged_attention(self.h, C.byref(kv.desc(pages)), _ptr(pages), C.byref(batch), _ptr(q),
+        self.check(self.lib.kmoe_paged_attention(self.h, self._pages(kv, pages), _ptr(pages), C.byref(batch), _ptr(q),
                                                  n_head, window, n_sink, _ptr(out)))
         return out
 
@@ -456,9 +461,7 @@ class Context:
         s, d = np.array(src, np.int32, ndmin=1), np.array(dst, np.int32, ndmin=1)
         if s.size != d.size:
             raise ValueError(f"{s.size} source pages, {d.size} destinations")
-        if not pages.is_contiguous():
-            raise ValueError("pages: not contiguous")
-        self.check(self.lib.kmoe_pages_copy(self.h, C.byref(kv.desc(pages, n_layer)), _ptr(pages), n_layer,
+        self.check(self.lib.kmoe_pages_copy(self.h, self._pages(kv, pages, n_layer), _ptr(pages), n_layer,
                                             pages.nbytes // max(1, n_layer), s.ctypes.data,
                                             d.ctypes.data, s.size))
 

@@ -702,11 +702,12 @@ def test_refusals(ctx):
     pages = torch.zeros((4, kv.page_bytes), dtype=torch.uint8, device="cuda")
     table, lens = _dev([[0, 1]], np.int32), _dev([40], np.int32)
     x, q, w = torch.zeros((1, 128), device="cuda"), torch.zeros((1, 256), device="cuda"), 128
+    out = torch.zeros_like(q)
     b = ctx.paged_batch(table, lens)
     inv = torch.ones(32, device="cuda")
     L, by = ctx.lib, C.byref
 
-    def att(d=None, bt=b, p=pages.data_ptr(), qp=q.data_ptr(), nh=4, win=0, sink=0, o=q.data_ptr()):
+    def att(d=None, bt=b, p=pages.data_ptr(), qp=q.data_ptr(), nh=4, win=0, sink=0, o=out.data_ptr()):
         return L.kmoe_paged_attention(ctx.h, by(d or kv.desc(pages)), p, by(bt), qp, nh, win, sink, o)
 
     def batch(**kw):
@@ -721,7 +722,7 @@ def test_refusals(ctx):
     INV, UNS = -1, -2
     for want, rc in [
             (0, att()), (INV, att(nh=3)), (INV, att(nh=0)), (UNS, att(nh=34)), (INV, att(win=-1)), (INV, att(sink=-1)),
-            (INV, att(p=None)), (INV, att(p=pages.data_ptr() + 4)), (INV, att(qp=None)), (INV, att(o=None)),
+            (INV, att(p=None)), (INV, att(p=pages.data_ptr() + 4)), (INV, att(qp=None)), (INV, att(o=None)), (INV, att(o=q.data_ptr())), (INV, att(o=q.data_ptr() + 4)),
             (UNS, att(D(F32, 2, 64, 32, 4))), (UNS, att(D(F16, 2, 96, 32, 4))), (UNS, att(D(F16, 2, 64, 16, 4))),
             (UNS, att(D(F16, 2, 64, 48, 4))), (INV, att(D(F16, 0, 64, 32, 4))), (INV, att(D(F16, 2, 64, 32, 0))),
             (INV, att(D(F16, 2, 64, 32, 1 << 31))), (INV, att(bt=batch(n_seq=-1))), (INV, att(bt=batch(n_seq=4097, s_rows=4097))),
@@ -742,6 +743,8 @@ def test_refusals(ctx):
     for bad in (lambda: ctx.paged_attention(kv, pages, b, q.half(), 4), lambda: ctx.paged_attention(kv, pages, b, q.cpu(), 4),
                 lambda: ctx.paged_attention(kv, pages, b, q, 2), lambda: ctx.paged_batch(table.long(), lens),
                 lambda: ctx.paged_batch(table, lens, lens, 1), lambda: ctx.paged_batch(table, lens, _dev([0, 1], np.int32)),
-                lambda: ctx.paged_kv_store(kv, pages, b, x[:, ::2], x)):
+                lambda: ctx.paged_kv_store(kv, pages, b, x[:, ::2], x), lambda: ctx.paged_attention(kv, pages.cpu(), b, q, 4),
+                lambda: ctx.paged_kv_read(kv, pages[::2], b), lambda: ctx.paged_kv_store(kv, pages.cpu(), b, x, x),
+                lambda: ctx.pages_copy(kv, pages.cpu(), [0], [1])):
         with pytest.raises(ValueError):
             bad()
