@@ -95,8 +95,11 @@ struct Frags<kPgQ8, HD, ONCE> {
 // Work-groups of a CU that the registers let reside.
 constexpr int paged_occ(int hd, int c) { return hd == 64 ? (c == 1 ? 4 : 3) : (c == 1 ? 3 : 2); }
 
-template <int COLS>
-using Work = Shares<COLS, 4, 8, 8, 24>;
+// (A unit of decode steps counts 8 tiles besides its own, 12 where they are half as
+// large: 200 rows of heads of 64, Q8_0, 8 tiles 54 us, 12 52, 16 52; 200 rows of heads
+// of 128, F16, 81, 83, 86.)
+template <int HD, int COLS>
+using Work = Shares<COLS, 4, (HD == 64 && COLS == 16 ? 12 : 8), 8, 24>;
 
 // Work-group: four waves, one segment of a column tile at a time; wave w takes
 // its tiles w, w + 4, ... (32 positions each) with its own running softmax, and
@@ -134,7 +137,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
   const int group = nh / a.n_kv, magic = 65536 / group + 1;  // x / group = x * magic >> 16 for x < 4096
   const int64_t bb = paged_block_bytes(T, a.page, HD);
   const int pshift = __builtin_ctz(a.page);
-  Cursor<Work<COLS>> cur(a, nh, window, sink, start, (int32_t *)(start + a.n_seq + 1), red);
+  Cursor<Work<HD, COLS>> cur(a, nh, window, sink, start, (int32_t *)(start + a.n_seq + 1), red);
   const int64_t cap = cur.cap;
 
   // wave 3 finds the next segment while this one's first loads are on their way (all
@@ -599,7 +602,8 @@ hipError_t launch_paged_attention(hipStream_t st, const PagedArgs &a, const floa
   const int cols = one ? 16 : 32, full = paged_grid(a.hd, one ? 1 : 2);
   // no more work-groups than the longest sequences that the table allows would fill
   const int64_t units = (a.s_rows * group / cols + a.n_seq) * a.n_kv;
-  const int64_t most = units * (((int64_t)a.table_cols * a.page / kTile + Work<16>::cost) / Work<16>::least + 2);
+  const int cost = one && a.hd == 64 ? Work<64, 16>::cost : Work<128, 16>::cost;
+  const int64_t most = units * (((int64_t)a.table_cols * a.page / kTile + cost) / Work<64, 16>::least + 2);
   const unsigned grid = (unsigned)std::min<int64_t>(full, (most + 7) / 8 * 8);
   const size_t lds = (size_t)(a.n_seq + 1) * 8 + (size_t)a.n_seq * 4;
   float *ml = part + (size_t)2 * full * cols * a.hd;
