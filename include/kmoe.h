@@ -511,7 +511,7 @@ typedef struct {
 } kmoe_paged_desc;
 typedef struct {
   int32_t n_seq;                 /* 1 .. KMOE_PAGED_MAX_SEQ */
-  int32_t table_cols;            /* pages per row of the table */
+  int32_t table_cols;            /* pages per row of the table: at most 2^30 positions */
   int64_t s_rows;                /* rows of the call's q, k, v and outputs, at most 2^22 */
   const int32_t *row_start_dev;  /* [n_seq + 1] ascending, or NULL: one row per sequence (s_rows == n_seq) */
   const int32_t *seq_len_dev;    /* [n_seq] */
@@ -541,10 +541,9 @@ int kmoe_paged_kv_read(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *p
                        const kmoe_paged_batch *batch, uint16_t *k_dev, uint16_t *v_dev);
 /* Causal GQA attention of the batch's rows q [s_rows, n_head, head_dim] (after
  * RoPE) over their sequences' pages: out [s_rows, n_head * head_dim], which must
- * not overlap q. A row at
- * position i sees the positions p <= i; with window > 0 only those with
- * p > i - window or p < n_sink (the first n_sink positions stay visible; window
- * 0: all, n_sink unused). Pages that no row sees are not read. A row that sees
+ * not overlap q. A row at position i sees the positions p <= i; with window > 0
+ * only those with p > i - window or p < n_sink (the first n_sink positions stay
+ * visible; window 0: all, n_sink unused). Pages that no row sees are not read. A row that sees
  * nothing gives zeros. Sums and softmax statistics are f32; a row's last bits
  * depend on the batch it is in (how the positions are shared out), a call's on
  * nothing else. n_head / n_kv <= 16 heads per kv head. The matrix cores take q,

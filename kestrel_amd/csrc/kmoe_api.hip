@@ -2542,6 +2542,8 @@ static int check_paged(kmoe_ctx *c, const kmoe_paged_desc *d, const void *pages,
   if (b->n_seq < 0 || b->n_seq > KMOE_PAGED_MAX_SEQ)
     return fail(c, KMOE_E_INVALID, "%d sequences (at most %d)", b->n_seq, KMOE_PAGED_MAX_SEQ);
   if (b->s_rows < 0 || b->s_rows > kPagedMaxRows || b->table_cols < 0) return fail(c, KMOE_E_INVALID, "negative or too large size");
+  if ((int64_t)b->table_cols * d->page > (int64_t)1 << 30)  // (tiles' ends are counted in 32 bits)
+    return fail(c, KMOE_E_INVALID, "%d pages of %d positions per sequence (at most 2^30 positions)", b->table_cols, d->page);
   if (!b->row_start_dev && b->s_rows != b->n_seq)
     return fail(c, KMOE_E_INVALID, "%lld rows of %d sequences need row_start", (long long)b->s_rows, b->n_seq);
   *a = PagedArgs{d->type, d->n_kv,          d->head_dim,     d->page,     d->n_pages, (uint8_t *)pages,

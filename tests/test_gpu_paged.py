@@ -727,7 +727,7 @@ def test_refusals(ctx):
             (UNS, att(D(F16, 2, 64, 48, 4))), (INV, att(D(F16, 0, 64, 32, 4))), (INV, att(D(F16, 2, 64, 32, 0))),
             (INV, att(D(F16, 2, 64, 32, 1 << 31))), (INV, att(bt=batch(n_seq=-1))), (INV, att(bt=batch(n_seq=4097, s_rows=4097))),
             (INV, att(bt=batch(s_rows=2))), (INV, att(bt=batch(s_rows=-1, row_start=lens.data_ptr()))),
-            (INV, att(bt=batch(seq_len=None))), (INV, att(bt=batch(table=None))), (INV, att(bt=batch(table_cols=-1))),
+            (INV, att(bt=batch(seq_len=None))), (INV, att(bt=batch(table=None))), (INV, att(bt=batch(table_cols=-1))), (INV, att(bt=batch(table_cols=(1 << 25) + 1))),
             (INV, att(bt=batch(s_rows=(1 << 22) + 1, row_start=lens.data_ptr()))),
             (0, att(bt=batch(n_seq=0, s_rows=0, seq_len=None, table=None), p=None, qp=None, o=None)),
             (INV, L.kmoe_paged_kv_store(ctx.h, by(kv.desc(pages)), pages.data_ptr(), by(b), x.data_ptr(), w - 1, x.data_ptr(), w)),

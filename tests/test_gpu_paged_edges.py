@@ -43,6 +43,26 @@ def test_windows_past_32_bits(ctx, rows):  # noqa: F811
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("nh,rows", [(4, None), (16, [3])])
+def test_lengths_past_the_table(ctx, t, nh, rows):  # noqa: F811
+    """Rows near position 2^31 of a table of 96 positions: they see those that the window leaves."""
+    nkv, hd = 1, 64
+    c = Cache(ctx, t, nkv, hd, 32, [96], 11)
+    S = 1 if rows is None else rows[0]
+    q = np.random.default_rng(11).standard_normal((S, nh, hd)).astype(np.float32)
+    b = c.batch(rows, lens=[2 ** 31 - 1])
+    for window, sink, n in ((0, 0, 96), (50, 0, 0), (50, 5, 5), (2 ** 31 - 96, 0, None), (2 ** 40, 0, 96)):
+        out = ctx.paged_attention(c.kv, c.pages, b, _dev(q.reshape(S, -1)), nh, window=window, n_sink=sink)
+        for i in range(S):
+            at = 2 ** 31 - 1 - S + i  # the row's position
+            p = np.arange(96)
+            see = p < n if n is not None else p > at - window
+            sub = SimpleNamespace(kv=c.kv, lens=[int(see.sum())], hk=[c.hk[0][see]], hv=[c.hv[0][see]])
+            ref, tol, _ = _reference(sub, q[i:i + 1], None, nh)
+            _close(out[i:i + 1].cpu().numpy(), ref, tol)
+
+
+@pytest.mark.parametrize("t", TYPES)
 def test_a_table_without_columns(ctx, t):  # noqa: F811
     import torch
 
