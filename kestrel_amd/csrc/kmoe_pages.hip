@@ -204,7 +204,7 @@ int kmoe_pages_trim(kmoe_pages *p, uint32_t seq, int64_t window, int64_t n_sink,
         p->give(s->pages[i]);
         s->pages[i] = -1;
         n += own;
-        s->kept = (i + 1) * p->page;
+        s->kept = std::max(s->kept, (i + 1) * p->page);  // (a smaller n_sink gives up front pages only)
         s->window = window;
       }
     if (freed) *freed = n;
