@@ -196,7 +196,7 @@ int kmoe_pages_trim(kmoe_pages *p, uint32_t seq, int64_t window, int64_t n_sink,
     // the next row sits at position len and sees p > len - window
     const int64_t lo = s->len - window + 1;
     if (lo <= 0) return KMOE_OK;
-    const int64_t first = (n_sink + p->page - 1) / p->page, last = lo / p->page;
+    const int64_t first = (std::min(n_sink, s->len) + p->page - 1) / p->page, last = lo / p->page;
     int64_t n = 0;
     for (int64_t i = first; i < last; ++i)
       if (s->pages[i] >= 0) {

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from kestrel_amd import kmoe
-from tests.test_pages import BUDGET, INVALID, Model
+from tests.test_pages import INVALID, Model
 
 pytestmark = pytest.mark.skipif(not os.path.exists(kmoe.LIB_PATH), reason="libkmoe.so not built (run __graft_entry__.build())")
 
@@ -104,3 +104,12 @@ def test_trims_between_truncations_and_forks(seed):
     for s in list(m.seqs):
         m.p.drop(s)
     assert m.p.usage() == (0, 60)
+
+
+@pytest.mark.parametrize("sink", [1 << 31, (1 << 63) - 1])
+def test_first_positions_past_the_sequence(sink):
+    """n_sink as large as it can be: every page is one of the first ones."""
+    p = kmoe.Pages(40, 32)
+    p.append(1, 1000)
+    assert p.trim(1, 1, sink) == 0 and p.usage() == (32, 40)
+    p.truncate(1, 5)
