@@ -73,7 +73,8 @@ __device__ void plain_head(const PagedArgs &a, int b, int g, const float *qp, co
     __syncthreads();
     const float mn = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), m);
     const float f = m == mn ? 1.0f : expf(m - mn);
-    const float e = blk ? expf(sc - mn) : -1.0f;  // -1: not seen
+    const float mb = mn == -INFINITY ? 0.0f : mn;  // (scores of -inf alone, so far: they weigh nothing)
+    const float e = blk ? expf(sc - mb) : -1.0f;  // -1: not seen
     w[t] = e;
     const float ws = group_sum<64>(blk ? e : 0.0f);
     if (lane == 0) sum[wave] = ws;
