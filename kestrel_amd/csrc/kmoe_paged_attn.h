@@ -5,6 +5,7 @@
 
 #include "kmoe_device.h"
 #include "kmoe_paged.h"
+#include "kmoe_paged_walk.h"
 
 namespace kmoe {
 namespace {
@@ -40,11 +41,13 @@ __device__ __forceinline__ int here(int x) {
 // One row's head by a work-group of 256, in plain f32: 256 positions at a time,
 // a thread per score, then a thread per dim (and 256 / HD parts of the
 // positions), running maximum and sum. Every position is read by itself, so a
-// NaN or an infinity reaches this row only if the row sees it.
+// NaN or an infinity reaches this row only if the row sees it. Stretches without pages
+// are passed over.
 template <int T, int HD>
 __device__ void plain_head(const PagedArgs &a, int b, int g, const float *qp, const Visible &vis, float *out) {
   constexpr int PARTS = 256 / HD;
   __shared__ float qs[HD], w[256], red[4], sum[4], accs[PARTS][HD];
+  __shared__ int held[4], nearest;
   const int t = here(threadIdx.x), wave = t >> 6, lane = t & 63;
   const int64_t bb = paged_block_bytes(T, a.page, HD);
   const float scale = 1.0f / sqrtf((float)HD);
@@ -52,14 +55,14 @@ __device__ void plain_head(const PagedArgs &a, int b, int g, const float *qp, co
   if (t < HD) qs[t] = qp[t];
   float m = -INFINITY, l = 0.0f, acc = 0.0f;
   bool any = false;
-  for (int64_t p0 = 0; p0 <= vis.pos; p0 += 256) {
-    if (p0 >= vis.sink && p0 + 256 <= vis.lo) {  // between the first positions and the window
-      p0 = vis.lo / 256 * 256 - 256;
-      continue;
-    }
+  auto block = [&](int64_t p0) {
     const int64_t p = p0 + t;
     const uint8_t *blk = vis(p) ? paged_block(a, bb, b, p, g) : nullptr;
-    __syncthreads();  // qs, and the last block's w read
+    const bool some = __builtin_amdgcn_ballot_w64(blk != nullptr);
+    if (lane == 0) held[wave] = some;
+    __syncthreads();  // (qs is there, too, and the last block's w read)
+    if (!(held[0] | held[1] | held[2] | held[3])) return false;
+    any = true;
     float sc = -INFINITY;
     if (blk) {
       const int pp = (int)(p % a.page);
@@ -78,7 +81,7 @@ __device__ void plain_head(const PagedArgs &a, int b, int g, const float *qp, co
     w[t] = e;
     const float ws = group_sum<64>(blk ? e : 0.0f);
     if (lane == 0) sum[wave] = ws;
-    any = __syncthreads_or(blk != nullptr) || any;
+    __syncthreads();
     m = mn;
     l = l * f + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
     acc *= f;
@@ -90,7 +93,24 @@ __device__ void plain_head(const PagedArgs &a, int b, int g, const float *qp, co
       const uint8_t *vb = paged_block(a, bb, b, p0 + j, g);
       acc = fmaf(e1, v_elem<T>(vb, a.page, HD, (int)((p0 + j) % a.page), d), acc);
     }
-  }
+    return true;
+  };
+  auto find = [&](int64_t col) {  // columns from col on that name no page, four a thread
+    const int32_t *row = a.table + (int64_t)b * a.table_cols;
+    __syncthreads();
+    if (t == 0) nearest = 1024;
+    __syncthreads();
+    int n = 1024;
+#pragma unroll
+    for (int i = 3; i >= 0; --i) {
+      const int64_t c = col + 256 * i + t, id = c < a.table_cols ? row[c] : -1;
+      n = id >= 0 && id < a.n_pages ? 256 * i + t : n;
+    }
+    if (n < 1024) atomicMin(&nearest, n);
+    __syncthreads();
+    return nearest;
+  };
+  plain_walk(vis.pos, vis.lo, vis.sink, (int64_t)a.table_cols * a.page, a.page, block, find);
   __syncthreads();
   accs[t / HD][t % HD] = acc;
   __syncthreads();

@@ -240,9 +240,11 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
 
     // one tile; `more`: its registers are refilled with the wave's next one on the
     // way (a branch around the loads would make every wait one for all of them)
+    bool paged = false;  // some tile of the wave has a page
     auto step = [&](auto more) {
       const int p0 = sp.tile(v) * kTile;
       const bool ok = exists(id);
+      paged |= ok;
       const int pp_next = more ? (sp.tile(v + 4) * kTile) & (a.page - 1) : 0;
       const uint8_t *p_next = more ? block(exists(id_next) ? id_next : 0) : nullptr;
       const int lq = here(lane);  // (q's pieces are read at each tile)
@@ -416,14 +418,15 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
       step(std::false_type());
     }
 
-    // the four waves' sums, O times kUp
+    // the four waves' sums, O times kUp; without a score above -inf the sum of weights
+    // says instead whether there was a page, here and in what is handed over
     lds_barrier();  // every wave is done with q
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const float ls = quad_sum(l[j]);
       if (kg == 0) {
         m_lds[wave][16 * j + c16] = m[j];
-        l_lds[wave][16 * j + c16] = ls;
+        l_lds[wave][16 * j + c16] = m[j] == -INFINITY && paged ? ls + 1.0f : ls;
       }
 #pragma unroll
       for (int u = 0; u < NU; ++u) *(f32x4 *)&L.o[wave][16 * j + c16][16 * u + 4 * kg] = O[j][u];
@@ -444,7 +447,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
         fin = fin && fabsf(r[k]) < INFINITY;
       }
       *(f32x4a4 *)(out + ((r0 + i) * nh + (int64_t)g * group + head_of(c)) * HD + d) = r;
-      if (!fin || (M == -INFINITY && pos0 + i >= 0)) atomicOr(&bad_cols, 1u << c);
+      if (!fin || (M == -INFINITY && Lsum > 0.0f && pos0 + i >= 0)) atomicOr(&bad_cols, 1u << c);
     };
     for (int e = tl; e < nv * (HD / 4); e += 256) {
       const int c = e / (HD / 4), d = e % (HD / 4) * 4;
@@ -454,7 +457,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
       float Ls = 0.0f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const float f = __builtin_amdgcn_exp2f(m_lds[w][c] - Mb);
+        const float f = M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_lds[w][c] - Mb);
         Ls = fmaf(l_lds[w][c], f, Ls);
         const f32x4 z = *(const f32x4 *)&L.o[w][c][d];
 #pragma unroll
@@ -491,12 +494,13 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
       float M = -INFINITY, Ls = 0.0f;
       for (int i = jp; i < ns; i += JP) {
         const f32x2 ml = ld2_agent(part_ml + (slot(i) * COLS + jc) * 2);
-        const float Mn = fmaxf(M, ml.x), Mb = Mn == -INFINITY ? 0.0f : Mn;
-        Ls = fmaf(ml.y, __builtin_amdgcn_exp2f(ml.x - Mb), Ls * __builtin_amdgcn_exp2f(M - Mb));
+        const float Mn = fmaxf(M, ml.x);
+        const bool none = Mn == -INFINITY;
+        Ls = fmaf(ml.y, none ? 1.0f : __builtin_amdgcn_exp2f(ml.x - Mn), Ls * (none ? 1.0f : __builtin_amdgcn_exp2f(M - Mn)));
         M = Mn;
       }
       const float Mc = group_max<JP>(M), Mb = Mc == -INFINITY ? 0.0f : Mc;
-      Ls = group_sum<JP>(Ls * __builtin_amdgcn_exp2f(M - Mb));
+      Ls = group_sum<JP>(Ls * (Mc == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - Mb)));
       if (jp == 0) {
         m_lds[0][jc] = Mc;
         l_lds[0][jc] = Ls;
@@ -564,7 +568,8 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
     lds_barrier();
     // an infinity or NaN among what a tile's columns see together spreads in the
     // products (0 * inf): such columns are formed again from their own positions,
-    // as are those without a score above -inf (no page at all, or every score -inf)
+    // as are those without a score above -inf where their sequence has a page (every
+    // score -inf, or no page that the row sees)
     uint32_t bad = bad_cols;
     while (bad) {
       const int c = __builtin_ctz(bad);
