@@ -591,8 +591,9 @@ int kmoe_pages_fork(kmoe_pages *p, uint32_t from, uint32_t to, int64_t n);
 int kmoe_pages_truncate(kmoe_pages *p, uint32_t seq, int64_t n);
 /* Gives up the pages that no later row of seq sees under kmoe_paged_attention's
  * window and n_sink (their table entries become -1); *freed (may be NULL)
- * counts those that are free now. Truncating or forking seq to where a trimmed
- * position would be seen again is refused. */
+ * counts those that are free now. Truncating or forking seq to a length whose
+ * next row would see a given up position within the window (that of the last trim
+ * that gave pages up) is refused; back to the first positions that were kept is not. */
 int kmoe_pages_trim(kmoe_pages *p, uint32_t seq, int64_t window, int64_t n_sink, int64_t *freed);
 int kmoe_pages_drop(kmoe_pages *p, uint32_t seq);
 int kmoe_pages_length(const kmoe_pages *p, uint32_t seq, int64_t *n);

@@ -17,9 +17,7 @@ namespace {
 struct Seq {
   int64_t len = 0;
   std::vector<int32_t> pages;  // -1: trimmed
-  // positions below `kept` that lie on trimmed pages are gone (the first pages,
-  // with the positions below `sink`, are still held); `window` as trimmed
-  int64_t kept = 0, window = 0;
+  int64_t window = 0;  // of the last trim that gave pages up; 0: none did
 };
 
 }  // namespace
@@ -71,6 +69,16 @@ int guarded(kmoe_pages *p, F &&f) {
   } catch (...) {
     return pfail(p, KMOE_E_INVALID, "unexpected error");
   }
+}
+
+// Whether s can be cut to n positions: the row that would come next sees, by the
+// window, none that was trimmed, and finds the page that it goes on.
+bool can_cut(const kmoe_pages *p, const Seq *s, int64_t n) {
+  if (!s->window || n >= s->len) return true;
+  const int64_t lo = std::max<int64_t>(0, n - s->window + 1), end = (n + p->page - 1) / p->page;
+  for (int64_t i = lo / p->page; i < end; ++i)
+    if (s->pages[i] < 0) return false;
+  return true;
 }
 
 Seq *find(kmoe_pages *p, uint32_t seq) {
@@ -153,11 +161,10 @@ int kmoe_pages_fork(kmoe_pages *p, uint32_t from, uint32_t to, int64_t n) {
     if (!s) return pfail(p, KMOE_E_NOT_LOADED, "fork: no sequence %u", from);
     if (find(p, to)) return pfail(p, KMOE_E_INVALID, "fork: sequence %u exists", to);
     if (n < 0 || n > s->len) return pfail(p, KMOE_E_INVALID, "fork: %lld of %lld positions", (long long)n, (long long)s->len);
-    if (s->kept && n < s->len && n + 1 - s->window < s->kept)
+    if (!can_cut(p, s, n))
       return pfail(p, KMOE_E_INVALID, "fork: position %lld's window was trimmed", (long long)n);
     Seq t;
     t.len = n;
-    t.kept = s->kept;
     t.window = s->window;
     t.pages.assign(s->pages.begin(), s->pages.begin() + (n + p->page - 1) / p->page);
     Seq &to_seq = p->seqs[to];
@@ -174,7 +181,7 @@ int kmoe_pages_truncate(kmoe_pages *p, uint32_t seq, int64_t n) {
     Seq *s = find(p, seq);
     if (!s) return pfail(p, KMOE_E_NOT_LOADED, "truncate: no sequence %u", seq);
     if (n < 0 || n > s->len) return pfail(p, KMOE_E_INVALID, "truncate: %lld of %lld positions", (long long)n, (long long)s->len);
-    if (s->kept && n < s->len && n + 1 - s->window < s->kept)
+    if (!can_cut(p, s, n))
       return pfail(p, KMOE_E_INVALID, "truncate: position %lld's window was trimmed", (long long)n);
     const size_t keep = (size_t)((n + p->page - 1) / p->page);
     while (s->pages.size() > keep) {
@@ -204,7 +211,6 @@ int kmoe_pages_trim(kmoe_pages *p, uint32_t seq, int64_t window, int64_t n_sink,
         p->give(s->pages[i]);
         s->pages[i] = -1;
         n += own;
-        s->kept = std::max(s->kept, (i + 1) * p->page);  // (a smaller n_sink gives up front pages only)
         s->window = window;
       }
     if (freed) *freed = n;

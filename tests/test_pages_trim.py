@@ -56,7 +56,7 @@ class Trimmed(Model):
         try:
             call()
         except kmoe.KmoeError as e:
-            assert e.status == INVALID and n < len(self.seqs[s])
+            assert e.status == INVALID and n < len(self.seqs[s]) and not self.held(s, n)
             return False
         assert n == len(self.seqs[s]) or self.held(s, n)
         return True
@@ -113,3 +113,24 @@ def test_first_positions_past_the_sequence(sink):
     p.append(1, 1000)
     assert p.trim(1, 1, sink) == 0 and p.usage() == (32, 40)
     p.truncate(1, 5)
+
+
+def test_back_to_the_first_positions():
+    """Lengths inside the first pages that a trim leaves are what they are left for: forks and truncations go there."""
+    p = kmoe.Pages(40, 32)
+    p.append(1, 1000)
+    p.trim(1, 100, 50)  # pages 0 and 1 stay, and 28 on
+    for n in (65, 96, 500, 990 - 100 + 5):
+        with pytest.raises(kmoe.KmoeError):
+            p.fork(1, 2, n)
+    for i, n in enumerate((0, 1, 32, 50, 64)):
+        p.fork(1, 10 + i, n)
+        assert p.length(10 + i) == n
+    assert p.append(13, 1) is not None  # inside a shared page: a copy of its own
+    used = p.usage()[0]
+    p.truncate(1, 40)
+    assert p.length(1) == 40 and p.usage()[0] == used - 4
+    p.append(1, 200)
+    (row,), _ = p.table([1], 8)
+    assert (row >= 0).all()
+    p.truncate(1, 0)
