@@ -581,9 +581,10 @@ typedef struct kmoe_pages kmoe_pages;
 int kmoe_pages_create(int64_t n_pages, int32_t page, kmoe_pages **out);
 int kmoe_pages_destroy(kmoe_pages *p);
 const char *kmoe_pages_last_error(const kmoe_pages *p);
-/* n more positions for seq (begun where it does not exist). Where they begin on
- * a page that other sequences hold too, seq gets a page of its own in its
- * place: *copies = 1 and *src must be copied onto *dst. Otherwise *copies = 0. */
+/* n more positions for seq (begun where it does not exist), 2^30 at most
+ * together (a page table's). Where they begin on a page that other sequences hold
+ * too, seq gets a page of its own in its place: *copies = 1 and *src must be copied
+ * onto *dst. Otherwise *copies = 0. */
 int kmoe_pages_append(kmoe_pages *p, uint32_t seq, int64_t n, int32_t *src, int32_t *dst, int32_t *copies);
 /* A new sequence `to` of the first n positions of `from`, on the same pages. */
 int kmoe_pages_fork(kmoe_pages *p, uint32_t from, uint32_t to, int64_t n);

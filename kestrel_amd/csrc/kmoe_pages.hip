@@ -14,6 +14,8 @@
 
 namespace {
 
+constexpr int64_t kMaxLen = (int64_t)1 << 30;  // what a page table spans at most (kmoe_paged_batch)
+
 struct Seq {
   int64_t len = 0;
   std::vector<int32_t> pages;  // -1: trimmed
@@ -126,7 +128,7 @@ int kmoe_pages_append(kmoe_pages *p, uint32_t seq, int64_t n, int32_t *src, int3
     *copies = 0;
     Seq *s = find(p, seq);
     const int64_t len = s ? s->len : 0, held = s ? (int64_t)s->pages.size() : 0;
-    if (n > INT32_MAX - len) return pfail(p, KMOE_E_INVALID, "append: a sequence ends at %d positions", INT32_MAX);
+    if (n > kMaxLen - len) return pfail(p, KMOE_E_INVALID, "append: a sequence ends at %lld positions", (long long)kMaxLen);
     const int64_t want = (len + n + p->page - 1) / p->page - held;
     // the new positions begin on a page that others hold too: it is copied first
     const bool cow = n > 0 && len % p->page && p->refs[s->pages.back()] > 1;

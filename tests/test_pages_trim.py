@@ -134,3 +134,16 @@ def test_back_to_the_first_positions():
     (row,), _ = p.table([1], 8)
     assert (row >= 0).all()
     p.truncate(1, 0)
+
+
+def test_a_sequence_ends_where_page_tables_do():
+    """2^30 positions: the most that a page table of the kernels spans."""
+    p = kmoe.Pages(4, 1 << 29)
+    p.append(1, (1 << 30) - 1)
+    with pytest.raises(kmoe.KmoeError) as e:
+        p.append(1, 2)
+    assert e.value.status == INVALID and p.length(1) == (1 << 30) - 1
+    p.append(1, 1)
+    with pytest.raises(kmoe.KmoeError) as e:
+        p.append(1, 1)
+    assert e.value.status == INVALID and p.usage() == (2, 4)
