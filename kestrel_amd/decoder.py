@@ -119,7 +119,7 @@ class Decoder:
         self.pos_dev = torch.zeros(1, dtype=torch.int32, device=dev)
         self.token_dev = torch.zeros(1, dtype=torch.int32, device=dev)
         self.graph = None
-        self._graph_gen = None  # the context's workspace generation the graph was captured at
+        self._graph_key = None  # what the graph was captured for (_key)
         self._graph_bufs = None
 
     def _make_cache(self):
@@ -254,6 +254,10 @@ class Decoder:
         return logits
 
     # --------------------------------------------------------- greedy decode
+    def _key(self):
+        """What a captured step depends on besides its buffers: the workspaces' addresses and the regime's kernels."""
+        return self.ctx.workspace_generation(), self.ctx.regime()
+
     def _decode_body(self):
         ty, dims, t = self.embed
         x = self.ctx.get_rows(ty, t, dims[1], dims[0], self.token_dev, out=self._graph_bufs["x"])
@@ -280,9 +284,10 @@ class Decoder:
                 out[i:i + 1].copy_(self.token_dev)
             self.cached += n
             return out
-        if self.graph is not None and self.ctx.workspace_generation() != self._graph_gen:
+        if self.graph is not None and self._key() != self._graph_key:
             # a workspace the graph points into was reallocated since the capture
-            # (a longer prompt chunk, another caller of the context): capture again
+            # (a longer prompt chunk, another caller of the context), or the regime
+            # is another: capture again
             self.graph = None
         if self.graph is None:
             # warm-up call at the same shapes grows every workspace first
@@ -299,7 +304,7 @@ class Decoder:
             finally:
                 self.ctx.set_stream(torch.cuda.current_stream())
             self.graph = g
-            self._graph_gen = self.ctx.workspace_generation()
+            self._graph_key = self._key()
             torch.cuda.synchronize()
         for i in range(n):
             self.graph.replay()
@@ -529,7 +534,7 @@ class PagedDecoder(Decoder):
             b["len"].copy_(at)
             b["tok"].copy_(tok)
             out = torch.empty((n, len(seqs)), dtype=torch.int32, device=self.dev)
-            if use_graph and (self.graph is None or self.ctx.workspace_generation() != self._graph_gen):
+            if use_graph and (self.graph is None or self._key() != self._graph_key):
                 self._decode_rows(b)  # grows every workspace first
                 b["len"].copy_(at)
                 b["tok"].copy_(tok)
@@ -541,7 +546,7 @@ class PagedDecoder(Decoder):
                         self._decode_rows(b)
                 finally:
                     self.ctx.set_stream(torch.cuda.current_stream())
-                self.graph, self._graph_gen = g, self.ctx.workspace_generation()
+                self.graph, self._graph_key = g, self._key()
                 torch.cuda.synchronize()
             for i in range(n):
                 if use_graph:

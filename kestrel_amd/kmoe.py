@@ -263,6 +263,9 @@ class Context:
     def set_regime(self, regime: int):
         self.check(self.lib.kmoe_set_regime(self.h, regime))
 
+    def regime(self) -> int:
+        return self.lib.kmoe_get_regime(self.h)
+
     def vram_set_limit(self, limit: int):
         self.check(self.lib.kmoe_vram_set_limit(self.h, limit))
 
