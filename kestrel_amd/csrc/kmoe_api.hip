@@ -2570,6 +2570,13 @@ int kmoe_paged_kv_store(kmoe_ctx *c, const kmoe_paged_desc *d, void *pages, cons
   return KMOE_OK;
 }
 
+// Whether `bytes` from out on touch one of `rows` rows of `width` floats, `stride` floats apart, from in on.
+static bool overlaps(const void *out, int64_t bytes, const void *in, int64_t rows, int64_t width, int64_t stride) {
+  const __int128 rel = (__int128)(uintptr_t)out - (__int128)(uintptr_t)in, w = 4 * (__int128)width, st = 4 * (__int128)stride;
+  const __int128 i = rel < w ? 0 : (rel - w) / st + 1;  // the first row that ends behind out's first byte
+  return i < rows && i * st < rel + bytes;
+}
+
 int kmoe_paged_rope_kv_store(kmoe_ctx *c, const kmoe_paged_desc *d, void *pages, const kmoe_paged_batch *b,
                              const float *q, int64_t q_stride, const float *k, int64_t k_stride, const float *v,
                              int64_t v_stride, int32_t n_head, int32_t rope_dim, const float *inv_freq, int32_t neox,
@@ -2585,6 +2592,11 @@ int kmoe_paged_rope_kv_store(kmoe_ctx *c, const kmoe_paged_desc *d, void *pages,
     return fail(c, KMOE_E_INVALID, "rows closer together than their width");
   if (a.s_rows == 0) return KMOE_OK;
   if (!q || !k || !v || !inv_freq || !q_out) return fail(c, KMOE_E_INVALID, "null pointer");
+  const int64_t out_bytes = a.s_rows * n_head * a.hd * (int64_t)sizeof(float);
+  if (overlaps(q_out, out_bytes, q, a.s_rows, (int64_t)n_head * a.hd, q_stride) ||
+      overlaps(q_out, out_bytes, k, a.s_rows, w, k_stride) || overlaps(q_out, out_bytes, v, a.s_rows, w, v_stride) ||
+      overlaps(q_out, out_bytes, inv_freq, 1, rope_dim / 2, rope_dim / 2))
+    return fail(c, KMOE_E_INVALID, "q_out overlaps an input");
   DeviceGuard g(c->device);
   LAUNCH(c, "paged_store",
          launch_paged_store(c->stream, a, q, q_stride, k, k_stride, v, v_stride, n_head, rope_dim, inv_freq, neox,
