@@ -2654,6 +2654,8 @@ int kmoe_pages_copy(kmoe_ctx *c, const kmoe_paged_desc *d, void *pages, int64_t 
   if (n == 0 || n_layer == 0) return KMOE_OK;
   if (!pages || !src || !dst) return fail(c, KMOE_E_INVALID, "null pointer");
   if ((uintptr_t)pages & 15) return fail(c, KMOE_E_INVALID, "pages not 16-byte aligned");
+  if (n > d->n_pages)  // (no page twice; before the arrays are read)
+    return fail(c, KMOE_E_INVALID, "%lld copies onto %lld pages", (long long)n, (long long)d->n_pages);
   try {
     std::vector<std::pair<int32_t, uint8_t>> seen;  // (page, 1: copied onto)
     seen.reserve(2 * (size_t)n);

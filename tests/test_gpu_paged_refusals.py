@@ -48,3 +48,15 @@ def test_rotated_q_over_an_input(ctx):  # noqa: F811
     with pytest.raises(KmoeError):
         ctx.paged_rope_kv_store(kv, pages, b, same, torch.ones((S, w), device="cuda"), torch.ones((S, w), device="cuda"), nh,
                                 hd, inv, True, q_out=same)
+
+
+def test_more_copies_than_pages(ctx):  # noqa: F811
+    """Some page would be copied onto twice: refused before the arrays are read."""
+    import torch
+
+    kv = PagedKV(F16, 1, 64, 32)
+    pages = torch.zeros((2, 4, kv.page_bytes), dtype=torch.uint8, device="cuda")
+    one = np.zeros(1, np.int32)
+    for n in (5, 2 ** 40, 2 ** 62, 2 ** 63 - 1):
+        assert ctx.lib.kmoe_pages_copy(ctx.h, C.byref(kv.desc(pages, 2)), pages.data_ptr(), 2, pages.nbytes // 2,
+                                       one.ctypes.data, one.ctypes.data, n) == -1
