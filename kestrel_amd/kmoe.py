@@ -461,7 +461,10 @@ class Context:
 
     def pages_copy(self, kv: PagedKV, pages, src, dst, n_layer: int = 1):
         """Pages src[i] onto dst[i] (host sequences) in each of the n_layer equal parts of pages."""
-        s, d = np.array(src, np.int32, ndmin=1), np.array(dst, np.int32, ndmin=1)
+        given = [np.array(x, ndmin=1) for x in (src, dst)]
+        s, d = (x.astype(np.int32) for x in given)
+        if (s != given[0]).any() or (d != given[1]).any():
+            raise ValueError("a page number is no 32-bit integer")
         if s.size != d.size:
             raise ValueError(f"{s.size} source pages, {d.size} destinations")
         self.check(self.lib.kmoe_pages_copy(self.h, self._pages(kv, pages, n_layer), _ptr(pages), n_layer,

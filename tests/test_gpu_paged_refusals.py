@@ -60,3 +60,22 @@ def test_more_copies_than_pages(ctx):  # noqa: F811
     for n in (5, 2 ** 40, 2 ** 62, 2 ** 63 - 1):
         assert ctx.lib.kmoe_pages_copy(ctx.h, C.byref(kv.desc(pages, 2)), pages.data_ptr(), 2, pages.nbytes // 2,
                                        one.ctypes.data, one.ctypes.data, n) == -1
+
+
+def test_page_numbers_past_32_bits(ctx):  # noqa: F811
+    """Page numbers are not taken modulo 2^32."""
+    import torch
+
+    kv = PagedKV(F16, 1, 64, 32)
+    pages = torch.arange(2 * 4 * kv.page_bytes, device="cuda").to(torch.uint8).view(2, 4, -1)
+    pages[:, 1:] = 0
+    keep = pages.clone()
+    for s, d in ((np.array([2 ** 32]), np.array([1])), (np.array([0]), np.array([2 ** 32 + 1])), ([2 ** 32], [1]),
+                 (torch.tensor([-2 ** 32]), [1])):
+        with pytest.raises((ValueError, KmoeError)):
+            ctx.pages_copy(kv, pages, s, d, n_layer=2)
+    torch.cuda.synchronize()
+    assert torch.equal(pages, keep)
+    ctx.pages_copy(kv, pages, np.array([0], np.int64), torch.tensor([3]), n_layer=2)
+    torch.cuda.synchronize()
+    assert torch.equal(pages[:, 3], keep[:, 0])
