@@ -467,8 +467,10 @@ class Context:
             raise ValueError("a page number is no 32-bit integer")
         if s.size != d.size:
             raise ValueError(f"{s.size} source pages, {d.size} destinations")
+        if n_layer < 1 or (n_layer > 1 and pages.nbytes % (n_layer * kv.page_bytes)):
+            raise ValueError(f"pages: need {n_layer} parts of whole pages ({kv.page_bytes} bytes), got {pages.nbytes} bytes")
         self.check(self.lib.kmoe_pages_copy(self.h, self._pages(kv, pages, n_layer), _ptr(pages), n_layer,
-                                            pages.nbytes // max(1, n_layer), s.ctypes.data,
+                                            pages.nbytes // n_layer, s.ctypes.data,
                                             d.ctypes.data, s.size))
 
     def swiglu(self, g, u, out=None):

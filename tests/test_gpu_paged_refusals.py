@@ -79,3 +79,17 @@ def test_page_numbers_past_32_bits(ctx):  # noqa: F811
     ctx.pages_copy(kv, pages, np.array([0], np.int64), torch.tensor([3]), n_layer=2)
     torch.cuda.synchronize()
     assert torch.equal(pages[:, 3], keep[:, 0])
+
+
+def test_layers_of_whole_pages(ctx):  # noqa: F811
+    """n_layer parts of a buffer whose parts are no whole pages: no layer begins where the copy would look for it."""
+    import torch
+
+    kv = PagedKV(F16, 1, 64, 32)
+    pages = torch.zeros((3, 5, kv.page_bytes), dtype=torch.uint8, device="cuda")
+    for n_layer in (2, 4, 0, -1):
+        with pytest.raises(ValueError):
+            ctx.pages_copy(kv, pages, [0], [1], n_layer=n_layer)
+    ctx.pages_copy(kv, pages, [0], [4], n_layer=3)
+    ctx.pages_copy(kv, pages, [0], [14], n_layer=1)
+    torch.cuda.synchronize()
