@@ -752,38 +752,47 @@ class Pages:
         if rc != 0:
             raise KmoeError(rc, self.lib.kmoe_pages_last_error(self.h).decode())
 
+    @staticmethod
+    def _seq(seq) -> int:
+        if not 0 <= seq < 1 << 32:
+            raise ValueError(f"sequence {seq}: named 0 .. 2^32 - 1")
+        return seq
+
     def append(self, seq: int, n: int):
         """n more positions for seq (begun where there is none); the (src, dst) page to copy, or None."""
         s, d, c = _i32(), _i32(), _i32()
-        self.check(self.lib.kmoe_pages_append(self.h, seq, n, C.byref(s), C.byref(d), C.byref(c)))
+        self.check(self.lib.kmoe_pages_append(self.h, self._seq(seq), n, C.byref(s), C.byref(d), C.byref(c)))
         return (s.value, d.value) if c.value else None
 
     def fork(self, src: int, dst: int, n: int):
         """A new sequence dst of the first n positions of src, on the same pages."""
-        self.check(self.lib.kmoe_pages_fork(self.h, src, dst, n))
+        self.check(self.lib.kmoe_pages_fork(self.h, self._seq(src), self._seq(dst), n))
 
     def truncate(self, seq: int, n: int):
-        self.check(self.lib.kmoe_pages_truncate(self.h, seq, n))
+        self.check(self.lib.kmoe_pages_truncate(self.h, self._seq(seq), n))
 
     def trim(self, seq: int, window: int, n_sink: int = 0) -> int:
         """Gives up the pages that no later row of seq sees; how many are free by it."""
         n = _i64()
-        self.check(self.lib.kmoe_pages_trim(self.h, seq, window, n_sink, C.byref(n)))
+        self.check(self.lib.kmoe_pages_trim(self.h, self._seq(seq), window, n_sink, C.byref(n)))
         return n.value
 
     def drop(self, seq: int):
-        self.check(self.lib.kmoe_pages_drop(self.h, seq))
+        self.check(self.lib.kmoe_pages_drop(self.h, self._seq(seq)))
 
     def length(self, seq: int) -> int:
         n = _i64()
-        rc = self.lib.kmoe_pages_length(self.h, seq, C.byref(n))
+        rc = self.lib.kmoe_pages_length(self.h, self._seq(seq), C.byref(n))
         if rc != 0:
             raise KmoeError(rc, f"no sequence {seq}")
         return n.value
 
     def table(self, seqs, table_cols: int):
         """(page table [n, table_cols], lengths [n]) of seqs, int32 on the host."""
-        ids = np.ascontiguousarray(seqs, dtype=np.uint32).reshape(-1)
+        given = np.asarray(seqs).reshape(-1)
+        ids = given.astype(np.uint32)
+        if (ids != given).any():
+            raise ValueError("a sequence is named 0 .. 2^32 - 1")
         t, n = np.empty((ids.size, table_cols), np.int32), np.empty(ids.size, np.int32)
         self.check(self.lib.kmoe_pages_table(self.h, ids.ctypes.data, ids.size, table_cols, t.ctypes.data,
                                              n.ctypes.data))

@@ -147,3 +147,19 @@ def test_a_sequence_ends_where_page_tables_do():
     with pytest.raises(kmoe.KmoeError) as e:
         p.append(1, 1)
     assert e.value.status == INVALID and p.usage() == (2, 4)
+
+
+@pytest.mark.parametrize("seq", [2 ** 32 + 1, -(2 ** 32) + 1, -1, 2 ** 32])
+def test_sequence_numbers_past_32_bits(seq):
+    """Sequences are not named modulo 2^32."""
+    p = kmoe.Pages(4, 32)
+    p.append(1, 5)
+    p.append(0, 3)
+    p.append(2 ** 32 - 1, 2)
+    for f in (lambda: p.append(seq, 1), lambda: p.drop(seq), lambda: p.truncate(seq, 1), lambda: p.fork(seq, 7, 1),
+              lambda: p.fork(1, seq, 1), lambda: p.trim(seq, 1), lambda: p.length(seq), lambda: p.table([1, seq], 2),
+              lambda: p.table(np.array([seq]), 2)):
+        with pytest.raises(ValueError):
+            f()
+    assert [p.length(s) for s in (0, 1, 2 ** 32 - 1)] == [3, 5, 2] and p.usage() == (3, 4)
+    assert p.table(np.array([1, 0]), 1)[1].tolist() == [5, 3]
