@@ -586,6 +586,11 @@ const char *kmoe_pages_last_error(const kmoe_pages *p);
  * too, seq gets a page of its own in its place: *copies = 1 and *src must be copied
  * onto *dst. Otherwise *copies = 0. */
 int kmoe_pages_append(kmoe_pages *p, uint32_t seq, int64_t n, int32_t *src, int32_t *dst, int32_t *copies);
+/* The same for `count` sequences, n[i] positions for seqs[i], all of them or none; a
+ * sequence is named once. src and dst have room for `count` pairs, *copies of them
+ * are written (no page is copied from and onto, so they may be made in one call). */
+int kmoe_pages_append_many(kmoe_pages *p, const uint32_t *seqs, const int64_t *n, int32_t count, int32_t *src,
+                           int32_t *dst, int32_t *copies);
 /* A new sequence `to` of the first n positions of `from`, on the same pages. */
 int kmoe_pages_fork(kmoe_pages *p, uint32_t from, uint32_t to, int64_t n);
 /* Back to the first n positions; pages past them are given up. */

@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <map>
 #include <new>
+#include <set>
 #include <string>
 #include <vector>
 
@@ -121,39 +122,65 @@ int kmoe_pages_destroy(kmoe_pages *p) {
 
 const char *kmoe_pages_last_error(const kmoe_pages *p) { return p ? p->err.c_str() : "null pages"; }
 
-int kmoe_pages_append(kmoe_pages *p, uint32_t seq, int64_t n, int32_t *src, int32_t *dst, int32_t *copies) {
+int kmoe_pages_append_many(kmoe_pages *p, const uint32_t *seqs, const int64_t *n, int32_t count, int32_t *src,
+                           int32_t *dst, int32_t *copies) {
   if (!p) return KMOE_E_INVALID;
-  if (n < 0 || !src || !dst || !copies) return pfail(p, KMOE_E_INVALID, "append: negative count or null pointer");
+  if (count < 0 || !copies || (count > 0 && (!seqs || !n || !src || !dst)))
+    return pfail(p, KMOE_E_INVALID, "append: negative count or null pointer");
   return guarded(p, [&]() -> int {
+    struct Part {
+      Seq *s;
+      int64_t len, want;
+      bool cow;  // the new positions begin on a page that others hold too: it is copied first
+    };
     *copies = 0;
-    Seq *s = find(p, seq);
-    const int64_t len = s ? s->len : 0, held = s ? (int64_t)s->pages.size() : 0;
-    if (n > kMaxLen - len) return pfail(p, KMOE_E_INVALID, "append: a sequence ends at %lld positions", (long long)kMaxLen);
-    const int64_t want = (len + n + p->page - 1) / p->page - held;
-    // the new positions begin on a page that others hold too: it is copied first
-    const bool cow = n > 0 && len % p->page && p->refs[s->pages.back()] > 1;
-    if (want + cow > (int64_t)p->free.size())
-      return pfail(p, KMOE_E_BUDGET, "append: %lld pages wanted, %lld free", (long long)(want + cow),
-                   (long long)p->free.size());
-    if (s) {
+    std::vector<Part> parts(count);
+    std::map<uint32_t, Seq> begun;
+    std::map<int32_t, int32_t> left;  // shared pages: holders that have left them so far
+    std::set<uint32_t> named;
+    int64_t total = 0;
+    for (int32_t i = 0; i < count; ++i) {
+      if (!named.insert(seqs[i]).second) return pfail(p, KMOE_E_INVALID, "append: sequence %u is named twice", seqs[i]);
+      Seq *s = find(p, seqs[i]);
+      const int64_t len = s ? s->len : 0, held = s ? (int64_t)s->pages.size() : 0;
+      if (n[i] < 0) return pfail(p, KMOE_E_INVALID, "append: negative count");
+      if (n[i] > kMaxLen - len) return pfail(p, KMOE_E_INVALID, "append: a sequence ends at %lld positions", (long long)kMaxLen);
+      const int64_t want = (len + n[i] + p->page - 1) / p->page - held;
+      bool cow = n[i] > 0 && len % p->page && p->refs[s->pages.back()] > 1;
+      if (cow) {
+        int32_t &l = left[s->pages.back()];
+        cow = p->refs[s->pages.back()] - l > 1;
+        l += cow;
+      }
+      total += want + cow;
+      if (total > (int64_t)p->free.size())
+        return pfail(p, KMOE_E_BUDGET, "append: %lld pages wanted, %lld free", (long long)total, (long long)p->free.size());
+      if (!s) s = &begun[seqs[i]];
       s->pages.reserve(held + want);
-    } else {
-      Seq t;
-      t.pages.reserve(want);
-      s = &(p->seqs[seq] = std::move(t));
+      parts[i] = Part{s, len, want, cow};
     }
-    if (cow) {
-      const int32_t old = s->pages.back(), id = p->take();
-      --p->refs[old];
-      s->pages.back() = id;
-      *src = old;
-      *dst = id;
-      *copies = 1;
+    // (from here on nothing fails)
+    int32_t m = 0;
+    for (int32_t i = 0; i < count; ++i) {
+      const Part &t = parts[i];
+      if (t.cow) {
+        const int32_t old = t.s->pages.back(), id = p->take();
+        --p->refs[old];
+        t.s->pages.back() = id;
+        src[m] = old;
+        dst[m++] = id;
+      }
+      for (int64_t k = 0; k < t.want; ++k) t.s->pages.push_back(p->take());
+      t.s->len = t.len + n[i];
     }
-    for (int64_t i = 0; i < want; ++i) s->pages.push_back(p->take());
-    s->len = len + n;
+    p->seqs.merge(begun);
+    *copies = m;
     return KMOE_OK;
   });
+}
+
+int kmoe_pages_append(kmoe_pages *p, uint32_t seq, int64_t n, int32_t *src, int32_t *dst, int32_t *copies) {
+  return kmoe_pages_append_many(p, &seq, &n, 1, src, dst, copies);
 }
 
 int kmoe_pages_fork(kmoe_pages *p, uint32_t from, uint32_t to, int64_t n) {

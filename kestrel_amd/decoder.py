@@ -391,18 +391,7 @@ class PagedDecoder(Decoder):
                 had[s] = None
             if (had[s] or 0) + n > self.n_ctx:
                 raise ValueError(f"context full: sequence {s} needs {(had[s] or 0) + n}, n_ctx {self.n_ctx}")
-        copies, done = [], {}
-        try:
-            for s, n in want.items():
-                c = self.account.append(s, n)
-                done[s] = had[s]
-                if c:
-                    copies.append(c)
-        except KmoeError:
-            self._copy(copies)  # (a page of one's own stays, and has to hold what the shared one does)
-            self._back(done)
-            raise
-        self._copy(copies)
+        self._copy(self.account.append_many(want))
         return had
 
     def _back(self, had: dict):

@@ -115,6 +115,7 @@ SIGNATURES = {
     "kmoe_pages_destroy": (C.c_int, [_P]),
     "kmoe_pages_last_error": (C.c_char_p, [_P]),
     "kmoe_pages_append": (C.c_int, [_P, _u32, _i64, C.POINTER(_i32), C.POINTER(_i32), C.POINTER(_i32)]),
+    "kmoe_pages_append_many": (C.c_int, [_P, _P, _P, _i32, _P, _P, C.POINTER(_i32)]),
     "kmoe_pages_fork": (C.c_int, [_P, _u32, _u32, _i64]),
     "kmoe_pages_truncate": (C.c_int, [_P, _u32, _i64]),
     "kmoe_pages_trim": (C.c_int, [_P, _u32, _i64, _i64, C.POINTER(_i64)]),
@@ -763,6 +764,15 @@ class Pages:
         s, d, c = _i32(), _i32(), _i32()
         self.check(self.lib.kmoe_pages_append(self.h, self._seq(seq), n, C.byref(s), C.byref(d), C.byref(c)))
         return (s.value, d.value) if c.value else None
+
+    def append_many(self, want: dict):
+        """append for several sequences {sequence: n}, all of them or none; the (src, dst) pages to copy."""
+        ids = np.array([self._seq(s) for s in want], np.uint32)
+        n = np.array(list(want.values()), np.int64)
+        s, d, k = np.empty(ids.size, np.int32), np.empty(ids.size, np.int32), _i32()
+        self.check(self.lib.kmoe_pages_append_many(self.h, ids.ctypes.data, n.ctypes.data, ids.size, s.ctypes.data,
+                                                   d.ctypes.data, C.byref(k)))
+        return list(zip(s[:k.value].tolist(), d[:k.value].tolist()))
 
     def fork(self, src: int, dst: int, n: int):
         """A new sequence dst of the first n positions of src, on the same pages."""
