@@ -484,11 +484,12 @@ class PagedDecoder(Decoder):
                     if len(last) < len(x):
                         x, f = (self.ctx.get_rows(F32, y, len(y), self.d, last) for y in (x, f))
                     logits.append(self._logits(x, f))
+            logits = logits[0] if len(logits) == 1 else self.torch.cat(logits)
         except BaseException:
             self._back(had)
             raise
         self._trim(rows)
-        return logits[0] if len(logits) == 1 else self.torch.cat(logits)
+        return logits
 
     # ------------------------------------------------------ greedy decode
     def _decode_rows(self, b):
