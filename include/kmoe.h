@@ -579,6 +579,9 @@ int kmoe_pages_copy(kmoe_ctx *ctx, const kmoe_paged_desc *desc, void *pages_dev,
  * to the kernels as kmoe_pages_table writes them. */
 typedef struct kmoe_pages kmoe_pages;
 int kmoe_pages_create(int64_t n_pages, int32_t page, kmoe_pages **out);
+/* An account of its own with the same sequences on the same pages: to find out
+ * whether a run of calls will succeed before making them. */
+int kmoe_pages_clone(const kmoe_pages *p, kmoe_pages **out);
 int kmoe_pages_destroy(kmoe_pages *p);
 const char *kmoe_pages_last_error(const kmoe_pages *p);
 /* n more positions for seq (begun where it does not exist), 2^30 at most

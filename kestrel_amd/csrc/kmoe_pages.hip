@@ -115,6 +115,24 @@ int kmoe_pages_create(int64_t n_pages, int32_t page, kmoe_pages **out) {
   return KMOE_OK;
 }
 
+int kmoe_pages_clone(const kmoe_pages *p, kmoe_pages **out) {
+  if (!out) return KMOE_E_INVALID;
+  *out = nullptr;
+  if (!p) return KMOE_E_INVALID;
+  kmoe_pages *q = nullptr;
+  const int rc = guarded(nullptr, [&]() {
+    q = new kmoe_pages(*p);
+    q->free.reserve(q->n);
+    return (int)KMOE_OK;
+  });
+  if (rc) {
+    delete q;
+    return rc;
+  }
+  *out = q;
+  return KMOE_OK;
+}
+
 int kmoe_pages_destroy(kmoe_pages *p) {
   delete p;
   return KMOE_OK;

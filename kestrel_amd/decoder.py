@@ -28,7 +28,7 @@ from __future__ import annotations
 
 import numpy as np
 
-from .kmoe import BLOCK, F16, F32, Q8_0, Context, KmoeError, PagedKV, Pages, bytes_for
+from .kmoe import BLOCK, F16, F32, Q8_0, STATUS, Context, KmoeError, PagedKV, Pages, bytes_for
 
 
 def _nbytes(t: int, dims) -> int:
@@ -326,9 +326,12 @@ class PagedDecoder(Decoder):
     prompts and single tokens together. Sequences are numbered by the caller and
     begin with their first tokens; forks share pages until one of them writes.
     With a window a row sees the last `window` positions and the first n_sink,
-    and pages that no later row sees are free again after a call. head_dim 64 or
-    128; a sequence has at most hp["n_ctx"] positions, a call at most 4096
-    sequences, and hp["n_batch"] rows at a time go through the layers."""
+    and pages that no later row sees are free again after a call, or during it
+    where its new positions find no pages all at once: then each part of it
+    (hp["n_batch"] rows of forward, as many greedy steps as a page has positions)
+    takes its pages before it runs. head_dim 64 or 128; a sequence has at most
+    hp["n_ctx"] positions, a call at most 4096 sequences, and hp["n_batch"] rows at
+    a time of a forward call go through the layers."""
 
     def __init__(self, ctx: Context, hp: dict, tensors: dict, n_pages: int, page: int = 64, kv_type: int = F16,
                  window: int = 0, n_sink: int = 0, layer_base: int = 1000):
@@ -379,8 +382,9 @@ class PagedDecoder(Decoder):
         if pairs:
             self.ctx.pages_copy(self.kv, self.pages, [s for s, _ in pairs], [d for _, d in pairs], self.n_layer)
 
-    def _reserve(self, want: dict) -> dict:
-        """Positions for new tokens, all of them or none; returns the lengths before (None: a new sequence)."""
+    def _reserve(self, want: dict, steps=()):
+        """Positions for new tokens {sequence: n}, all of them or none: the lengths before (None: a new sequence),
+        and whether the call's steps {sequence: n} have to take theirs one by one, as a window's pages become free."""
         if not want or len(want) > 4096:
             raise ValueError(f"{len(want)} sequences: a call takes 1 to 4096")
         had = {}
@@ -391,20 +395,36 @@ class PagedDecoder(Decoder):
                 had[s] = None
             if (had[s] or 0) + n > self.n_ctx:
                 raise ValueError(f"context full: sequence {s} needs {(had[s] or 0) + n}, n_ctx {self.n_ctx}")
+        try:
+            self._append(want)
+            return had, False
+        except KmoeError as e:
+            if STATUS.get(e.status) != "BUDGET" or not self.window or len(steps) < 2:
+                raise
+        trial = self.account.clone()  # (fails here, or not at all)
+        try:
+            for step in steps:
+                trial.append_many(step)
+                self._trim(step, had, trial)
+        finally:
+            trial.close()
+        return had, True
+
+    def _append(self, want: dict):
         self._copy(self.account.append_many(want))
-        return had
 
     def _back(self, had: dict):
         for s, n in had.items():
-            if n is None:
-                self.account.drop(s)
-            else:
+            if n is not None:
                 self.account.truncate(s, n)
+            elif self.length(s):
+                self.account.drop(s)
 
-    def _trim(self, seqs):
+    def _trim(self, seqs, had=None, account=None):
+        """Gives up what no later row sees; with `had` not yet what the sequences need at those lengths."""
         if self.window:
             for s in seqs:
-                self.account.trim(s, self.window, self.n_sink)
+                (account or self.account).trim(s, self.window, max(self.n_sink, had[s] or 0) if had else self.n_sink)
 
     # -------------------------------------------------------------- steps
     def _paged_layer(self, L, pages, batch, x, f_prev):
@@ -452,6 +472,20 @@ class PagedDecoder(Decoder):
         rs = None if max(counts) == 1 else d[n:2 * n + 1]
         return self.ctx.paged_batch(d[2 * n + 1:].view(n, cols), d[:n], rs, int(starts[-1]))
 
+    def _parts(self, rows: dict):
+        """The rows in parts of n_batch: lists of (sequence, first token, end), a sequence at most once in each."""
+        parts, part, room = [], [], self.n_batch
+        for s, ts in rows.items():
+            i = 0
+            while i < len(ts):
+                m = min(room, len(ts) - i)
+                part.append((s, i, i + m))
+                i, room = i + m, room - m
+                if not room:
+                    parts.append(part)
+                    part, room = [], self.n_batch
+        return parts + [part] if part else parts
+
     def forward(self, rows: dict):
         """Feeds rows {sequence: its next tokens}; returns the logits of each one's last token [len(rows), n_vocab],
         in the order of rows. A call that fails leaves the sequences as they were."""
@@ -459,22 +493,13 @@ class PagedDecoder(Decoder):
         for s, ts in rows.items():
             if not ts or min(ts) < 0 or max(ts) >= self.n_vocab:
                 raise ValueError(f"sequence {s}: need at least one token, each below {self.n_vocab}")
-        had = self._reserve({s: len(ts) for s, ts in rows.items()})
+        parts = self._parts(rows)
+        had, by_parts = self._reserve({s: len(ts) for s, ts in rows.items()}, [{s: j - i for s, i, j in p} for p in parts])
         try:
-            pieces = [(s, i, min(i + self.n_batch, len(ts))) for s, ts in rows.items()
-                      for i in range(0, len(ts), self.n_batch)]
             logits = []
-            while pieces:
-                part, room = [], self.n_batch
-                while pieces and room:
-                    s, i, j = pieces.pop(0)
-                    m = min(room, j - i)
-                    if i + m < j:
-                        pieces.insert(0, (s, i + m, j))
-                    part.append((s, i, i + m))
-                    room -= m
-                    if len(part) > 1 and part[-2][0] == s:  # (two pieces of one sequence are one)
-                        part[-2:] = [(s, part[-2][1], i + m)]
+            for part in parts:
+                if by_parts:
+                    self._append({s: j - i for s, i, j in part})
                 ty, dims, t = self.embed
                 x = self.ctx.get_rows(ty, t, dims[1], dims[0], [tk for s, i, j in part for tk in rows[s][i:j]])
                 counts = [j - i for _, i, j in part]
@@ -484,6 +509,8 @@ class PagedDecoder(Decoder):
                     if len(last) < len(x):
                         x, f = (self.ctx.get_rows(F32, y, len(y), self.d, last) for y in (x, f))
                     logits.append(self._logits(x, f))
+                if by_parts:
+                    self._trim([s for s, _, _ in part], had)
             logits = logits[0] if len(logits) == 1 else self.torch.cat(logits)
         except BaseException:
             self._back(had)
@@ -508,8 +535,12 @@ class PagedDecoder(Decoder):
             raise ValueError("n: at least one step")
         if any(not 0 <= int(t) < self.n_vocab for t in first.values()):
             raise ValueError(f"a token is not below {self.n_vocab}")
-        had = self._reserve({s: n for s in seqs})
+        page = self.kv.page
+        blocks = [min(page, n - i) for i in range(0, n, page)]
+        had, by_blocks = self._reserve({s: n for s in seqs}, [{s: m for s in seqs} for m in blocks])
         try:
+            if by_blocks:
+                self._append({s: blocks[0] for s in seqs})
             b = self._graph_bufs
             if b is None or self._graph_n != len(seqs):
                 i32 = dict(dtype=torch.int32, device=self.dev)
@@ -539,6 +570,10 @@ class PagedDecoder(Decoder):
                 self.graph, self._graph_key = g, self._key()
                 torch.cuda.synchronize()
             for i in range(n):
+                if by_blocks and i and i % page == 0:
+                    self._trim(seqs, had)
+                    self._append({s: blocks[i // page] for s in seqs})
+                    b["table"].copy_(torch.from_numpy(self.account.table(seqs, self.cols)[0]))
                 if use_graph:
                     self.graph.replay()
                 else:

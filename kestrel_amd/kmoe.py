@@ -112,6 +112,7 @@ SIGNATURES = {
     "kmoe_paged_attention": (C.c_int, [_P, _P, _P, _P, _P, _i32, _i64, _i64, _P]),
     "kmoe_pages_copy": (C.c_int, [_P, _P, _P, _i64, _i64, _P, _P, _i64]),
     "kmoe_pages_create": (C.c_int, [_i64, _i32, C.POINTER(_P)]),
+    "kmoe_pages_clone": (C.c_int, [_P, C.POINTER(_P)]),
     "kmoe_pages_destroy": (C.c_int, [_P]),
     "kmoe_pages_last_error": (C.c_char_p, [_P]),
     "kmoe_pages_append": (C.c_int, [_P, _u32, _i64, C.POINTER(_i32), C.POINTER(_i32), C.POINTER(_i32)]),
@@ -737,6 +738,16 @@ class Pages:
         if rc != 0:
             raise KmoeError(rc, "kmoe_pages_create failed")
         self.h, self.page, self.n_pages = h, page, n_pages
+
+    def clone(self) -> "Pages":
+        """An account of its own with the same sequences on the same pages."""
+        h = _P()
+        rc = self.lib.kmoe_pages_clone(self.h, C.byref(h))
+        if rc != 0:
+            raise KmoeError(rc, "kmoe_pages_clone failed")
+        c = Pages.__new__(Pages)
+        c.lib, c.h, c.page, c.n_pages = self.lib, h, self.page, self.n_pages
+        return c
 
     def close(self):
         if getattr(self, "h", None):

@@ -113,3 +113,68 @@ def test_refusals():
         assert p.lib.kmoe_pages_append_many(p.h, *args) == INVALID
     assert p.lib.kmoe_pages_append_many(None, ids, n, 1, out, out, C.byref(k)) == INVALID
     assert p.length(1) == 40 and p.usage() == (2, 4)
+
+
+def test_a_clone_goes_its_own_way():
+    p = kmoe.Pages(6, 32)
+    p.append(1, 40)
+    p.fork(1, 2, 40)
+    q = p.clone()
+    assert q.append(1, 1) is not None and q.append(3, 96) is None and q.usage() == (6, 6)
+    q.drop(2)
+    assert p.usage() == (2, 6) and [p.length(s) for s in (1, 2)] == [40, 40]
+    p.append(1, 1)
+    p.drop(1)
+    p.drop(2)
+    assert p.usage() == (0, 6) and q.length(1) == 41 and q.usage()[0] == 5
+    q.close()
+    p.append(9, 6 * 32)
+    assert p.lib.kmoe_pages_clone(None, C.byref(C.c_void_p())) == INVALID and p.lib.kmoe_pages_clone(p.h, None) == INVALID
+
+
+@pytest.mark.parametrize("window,sink,had", [(40, 0, 0), (40, 5, 70), (1, 0, 33), (100, 40, 64)])
+def test_a_window_serves_more_positions_than_pages(window, sink, had):
+    """By steps where the pages are too few for all at once; every step's rows find what they see, and so does the
+    sequence's old end until the call is over."""
+    page = 32
+    want = 12 * page
+    steps = [{0: 16}] * (want // 16)
+    need = -(-window // page) + 1 + -(-sink // page) + (-(-window // page) + 1 if had else 0) + 1
+    dec = _decoder(need, page)
+    dec.window, dec.n_sink = window, sink
+    if had:
+        dec._reserve({0: had})
+        dec._trim([0])
+    used = dec.account.usage()
+    got, by_steps = dec._reserve({0: want}, steps)
+    assert by_steps and got == {0: had or None} and dec.account.usage() == used
+    n = had
+    for step in steps:
+        dec._append(step)
+        (row,), _ = dec.account.table([0], 64)
+        for pos in range(n, n + 16):
+            for p in range(pos + 1):
+                assert not (p > pos - window or p < sink) or row[p // page] >= 0
+        n += 16
+        dec._trim([0], got)
+    if had:
+        dec._back(got)
+        (row,), _ = dec.account.table([0], 64)
+        assert dec.length(0) == had and all(row[p // page] >= 0 for p in range(had) if p > had - window or p < sink)
+    else:
+        dec._back(got)
+        assert dec.account.usage() == (0, need)
+
+
+def test_a_window_that_does_not_fit_keeps_nothing():
+    dec = _decoder(3, 32)
+    dec.window = 100
+    dec._reserve({0: 50})
+    for steps in ([{0: 16}] * 20, [{0: 320}], []):
+        with pytest.raises(kmoe.KmoeError) as e:
+            dec._reserve({0: 320}, steps)
+        assert e.value.status == BUDGET and dec.account.usage() == (2, 3) and dec.length(0) == 50
+    dec.window = 0
+    with pytest.raises(kmoe.KmoeError):
+        dec._reserve({0: 320}, [{0: 16}] * 20)
+    assert dec.account.usage() == (2, 3)
