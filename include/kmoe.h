@@ -557,8 +557,10 @@ int kmoe_paged_kv_read(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *p
  * MB, counted against the VRAM budget; KMOE_E_BUDGET where the first call finds no
  * room). It is allocated once, also inside a capture, and never moves, so graphs
  * stay valid; calls on several streams of one context are ordered by the library,
- * but replays of graphs that hold such calls of one context must not overlap with
- * each other or with a call. */
+ * also those on several streams of one capture (not a call outside a capture after
+ * the stream of the last one has begun a capture: nothing can wait for what it did
+ * before). But replays of graphs that hold such calls of one context must not overlap
+ * with each other or with a call. */
 int kmoe_paged_attention(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *pages_dev,
                          const kmoe_paged_batch *batch, const float *q_dev, int32_t n_head, int64_t window,
                          int64_t n_sink, float *out_dev);

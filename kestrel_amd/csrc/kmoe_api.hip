@@ -219,6 +219,9 @@ struct kmoe_ctx {
   bool gws_used = false, gws_wait = false;
   hipStream_t gws_stream = nullptr;  // of the last use outside a capture
   hipEvent_t gws_event = nullptr;
+  unsigned long long gws_cap = 0;  // the last capture that used them, on that stream
+  hipStream_t gws_cap_stream = nullptr;
+  hipEvent_t gws_cap_event = nullptr;
   // last moe_ffn routing (pointers into ws) and its sizes
   uint32_t *last_idx = nullptr, *last_perm = nullptr, *last_off = nullptr;
   float *last_w = nullptr;
@@ -675,7 +678,8 @@ uint8_t *pieces(kmoe_ctx *c, size_t need) {
 
 // The paged attention's partials: allocated once (in a capture too) and never
 // moved, so graphs that hold them stay valid. A call on another stream than the
-// last one waits for that one's use, as with the pieces.
+// last one waits for that one's use, as with the pieces, and so does one on another
+// stream of the same capture (the graph's nodes follow each other then).
 int paged_ws(kmoe_ctx *c, float **p) {
   const bool cap = capturing(c->stream);
   if (!c->gws) {
@@ -688,7 +692,19 @@ int paged_ws(kmoe_ctx *c, float **p) {
     c->gws = (float *)d;
   }
   *p = c->gws;
-  if (cap) return KMOE_OK;
+  if (cap) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    HIP_OK(c, hipStreamGetCaptureInfo(c->stream, &st, &id));
+    if (id == c->gws_cap && c->stream != c->gws_cap_stream) {
+      if (!c->gws_cap_event) HIP_OK(c, hipEventCreateWithFlags(&c->gws_cap_event, hipEventDisableTiming));
+      HIP_OK(c, hipEventRecord(c->gws_cap_event, c->gws_cap_stream));
+      HIP_OK(c, hipStreamWaitEvent(c->stream, c->gws_cap_event, 0));
+    }
+    c->gws_cap = id;
+    c->gws_cap_stream = c->stream;
+    return KMOE_OK;
+  }
   if (c->gws_wait) HIP_OK(c, hipStreamWaitEvent(c->stream, c->gws_event, 0));
   c->gws_wait = false;
   c->gws_used = true;
@@ -877,6 +893,7 @@ int kmoe_destroy(kmoe_ctx *c) {
   if (c->pws_event) (void)hipEventDestroy(c->pws_event);
   if (c->gws) (void)hipFree(c->gws);
   if (c->gws_event) (void)hipEventDestroy(c->gws_event);
+  if (c->gws_cap_event) (void)hipEventDestroy(c->gws_cap_event);
   if (c->counters) (void)hipFree(c->counters);
   if (c->own) (void)hipStreamDestroy(c->own);
   delete c;
