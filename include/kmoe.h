@@ -547,12 +547,12 @@ int kmoe_paged_kv_read(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *p
  * nothing gives zeros. Sums and softmax statistics are f32; a row's last bits
  * depend on the batch it is in (how the positions are shared out), a call's on
  * nothing else. n_head / n_kv <= 16 heads per kv head. The matrix cores take q,
- * the weights and Q8_0 values as two f16 pieces each: F16 pages as f32 arithmetic,
- * Q8_0 pages with weights off by up to 2^-36 of a row's largest and q's elements by
- * 2^-40 of its largest. Rows whose result is not finite, or whose scores are all
- * -inf, are formed again in plain f32, so that an infinity or NaN at a position
- * reaches the rows that see it only (slower; so are Q8_0 rows that see a value
- * past f16's range).
+ * the weights and Q8_0 values as two f16 pieces each, as f32 arithmetic does (a
+ * weight is off by up to 2^-48 of the row's largest besides 2^-23 of itself, an
+ * element of q by 2^-52 of its row's largest). Rows whose result is not finite, or
+ * whose scores are all -inf, are formed again in plain f32, so that an infinity or
+ * NaN at a position reaches the rows that see it only (slower; so are Q8_0 rows
+ * that see a value past f16's range).
  * Work-groups that share a row join their sums in a workspace of the context (17
  * MB, counted against the VRAM budget; KMOE_E_BUDGET where the first call finds no
  * room). It is allocated once, also inside a capture, and never moves, so graphs

@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           uint32_t u, w;
-          split2(ldexpf(y[t][e >> 1][2 * (e & 1)], sh), ldexpf(y[t][e >> 1][2 * (e & 1) + 1], sh), 1.0f, lo_up(T), u, w);
+          split2(ldexpf(y[t][e >> 1][2 * (e & 1)], sh), ldexpf(y[t][e >> 1][2 * (e & 1) + 1], sh), 1.0f, kLoUp, u, w);
           hi[e] = u;
           lo[e] = w;
         }
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
 #pragma unroll
           for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) S[j][s][i] = fmaf(lo[j][s][i], 1.0f / lo_up(T), hi[j][s][i]);
+            for (int i = 0; i < 4; ++i) S[j][s][i] = fmaf(lo[j][s][i], 1.0f / kLoUp, hi[j][s][i]);
       } else {
 #pragma unroll
         for (int j = 0; j < C; ++j) S[j][0] = S[j][1] = f32x4{0};
@@ -296,9 +296,10 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             const h8 k = i8_h8(here(fr.k[s][t >> 1][2 * (t & 1)]), here(fr.k[s][t >> 1][2 * (t & 1) + 1]));
+            const h8 kl = k * (_Float16)(1.0f / kLoUp);  // (exact: whole numbers up to 127)
 #pragma unroll
             for (int j = 0; j < C; ++j) {
-              f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, x[t & 1][j][1], f32x4{0}, 0, 0, 0);
+              f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, x[t & 1][j][1], f32x4{0}, 0, 0, 0);
               y = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, x[t & 1][j][0], y, 0, 0, 0);
 #pragma unroll
               for (int i = 0; i < 4; ++i) S[j][s][i] = fmaf(y[i], half_of(fr.ks[s][t >> 1], 4 * (t & 1) + i), S[j][s][i]);
@@ -359,7 +360,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           uint32_t x, z;
-          split2(e8[2 * i], e8[2 * i + 1], kUp, lo_up(T), x, z);
+          split2(e8[2 * i], e8[2 * i + 1], kUp, kLoUp, x, z);
           ph[j][i] = x;
           pl[j][i] = z;
         }
@@ -388,7 +389,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
 #pragma unroll
             for (int j = 0; j < C; ++j)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) O[j][u0 + u][i] = fmaf(t[u][j][i], 1.0f / lo_up(T), O[j][u0 + u][i]);
+              for (int i = 0; i < 4; ++i) O[j][u0 + u][i] = fmaf(t[u][j][i], 1.0f / kLoUp, O[j][u0 + u][i]);
         }
       } else {
 #pragma unroll
@@ -401,10 +402,15 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
             O[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, __builtin_bit_cast(h8, ph[j]), O[j][u], 0, 0, 0);
 #pragma unroll
           for (int j = 0; j < C; ++j)
-            O[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, __builtin_bit_cast(h8, pl[j]), O[j][u], 0, 0, 0);
+            O[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, __builtin_bit_cast(h8, ph[j]), O[j][u], 0, 0, 0);
+          f32x4 t[C];
 #pragma unroll
           for (int j = 0; j < C; ++j)
-            O[j][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, __builtin_bit_cast(h8, ph[j]), O[j][u], 0, 0, 0);
+            t[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, __builtin_bit_cast(h8, pl[j]), f32x4{0}, 0, 0, 0);
+#pragma unroll
+          for (int j = 0; j < C; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) O[j][u][i] = fmaf(t[j][i], 1.0f / kLoUp, O[j][u][i]);
           if (u & 1) __builtin_amdgcn_sched_barrier(0);
         }
       }
