@@ -461,12 +461,22 @@ class Context:
                                                  n_head, window, n_sink, _ptr(out)))
         return out
 
+    @staticmethod
+    def _page_ids(x):
+        try:
+            if isinstance(x, (list, tuple)):  # (numpy takes no whole number past 32 bits from these)
+                return np.array(x, np.int32, ndmin=1)
+            wide = np.array(x, ndmin=1)
+            ids = wide.astype(np.int32)
+            if not (ids != wide).any():
+                return ids
+        except OverflowError:
+            pass
+        raise ValueError("a page number is no 32-bit integer")
+
     def pages_copy(self, kv: PagedKV, pages, src, dst, n_layer: int = 1):
         """Pages src[i] onto dst[i] (host sequences) in each of the n_layer equal parts of pages."""
-        given = [np.array(x, ndmin=1) for x in (src, dst)]
-        s, d = (x.astype(np.int32) for x in given)
-        if (s != given[0]).any() or (d != given[1]).any():
-            raise ValueError("a page number is no 32-bit integer")
+        s, d = self._page_ids(src), self._page_ids(dst)
         if s.size != d.size:
             raise ValueError(f"{s.size} source pages, {d.size} destinations")
         if n_layer < 1 or (n_layer > 1 and pages.nbytes % (n_layer * kv.page_bytes)):
