@@ -91,7 +91,7 @@ constexpr int kQHeads = 8, kQRows = 8;  // of a work-group that rotates q
 // piece to eight, and is stored whole where the call has all of them). Behind them,
 // work-groups of kQHeads heads by kQRows rows rotate q. A thread's values are all on
 // their way before the angles are formed; sincosf of a row's angles is what costs
-// most. 1777 rows, 16 heads over 4, Q8_0: 13 us for 38 MB (a work-group of all 32
+// most. 1777 rows, 16 heads over 4, Q8_0: 12 us for 38 MB (a work-group of all 32
 // rows and 2 heads of q: 17); a copy of as many bytes takes 7.
 template <int T, int HD>
 __global__ void __launch_bounds__(256) k_paged_store(PagedArgs a, const float *__restrict__ q, int64_t q_stride,

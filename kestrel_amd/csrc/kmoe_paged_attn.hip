@@ -5,7 +5,7 @@
 // positions, heads of 128 unless said): one row per sequence reads every K and V
 // once for all heads of a group, 64 rows at 100 .. 8192 positions 88 us = 5.6 TB/s
 // of pages, one row at 131000 positions (8 kv heads) 95 us; with Q8_0 pages (half
-// the bytes) the vector units, which make f16 of the quants: 64 us for 286 MB.
+// the bytes) the vector units, which make f16 of the quants: 65 us for 286 MB.
 // Prompts are bound by the vector and matrix units together, which overlap little
 // with two waves a SIMD (4096 rows, 32 heads over 8: 375 us, 730 Tflop/s of f16
 // products, at 2.05 GHz; a wave's next scores beside its own softmax, in whatever
@@ -24,7 +24,7 @@ namespace {
 // 16 bytes per lane, each line whole by one load. ONCE: by one work-group only, past
 // the caches' order of use (decode steps, 64 rows at 2000 positions 100 -> 90 us).
 // Column tiles of many rows read the same pages (with it two chunks of 512 rows and
-// seven single rows, Q8_0, 250 -> 281 us; 4096 rows 382 -> 405).
+// seven single rows, Q8_0, 272 -> 303 us; 4096 rows 359 -> 385).
 template <bool ONCE>
 __device__ __forceinline__ u32x4 load16(const uint8_t *p) {
   if constexpr (ONCE) return __builtin_nontemporal_load((const u32x4 *)p);
@@ -96,8 +96,8 @@ struct Frags<kPgQ8, HD, ONCE> {
 constexpr int paged_occ(int hd, int c) { return hd == 64 ? (c == 1 ? 4 : 3) : (c == 1 ? 3 : 2); }
 
 // (A unit of decode steps counts 8 tiles besides its own, 12 where they are half as
-// large: 200 rows of heads of 64, Q8_0, 8 tiles 54 us, 12 52, 16 52; 200 rows of heads
-// of 128, F16, 81, 83, 86.)
+// large: 200 rows of heads of 64, Q8_0, 8 tiles 55.6 us, 12 54.4, 16 55.5; 200 rows of
+// heads of 128, F16, 81, 83, 86.)
 template <int HD, int COLS>
 using Work = Shares<COLS, 4, (HD == 64 && COLS == 16 ? 12 : 8), 8, 24>;
 
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
       const uint8_t *p_next = more ? block(exists(id_next) ? id_next : 0) : nullptr;
       const int lq = here(lane);  // (q's pieces are read at each tile)
       // (Q8_0: the wave at its products goes first, the others have the quants and
-      // the softmax to do: 4096 rows 470 -> 458 us; with F16 pages the same)
+      // the softmax to do: 4096 rows 560 -> 546 us; with F16 pages the same)
       if constexpr (T == kPgQ8) __builtin_amdgcn_s_setprio(1);
       // scores, in q's scale
       f32x4 S[C][2];
