@@ -548,7 +548,7 @@ int kmoe_paged_kv_read(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *p
  * depend on the batch it is in (how the positions are shared out), a call's on
  * nothing else. n_head / n_kv <= 16 heads per kv head. The matrix cores take q,
  * the weights and Q8_0 values as two f16 pieces each, as f32 arithmetic does (a
- * weight is off by up to 2^-48 of the row's largest besides 2^-23 of itself, an
+ * weight is off by up to 2^-47 of the row's largest besides 2^-23 of itself, an
  * element of q by 2^-52 of its row's largest). Rows whose result is not finite, or
  * whose scores are all -inf, are formed again in plain f32, so that an infinity or
  * NaN at a position reaches the rows that see it only (slower; so are Q8_0 rows

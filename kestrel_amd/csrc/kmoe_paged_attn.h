@@ -164,13 +164,14 @@ __device__ __forceinline__ void split2(float a, float b, float up, float lo_up, 
   lo = __builtin_bit_cast(uint32_t, (h2){(_Float16)fmaf((float)h.x, -lo_up, a * (up * lo_up)),
                                          (_Float16)fmaf((float)h.y, -lo_up, b * (up * lo_up))});
 }
-// lo_up of q and of the weights: errors beside 2^-23 of 2^-48 of the largest weight (1)
-// and 2^-52 of q's largest element. The products of the weights' lo have a sum of
-// their own, joined tile by tile; q's lo has too on F16 pages, and on Q8_0 pages is
-// multiplied by the quants / lo_up, exact in f16. (One sum for hi and an unscaled lo:
-// 2^-36 and 2^-40, so that beside a first position with a zero value that takes all but
-// e^-20 of the weight the others have seven bits. It took two chunks of 512 rows and seven
-// single rows, Q8_0, 249 -> 234 us, 4096 rows, F16, 408 -> 385.)
+// lo_up of q and of the weights: errors beside 2^-23 of 2^-48 of the largest weight (1;
+// Q8_0: 2^-47, the product of what both first pieces leave) and 2^-52 of q's largest
+// element. The products of the weights' lo have a sum of their own, joined tile by
+// tile; q's lo has too on F16 pages, and on Q8_0 pages is multiplied by the quants /
+// lo_up, exact in f16. (One sum for hi and an unscaled lo: 2^-36 and 2^-40, so that
+// beside a first position with a zero value that takes all but e^-20 of the weight the
+// others have seven bits. It took two chunks of 512 rows and seven single rows, Q8_0,
+// 249 -> 234 us, 4096 rows, F16, 408 -> 385.)
 constexpr float kLoUp = 0x1p12f;
 
 // Largest of the four lanes l, l ^ 16, l ^ 32, l ^ 48 (a column's share of one

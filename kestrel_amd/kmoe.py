@@ -466,7 +466,7 @@ class Context:
         try:
             if isinstance(x, (list, tuple)):  # (numpy takes no whole number past 32 bits from these)
                 return np.array(x, np.int32, ndmin=1)
-            wide = np.array(x, ndmin=1)
+            wide = np.atleast_1d(np.asarray(x))
             ids = wide.astype(np.int32)
             if not (ids != wide).any():
                 return ids
