@@ -696,7 +696,7 @@ int paged_ws(kmoe_ctx *c, float **p) {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     unsigned long long id = 0;
     HIP_OK(c, hipStreamGetCaptureInfo(c->stream, &st, &id));
-    if (id == c->gws_cap && c->stream != c->gws_cap_stream) {
+    if (c->gws_cap_stream && id == c->gws_cap && c->stream != c->gws_cap_stream) {
       if (!c->gws_cap_event) HIP_OK(c, hipEventCreateWithFlags(&c->gws_cap_event, hipEventDisableTiming));
       HIP_OK(c, hipEventRecord(c->gws_cap_event, c->gws_cap_stream));
       HIP_OK(c, hipStreamWaitEvent(c->stream, c->gws_cap_event, 0));
