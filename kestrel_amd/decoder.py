@@ -396,11 +396,17 @@ class PagedDecoder(Decoder):
             if (had[s] or 0) + n > self.n_ctx:
                 raise ValueError(f"context full: sequence {s} needs {(had[s] or 0) + n}, n_ctx {self.n_ctx}")
         try:
-            self._append(want)
-            return had, False
+            copies = self.account.append_many(want)
         except KmoeError as e:
             if STATUS.get(e.status) != "BUDGET" or not self.window or len(steps) < 2:
                 raise
+        else:
+            try:
+                self._copy(copies)
+            except BaseException:
+                self._back(had)
+                raise
+            return had, False
         trial = self.account.clone()  # (fails here, or not at all)
         try:
             for step in steps:

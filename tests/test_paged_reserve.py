@@ -178,3 +178,21 @@ def test_a_window_that_does_not_fit_keeps_nothing():
     with pytest.raises(kmoe.KmoeError):
         dec._reserve({0: 320}, [{0: 16}] * 20)
     assert dec.account.usage() == (2, 3)
+
+
+@pytest.mark.parametrize("status", [-3, -4])
+def test_copies_that_fail_take_the_reservation_back(status):
+    """Whatever the copies fail with, the positions are not kept, nor taken twice."""
+    dec = _decoder(8, 32)
+    dec.window = 100
+    dec._reserve({0: 40})
+    dec.fork(0, 1)
+
+    def fails(pairs):
+        assert pairs
+        raise kmoe.KmoeError(status, "no")
+
+    dec._copy = fails
+    with pytest.raises(kmoe.KmoeError) as e:
+        dec._reserve({0: 50, 2: 33}, [{0: 25, 2: 16}, {0: 25, 2: 17}])
+    assert e.value.status == status and [dec.length(s) for s in range(3)] == [40, 40, 0]
