@@ -467,6 +467,38 @@ int kmoe_add_rows(kmoe_ctx *ctx, float *x_dev, const float *b_dev, int64_t rows,
  * *pos_dev += advance afterwards (the end of a graph-captured decode step). */
 int kmoe_argmax(kmoe_ctx *ctx, const float *logits_dev, int64_t n, uint32_t *out_dev, int32_t *pos_dev,
                 int32_t advance);
+/* The next token of each of s_rows rows of n logits (1 .. KMOE_SAMPLE_MAX), `stride`
+ * floats apart. (The reference samples on the host, sampler.rs:30-112, with random
+ * numbers of its own; the order of the steps here is this call's.) A row's weights are
+ * w_i = exp((l_i - max l) / T). In the order of descending logits, equal ones by
+ * index, the first top_k tokens are kept, of those the shortest beginning that holds
+ * top_p of their weight, of those the ones with w_i >= min_p (the largest is always
+ * kept). Drawn is the first kept token, by index, at which the running sum of w
+ * passes u times the sum over all kept. u [s_rows] are the caller's random numbers
+ * in [0, 1) (below 0 and NaN count as 0, from 1 on the last kept token is drawn). The
+ * settings are device arrays of a value per row, or NULL; they, too, are read when
+ * the kernels run, so that a captured call may be replayed with others:
+ *   temperature  NULL: 1; 0, negative or NaN: the first largest logit (greedy)
+ *   top_k        NULL, 0 or negative, n or more: all
+ *   top_p        NULL, NaN, 1 or more: all; 0 or less: the first largest
+ *   min_p        NULL, NaN, 0 or less: all; above 1 counts as 1
+ * A NaN logit counts as -inf; if all are, the token is 0 and its probability 0. With
+ * +inf logits only those are drawn. Weights are 64-bit floats, summed as multiples of
+ * 2^-43 (a token of less than half of that is not drawn), so a row's token does not
+ * depend on the other rows or on how the work is shared out. out [s_rows] receives the
+ * tokens, prob (may be NULL) the probabilities they were drawn with among the kept. When
+ * pos_dev [s_rows] is non-NULL, each is advanced by `advance` afterwards. out, prob and
+ * pos must not overlap each other or the inputs. */
+#define KMOE_SAMPLE_MAX 1048576
+typedef struct {
+  const float *temperature_dev;
+  const int32_t *top_k_dev;
+  const float *top_p_dev;
+  const float *min_p_dev;
+} kmoe_sampling;
+int kmoe_sample(kmoe_ctx *ctx, const float *logits_dev, int64_t s_rows, int64_t n, int64_t stride,
+                const kmoe_sampling *how, const float *u_dev, uint32_t *out_dev, float *prob_dev, int32_t *pos_dev,
+                int32_t advance);
 /* *pos_dev += by on the device (no counterpart: the position counter of
  * graph-captured steps). */
 int kmoe_pos_advance(kmoe_ctx *ctx, int32_t *pos_dev, int32_t by);

@@ -2507,12 +2507,47 @@ int kmoe_add_rows(kmoe_ctx *c, float *x, const float *b, int64_t rows, int64_t c
   return KMOE_OK;
 }
 
+constexpr int64_t kPagedMaxRows = (int64_t)1 << 22;  // (a work-group of 256 per row stays a valid grid)
+
+// Whether `bytes` from out on touch one of `rows` rows of `width` floats, `stride` floats apart, from in on.
+static bool overlaps(const void *out, int64_t bytes, const void *in, int64_t rows, int64_t width, int64_t stride) {
+  const __int128 rel = (__int128)(uintptr_t)out - (__int128)(uintptr_t)in, w = 4 * (__int128)width, st = 4 * (__int128)stride;
+  const __int128 i = rel < w ? 0 : (rel - w) / st + 1;  // the first row that ends behind out's first byte
+  return i < rows && i * st < rel + bytes;
+}
+
 int kmoe_argmax(kmoe_ctx *c, const float *logits, int64_t n, uint32_t *out, int32_t *pos_dev, int32_t advance) {
   if (!c) return KMOE_E_INVALID;
   if (n <= 0) return fail(c, KMOE_E_INVALID, "argmax of an empty vector");
   if (!logits || !out) return fail(c, KMOE_E_INVALID, "null pointer");
   DeviceGuard g(c->device);
   LAUNCH(c, "argmax", launch_argmax(c->stream, logits, n, out, pos_dev, advance));
+  return KMOE_OK;
+}
+
+int kmoe_sample(kmoe_ctx *c, const float *logits, int64_t s_rows, int64_t n, int64_t stride, const kmoe_sampling *how,
+                const float *u, uint32_t *out, float *prob, int32_t *pos, int32_t advance) {
+  if (!c) return KMOE_E_INVALID;
+  if (n <= 0 || n > KMOE_SAMPLE_MAX) return fail(c, KMOE_E_INVALID, "%lld logits a row (1 .. %d)", (long long)n, KMOE_SAMPLE_MAX);
+  if (s_rows < 0 || s_rows > kPagedMaxRows) return fail(c, KMOE_E_INVALID, "negative or too large size");
+  if (stride < n || stride > INT64_MAX / 8 / kPagedMaxRows)
+    return fail(c, KMOE_E_INVALID, "rows of %lld floats %lld apart", (long long)n, (long long)stride);
+  if (s_rows == 0) return KMOE_OK;
+  if (!logits || !u || !out) return fail(c, KMOE_E_INVALID, "null pointer");
+  const kmoe_sampling h = how ? *how : kmoe_sampling{};
+  const int64_t b = s_rows * 4;
+  void *const outs[] = {out, prob, pos};
+  const void *const ins[] = {u, h.temperature_dev, h.top_k_dev, h.top_p_dev, h.min_p_dev};
+  for (int i = 0; i < 3; ++i) {
+    if (!outs[i]) continue;
+    bool bad = overlaps(outs[i], b, logits, s_rows, n, stride);
+    for (const void *in : ins) bad = bad || (in && overlaps(outs[i], b, in, 1, s_rows, s_rows));
+    for (int j = 0; j < i; ++j) bad = bad || (outs[j] && overlaps(outs[i], b, outs[j], 1, s_rows, s_rows));
+    if (bad) return fail(c, KMOE_E_INVALID, "an output overlaps an input or another output");
+  }
+  DeviceGuard g(c->device);
+  const SampleArgs a{logits, s_rows, n, stride, u, h.temperature_dev, h.top_k_dev, h.top_p_dev, h.min_p_dev, out, prob, pos, advance};
+  LAUNCH(c, "sample", launch_sample(c->stream, a));
   return KMOE_OK;
 }
 
@@ -2534,8 +2569,6 @@ int kmoe_paged_page_bytes(const kmoe_paged_desc *d, uint64_t *bytes) {
   *bytes = (uint64_t)d->n_kv * (uint64_t)paged_block_bytes(d->type, d->page, d->head_dim);
   return KMOE_OK;
 }
-
-constexpr int64_t kPagedMaxRows = (int64_t)1 << 22;  // (a work-group of 256 per row stays a valid grid)
 
 static int check_paged_desc(kmoe_ctx *c, const kmoe_paged_desc *d) {
   if (!d) return fail(c, KMOE_E_INVALID, "null pointer");
@@ -2585,13 +2618,6 @@ int kmoe_paged_kv_store(kmoe_ctx *c, const kmoe_paged_desc *d, void *pages, cons
   LAUNCH(c, "paged_store",
          launch_paged_store(c->stream, a, nullptr, 0, k, k_stride, v, v_stride, 0, 0, nullptr, 0, nullptr));
   return KMOE_OK;
-}
-
-// Whether `bytes` from out on touch one of `rows` rows of `width` floats, `stride` floats apart, from in on.
-static bool overlaps(const void *out, int64_t bytes, const void *in, int64_t rows, int64_t width, int64_t stride) {
-  const __int128 rel = (__int128)(uintptr_t)out - (__int128)(uintptr_t)in, w = 4 * (__int128)width, st = 4 * (__int128)stride;
-  const __int128 i = rel < w ? 0 : (rel - w) / st + 1;  // the first row that ends behind out's first byte
-  return i < rows && i * st < rel + bytes;
 }
 
 int kmoe_paged_rope_kv_store(kmoe_ctx *c, const kmoe_paged_desc *d, void *pages, const kmoe_paged_batch *b,

@@ -105,6 +105,7 @@ SIGNATURES = {
     "kmoe_add_rows": (C.c_int, [_P, _P, _P, _i64, _i64]),
     "kmoe_argmax": (C.c_int, [_P, _P, _i64, _P, _P, _i32]),
     "kmoe_pos_advance": (C.c_int, [_P, _P, _i32]),
+    "kmoe_sample": (C.c_int, [_P, _P, _i64, _i64, _i64, _P, _P, _P, _P, _P, _i32]),
     "kmoe_paged_page_bytes": (C.c_int, [_P, C.POINTER(_u64)]),
     "kmoe_paged_kv_store": (C.c_int, [_P, _P, _P, _P, _P, _i64, _P, _i64]),
     "kmoe_paged_rope_kv_store": (C.c_int, [_P, _P, _P, _P, _P, _i64, _P, _i64, _P, _i64, _i32, _i32, _P, _i32, _P]),
@@ -145,6 +146,12 @@ class MoeDesc(C.Structure):
         ("up_type", _i32),
         ("down_type", _i32),
     ]
+
+
+class Sampling(C.Structure):
+    """kmoe_sampling (include/kmoe.h): device arrays of a value per row."""
+
+    _fields_ = [("temperature", _P), ("top_k", _P), ("top_p", _P), ("min_p", _P)]
 
 
 class PagedDesc(C.Structure):
@@ -498,6 +505,26 @@ class Context:
     def argmax(self, logits, out=None, pos_dev=None, advance: int = 0):
         out = self._empty((1,), self.torch.int32) if out is None else out
         self.check(self.lib.kmoe_argmax(self.h, _ptr(logits), logits.numel(), _ptr(out), _ptr(pos_dev), advance))
+        return out
+
+    def sample(self, logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out=None, prob=None, pos_dev=None,
+               advance: int = 0):
+        """kmoe_sample: the next token (int32 [S]) of each row of logits [S, n], drawn by u [S]. temperature, top_p,
+        min_p (f32) and top_k (int32): device tensors of a value per row, or None. prob [S] f32 receives the tokens'
+        probabilities."""
+        f, i32 = self.torch.float32, self.torch.int32
+        if logits.dim() != 2:
+            raise ValueError(f"logits: need [rows, tokens], got {list(logits.shape)}")
+        S, n = logits.shape
+        stride = self._need("logits", logits, f, S, n, True)
+        out = self._empty((S,), i32) if out is None else out
+        for name, t, dtype in (("u", u, f), ("temperature", temperature, f), ("top_k", top_k, i32), ("top_p", top_p, f),
+                               ("min_p", min_p, f), ("out", out, i32), ("prob", prob, f), ("pos_dev", pos_dev, i32)):
+            if t is not None:
+                self._need(name, t, dtype, 1, S)
+        how = Sampling(*[_ptr(t) or None for t in (temperature, top_k, top_p, min_p)])
+        self.check(self.lib.kmoe_sample(self.h, _ptr(logits), S, n, stride, C.byref(how), _ptr(u), _ptr(out),
+                                        _ptr(prob) or None, _ptr(pos_dev) or None, advance))
         return out
 
     def pos_advance(self, pos_dev, by: int = 1):
