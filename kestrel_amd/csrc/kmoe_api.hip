@@ -175,6 +175,17 @@ bool f16_down(int t, int64_t d, int64_t F, int64_t slots, int64_t max_active) {
 }
 constexpr int kFewRows = 3;   // decode batches over narrow rows: experts of 1..3 rows take launch_few_int
 
+// Scratch that never moves, so graphs that hold it stay valid, and the order of its uses.
+struct Kept {
+  uint8_t *p = nullptr;
+  bool used = false, wait = false;
+  hipStream_t stream = nullptr;  // of the last use outside a capture
+  hipEvent_t event = nullptr;
+  unsigned long long cap = 0;  // the last capture that used it, on that stream
+  hipStream_t cap_stream = nullptr;
+  hipEvent_t cap_event = nullptr;
+};
+
 struct kmoe_ctx {
   int device = 0;
   hipStream_t own = nullptr;
@@ -213,15 +224,9 @@ struct kmoe_ctx {
   hipStream_t pws_stream = nullptr;  // of the last use outside a capture
   hipEvent_t pws_event = nullptr;
   std::vector<void *> pws_retired;
-  // partials of the paged attention's split units: one size, allocated at the
-  // first call and kept
-  float *gws = nullptr;
-  bool gws_used = false, gws_wait = false;
-  hipStream_t gws_stream = nullptr;  // of the last use outside a capture
-  hipEvent_t gws_event = nullptr;
-  unsigned long long gws_cap = 0;  // the last capture that used them, on that stream
-  hipStream_t gws_cap_stream = nullptr;
-  hipEvent_t gws_cap_event = nullptr;
+  // scratch of one size each, allocated at the first call that takes it and kept:
+  // partials of the paged attention's split units, what sampling finds of the chunks
+  Kept paged, sample;
   // last moe_ffn routing (pointers into ws) and its sizes
   uint32_t *last_idx = nullptr, *last_perm = nullptr, *last_off = nullptr;
   float *last_w = nullptr;
@@ -676,57 +681,57 @@ uint8_t *pieces(kmoe_ctx *c, size_t need) {
   return c->pws;
 }
 
-// The paged attention's partials: allocated once (in a capture too) and never
-// moved, so graphs that hold them stay valid. A call on another stream than the
+// Scratch of `bytes` (the same at every call): allocated once (in a capture too) and never
+// moved, so graphs that hold it stay valid. A call on another stream than the
 // last one waits for that one's use, as with the pieces, and so does one on another
 // stream of the same capture (the graph's nodes follow each other then).
-int paged_ws(kmoe_ctx *c, float **p) {
+int kept_ws(kmoe_ctx *c, Kept &k, size_t bytes, const char *purpose, uint8_t **p) {
   const bool cap = capturing(c->stream);
-  if (!c->gws) {
+  if (!k.p) {
     void *d = nullptr;
     hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
     if (cap) (void)hipThreadExchangeStreamCaptureMode(&mode);
-    const int rc = dev_alloc(c, paged_part_floats() * sizeof(float), &d, "paged attention partials");
+    const int rc = dev_alloc(c, bytes, &d, purpose);
     if (cap) (void)hipThreadExchangeStreamCaptureMode(&mode);
     if (rc) return rc;
-    c->gws = (float *)d;
+    k.p = (uint8_t *)d;
   }
-  *p = c->gws;
+  *p = k.p;
   if (cap) {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     unsigned long long id = 0;
     HIP_OK(c, hipStreamGetCaptureInfo(c->stream, &st, &id));
-    if (c->gws_cap_stream && id == c->gws_cap && c->stream != c->gws_cap_stream) {
-      if (!c->gws_cap_event) HIP_OK(c, hipEventCreateWithFlags(&c->gws_cap_event, hipEventDisableTiming));
-      HIP_OK(c, hipEventRecord(c->gws_cap_event, c->gws_cap_stream));
-      HIP_OK(c, hipStreamWaitEvent(c->stream, c->gws_cap_event, 0));
+    if (k.cap_stream && id == k.cap && c->stream != k.cap_stream) {
+      if (!k.cap_event) HIP_OK(c, hipEventCreateWithFlags(&k.cap_event, hipEventDisableTiming));
+      HIP_OK(c, hipEventRecord(k.cap_event, k.cap_stream));
+      HIP_OK(c, hipStreamWaitEvent(c->stream, k.cap_event, 0));
     }
-    c->gws_cap = id;
-    c->gws_cap_stream = c->stream;
+    k.cap = id;
+    k.cap_stream = c->stream;
     return KMOE_OK;
   }
-  if (c->gws_wait) HIP_OK(c, hipStreamWaitEvent(c->stream, c->gws_event, 0));
-  c->gws_wait = false;
-  c->gws_used = true;
-  c->gws_stream = c->stream;
+  if (k.wait) HIP_OK(c, hipStreamWaitEvent(c->stream, k.event, 0));
+  k.wait = false;
+  k.used = true;
+  k.stream = c->stream;
   return KMOE_OK;
 }
 
-void leave_paged(kmoe_ctx *c, hipStream_t next) {
-  if (!c->gws_used || next == c->gws_stream || capturing(c->gws_stream) || capturing(next)) return;
+void leave_kept(kmoe_ctx *c, Kept &k, hipStream_t next) {
+  if (!k.used || next == k.stream || capturing(k.stream) || capturing(next)) return;
   DeviceGuard g(c->device);
-  if ((!c->gws_event && hipEventCreateWithFlags(&c->gws_event, hipEventDisableTiming) != hipSuccess) ||
-      hipEventRecord(c->gws_event, c->gws_stream) != hipSuccess) {
+  if ((!k.event && hipEventCreateWithFlags(&k.event, hipEventDisableTiming) != hipSuccess) ||
+      hipEventRecord(k.event, k.stream) != hipSuccess) {
     (void)hipGetLastError();  // no such stream any more
     return;
   }
-  c->gws_wait = true;
-  c->gws_used = false;
+  k.wait = true;
+  k.used = false;
 }
 
 // The stream is about to change: the last use of the pieces is marked on its own.
 void leave_stream(kmoe_ctx *c, hipStream_t next) {
-  leave_paged(c, next);
+  for (Kept *k : {&c->paged, &c->sample}) leave_kept(c, *k, next);
   if (!c->pws_used || next == c->pws_stream || capturing(c->pws_stream) || capturing(next)) return;
   DeviceGuard g(c->device);
   if ((!c->pws_event && hipEventCreateWithFlags(&c->pws_event, hipEventDisableTiming) != hipSuccess) ||
@@ -891,9 +896,11 @@ int kmoe_destroy(kmoe_ctx *c) {
   if (c->pws) (void)hipFree(c->pws);
   for (void *p : c->pws_retired) (void)hipFree(p);
   if (c->pws_event) (void)hipEventDestroy(c->pws_event);
-  if (c->gws) (void)hipFree(c->gws);
-  if (c->gws_event) (void)hipEventDestroy(c->gws_event);
-  if (c->gws_cap_event) (void)hipEventDestroy(c->gws_cap_event);
+  for (Kept *k : {&c->paged, &c->sample}) {
+    if (k->p) (void)hipFree(k->p);
+    if (k->event) (void)hipEventDestroy(k->event);
+    if (k->cap_event) (void)hipEventDestroy(k->cap_event);
+  }
   if (c->counters) (void)hipFree(c->counters);
   if (c->own) (void)hipStreamDestroy(c->own);
   delete c;
@@ -2529,8 +2536,9 @@ int kmoe_sample(kmoe_ctx *c, const float *logits, int64_t s_rows, int64_t n, int
                 const float *u, uint32_t *out, float *prob, int32_t *pos, int32_t advance) {
   if (!c) return KMOE_E_INVALID;
   if (n <= 0 || n > KMOE_SAMPLE_MAX) return fail(c, KMOE_E_INVALID, "%lld logits a row (1 .. %d)", (long long)n, KMOE_SAMPLE_MAX);
-  if (s_rows < 0 || s_rows > kPagedMaxRows) return fail(c, KMOE_E_INVALID, "negative or too large size");
-  if (stride < n || stride > INT64_MAX / 8 / kPagedMaxRows)
+  constexpr int64_t kMaxRows = (int64_t)1 << 20;  // (a work-group of 1024 per row stays a valid grid)
+  if (s_rows < 0 || s_rows > kMaxRows) return fail(c, KMOE_E_INVALID, "%lld rows (at most 2^20)", (long long)s_rows);
+  if (stride < n || stride > INT64_MAX / 8 / kMaxRows)
     return fail(c, KMOE_E_INVALID, "rows of %lld floats %lld apart", (long long)n, (long long)stride);
   if (s_rows == 0) return KMOE_OK;
   if (!logits || !u || !out) return fail(c, KMOE_E_INVALID, "null pointer");
@@ -2547,7 +2555,10 @@ int kmoe_sample(kmoe_ctx *c, const float *logits, int64_t s_rows, int64_t n, int
   }
   DeviceGuard g(c->device);
   const SampleArgs a{logits, s_rows, n, stride, u, h.temperature_dev, h.top_k_dev, h.top_p_dev, h.min_p_dev, out, prob, pos, advance};
-  LAUNCH(c, "sample", launch_sample(c->stream, a));
+  uint8_t *ws = nullptr;
+  const int rc = kept_ws(c, c->sample, sample_ws_bytes(), "sampling", &ws);
+  if (rc) return rc;
+  LAUNCH(c, "sample", launch_sample(c->stream, a, ws));
   return KMOE_OK;
 }
 
@@ -2676,10 +2687,10 @@ int kmoe_paged_attention(kmoe_ctx *c, const kmoe_paged_desc *d, const void *page
   if ((uintptr_t)q < (uintptr_t)out + bytes && (uintptr_t)out < (uintptr_t)q + bytes)
     return fail(c, KMOE_E_INVALID, "out overlaps q");
   DeviceGuard g(c->device);
-  float *part = nullptr;
-  rc = paged_ws(c, &part);
+  uint8_t *part = nullptr;
+  rc = kept_ws(c, c->paged, paged_part_floats() * sizeof(float), "paged attention partials", &part);
   if (rc) return rc;
-  LAUNCH(c, "paged_attention", launch_paged_attention(c->stream, a, q, n_head, window, n_sink, out, part,
+  LAUNCH(c, "paged_attention", launch_paged_attention(c->stream, a, q, n_head, window, n_sink, out, (float *)part,
                                                       c->counters + kCounterWords));
   return KMOE_OK;
 }

@@ -463,7 +463,13 @@ struct SampleArgs {
   float *prob;
   int32_t *pos, advance;
 };
-hipError_t launch_sample(hipStream_t st, const SampleArgs &a);
+// What k_sample_stats finds of a row's chunks, for as many rows as the workspace holds.
+struct SampleStats {
+  unsigned long long *chunk_sum;
+  float *chunk_max, *group_max;
+};
+size_t sample_ws_bytes();
+hipError_t launch_sample(hipStream_t st, const SampleArgs &a, uint8_t *ws);
 hipError_t launch_argmax(hipStream_t st, const float *l, int64_t n, uint32_t *out, int32_t *pos_dev,
                          int32_t advance);
 hipError_t launch_pos_advance(hipStream_t st, int32_t *pos_dev, int32_t by);

@@ -29,6 +29,8 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kFix = 43;    // weights in units of 2^-43
 constexpr int kBins = 2048;
 constexpr u64 kOne = 1ull << kFix;
+constexpr int kGroup = 64, kChunk = 4096;  // elements of which k_sample_stats finds the largest, and the sum
+constexpr int kCand = 2048, kGroups = 1024;
 constexpr float kSpan = 24.0f;  // distances from the largest logit that the even bins tell apart, in units of T
 
 // Order of the logits as whole numbers: the larger the logit, the smaller its rank
@@ -45,15 +47,23 @@ __device__ __forceinline__ float of_rank(uint32_t r) {
 
 // What one row is drawn by.
 struct Row {
-  const float *l;
-  int n;
   float max;     // largest logit
   double inv_t;  // 1 / T
   float scale;   // bins per unit of logit
-  int k;         // tokens kept at most
-  float p;       // >= 1: all
   double min_p;  // 0: all
   float u;
+};
+
+// Elements of a row: of the logits themselves, or candidates in LDS, in the order of their index.
+struct Logits {
+  const float *l;
+  int n;
+  __device__ __forceinline__ float at(int i) const { return clean(l[i]); }
+};
+struct Candidates {
+  const float *l;
+  int n;
+  __device__ __forceinline__ float at(int i) const { return l[i]; }
 };
 
 // exp(x), -31 <= x <= 0: 2^(i / 64) from a table (LDS) times the exponential of what is
@@ -93,8 +103,13 @@ struct Shared {
   uint32_t count[kBins];
   u64 red[kWaves];
   uint32_t redi[kWaves];
+  float redf[kWaves];
   u64 before;
   int at;
+  // candidates, and the groups that they are in with how many candidates each has
+  float cand[kCand];
+  int index[kCand];
+  uint16_t group[kGroups], in_group[kGroups];
 };
 
 __device__ __forceinline__ u64 shfl_up64(u64 x, int d) {
@@ -146,19 +161,19 @@ __device__ __forceinline__ int crossing(const T *hist, u64 target, u64 &before, 
   return sh.at;
 }
 
-// f(i, l) for every element i of the row, a work-group together.
-template <class F>
-__device__ __forceinline__ void each(const Row &r, F &&f) {
+// f(i, l) for every element i, a work-group together.
+template <class S, class F>
+__device__ __forceinline__ void each(const S &src, F &&f) {
   constexpr int U = 8;
   int i = threadIdx.x;
-  for (; i + (U - 1) * kThreads < r.n; i += U * kThreads) {
+  for (; i + (U - 1) * kThreads < src.n; i += U * kThreads) {
     float x[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) x[j] = r.l[i + j * kThreads];
+    for (int j = 0; j < U; ++j) x[j] = src.at(i + j * kThreads);
 #pragma unroll
-    for (int j = 0; j < U; ++j) f(i + j * kThreads, clean(x[j]));
+    for (int j = 0; j < U; ++j) f(i + j * kThreads, x[j]);
   }
-  for (; i < r.n; i += kThreads) f(i, clean(r.l[i]));
+  for (; i < src.n; i += kThreads) f(i, src.at(i));
 }
 
 template <class T>
@@ -175,8 +190,8 @@ struct Cut {
 // Where the running sum over the elements of an even bin whose rank is below `limit`
 // reaches target (1 .. their sum): the value's rank, and what is left of the target
 // there. MASS: sums of weights, otherwise numbers of elements. Digit by digit.
-template <bool MASS>
-__device__ Cut cut_in_bin(const Row &r, int bin, uint32_t limit, u64 target, Shared &sh) {
+template <bool MASS, class S>
+__device__ __forceinline__ Cut cut_in_bin(const Row &r, const S &src, int bin, uint32_t limit, u64 target, Shared &sh) {
   uint32_t found = 0;
 #pragma unroll 1
   for (int d = 0; d < 3; ++d) {  // 11, 11 and 10 bits
@@ -185,7 +200,7 @@ __device__ Cut cut_in_bin(const Row &r, int bin, uint32_t limit, u64 target, Sha
     if (MASS) clear(sh.mass);
     else clear(sh.count);
     __syncthreads();
-    each(r, [&](int, float l) {
+    each(src, [&](int, float l) {
       if (bin_of(r, l) != bin) return;
       const uint32_t k = rank_of(l);
       if (k >= limit || (d && k >> top != found >> top)) return;
@@ -202,28 +217,96 @@ __device__ Cut cut_in_bin(const Row &r, int bin, uint32_t limit, u64 target, Sha
   return Cut{found, target};
 }
 
-// Sum of f(i, l) over the row, to every thread.
-template <class F>
-__device__ __forceinline__ u64 sum_of(const Row &r, Shared &sh, F &&f) {
+// Sum of f(i, l) over the elements, to every thread.
+template <class S, class F>
+__device__ __forceinline__ u64 sum_of(const S &src, Shared &sh, F &&f) {
   u64 s = 0, total;
-  each(r, [&](int i, float l) { s += f(i, l); });
+  each(src, [&](int i, float l) { s += f(i, l); });
   block_scan(s, total, sh);
   return total;
 }
 
-// The first kept token, by index, at which the running sum passes u times the whole:
-// the range is cut into 16 parts by sums of its waves until it has an element per thread.
-// Returns its weight and the sum.
-__device__ int draw(const Row &r, const Cut &cut, u64 &w, u64 &sum, Shared &sh) {
+// The cut by top_k (src.n or more: none) and top_p (1 or more: none) among the elements. all_: the
+// whole row's sum where the elements are not all that top_p counts, or 0.
+template <class S>
+__device__ __forceinline__ Cut find_cut(const Row &r, const S &src, int k, float p, u64 all_, Shared &sh) {
+  const int t = threadIdx.x;
+  Cut cut{0xffffffffu, ~0ull};
+  if (k >= src.n && p >= 1.0f) return cut;
+  __syncthreads();
+  clear(sh.mass);
+  clear(sh.count);
+  __syncthreads();
+  each(src, [&](int, float l) {
+    const int b = bin_of(r, l);
+    atomicAdd(&sh.count[b], 1u);
+    const u64 w = p < 1.0f ? fixed(weight(r, l, sh.tab)) : 0;
+    if (w) atomicAdd(&sh.mass[b], w);
+  });
+  __syncthreads();
+  // k falls into bin kb; m_bins: the sum of the bins before it, m_above: of all elements
+  // before the k-th's value
+  u64 n_before = 0, m_bins = 0, w_tie = 0;
+  int kb = kBins;
+  if (k < src.n) kb = crossing(sh.count, (u64)k, n_before, sh);
+  block_scan((2 * t < kb ? sh.mass[2 * t] : 0) + (2 * t + 1 < kb ? sh.mass[2 * t + 1] : 0), m_bins, sh);
+  u64 m_above = m_bins, all = m_bins;
+  if (kb < kBins) {
+    cut = cut_in_bin<false>(r, src, kb, 0xffffffffu, (u64)k - n_before, sh);  // (the masses stay)
+    if (p >= 1.0f) return cut;
+    w_tie = fixed(weight(r, of_rank(cut.rank), sh.tab));
+    m_above += sum_of(src, sh, [&](int, float l) {
+      return bin_of(r, l) == kb && rank_of(l) < cut.rank ? fixed(weight(r, l, sh.tab)) : 0;
+    });
+    all = m_above + cut.ties * w_tie;
+  }
+  const u64 whole = all_ ? all_ : all;
+  const double x = (double)p * (double)whole;
+  u64 target = (u64)x;
+  target += (double)target < x;
+  target = target > 1 ? target : 1;
+  if (target > all) {
+    if (all_) return cut;  // further down than the elements go
+    target = all;
+  }
+  if (target > m_above) {
+    cut.ties = (target - m_above + w_tie - 1) / w_tie;
+    return cut;
+  }
+  u64 before = m_bins;
+  int b = kb;
+  uint32_t limit = cut.rank;
+  if (target <= m_bins) {
+    b = crossing(sh.mass, target, before, sh);
+    limit = 0xffffffffu;
+  }
+  cut = cut_in_bin<true>(r, src, b, limit, target - before, sh);
+  w_tie = fixed(weight(r, of_rank(cut.rank), sh.tab));
+  cut.ties = (cut.ties + w_tie - 1) / w_tie;
+  return cut;
+}
+
+// The first kept element from `start` on at which the running sum passes u times the
+// sum, or `goal` where `whole` is given (the sum of a row of which src is a part): the
+// range is cut into 16 parts by sums of its waves until it has an element per thread.
+// Returns its weight and the sum; -1 where all weights are 0.
+template <class S>
+__device__ __forceinline__ int draw(const Row &r, const S &src, const Cut &cut, int start, int len, u64 goal, u64 whole,
+                                    u64 &w, u64 &sum, Shared &sh) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   auto kept = [&](float l) -> u64 {
     const double x = weight(r, l, sh.tab);
     return x >= r.min_p ? fixed(x) : 0;
   };
   const u64 w_tie = kept(of_rank(cut.rank));
-  int start = 0, len = r.n;
-  u64 goal = 0, ties = cut.ties;
+  u64 ties = cut.ties;
   bool first = true;
+  auto begin = [&](u64 total) {
+    sum = whole ? whole : total;
+    if (!whole) goal = (u64)((double)r.u * (double)sum);
+    goal = goal < total ? goal : total - 1;  // (a part's sum, as the row's was formed, may be some units off)
+    first = false;
+  };
   while (len > kThreads) {
     const int part = (len + kThreads - 1) / kThreads * 64, a = start + wave * part;
     const int b = a + part < start + len ? a + part : start + len;
@@ -231,7 +314,7 @@ __device__ int draw(const Row &r, const Cut &cut, u64 &w, u64 &sum, Shared &sh) 
     uint32_t c = 0;
 #pragma unroll 4
     for (int i = a + lane; i < b; i += 64) {
-      const float l = clean(r.l[i]);
+      const float l = src.at(i);
       const uint32_t k = rank_of(l);
       if (k < cut.rank) s += kept(l);
       c += k == cut.rank;
@@ -246,15 +329,13 @@ __device__ int draw(const Row &r, const Cut &cut, u64 &w, u64 &sum, Shared &sh) 
     __syncthreads();
     auto of_part = [&](int i, u64 left) { return sh.red[i] + (sh.redi[i] < left ? sh.redi[i] : left) * w_tie; };
     if (first) {
-      u64 left = ties;
-      sum = 0;
+      u64 left = ties, total = 0;
       for (int i = 0; i < kWaves; ++i) {
-        sum += of_part(i, left);
+        total += of_part(i, left);
         left -= sh.redi[i] < left ? sh.redi[i] : left;
       }
-      goal = (u64)((double)r.u * (double)sum);
-      goal = goal < sum ? goal : sum - 1;
-      first = false;
+      if (!total) return -1;
+      begin(total);
     }
     int i = 0;
     for (; i < kWaves - 1; ++i) {
@@ -267,7 +348,7 @@ __device__ int draw(const Row &r, const Cut &cut, u64 &w, u64 &sum, Shared &sh) 
     start += i * part;
     len = start + part < end ? part : end - start;
   }
-  const float l = t < len ? clean(r.l[start + t]) : 0.0f;
+  const float l = t < len ? src.at(start + t) : 0.0f;
   const uint32_t k = rank_of(l);
   const bool tie = t < len && k == cut.rank;
   u64 total;
@@ -275,9 +356,8 @@ __device__ int draw(const Row &r, const Cut &cut, u64 &w, u64 &sum, Shared &sh) 
   const u64 m = t < len && (k < cut.rank || (tie && nth < ties)) ? kept(l) : 0;
   const u64 x = block_scan(m, total, sh);
   if (first) {
-    sum = total;
-    goal = (u64)((double)r.u * (double)sum);
-    goal = goal < sum ? goal : sum - 1;
+    if (!total) return -1;
+    begin(total);
   }
   if (x <= goal && goal < x + m) {
     sh.at = start + t;
@@ -288,116 +368,304 @@ __device__ int draw(const Row &r, const Cut &cut, u64 &w, u64 &sum, Shared &sh) 
   return sh.at;
 }
 
-__global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a) {
+// A row's settings, as they are used.
+struct Settings {
+  float temp, p, min_p;
+  int k;
+  bool greedy;
+  __device__ __forceinline__ Settings(const SampleArgs &a, int64_t row) {
+    temp = a.temperature ? a.temperature[row] : 1.0f;
+    k = a.top_k ? a.top_k[row] : 0;
+    k = k > 0 && k < (int)a.n ? k : (int)a.n;
+    p = a.top_p ? a.top_p[row] : 1.0f;
+    p = p == p ? p : 1.0f;
+    min_p = a.min_p ? a.min_p[row] : 0.0f;
+    min_p = min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f;
+    greedy = !(temp > 0.0f) || k == 1 || p <= 0.0f;
+  }
+  // whether the sum of all weights is asked for
+  __device__ __forceinline__ bool sums(const SampleArgs &a) const { return !greedy && k >= (int)a.n && (p < 1.0f || min_p == 0.0f); }
+};
+
+typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// Per chunk of kChunk logits, the largest, the sum of the weights by that one (kFix
+// units) where it is asked for, and the largest of every kGroup.
+__global__ void __launch_bounds__(256) k_sample_stats(SampleArgs a, int64_t row0, SampleStats st) {
+  __shared__ double tab[64];
+  __shared__ float red[4];
+  __shared__ u64 redu[4];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = blockIdx.x;
+  const int64_t row = row0 + blockIdx.y;
+  const float *l = a.logits + row * a.stride;
+  const int n = (int)a.n, base = c * kChunk;
+  const Settings s(a, row);
+  const bool sums = s.sums(a);
+  if (sums && t < 64) tab[t] = exp2((double)t / 64);
+  float x[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int i = base + j * 1024 + 4 * t;
+    if (i + 4 <= n) {
+      const f32x4a4 y = *(const f32x4a4 *)(l + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[j][e] = clean(y[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[j][e] = i + e < n ? clean(l[i + e]) : -INFINITY;
+    }
+  }
+  float *gm = st.group_max + ((int64_t)blockIdx.y * gridDim.x + c) * (kChunk / kGroup);
+  float m = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float g = group_max<16>(fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])));
+    if ((lane & 15) == 0) gm[j * 16 + (t >> 4)] = g;
+    m = fmaxf(m, g);
+  }
+  m = group_max<64>(m);
+  if (lane == 0) red[wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  u64 sum = 0;
+  if (sums) {
+    Row r;
+    r.max = m;
+    r.inv_t = 1.0 / (double)s.temp;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (base + j * 1024 + 4 * t + e < n) sum += fixed(weight(r, x[j][e], tab));
+    sum = wave_scan(sum);
+    if (lane == 63) redu[wave] = sum;
+    __syncthreads();
+    sum = redu[0] + redu[1] + redu[2] + redu[3];
+  }
+  if (t == 0) {
+    st.chunk_max[(int64_t)blockIdx.y * gridDim.x + c] = m;
+    st.chunk_sum[(int64_t)blockIdx.y * gridDim.x + c] = sum;
+  }
+}
+
+// The first element of [start, end) that is l.
+__device__ __forceinline__ int first_equal(const Logits &src, int start, int end, float l, Shared &sh) {
+  __syncthreads();
+  if (threadIdx.x == 0) sh.at = end;
+  __syncthreads();
+  int first = end;
+  for (int i = start + threadIdx.x; i < end && first == end; i += kThreads) first = src.at(i) == l ? i : end;
+  if (first < end) atomicMin(&sh.at, first);
+  __syncthreads();
+  return sh.at;
+}
+
+// The elements whose even bin is at most b0, in sh.cand and sh.index, in their order;
+// -1 where they are too many. A group's largest says whether it has any.
+__device__ __forceinline__ int gather(const Row &r, const Logits &src, const float *gm, int n_group, int b0, Shared &sh) {
+  const int t = threadIdx.x, l16 = t & 15;
+  int n = 0;
+  for (int g0 = 0; g0 < n_group; g0 += kThreads) {
+    const int g = g0 + t;
+    const float x = g < n_group ? gm[g] : -INFINITY;
+    const bool in = x != -INFINITY && bin_of(r, x) <= b0;
+    u64 total;
+    const int at = n + (int)block_scan(in, total, sh);
+    if (in && at < kGroups) sh.group[at] = (uint16_t)g;
+    n += (int)total;
+  }
+  if (n > kGroups) return -1;
+  __syncthreads();
+  auto load = [&](int i, float (&x)[4]) {
+    const int at = sh.group[i] * kGroup + 4 * l16;
+    uint32_t in = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[e] = at + e < src.n ? src.at(at + e) : -INFINITY;
+      if (x[e] != -INFINITY && bin_of(r, x[e]) <= b0) in |= 1u << e;
+    }
+    return in;
+  };
+  for (int i = t >> 4; i < n; i += kThreads / 16) {
+    float x[4];
+    const int m = group_sum_i<16>(__builtin_popcount(load(i, x)));
+    if (l16 == 0) sh.in_group[i] = (uint16_t)m;
+  }
+  __syncthreads();
+  u64 total;
+  const uint32_t mine = t < n ? sh.in_group[t] : 0;
+  const int at = (int)block_scan(mine, total, sh);
+  if (total > kCand) return -1;
+  if (t < n) sh.in_group[t] = (uint16_t)at;
+  __syncthreads();
+  for (int i = t >> 4; i < n; i += kThreads / 16) {
+    float x[4];
+    const uint32_t in = load(i, x);
+    int before = __builtin_popcount(in);
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+      const int y = __shfl_up(before, d, 16);
+      if (l16 >= d) before += y;
+    }
+    int to = sh.in_group[i] + before - __builtin_popcount(in);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (in & (1u << e)) {
+        sh.cand[to] = x[e];
+        sh.index[to++] = sh.group[i] * kGroup + 4 * l16 + e;
+      }
+  }
+  __syncthreads();
+  return (int)total;
+}
+
+// chunks: 0 without k_sample_stats before it.
+__global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t row0, SampleStats st, int chunks) {
   __shared__ Shared sh;
   const int t = threadIdx.x;
-  const int64_t row = blockIdx.x;
+  const int64_t row = row0 + blockIdx.x;
   if (t < 64) sh.tab[t] = exp2((double)t / 64);
-  Row r;
-  r.l = a.logits + row * a.stride;
-  r.n = (int)a.n;
-  const float temp = a.temperature ? a.temperature[row] : 1.0f;
-  r.k = a.top_k ? a.top_k[row] : 0;
-  r.k = r.k > 0 && r.k < r.n ? r.k : r.n;
-  r.p = a.top_p ? a.top_p[row] : 1.0f;
-  r.p = r.p == r.p ? r.p : 1.0f;
-  const float mp = a.min_p ? a.min_p[row] : 0.0f;
-  r.min_p = mp > 0.0f ? (double)fminf(mp, 1.0f) : 0.0;
-  r.u = a.u[row];
-  r.u = r.u > 0.0f ? fminf(r.u, 1.0f) : 0.0f;
+  const Logits src{a.logits + row * a.stride, (int)a.n};
+  const Settings s(a, row);
+  const float *cm = st.chunk_max + (int64_t)blockIdx.x * chunks;
   // the largest logit
   float m = -INFINITY;
-  each(r, [&](int, float l) { m = fmaxf(m, l); });
+  if (chunks) {
+    for (int i = t; i < chunks; i += kThreads) m = fmaxf(m, cm[i]);
+  } else {
+    each(src, [&](int, float l) { m = fmaxf(m, l); });
+  }
   m = group_max<64>(m);
-  __shared__ float red[kWaves];
-  if ((t & 63) == 0) red[t >> 6] = m;
+  if ((t & 63) == 0) sh.redf[t >> 6] = m;
   __syncthreads();
-  for (int i = 0; i < kWaves; ++i) m = fmaxf(m, red[i]);
+  for (int i = 0; i < kWaves; ++i) m = fmaxf(m, sh.redf[i]);
+  Row r;
   r.max = m;
-  uint32_t id = 0;
+  r.u = a.u[row];
+  r.u = r.u > 0.0f ? fminf(r.u, 1.0f) : 0.0f;
+  r.min_p = s.min_p;
+  r.inv_t = 1.0 / (double)s.temp;
+  r.scale = fminf((float)(kBins / kSpan * r.inv_t), 3.0e38f);
+  int id = 0;
   float prob = 0.0f;
   if (m == -INFINITY) {  // nothing to draw from
-  } else if (!(temp > 0.0f) || r.k == 1 || r.p <= 0.0f) {
-    if (t == 0) sh.at = r.n;
-    __syncthreads();
-    int first = r.n;
-    each(r, [&](int i, float l) { first = l == m && i < first ? i : first; });
-    if (first < r.n) atomicMin(&sh.at, first);
-    __syncthreads();
-    id = (uint32_t)sh.at;
+  } else if (s.greedy) {
+    int start = 0, end = src.n;
+    if (chunks) {
+      if (t == 0) sh.at = chunks;
+      __syncthreads();
+      if (t < chunks && cm[t] == m) atomicMin(&sh.at, t);
+      __syncthreads();
+      start = sh.at * kChunk;
+      end = start + kChunk < end ? start + kChunk : end;
+    }
+    id = first_equal(src, start, end, m, sh);
     prob = 1.0f;
   } else {
-    r.inv_t = 1.0 / (double)temp;
-    r.scale = fminf((float)(kBins / kSpan * r.inv_t), 3.0e38f);
-    Cut cut{0xffffffffu, ~0ull};
-    if (r.k < r.n || r.p < 1.0f) {
+    // the chunks' sums by the row's largest
+    u64 sum = 0, w = 0, mine = 0, before = 0;
+    if (chunks && s.sums(a)) {
+      if (t < chunks) {
+        Row q = r;
+        mine = (u64)__builtin_rint((double)st.chunk_sum[(int64_t)blockIdx.x * chunks + t] * weight(q, cm[t], sh.tab));
+      }
+      before = block_scan(mine, sum, sh);
+    }
+    int at = -1;
+    if (sum && s.p >= 1.0f) {  // everything is kept: the chunk, then the token in it
+      u64 goal = (u64)((double)r.u * (double)sum);
+      goal = goal < sum ? goal : sum - 1;
+      if (before <= goal && goal < before + mine) {
+        sh.at = t;
+        sh.before = before;
+      }
+      __syncthreads();
+      const int start = sh.at * kChunk, end = start + kChunk < src.n ? start + kChunk : src.n;
+      goal -= sh.before;
+      const float cl = cm[sh.at];
+      __syncthreads();
+      at = draw(r, src, Cut{0xffffffffu, ~0ull}, start, end - start, goal, sum, w, sum, sh);
+      id = at >= 0 ? at : first_equal(src, start, end, cl, sh);  // (a chunk of many weights of under half a unit)
+      w = at >= 0 ? w : 1;
+      at = 0;
+    } else if (chunks) {
+      // a bin that holds the last kept token, or one after it, by the groups' largest: as
+      // many of them as tokens are kept, or of as much weight
+      const float *gm = st.group_max + (int64_t)blockIdx.x * chunks * (kChunk / kGroup);
+      const int n_group = (src.n + kGroup - 1) / kGroup;
+      int b0 = kBins;
       clear(sh.mass);
       clear(sh.count);
       __syncthreads();
-      each(r, [&](int, float l) {
-        const int b = bin_of(r, l);
-        atomicAdd(&sh.count[b], 1u);
-        const u64 w = fixed(weight(r, l, sh.tab));
-        if (w) atomicAdd(&sh.mass[b], w);
-      });
+      for (int g = t; g < n_group; g += kThreads) {
+        const float x = gm[g];
+        if (x == -INFINITY) continue;
+        const int b = bin_of(r, x);
+        if (s.k < src.n) atomicAdd(&sh.count[b], 1u);
+        else if (s.p < 1.0f) atomicAdd(&sh.mass[b], fixed(weight(r, x, sh.tab)));
+      }
       __syncthreads();
-      // the bins' sums are used up by the digits' later: everything that is needed of
-      // them is found first
-      u64 n_before = 0, m_bins = 0, total;
-      int kb = kBins;
-      if (r.k < r.n) {
-        kb = crossing(sh.count, (u64)r.k, n_before, sh);
-        const u64 x = (2 * t < kb ? sh.mass[2 * t] : 0) + (2 * t + 1 < kb ? sh.mass[2 * t + 1] : 0);
-        block_scan(x, m_bins, sh);
-      } else {
-        block_scan(sh.mass[2 * t] + sh.mass[2 * t + 1], m_bins, sh);
-      }
-      u64 all = m_bins, w_tie = 0, m_above = m_bins;
-      if (kb < kBins) {
-        // (the masses are kept: this counts)
-        cut = cut_in_bin<false>(r, kb, 0xffffffffu, (u64)r.k - n_before, sh);
-        w_tie = fixed(weight(r, of_rank(cut.rank), sh.tab));
-        m_above += sum_of(r, sh, [&](int, float l) {
-          return bin_of(r, l) == kb && rank_of(l) < cut.rank ? fixed(weight(r, l, sh.tab)) : 0;
-        });
-        all = m_above + cut.ties * w_tie;
-      }
-      if (r.p < 1.0f) {
-        const double x = (double)r.p * (double)all;
+      u64 total, none;
+      if (s.k < src.n) {
+        block_scan((u64)sh.count[2 * t] + sh.count[2 * t + 1], total, sh);
+        if ((u64)s.k <= total) b0 = crossing(sh.count, (u64)s.k, none, sh);
+      } else if (s.p < 1.0f) {
+        const double x = (double)s.p * (double)sum;
         u64 target = (u64)x;
         target += (double)target < x;
         target = target > 1 ? target : 1;
-        target = target < all ? target : all;
-        if (target <= m_bins) {
-          u64 before;
-          const int b = crossing(sh.mass, target, before, sh);
-          cut = cut_in_bin<true>(r, b, 0xffffffffu, target - before, sh);
-          w_tie = fixed(weight(r, of_rank(cut.rank), sh.tab));
-          cut.ties = (cut.ties + w_tie - 1) / w_tie;
-        } else if (target <= m_above) {
-          cut = cut_in_bin<true>(r, kb, cut.rank, target - m_bins, sh);
-          w_tie = fixed(weight(r, of_rank(cut.rank), sh.tab));
-          cut.ties = (cut.ties + w_tie - 1) / w_tie;
-        } else {
-          cut.ties = (target - m_above + w_tie - 1) / w_tie;
+        block_scan(sh.mass[2 * t] + sh.mass[2 * t + 1], total, sh);
+        if (target <= total) b0 = crossing(sh.mass, target, none, sh);
+      }
+      if (r.min_p > 0.0 && (s.k >= src.n || s.p >= 1.0f)) {
+        // (where top_p counts among the top_k all of those are needed)
+        const float x = (float)(-log(r.min_p) * (double)s.temp) * r.scale + 1.0f;
+        b0 = x < (float)b0 ? (int)x : b0;
+      }
+      if (b0 < kBins - 1) {
+        const int n = gather(r, src, gm, n_group, b0, sh);
+        if (n >= 0) {
+          const Candidates cand{sh.cand, n};
+          Row f = r;
+          f.scale = r.scale * ((float)kBins / (float)(b0 + 1));  // (their bins, finer)
+          const Cut cut = find_cut(f, cand, s.k, s.p, s.k < src.n ? 0 : sum, sh);
+          at = draw(f, cand, cut, 0, n, 0, 0, w, sum, sh);
+          id = sh.index[at];
         }
       }
     }
-    u64 w, sum;
-    id = (uint32_t)draw(r, cut, w, sum, sh);
+    if (at < 0) {
+      const Cut cut = find_cut(r, src, s.k, s.p, 0, sh);
+      id = draw(r, src, cut, 0, src.n, 0, 0, w, sum, sh);
+    }
     prob = (float)((double)w / (double)sum);
   }
   if (t == 0) {
-    a.out[row] = id;
+    a.out[row] = (uint32_t)id;
     if (a.prob) a.prob[row] = prob;
     if (a.pos) a.pos[row] += a.advance;
   }
 }
 
+constexpr int64_t kFewTokens = 8192;  // a work-group reads so many as quickly as another launch comes
+
 }  // namespace
 
-hipError_t launch_sample(hipStream_t st, const SampleArgs &a) {
-  KMOE_LAUNCH(k_sample, dim3((unsigned)a.rows), dim3(kThreads), 0, st, a);
+size_t sample_ws_bytes() { return (size_t)16 << 20; }
+
+hipError_t launch_sample(hipStream_t st, const SampleArgs &a, uint8_t *ws) {
+  if (a.n <= kFewTokens) {
+    KMOE_LAUNCH(k_sample, dim3((unsigned)a.rows), dim3(kThreads), 0, st, a, (int64_t)0, SampleStats{}, 0);
+    return hipGetLastError();
+  }
+  const int chunks = (int)((a.n + kChunk - 1) / kChunk);
+  const int64_t each = (int64_t)chunks * (12 + 4 * (kChunk / kGroup)), most = (int64_t)sample_ws_bytes() / each;
+  for (int64_t row = 0; row < a.rows; row += most) {
+    const int64_t n = a.rows - row < most ? a.rows - row : most;
+    const SampleStats s{(unsigned long long *)ws, (float *)(ws + 8 * most * chunks), (float *)(ws + 12 * most * chunks)};
+    KMOE_LAUNCH(k_sample_stats, dim3((unsigned)chunks, (unsigned)n), dim3(256), 0, st, a, row, s);
+    KMOE_LAUNCH(k_sample, dim3((unsigned)n), dim3(kThreads), 0, st, a, row, s, chunks);
+  }
   return hipGetLastError();
 }
 

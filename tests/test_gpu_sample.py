@@ -235,7 +235,7 @@ def test_refusals(ctx):
     ctx.sample(buf[:480].view(4, 120)[:, :100], u, out=i32[100:104], prob=buf[224:228])
     f = ctx.lib.kmoe_sample
     o = torch.zeros(8, dtype=torch.int32, device="cuda")
-    for rows, n, stride in ((4, 0, 0), (4, -1, 5), (4, (1 << 20) + 1, 1 << 21), (-1, 100, 100), (4, 100, 99), (1 << 23, 1, 1), (2, 100, 2 ** 62)):
+    for rows, n, stride in ((4, 0, 0), (4, -1, 5), (4, (1 << 20) + 1, 1 << 21), (-1, 100, 100), (4, 100, 99), ((1 << 20) + 1, 1, 1), (2, 100, 2 ** 62)):
         assert f(ctx.h, x.data_ptr(), rows, n, stride, None, u.data_ptr(), o.data_ptr(), None, None, 0) == -1, (rows, n, stride)
     for args in ((0, u.data_ptr(), o.data_ptr()), (x.data_ptr(), 0, o.data_ptr()), (x.data_ptr(), u.data_ptr(), 0)):
         assert f(ctx.h, args[0], 4, 100, 100, None, args[1], args[2], None, None, 0) == -1
@@ -243,3 +243,37 @@ def test_refusals(ctx):
     assert f(ctx.h, 0, 0, 100, 100, None, 0, 0, None, None, 0) == 0
     assert f(ctx.h, x.data_ptr(), 4, 100, 100, None, u.data_ptr(), o.data_ptr(), None, None, 0) == 0
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("n", [8191, 8193, 12289, 1 << 20])
+def test_the_last_token_of_long_rows(ctx, n):
+    """The largest logit, the k-th and the drawn one at the ends of chunks and rows."""
+    rng = np.random.default_rng(n)
+    at = sorted({i for i in (0, 63, 64, 4095, 4096, 8191, n - 2, n - 1) if i < n})
+    x = rng.standard_normal((len(at), n)).astype(np.float32)
+    x[np.arange(len(at)), at] = 30.0
+    for how in (dict(temp=0.0), dict(k=5), dict(), dict(p=0.9)):
+        assert (_check(ctx, x, np.full(len(at), 0.5, np.float32), **how) == at).all()
+    x[:, n - 64:] = 40.0  # a whole group of equal ones at the end
+    for how in (dict(k=5), dict(p=0.5), dict(m=0.9), dict()):
+        _check(ctx, x[:2], [0.1, 0.99], **how)
+
+
+@pytest.mark.parametrize("how", [dict(k=900), dict(k=5000), dict(p=0.9999), dict(m=1e-6), dict(temp=1.3, p=0.9), dict(temp=50.0, k=3000, p=0.7, m=0.9)])
+def test_more_tokens_kept_than_fit_the_candidates(ctx, how):
+    rng = np.random.default_rng(3)
+    x = (rng.standard_normal((4, 60001)) * np.array([[0.01], [0.5], [2], [6]])).astype(np.float32)
+    _check(ctx, x, np.array([0.001, 0.3, 0.9, 0.9999], np.float32), **how)
+
+
+def test_more_rows_than_the_workspace_holds(ctx):
+    """The rows go by parts then: 16 MB hold 20867 rows of 3 chunks."""
+    import torch
+
+    S, n = 20900, 8200
+    x = torch.randn((S, n), device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    u = torch.rand(S, device="cuda", generator=torch.Generator("cuda").manual_seed(2))
+    k = torch.full((S,), 30, dtype=torch.int32, device="cuda")
+    got = ctx.sample(x, u, top_k=k)
+    for i in list(range(20860, 20880)) + [0, S - 1]:
+        assert got[i].item() == _reference(x[i].cpu().numpy(), u[i].item(), k=30)[0]
