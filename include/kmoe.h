@@ -598,6 +598,26 @@ int kmoe_paged_kv_read(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *p
 int kmoe_paged_attention(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *pages_dev,
                          const kmoe_paged_batch *batch, const float *q_dev, int32_t n_head, int64_t window,
                          int64_t n_sink, float *out_dev);
+/* kmoe_paged_attention (without a window) for a batch whose sequences have pages in
+ * common, as forks of one prompt do: what a group shares is read once for all its rows.
+ * Group i holds the sequences start[i] .. start[i + 1] - 1 of the batch (start
+ * [n_group + 1] ascending, so that groups lie one behind the other; sequences before the
+ * first and behind the last are in none), and the first pages[i] columns of its sequences' table
+ * rows name the same pages: they are read from the first one's row. Both arrays are device memory, read when the
+ * kernels run; entries past the batch or the table are cut off. A sequence whose rows do not all lie
+ * behind the shared pages is worked by itself, from its own row of the table, and so is a group of one. The
+ * result is kmoe_paged_attention's up to the last bits: a row's shared part and its own
+ * are formed apart, in f32, and joined by their maxima and sums; rows that come out not finite
+ * are formed again over their own table as there. s_rows * n_head is at most 2^21
+ * (KMOE_E_UNSUPPORTED past it). Besides that call's workspace it keeps one of 17 MB, with the
+ * same rules. */
+typedef struct {
+  int32_t n_group; /* 0 .. KMOE_PAGED_MAX_SEQ */
+  const int32_t *start_dev, *pages_dev;
+} kmoe_paged_groups;
+int kmoe_paged_attention_shared(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *pages_dev,
+                                const kmoe_paged_batch *batch, const kmoe_paged_groups *groups, const float *q_dev,
+                                int32_t n_head, float *out_dev);
 /* Pages src[i] onto dst[i], i < n, in each of n_layer buffers layer_stride
  * bytes apart (16-byte aligned; desc->n_pages pages each). src and dst are
  * host arrays, read before the call returns (the copies are asynchronous and

@@ -225,8 +225,9 @@ struct kmoe_ctx {
   hipEvent_t pws_event = nullptr;
   std::vector<void *> pws_retired;
   // scratch of one size each, allocated at the first call that takes it and kept:
-  // partials of the paged attention's split units, what sampling finds of the chunks
-  Kept paged, sample;
+  // partials of the paged attention's split units, the shared parts of its rows, what
+  // sampling finds of the chunks
+  Kept paged, shared, sample;
   // last moe_ffn routing (pointers into ws) and its sizes
   uint32_t *last_idx = nullptr, *last_perm = nullptr, *last_off = nullptr;
   float *last_w = nullptr;
@@ -731,7 +732,7 @@ void leave_kept(kmoe_ctx *c, Kept &k, hipStream_t next) {
 
 // The stream is about to change: the last use of the pieces is marked on its own.
 void leave_stream(kmoe_ctx *c, hipStream_t next) {
-  for (Kept *k : {&c->paged, &c->sample}) leave_kept(c, *k, next);
+  for (Kept *k : {&c->paged, &c->shared, &c->sample}) leave_kept(c, *k, next);
   if (!c->pws_used || next == c->pws_stream || capturing(c->pws_stream) || capturing(next)) return;
   DeviceGuard g(c->device);
   if ((!c->pws_event && hipEventCreateWithFlags(&c->pws_event, hipEventDisableTiming) != hipSuccess) ||
@@ -896,7 +897,7 @@ int kmoe_destroy(kmoe_ctx *c) {
   if (c->pws) (void)hipFree(c->pws);
   for (void *p : c->pws_retired) (void)hipFree(p);
   if (c->pws_event) (void)hipEventDestroy(c->pws_event);
-  for (Kept *k : {&c->paged, &c->sample}) {
+  for (Kept *k : {&c->paged, &c->shared, &c->sample}) {
     if (k->p) (void)hipFree(k->p);
     if (k->event) (void)hipEventDestroy(k->event);
     if (k->cap_event) (void)hipEventDestroy(k->cap_event);
@@ -2671,27 +2672,60 @@ int kmoe_paged_kv_read(kmoe_ctx *c, const kmoe_paged_desc *d, const void *pages,
   return KMOE_OK;
 }
 
+// Checks of the attention calls besides the batch's.
+static int check_paged_q(kmoe_ctx *c, const PagedArgs &a, const float *q, int32_t n_head, const float *out) {
+  if (n_head <= 0 || n_head % a.n_kv) return fail(c, KMOE_E_INVALID, "attention: need n_head %% n_kv == 0");
+  if (n_head / a.n_kv > 16)
+    return fail(c, KMOE_E_UNSUPPORTED, "%d query heads per kv head (kernels: <= 16)", n_head / a.n_kv);
+  if (a.s_rows == 0) return KMOE_OK;
+  if (!q || !out) return fail(c, KMOE_E_INVALID, "null pointer");
+  const uintptr_t bytes = (uintptr_t)a.s_rows * n_head * a.hd * sizeof(float);
+  if ((uintptr_t)q < (uintptr_t)out + bytes && (uintptr_t)out < (uintptr_t)q + bytes)
+    return fail(c, KMOE_E_INVALID, "out overlaps q");
+  return KMOE_OK;
+}
+
 int kmoe_paged_attention(kmoe_ctx *c, const kmoe_paged_desc *d, const void *pages, const kmoe_paged_batch *b,
                          const float *q, int32_t n_head, int64_t window, int64_t n_sink, float *out) {
   if (!c) return KMOE_E_INVALID;
   PagedArgs a;
   int rc = check_paged(c, d, pages, b, &a);
   if (rc) return rc;
-  if (n_head <= 0 || n_head % a.n_kv) return fail(c, KMOE_E_INVALID, "attention: need n_head %% n_kv == 0");
-  if (n_head / a.n_kv > 16)
-    return fail(c, KMOE_E_UNSUPPORTED, "%d query heads per kv head (kernels: <= 16)", n_head / a.n_kv);
   if (window < 0 || n_sink < 0) return fail(c, KMOE_E_INVALID, "negative window or n_sink");
-  if (a.s_rows == 0) return KMOE_OK;
-  if (!q || !out) return fail(c, KMOE_E_INVALID, "null pointer");
-  const uintptr_t bytes = (uintptr_t)a.s_rows * n_head * a.hd * sizeof(float);
-  if ((uintptr_t)q < (uintptr_t)out + bytes && (uintptr_t)out < (uintptr_t)q + bytes)
-    return fail(c, KMOE_E_INVALID, "out overlaps q");
+  rc = check_paged_q(c, a, q, n_head, out);
+  if (rc || a.s_rows == 0) return rc;
   DeviceGuard g(c->device);
   uint8_t *part = nullptr;
   rc = kept_ws(c, c->paged, paged_part_floats() * sizeof(float), "paged attention partials", &part);
   if (rc) return rc;
   LAUNCH(c, "paged_attention", launch_paged_attention(c->stream, a, q, n_head, window, n_sink, out, (float *)part,
                                                       c->counters + kCounterWords));
+  return KMOE_OK;
+}
+
+int kmoe_paged_attention_shared(kmoe_ctx *c, const kmoe_paged_desc *d, const void *pages, const kmoe_paged_batch *b,
+                                const kmoe_paged_groups *groups, const float *q, int32_t n_head, float *out) {
+  if (!c) return KMOE_E_INVALID;
+  PagedArgs a;
+  int rc = check_paged(c, d, pages, b, &a);
+  if (rc) return rc;
+  if (!groups) return fail(c, KMOE_E_INVALID, "null pointer");
+  if (groups->n_group < 0 || groups->n_group > KMOE_PAGED_MAX_SEQ)
+    return fail(c, KMOE_E_INVALID, "%d groups (at most %d)", groups->n_group, KMOE_PAGED_MAX_SEQ);
+  rc = check_paged_q(c, a, q, n_head, out);
+  if (rc || a.s_rows == 0) return rc;
+  if (groups->n_group == 0) return kmoe_paged_attention(c, d, pages, b, q, n_head, 0, 0, out);
+  if (!groups->start_dev || !groups->pages_dev) return fail(c, KMOE_E_INVALID, "null pointer");
+  if (a.s_rows * n_head > kSharedHeads)
+    return fail(c, KMOE_E_UNSUPPORTED, "%lld rows of %d heads (at most 2^21 together)", (long long)a.s_rows, n_head);
+  DeviceGuard g(c->device);
+  uint8_t *part = nullptr, *ml = nullptr;
+  rc = kept_ws(c, c->paged, paged_part_floats() * sizeof(float), "paged attention partials", &part);
+  if (!rc) rc = kept_ws(c, c->shared, kSharedHeads * 8 + KMOE_PAGED_MAX_SEQ * 4, "shared parts of rows", &ml);
+  if (rc) return rc;
+  const SharedArgs sa{groups->start_dev, groups->pages_dev, groups->n_group, (int32_t *)(ml + kSharedHeads * 8), (float *)ml};
+  LAUNCH(c, "paged_attention_shared", launch_paged_attention_shared(c->stream, a, sa, q, n_head, out, (float *)part,
+                                                                    c->counters + kCounterWords));
   return KMOE_OK;
 }
 

@@ -94,6 +94,17 @@ __device__ __forceinline__ uint8_t *paged_block(const PagedArgs &a, int64_t bloc
   return a.pages + (id * a.n_kv + g) * block_bytes;
 }
 
+// Sequences with pages in common (kmoe_paged_groups): group i holds sequences start[i] ..
+// start[i + 1] - 1 and the first pages[i] columns of its first one's table. skip: tiles
+// of 32 positions that a sequence leaves to its group; ml: maximum and sum of the weights
+// of what the group's positions give a row's head, whose weighted mean stands in out.
+struct SharedArgs {
+  const int32_t *start, *pages;
+  int n_group;
+  int32_t *skip;
+  float *ml;
+};
+
 hipError_t launch_paged_store(hipStream_t st, const PagedArgs &a, const float *q, int64_t q_stride, const float *k,
                               int64_t k_stride, const float *v, int64_t v_stride, int n_head, int rope_dim,
                               const float *inv_freq, int neox, float *q_out);
@@ -106,5 +117,10 @@ size_t paged_part_floats();
 int paged_counters();
 hipError_t launch_paged_attention(hipStream_t st, const PagedArgs &a, const float *q, int n_head, int64_t window,
                                   int64_t n_sink, float *out, float *part, uint32_t *counters);
+
+// Rows by heads that ml holds.
+constexpr int64_t kSharedHeads = (int64_t)1 << 21;
+hipError_t launch_paged_attention_shared(hipStream_t st, const PagedArgs &a, const SharedArgs &sa, const float *q,
+                                         int n_head, float *out, float *part, uint32_t *counters);
 
 }  // namespace kmoe

@@ -214,17 +214,40 @@ struct Span {
   int n_first, first, vt;
   __device__ __forceinline__ int tile(int v) const { return v < n_first ? v : first + (v - n_first); }
 };
-__device__ __forceinline__ Span span_of(int64_t pos_lo, int64_t pos_hi, int64_t cap, int window, int sink) {
+__device__ __forceinline__ Span span_of(int64_t pos_lo, int64_t pos_hi, int64_t cap, int window, int sink, int skip = 0) {
   const int64_t hi = pos_hi + 1 < cap ? pos_hi + 1 : cap;
   if (hi <= 0) return Span{0, 0, 0};
   const int t_hi = (int)((hi + kTile - 1) / kTile);
-  if (window == 0) return Span{0, 0, t_hi};
+  if (window == 0) return Span{0, skip, t_hi > skip ? t_hi - skip : 0};  // (skip: without a window only)
   const int64_t lo = pos_lo - window + 1 > 0 ? pos_lo - window + 1 : 0;
   int t_lo = (int)(lo / kTile);
   t_lo = t_lo < t_hi ? t_lo : t_hi;
   const int s_hi = (int)(((sink < hi ? sink : hi) + kTile - 1) / kTile);
   const int n = s_hi < t_lo ? s_hi : t_lo;
   return Span{n, t_lo, n + t_hi - t_lo};
+}
+
+// What a launch works: whole sequences; what the sequences of each group have in common
+// (kShared: a group counts as a sequence, all its rows see all of it); or what is left of
+// the sequences then (kOwn).
+enum { kWhole = 0, kShared = 1, kOwn = 2 };
+
+// Rows of group i together, its first sequence, and its positions in common.
+__device__ __forceinline__ void group_rows(const PagedArgs &a, const SharedArgs &s, int i, int &b0, int64_t &r0, int64_t &n,
+                                           int64_t &len) {
+  int lo = s.start[i], hi = s.start[i + 1];
+  lo = lo < 0 ? 0 : lo;
+  hi = hi > a.n_seq ? a.n_seq : hi;
+  int32_t pages = s.pages[i];
+  pages = pages < 0 ? 0 : pages < a.table_cols ? pages : a.table_cols;
+  len = (int64_t)pages * a.page;
+  b0 = lo;
+  r0 = n = 0;
+  if (hi - lo <= 1 || !pages) return;  // (one sequence alone has nothing in common)
+  int64_t r1, m;
+  paged_rows(a, lo, r0, n);
+  paged_rows(a, hi - 1, r1, m);
+  n = r1 + m > r0 ? r1 + m - r0 : 0;
 }
 
 // How a call's work is shared out. A column tile is COLS columns: the sequence's
@@ -247,20 +270,25 @@ struct Shares {
 };
 
 struct SeqPlan {
-  int n_ct, per;  // column tiles; tiles of the line per unit
-  __device__ __forceinline__ int pairs() const { return (n_ct + 1) >> 1; }
+  int n_ct, per, units;  // column tiles; tiles of the line per unit; units per kv head
 };
-template <class SH>
-__device__ __forceinline__ SeqPlan seq_plan(int64_t n, int64_t len, int group, int64_t cap, int window, int sink) {
+template <class SH, int MODE>
+__device__ __forceinline__ SeqPlan seq_plan(int64_t n, int64_t len, int group, int64_t cap, int window, int sink, int skip) {
   constexpr int COLS = SH::COLS;
-  SeqPlan r{((int)n * group + COLS - 1) / COLS, 0};
+  SeqPlan r{((int)n * group + COLS - 1) / COLS, 0, 0};
   if (r.n_ct == 0) return r;
-  const int all = span_of(0, len - 1, cap, 0, 0).vt;  // of the last row without a window
+  if constexpr (MODE == kShared) {  // every column tile sees everything: a unit of its own
+    r.per = SH::cost + SH::up((int)(len / kTile));
+    r.units = r.n_ct;
+    return r;
+  }
+  r.units = (r.n_ct + 1) >> 1;
+  const int all = span_of(0, len - 1, cap, 0, 0, skip).vt;  // of the last row without a window
   // most of a column tile, and most of two that are paired: their last rows lie
   // (n_ct - 1) COLS / group + COLS / group positions after the first row together
   int one = all;
   const int64_t base = len - n > 0 ? len - n : 0;
-  int64_t two = (2 * base + (uint32_t)((r.n_ct + 1) * COLS) / (uint32_t)group + 3 + kTile - 1) / kTile + 2;
+  int64_t two = (2 * base + (uint32_t)((r.n_ct + 1) * COLS) / (uint32_t)group + 3 + kTile - 1) / kTile + 2 - 2 * skip;
   two = two < 2 * (int64_t)all ? two : 2 * (int64_t)all;
   if (window) {
     const int64_t w = (int64_t)(sink + kTile - 1) / kTile + (window + (n < COLS ? n : COLS) + kTile - 2) / kTile + 1;
@@ -293,20 +321,31 @@ __device__ __forceinline__ int64_t scan(int64_t x, int64_t &total, int64_t *red)
   return x;
 }
 
-// start[b] (b <= n_seq): the line's tiles before sequence b; lens[b]: its length.
-template <class SH>
-__device__ void make_plan(const PagedArgs &a, int group, int64_t cap, int window, int sink, int64_t *start,
-                          int32_t *lens, int64_t *red) {
-  const int per = (a.n_seq + 255) / 256, b0 = threadIdx.x * per;
+// start[b] (b <= n, the sequences or groups): the line's tiles before sequence b; lens[b]: its length, kOwn:
+// lens[n + b]: the tiles of it that its group works.
+template <class SH, int MODE>
+__device__ void make_plan(const PagedArgs &a, const SharedArgs &sa, int n_seq, int group, int64_t cap, int window, int sink,
+                          int64_t *start, int32_t *lens, int64_t *red) {
+  const int per = (n_seq + 255) / 256, b0 = threadIdx.x * per;
   auto space = [&](int b) -> int64_t {
-    int64_t r0, n;
-    paged_rows(a, b, r0, n);
-    const int32_t len = a.seq_len[b] > 0 ? a.seq_len[b] : 0;  // (a length below the rows leaves them nothing)
-    lens[b] = len;
-    const SeqPlan s = seq_plan<SH>(n, len, group, cap, window, sink);
-    return (int64_t)s.pairs() * a.n_kv * s.per;
+    int64_t r0, n, len;
+    int skip = 0;
+    if constexpr (MODE == kShared) {
+      int first;
+      group_rows(a, sa, b, first, r0, n, len);
+    } else {
+      paged_rows(a, b, r0, n);
+      len = a.seq_len[b] > 0 ? a.seq_len[b] : 0;  // (a length below the rows leaves them nothing)
+      if constexpr (MODE == kOwn) {
+        skip = sa.skip[b];
+        lens[n_seq + b] = skip;
+      }
+    }
+    lens[b] = (int32_t)len;
+    const SeqPlan s = seq_plan<SH, MODE>(n, len, group, cap, window, sink, skip);
+    return (int64_t)s.units * a.n_kv * s.per;
   };
-  if (a.n_seq == 1) {  // (no scan: 37 positions 9.3 -> 8.6 us)
+  if (n_seq == 1) {  // (no scan: 37 positions 9.3 -> 8.6 us)
     const int64_t x = space(0);
     if (threadIdx.x == 0) {
       start[0] = 0;
@@ -316,17 +355,17 @@ __device__ void make_plan(const PagedArgs &a, int group, int64_t cap, int window
     return;
   }
   int64_t sum = 0, total;
-  for (int b = b0; b < b0 + per && b < a.n_seq; ++b) sum += space(b);
+  for (int b = b0; b < b0 + per && b < n_seq; ++b) sum += space(b);
   int64_t at = scan(sum, total, red);
   if (per == 1) {
-    if (b0 < a.n_seq) start[b0] = at;
+    if (b0 < n_seq) start[b0] = at;
   } else {
-    for (int b = b0; b < b0 + per && b < a.n_seq; ++b) {
+    for (int b = b0; b < b0 + per && b < n_seq; ++b) {
       start[b] = at;
       at += space(b);
     }
   }
-  if (threadIdx.x == 0) start[a.n_seq] = total;
+  if (threadIdx.x == 0) start[n_seq] = total;
   __syncthreads();
 }
 
@@ -344,13 +383,14 @@ __device__ __forceinline__ int64_t uniform64(int64_t x) {
 // columns are c0 .. c0 + nv - 1; column c is row i0 + (h0 + c) / group, head
 // (h0 + c) % group of the sequence's rows.
 struct Seg {
-  int b, g, n, len, pos0;  // pos0: the position of row 0
+  int b, g, n, len, pos0;  // pos0: the position of row 0 (kShared: of every row); b: the sequence whose pages are read
   int r0;
   int nv, i0, h0;
   Span sp;
   int at, v_last;
   int w_first, n_seg;  // the stretches that the column tile lies in
   int first;           // it starts in this one
+  int skip;            // tiles that the sequence's group works
 };
 
 // Of a segment that every lane reads at one place.
@@ -364,21 +404,22 @@ __device__ __forceinline__ Seg uniform(const Seg &x) {
   return __builtin_bit_cast(Seg, r);
 }
 
-template <class SH>
+template <class SH, int MODE>
 struct Cursor {
   const PagedArgs &a;
+  const SharedArgs &sa;
   const int64_t *start;
   const int32_t *lens;
-  int group, window, sink, rank, b;
+  int n_seq, group, window, sink, rank, b;
   int64_t cap, share, x0, x1, x;
 
   // This work-group's stretch; neighbours in the line share an XCD's L2.
-  __device__ __forceinline__ Cursor(const PagedArgs &a_, int nh, int window_, int sink_, int64_t *start_, int32_t *lens_,
-                                    int64_t *red)
-      : a(a_), start(start_), lens(lens_), group(nh / a_.n_kv), window(window_), sink(sink_),
-        cap((int64_t)a_.table_cols * a_.page) {
-    make_plan<SH>(a, group, cap, window, sink, start_, lens_, red);
-    const int64_t total = uniform64(start[a.n_seq]);
+  __device__ __forceinline__ Cursor(const PagedArgs &a_, const SharedArgs &sa_, int nh, int window_, int sink_,
+                                    int64_t *start_, int32_t *lens_, int64_t *red)
+      : a(a_), sa(sa_), start(start_), lens(lens_), n_seq(MODE == kShared ? sa_.n_group : a_.n_seq), group(nh / a_.n_kv),
+        window(window_), sink(sink_), cap((int64_t)a_.table_cols * a_.page) {
+    make_plan<SH, MODE>(a, sa, n_seq, group, cap, window, sink, start_, lens_, red);
+    const int64_t total = uniform64(start[n_seq]);
     rank = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
     share = div64(total + gridDim.x - 1, gridDim.x);
     share = share < SH::least ? SH::least : share < 4 * SH::STEP ? SH::up((int)share) : share;
@@ -387,11 +428,11 @@ struct Cursor {
     // 58 us; 4000 rows, 32 heads: 434 -> 380; twice that many tiles: 1200 rows, 32
     // heads, 66 -> 84). Where not all work-groups are needed, equal parts of a unit
     // (64 rows at 700 positions, 32 heads: 30 -> 23 us).
-    if (SH::COLS > 16 && a.n_seq == 1) {
+    if (MODE == kWhole && SH::COLS > 16 && n_seq == 1) {
       int64_t r0, n;
       paged_rows(a, 0, r0, n);
-      const SeqPlan p = seq_plan<SH>(n, lens[0], group, cap, window, sink);
-      const int64_t units = (int64_t)p.pairs() * a.n_kv;
+      const SeqPlan p = seq_plan<SH, MODE>(n, lens[0], group, cap, window, sink, 0);
+      const int64_t units = (int64_t)p.units * a.n_kv;
       if (share <= SH::least) {
         const int parts = p.per / SH::least;
         if (parts) share = SH::up((p.per + parts - 1) / parts);
@@ -405,7 +446,7 @@ struct Cursor {
     x = x0;
     int lo = 0;
     if (x0 < x1)  // the last sequence that starts at or before x0
-      for (int hi = a.n_seq; hi - lo > 1;) {
+      for (int hi = n_seq; hi - lo > 1;) {
         const int mid = (lo + hi) >> 1;
         if (start[mid] <= x0) lo = mid;
         else hi = mid;
@@ -419,7 +460,14 @@ struct Cursor {
       while (uniform64(start[b + 1]) <= x) ++b;
       const int64_t sb = uniform64(start[b]);
       s.b = b;
-      if (a.row_start) {
+      s.skip = 0;
+      if constexpr (MODE == kShared) {
+        int64_t r0, n, len;
+        group_rows(a, sa, b, s.b, r0, n, len);
+        s.b = __builtin_amdgcn_readfirstlane(s.b);
+        s.r0 = __builtin_amdgcn_readfirstlane((int)r0);
+        s.n = __builtin_amdgcn_readfirstlane((int)n);
+      } else if (a.row_start) {
         const const_i32 rs = (const_i32)(uintptr_t)a.row_start + b;
         s.r0 = rs[0] < 0 ? 0 : rs[0];
         const int hi = rs[1] < (int)a.s_rows ? rs[1] : (int)a.s_rows;
@@ -429,19 +477,21 @@ struct Cursor {
         s.n = b < a.s_rows ? 1 : 0;
       }
       s.len = __builtin_amdgcn_readfirstlane(lens[b]);
-      s.pos0 = s.len - s.n;
+      if constexpr (MODE == kOwn) s.skip = __builtin_amdgcn_readfirstlane(lens[n_seq + b]);
+      s.pos0 = MODE == kShared ? s.len - 1 : s.len - s.n;
       const int n_cols = s.n * group;
-      const SeqPlan plan = seq_plan<SH>(s.n, s.len, group, cap, window, sink);
+      const SeqPlan plan = seq_plan<SH, MODE>(s.n, s.len, group, cap, window, sink, s.skip);
       const int64_t unit = div64(x - sb, plan.per);
       const int off = (int)(x - sb - unit * plan.per);
-      s.g = (int)div64(unit, plan.pairs());
-      const int pair = (int)(unit - (int64_t)s.g * plan.pairs());
+      s.g = (int)div64(unit, plan.units);
+      const int pair = (int)(unit - (int64_t)s.g * plan.units);
       auto span = [&](int ct) {
+        if constexpr (MODE == kShared) return Span{0, 0, s.len / kTile};
         const int c = ct * COLS, e = c + COLS < n_cols ? c + COLS : n_cols;
         return span_of(s.pos0 + (int)((uint32_t)c / (uint32_t)group), s.pos0 + (int)((uint32_t)(e - 1) / (uint32_t)group),
-                       cap, window, sink);
+                       cap, window, sink, s.skip);
       };
-      const int ct_a = plan.n_ct - 1 - pair;
+      const int ct_a = MODE == kShared ? pair : plan.n_ct - 1 - pair;
       const Span sp_a = span(ct_a);
       const int len_a = SH::up(sp_a.vt > 0 ? sp_a.vt : 1);
       const bool second = off >= len_a;

@@ -101,6 +101,24 @@ constexpr int paged_occ(int hd, int c) { return hd == 64 ? (c == 1 ? 4 : 3) : (c
 template <int HD, int COLS>
 using Work = Shares<COLS, 4, (HD == 64 && COLS == 16 ? 12 : 8), 8, 24>;
 
+// sa.skip: what a sequence's group works of it, where all its rows lie behind that.
+__device__ void find_skip(const PagedArgs &a, const SharedArgs &sa) {
+  for (int b = threadIdx.x; b < a.n_seq; b += 256) {
+    int lo = 0;  // the last group that starts at or before b
+    for (int hi = sa.n_group; hi - lo > 1;) {
+      const int mid = (lo + hi) >> 1;
+      if (sa.start[mid] <= b) lo = mid;
+      else hi = mid;
+    }
+    int b0;
+    int64_t r0, n, len, at, m;
+    group_rows(a, sa, lo, b0, r0, n, len);
+    paged_rows(a, b, at, m);
+    const bool in = sa.start[lo] <= b && b < sa.start[lo + 1] && m > 0 && at >= r0 && at + m <= r0 + n;
+    sa.skip[b] = in && (int64_t)a.seq_len[b] - m >= len ? (int)(len / kTile) : 0;
+  }
+}
+
 // Work-group: four waves, one segment of a column tile at a time; wave w takes
 // its tiles w, w + 4, ... (32 positions each) with its own running softmax, and
 // the waves are merged through LDS.
@@ -117,12 +135,15 @@ using Work = Shares<COLS, 4, (HD == 64 && COLS == 16 ? 12 : 8), 8, 24>;
 // is summed 32 dims at a time, one K step, and scaled by the position's scale of
 // those; a value, eight bits times eleven, is the sum of two f16 exactly.
 // The running maximum is in units of log2 e.
-template <int T, int HD, int C>
+//
+// MODE (see kmoe_paged_attn.h): kShared leaves a row's mean over its group's positions in
+// out, with the maximum and sum of the weights in sa.ml; kOwn joins that with its own.
+template <int T, int HD, int C, int MODE>
 __global__ void __launch_bounds__(256, paged_occ(HD, C))
-    k_paged_attn(PagedArgs a, const float *__restrict__ q, int nh, int window, int sink, float *__restrict__ part,
-                 float *__restrict__ part_ml, uint32_t *counters, float *__restrict__ out) {
+    k_paged_attn(PagedArgs a, SharedArgs sa, const float *__restrict__ q, int nh, int window, int sink,
+                 float *__restrict__ part, float *__restrict__ part_ml, uint32_t *counters, float *__restrict__ out) {
   constexpr int NT = HD / 32, NU = HD / 16, COLS = 16 * C, OROW = HD + 4;
-  extern __shared__ int64_t start[];  // [n_seq + 1], then the lengths [n_seq]
+  extern __shared__ int64_t start[];  // [n + 1] for n sequences (kShared: groups), then the lengths [n], kOwn: and what is skipped [n]
   __shared__ union {
     u32x4 q[C][NT][2][64];
     float o[4][COLS][OROW];
@@ -137,7 +158,10 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
   const int group = nh / a.n_kv, magic = 65536 / group + 1;  // x / group = x * magic >> 16 for x < 4096
   const int64_t bb = paged_block_bytes(T, a.page, HD);
   const int pshift = __builtin_ctz(a.page);
-  Cursor<Work<HD, COLS>> cur(a, nh, window, sink, start, (int32_t *)(start + a.n_seq + 1), red);
+  if constexpr (MODE == kShared)
+    if (blockIdx.x == gridDim.x - 1) find_skip(a, sa);
+  Cursor<Work<HD, COLS>, MODE> cur(a, sa, nh, window, sink, start,
+                                   (int32_t *)(start + (MODE == kShared ? sa.n_group : a.n_seq) + 1), red);
   const int64_t cap = cur.cap;
 
   // wave 3 finds the next segment while this one's first loads are on their way (all
@@ -159,7 +183,8 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
     const Span sp = s_.sp;
     auto row_of = [&](int c) { return s_.i0 + (((s_.h0 + c) * magic) >> 16); };
     auto head_of = [&](int c) { return s_.h0 + c - (((s_.h0 + c) * magic) >> 16) * group; };
-    const int64_t pos_lo = pos0 + s_.i0, pos_hi = pos0 + row_of(nv - 1);
+    auto pos_of = [&](int c) { return MODE == kShared ? pos0 : pos0 + row_of(c); };
+    const int64_t pos_lo = MODE == kShared ? pos0 : pos0 + s_.i0, pos_hi = pos_of(nv - 1);
     const int hi_pos = (int)(pos_hi + 1 < cap ? pos_hi + 1 : cap);  // the columns' positions end here
     const int lo_pos = window && pos_lo - window + 1 > 0 ? (int)(pos_lo - window + 1) : 0;
 
@@ -222,7 +247,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const int cc = 16 * j + c16;
-      const int64_t p = pos0 + row_of(cc < nv ? cc : nv - 1);
+      const int64_t p = pos_of(cc < nv ? cc : nv - 1);
       pos_c[j] = cc < nv ? (int)(p < cap ? p : cap - 1) : -1;
       lo_c[j] = window && p - window + 1 > 0 ? (int)(p - window + 1) : 0;
     }
@@ -445,15 +470,31 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
     auto finish = [&](int c, int d, const f32x4 &y, float M, float Lsum) {
       const float inv = M == -INFINITY ? 0.0f : 1.0f / (kUp * Lsum);  // nothing seen: zeros
       const int i = row_of(c);
+      const int64_t at = (r0 + i) * nh + (int64_t)g * group + head_of(c);
       bool fin = true;
       f32x4a4 r;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        r[k] = y[k] * inv;
-        fin = fin && fabsf(r[k]) < INFINITY;
+      for (int k = 0; k < 4; ++k) r[k] = y[k] * inv;
+      if constexpr (MODE == kShared) {  // (one that is not finite makes the joined one so)
+        if (d == 0) *(f32x2 *)(sa.ml + 2 * at) = f32x2{M, Lsum};
       }
-      *(f32x4a4 *)(out + ((r0 + i) * nh + (int64_t)g * group + head_of(c)) * HD + d) = r;
-      if (!fin || (M == -INFINITY && Lsum > 0.0f && pos0 + i >= 0)) atomicOr(&bad_cols, 1u << c);
+      if constexpr (MODE == kOwn) {
+        if (s_.skip) {
+          const f32x2 gs = *(const f32x2 *)(sa.ml + 2 * at);
+          const f32x4a4 o = *(const f32x4a4 *)(out + at * HD + d);
+          const float Mj = fmaxf(M, gs.x), Mb = Mj == -INFINITY ? 0.0f : Mj;
+          const float wo = Lsum * __builtin_amdgcn_exp2f(M - Mb), wg = gs.y * __builtin_amdgcn_exp2f(gs.x - Mb);
+          const float ij = Mj == -INFINITY ? 0.0f : 1.0f / (wo + wg);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) r[k] = (r[k] * wo + o[k] * wg) * ij;
+          M = Mj;
+          Lsum += gs.y;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) fin = fin && fabsf(r[k]) < INFINITY;
+      *(f32x4a4 *)(out + at * HD + d) = r;
+      if (MODE != kShared && (!fin || (M == -INFINITY && Lsum > 0.0f && pos0 + i >= 0))) atomicOr(&bad_cols, 1u << c);
     };
     for (int e = tl; e < nv * (HD / 4); e += 256) {
       const int c = e / (HD / 4), d = e % (HD / 4) * 4;
@@ -602,24 +643,25 @@ size_t paged_part_floats() {
 }
 int paged_counters() { return paged_grid(64, 1); }
 
-hipError_t launch_paged_attention(hipStream_t st, const PagedArgs &a, const float *q, int n_head, int64_t window,
-                                  int64_t n_sink, float *out, float *part, uint32_t *counters) {
-  const int group = n_head / a.n_kv;
-  const int w = window >= INT32_MAX ? 0 : (int)window, sink = (int)(n_sink < (1 << 30) ? n_sink : (1 << 30));
+// sa: of a launch over groups, or over what they leave (MODE).
+template <int MODE>
+static hipError_t launch_mode(hipStream_t st, const PagedArgs &a, const SharedArgs &sa, const float *q, int n_head, int w,
+                              int sink, float *out, float *part, uint32_t *counters) {
+  const int group = n_head / a.n_kv, n_seq = MODE == kShared ? sa.n_group : a.n_seq;
   // 16 columns per tile where sequences have few rows: at 32 columns each 36 us with
   // 16, 23 with 32 (16 sequences of 2000 positions, Q8_0, heads of 64); decode steps
   // of 8 heads would leave three quarters of 32 idle
-  const bool one = a.s_rows * group <= (int64_t)24 * a.n_seq;
+  const bool one = a.s_rows * group <= (int64_t)24 * n_seq;
   const int cols = one ? 16 : 32, full = paged_grid(a.hd, one ? 1 : 2);
   // no more work-groups than the longest sequences that the table allows would fill
-  const int64_t units = (a.s_rows * group / cols + a.n_seq) * a.n_kv;
+  const int64_t units = (a.s_rows * group / cols + n_seq) * a.n_kv;
   const int cost = one && a.hd == 64 ? Work<64, 16>::cost : Work<128, 16>::cost;
   const int64_t most = units * (((int64_t)a.table_cols * a.page / kTile + cost) / Work<64, 16>::least + 2);
   const unsigned grid = (unsigned)std::min<int64_t>(full, (most + 7) / 8 * 8);
-  const size_t lds = (size_t)(a.n_seq + 1) * 8 + (size_t)a.n_seq * 4;
+  const size_t lds = (size_t)(n_seq + 1) * 8 + (size_t)n_seq * (MODE == kOwn ? 8 : 4);
   float *ml = part + (size_t)2 * full * cols * a.hd;
 #define KMOE_PAGED(T, H, C) \
-  KMOE_LAUNCH((k_paged_attn<T, H, C>), dim3(grid), dim3(256), lds, st, a, q, n_head, w, sink, part, ml, counters, out)
+  KMOE_LAUNCH((k_paged_attn<T, H, C, MODE>), dim3(grid), dim3(256), lds, st, a, sa, q, n_head, w, sink, part, ml, counters, out)
 #define KMOE_PAGED_C(T, H)        \
   do {                            \
     if (one) KMOE_PAGED(T, H, 1); \
@@ -635,6 +677,18 @@ hipError_t launch_paged_attention(hipStream_t st, const PagedArgs &a, const floa
 #undef KMOE_PAGED_C
 #undef KMOE_PAGED
   return hipGetLastError();
+}
+
+hipError_t launch_paged_attention(hipStream_t st, const PagedArgs &a, const float *q, int n_head, int64_t window,
+                                  int64_t n_sink, float *out, float *part, uint32_t *counters) {
+  const int w = window >= INT32_MAX ? 0 : (int)window, sink = (int)(n_sink < (1 << 30) ? n_sink : (1 << 30));
+  return launch_mode<kWhole>(st, a, SharedArgs{}, q, n_head, w, sink, out, part, counters);
+}
+
+hipError_t launch_paged_attention_shared(hipStream_t st, const PagedArgs &a, const SharedArgs &sa, const float *q,
+                                         int n_head, float *out, float *part, uint32_t *counters) {
+  const hipError_t e = launch_mode<kShared>(st, a, sa, q, n_head, 0, 0, out, part, counters);
+  return e == hipSuccess ? launch_mode<kOwn>(st, a, sa, q, n_head, 0, 0, out, part, counters) : e;
 }
 
 }  // namespace kmoe

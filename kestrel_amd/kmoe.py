@@ -111,6 +111,7 @@ SIGNATURES = {
     "kmoe_paged_rope_kv_store": (C.c_int, [_P, _P, _P, _P, _P, _i64, _P, _i64, _P, _i64, _i32, _i32, _P, _i32, _P]),
     "kmoe_paged_kv_read": (C.c_int, [_P, _P, _P, _P, _P, _P]),
     "kmoe_paged_attention": (C.c_int, [_P, _P, _P, _P, _P, _i32, _i64, _i64, _P]),
+    "kmoe_paged_attention_shared": (C.c_int, [_P, _P, _P, _P, _P, _P, _i32, _P]),
     "kmoe_pages_copy": (C.c_int, [_P, _P, _P, _i64, _i64, _P, _P, _i64]),
     "kmoe_pages_create": (C.c_int, [_i64, _i32, C.POINTER(_P)]),
     "kmoe_pages_clone": (C.c_int, [_P, C.POINTER(_P)]),
@@ -165,6 +166,12 @@ class PagedBatch(C.Structure):
 
     _fields_ = [("n_seq", _i32), ("table_cols", _i32), ("s_rows", _i64), ("row_start", _P), ("seq_len", _P),
                 ("table", _P)]
+
+
+class PagedGroups(C.Structure):
+    """kmoe_paged_groups (include/kmoe.h), with the tensors it points into."""
+
+    _fields_ = [("n_group", _i32), ("start", _P), ("pages", _P)]
 
 
 @dataclass(frozen=True)
@@ -466,6 +473,29 @@ class Context:
             self._need("out", out, f, *shape)
         self.check(self.lib.kmoe_paged_attention(self.h, self._pages(kv, pages), _ptr(pages), C.byref(batch), _ptr(q),
                                                  n_head, window, n_sink, _ptr(out)))
+        return out
+
+    def paged_groups(self, start, pages) -> PagedGroups:
+        """kmoe_paged_groups: sequences start[i] .. start[i + 1] - 1 of a batch share the first pages[i] pages; int32 on
+        the device (start [n + 1], pages [n]), read when a call's kernels run. The struct keeps them alive."""
+        i32, n = self.torch.int32, pages.numel()
+        self._need("pages", pages, i32, 1, n)
+        self._need("start", start, i32, 1, n + 1)
+        g = PagedGroups(n, _ptr(start), _ptr(pages) or None)
+        g.keep = (start, pages)
+        return g
+
+    def paged_attention_shared(self, kv: PagedKV, pages, batch: PagedBatch, groups: PagedGroups, q, n_head: int, out=None):
+        """paged_attention of a batch whose groups of sequences have their first pages in common, read once for all of
+        a group's rows."""
+        shape, f = (batch.s_rows, n_head * kv.head_dim), self.torch.float32
+        self._need("q", q, f, *shape)
+        if out is None:
+            out = self._empty(shape, f)
+        else:
+            self._need("out", out, f, *shape)
+        self.check(self.lib.kmoe_paged_attention_shared(self.h, self._pages(kv, pages), _ptr(pages), C.byref(batch),
+                                                        C.byref(groups), _ptr(q), n_head, _ptr(out)))
         return out
 
     @staticmethod
