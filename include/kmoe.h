@@ -618,6 +618,31 @@ typedef struct {
 int kmoe_paged_attention_shared(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *pages_dev,
                                 const kmoe_paged_batch *batch, const kmoe_paged_groups *groups, const float *q_dev,
                                 int32_t n_head, float *out_dev);
+/* Bounds of the pages' keys, for kmoe_paged_attention_selected: bounds [n_pages, n_kv, 2,
+ * head_dim] f16 (16-byte aligned), kept by the caller beside the pages of a layer, receives for
+ * every page that the batch's rows lie on the least and the largest value of each dim
+ * among its sequence's positions on that page (from its first position on, the new rows
+ * included; KMOE_Q8_0: quant * scale, rounded to the nearest f16 and kept finite). So a call
+ * after every store keeps them up to date; they are formed anew from the page each
+ * time, and do not depend on what was there. A NaN key is passed over. A page without an
+ * entry in the table, and the others, are left as they were. Copies of pages need
+ * copies of their bounds. */
+int kmoe_paged_bounds(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *pages_dev, const kmoe_paged_batch *batch,
+                      uint16_t *bounds_dev);
+/* kmoe_paged_attention (without a window) over some of the pages, chosen for each row
+ * and kv head: the row's own page, up to its position; the first n_first; and of
+ * those between them the ones with the largest
+ *   sum over the kv head's heads, sum over dims d of max(q_d lo_d, q_d hi_d)
+ * by the pages' bounds, in 64 bits, equal ones by position; n_select pages in all (0 <=
+ * n_first < n_select), all that there are where they are fewer. A page without an entry
+ * in the table is not chosen. A NaN score counts as the best. No score of a position
+ * passes its page's, summed over the heads; pages whose keys lie apart from the query's direction are not read. With
+ * n_select >= table_cols it is kmoe_paged_attention itself. table_cols up to 2^20 and
+ * n_pages * n_kv up to 2^31 - 1 (KMOE_E_UNSUPPORTED past them). Besides that call's workspace it keeps one of
+ * 50 MB, with the same rules. */
+int kmoe_paged_attention_selected(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *pages_dev,
+                                  const uint16_t *bounds_dev, const kmoe_paged_batch *batch, const float *q_dev,
+                                  int32_t n_head, int32_t n_select, int32_t n_first, float *out_dev);
 /* Pages src[i] onto dst[i], i < n, in each of n_layer buffers layer_stride
  * bytes apart (16-byte aligned; desc->n_pages pages each). src and dst are
  * host arrays, read before the call returns (the copies are asynchronous and

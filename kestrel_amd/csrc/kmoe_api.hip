@@ -193,6 +193,7 @@ struct kmoe_ctx {
   std::string err;
   int regime = KMOE_REGIME_AVX2;
   // device, zero between calls: kCounterWords completion counters, then the paged attention's
+  // and its choice of pages'
   uint32_t *counters = nullptr;
   uint64_t vram_limit = 0;
   uint64_t vram_reserved = 0;
@@ -225,9 +226,9 @@ struct kmoe_ctx {
   hipEvent_t pws_event = nullptr;
   std::vector<void *> pws_retired;
   // scratch of one size each, allocated at the first call that takes it and kept:
-  // partials of the paged attention's split units, the shared parts of its rows, what
-  // sampling finds of the chunks
-  Kept paged, shared, sample;
+  // partials of the paged attention's split units, the shared parts of its rows, the choice
+  // of pages, what sampling finds of the chunks
+  Kept paged, shared, select, sample;
   // last moe_ffn routing (pointers into ws) and its sizes
   uint32_t *last_idx = nullptr, *last_perm = nullptr, *last_off = nullptr;
   float *last_w = nullptr;
@@ -732,7 +733,7 @@ void leave_kept(kmoe_ctx *c, Kept &k, hipStream_t next) {
 
 // The stream is about to change: the last use of the pieces is marked on its own.
 void leave_stream(kmoe_ctx *c, hipStream_t next) {
-  for (Kept *k : {&c->paged, &c->shared, &c->sample}) leave_kept(c, *k, next);
+  for (Kept *k : {&c->paged, &c->shared, &c->select, &c->sample}) leave_kept(c, *k, next);
   if (!c->pws_used || next == c->pws_stream || capturing(c->pws_stream) || capturing(next)) return;
   DeviceGuard g(c->device);
   if ((!c->pws_event && hipEventCreateWithFlags(&c->pws_event, hipEventDisableTiming) != hipSuccess) ||
@@ -852,7 +853,7 @@ int kmoe_create(int device, kmoe_ctx **out) {
   }
   c->stream = c->own;
   // completion counters of multi-work-group kernels; zero between calls
-  const size_t cw = ((size_t)kCounterWords + paged_counters()) * 4;
+  const size_t cw = ((size_t)kCounterWords + paged_counters() + select_counters()) * 4;
   if (hipMalloc((void **)&c->counters, cw) != hipSuccess || hipMemset(c->counters, 0, cw) != hipSuccess) {
     (void)hipStreamDestroy(c->own);
     delete c;
@@ -897,7 +898,7 @@ int kmoe_destroy(kmoe_ctx *c) {
   if (c->pws) (void)hipFree(c->pws);
   for (void *p : c->pws_retired) (void)hipFree(p);
   if (c->pws_event) (void)hipEventDestroy(c->pws_event);
-  for (Kept *k : {&c->paged, &c->shared, &c->sample}) {
+  for (Kept *k : {&c->paged, &c->shared, &c->select, &c->sample}) {
     if (k->p) (void)hipFree(k->p);
     if (k->event) (void)hipEventDestroy(k->event);
     if (k->cap_event) (void)hipEventDestroy(k->cap_event);
@@ -2726,6 +2727,54 @@ int kmoe_paged_attention_shared(kmoe_ctx *c, const kmoe_paged_desc *d, const voi
   const SharedArgs sa{groups->start_dev, groups->pages_dev, groups->n_group, (int32_t *)(ml + kSharedHeads * 8), (float *)ml};
   LAUNCH(c, "paged_attention_shared", launch_paged_attention_shared(c->stream, a, sa, q, n_head, out, (float *)part,
                                                                     c->counters + kCounterWords));
+  return KMOE_OK;
+}
+
+int kmoe_paged_bounds(kmoe_ctx *c, const kmoe_paged_desc *d, const void *pages, const kmoe_paged_batch *b,
+                      uint16_t *bounds) {
+  if (!c) return KMOE_E_INVALID;
+  PagedArgs a;
+  int rc = check_paged(c, d, pages, b, &a);
+  if (rc || a.s_rows == 0) return rc;
+  if (!bounds) return fail(c, KMOE_E_INVALID, "null pointer");
+  if ((uintptr_t)bounds & 15) return fail(c, KMOE_E_INVALID, "bounds not 16-byte aligned");
+  const uintptr_t pb = (uintptr_t)a.n_pages * a.n_kv * paged_block_bytes(a.type, a.page, a.hd), bytes = (uintptr_t)a.n_pages * a.n_kv * a.hd * 4;
+  if ((uintptr_t)pages < (uintptr_t)bounds + bytes && (uintptr_t)bounds < (uintptr_t)pages + pb)
+    return fail(c, KMOE_E_INVALID, "bounds overlap the pages");
+  DeviceGuard g(c->device);
+  LAUNCH(c, "paged_bounds", launch_paged_bounds(c->stream, a, bounds));
+  return KMOE_OK;
+}
+
+int kmoe_paged_attention_selected(kmoe_ctx *c, const kmoe_paged_desc *d, const void *pages, const uint16_t *bounds,
+                                  const kmoe_paged_batch *b, const float *q, int32_t n_head, int32_t n_select,
+                                  int32_t n_first, float *out) {
+  if (!c) return KMOE_E_INVALID;
+  PagedArgs a;
+  int rc = check_paged(c, d, pages, b, &a);
+  if (rc) return rc;
+  if (n_first < 0 || n_select <= n_first)
+    return fail(c, KMOE_E_INVALID, "%d pages with the first %d among them (need 0 <= n_first < n_select)", n_select, n_first);
+  if (a.table_cols > select_max_cols() || a.n_pages * a.n_kv > INT32_MAX)
+    return fail(c, KMOE_E_UNSUPPORTED, "%d columns, %lld pages of %d kv heads (at most 2^20, and 2^31 - 1 together)",
+                a.table_cols, (long long)a.n_pages, a.n_kv);
+  rc = check_paged_q(c, a, q, n_head, out);
+  if (rc || a.s_rows == 0) return rc;
+  if (!bounds) return fail(c, KMOE_E_INVALID, "null pointer");
+  if ((uintptr_t)bounds & 15) return fail(c, KMOE_E_INVALID, "bounds not 16-byte aligned");
+  const uintptr_t bb = (uintptr_t)a.n_pages * a.n_kv * a.hd * 4, ob = (uintptr_t)a.s_rows * n_head * a.hd * 4;
+  if ((uintptr_t)out < (uintptr_t)bounds + bb && (uintptr_t)bounds < (uintptr_t)out + ob)
+    return fail(c, KMOE_E_INVALID, "out overlaps the bounds");
+  if (n_select >= a.table_cols) return kmoe_paged_attention(c, d, pages, b, q, n_head, 0, 0, out);
+  DeviceGuard g(c->device);
+  uint8_t *part = nullptr, *ws = nullptr;
+  rc = kept_ws(c, c->paged, paged_part_floats() * sizeof(float), "paged attention partials", &part);
+  if (!rc) rc = kept_ws(c, c->select, select_ws_bytes(), "choice of pages", &ws);
+  if (rc) return rc;
+  uint32_t *counters = c->counters + kCounterWords;
+  LAUNCH(c, "paged_attention_selected",
+         launch_paged_attention_selected(c->stream, a, bounds, q, n_head, n_select, n_first, out, (float *)part, counters,
+                                         ws, counters + paged_counters()));
   return KMOE_OK;
 }
 

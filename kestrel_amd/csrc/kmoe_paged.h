@@ -118,6 +118,26 @@ int paged_counters();
 hipError_t launch_paged_attention(hipStream_t st, const PagedArgs &a, const float *q, int n_head, int64_t window,
                                   int64_t n_sink, float *out, float *part, uint32_t *counters);
 
+// A choice of pages (kmoe_paged_attention_selected), for some of the rows by kv heads at a
+// time: scores holds the ranks of pages that several work-groups score, counters (zero
+// between calls) who has arrived, table, len and row_start the batch that is left, a
+// sequence of one row per row and kv head.
+struct SelectArgs {
+  PagedArgs a;
+  const uint16_t *bounds;
+  const float *q;
+  int n_head, group, n_select, n_first;
+  unsigned long long *scores;
+  int32_t *table, *len, *row_start;
+  uint32_t *counters;
+};
+int64_t select_max_cols();
+int select_counters();
+size_t select_ws_bytes();
+hipError_t launch_paged_bounds(hipStream_t st, const PagedArgs &a, uint16_t *bounds);
+hipError_t launch_paged_attention_selected(hipStream_t st, const PagedArgs &a, const uint16_t *bounds, const float *q,
+                                           int n_head, int n_select, int n_first, float *out, float *part,
+                                           uint32_t *counters, uint8_t *ws, uint32_t *select_counters);
 // Rows by heads that ml holds.
 constexpr int64_t kSharedHeads = (int64_t)1 << 21;
 hipError_t launch_paged_attention_shared(hipStream_t st, const PagedArgs &a, const SharedArgs &sa, const float *q,

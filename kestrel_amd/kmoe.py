@@ -112,6 +112,8 @@ SIGNATURES = {
     "kmoe_paged_kv_read": (C.c_int, [_P, _P, _P, _P, _P, _P]),
     "kmoe_paged_attention": (C.c_int, [_P, _P, _P, _P, _P, _i32, _i64, _i64, _P]),
     "kmoe_paged_attention_shared": (C.c_int, [_P, _P, _P, _P, _P, _P, _i32, _P]),
+    "kmoe_paged_bounds": (C.c_int, [_P, _P, _P, _P, _P]),
+    "kmoe_paged_attention_selected": (C.c_int, [_P, _P, _P, _P, _P, _P, _i32, _i32, _i32, _P]),
     "kmoe_pages_copy": (C.c_int, [_P, _P, _P, _i64, _i64, _P, _P, _i64]),
     "kmoe_pages_create": (C.c_int, [_i64, _i32, C.POINTER(_P)]),
     "kmoe_pages_clone": (C.c_int, [_P, C.POINTER(_P)]),
@@ -496,6 +498,33 @@ class Context:
             self._need("out", out, f, *shape)
         self.check(self.lib.kmoe_paged_attention_shared(self.h, self._pages(kv, pages), _ptr(pages), C.byref(batch),
                                                         C.byref(groups), _ptr(q), n_head, _ptr(out)))
+        return out
+
+    def _bounds(self, kv: PagedKV, pages, bounds):
+        n = kv.desc(pages).n_pages
+        self._need("bounds", bounds, self.torch.float16, n, kv.n_kv * 2 * kv.head_dim)
+        return _ptr(bounds)
+
+    def paged_bounds(self, kv: PagedKV, pages, batch: PagedBatch, bounds):
+        """The least and largest keys of the pages that the batch's rows lie on, into bounds [n_pages, n_kv, 2, head_dim]
+        f16 (returned): after every store, for paged_attention_selected."""
+        self.check(self.lib.kmoe_paged_bounds(self.h, self._pages(kv, pages), _ptr(pages), C.byref(batch),
+                                              self._bounds(kv, pages, bounds)))
+        return bounds
+
+    def paged_attention_selected(self, kv: PagedKV, pages, bounds, batch: PagedBatch, q, n_head: int, n_select: int,
+                                 n_first: int = 0, out=None):
+        """paged_attention of every row and kv head over n_select pages: its own, the first n_first, and those whose bounds
+        promise the largest scores."""
+        shape, f = (batch.s_rows, n_head * kv.head_dim), self.torch.float32
+        self._need("q", q, f, *shape)
+        if out is None:
+            out = self._empty(shape, f)
+        else:
+            self._need("out", out, f, *shape)
+        self.check(self.lib.kmoe_paged_attention_selected(
+            self.h, self._pages(kv, pages), _ptr(pages), self._bounds(kv, pages, bounds), C.byref(batch), _ptr(q), n_head,
+            n_select, n_first, _ptr(out)))
         return out
 
     @staticmethod
