@@ -308,6 +308,120 @@ int kmoe_pages_table(kmoe_pages *p, const uint32_t *seqs, int32_t n_seq, int32_t
   });
 }
 
+int kmoe_pages_groups(kmoe_pages *p, const uint32_t *seqs, int32_t n_seq, int64_t least, int32_t *order, int32_t *start,
+                      int32_t *shared, int32_t *n_group) {
+  if (!p) return KMOE_E_INVALID;
+  if (n_seq < 0 || least < 0 || !n_group || !start || (n_seq > 0 && (!seqs || !order || !shared)))
+    return pfail(p, KMOE_E_INVALID, "groups: bad size or null pointer");
+  return guarded(p, [&]() -> int {
+    std::vector<const Seq *> s(n_seq);
+    std::vector<int32_t> by(n_seq);  // sequences with a common beginning lie beside each other
+    std::set<uint32_t> named;
+    for (int32_t i = 0; i < n_seq; ++i) {
+      s[i] = find(p, seqs[i]);
+      if (!s[i]) return pfail(p, KMOE_E_NOT_LOADED, "groups: no sequence %u", seqs[i]);
+      if (!named.insert(seqs[i]).second) return pfail(p, KMOE_E_INVALID, "groups: sequence %u is named twice", seqs[i]);
+      by[i] = i;
+    }
+    std::sort(by.begin(), by.end(), [&](int32_t x, int32_t y) {
+      return s[x]->pages != s[y]->pages ? s[x]->pages < s[y]->pages : x < y;
+    });
+    std::vector<int64_t> lcp(n_seq, 0);  // pages that by[i] has in common with by[i - 1]
+    for (int32_t i = 1; i < n_seq; ++i) {
+      const std::vector<int32_t> &a = s[by[i - 1]]->pages, &b = s[by[i]]->pages;
+      while (lcp[i] < (int64_t)std::min(a.size(), b.size()) && a[lcp[i]] == b[lcp[i]] && a[lcp[i]] >= 0) ++lcp[i];
+    }
+    // A tree of common beginnings: a node is the first d pages of all that lie below it.
+    struct Node {
+      int64_t d;
+      std::vector<int32_t> kids;  // nodes, or ~ sequences (places in `by`)
+      int32_t level = 0, closed = 0;  // closed: levels of the nearest group above from which on it makes none
+      std::vector<int32_t> members;
+    };
+    std::vector<Node> tree(1, Node{0, {}});
+    std::vector<int32_t> path(1, 0);
+    for (int32_t i = 1; i <= n_seq; ++i) {
+      const int64_t m = i < n_seq ? lcp[i] : 0;
+      int32_t kid = ~(i - 1);
+      while (tree[path.back()].d > m) {
+        tree[path.back()].kids.push_back(kid);
+        kid = path.back();
+        path.pop_back();
+      }
+      if (tree[path.back()].d == m) {
+        tree[path.back()].kids.push_back(kid);
+      } else {
+        path.push_back((int32_t)tree.size());
+        tree.push_back(Node{m, {kid}});
+      }
+    }
+    // Nodes chosen for groups: a sequence belongs to the lowest one above it. Together they
+    // save the sum over the sequences of their node's d, less d once per node: the most
+    // of that, by the level of the lowest chosen node above (0: none), from the leaves up.
+    // (An explicit stack: nodes may nest n_seq deep.)
+    struct Step {
+      int32_t node;
+      size_t kid;
+      std::vector<int64_t> best;  // by that level, its own among them
+    };
+    std::vector<Step> todo;
+    std::vector<int64_t> depth;
+    auto enter = [&](int32_t x) {
+      tree[x].level = (int32_t)depth.size();
+      depth.push_back(tree[x].d);
+      todo.push_back(Step{x, 0, std::vector<int64_t>(depth.size(), 0)});
+    };
+    enter(0);
+    while (!todo.empty()) {
+      Step &t = todo.back();
+      Node &v = tree[t.node];
+      if (t.kid < v.kids.size()) {
+        const int32_t kid = v.kids[t.kid++];
+        if (kid >= 0) {
+          enter(kid);  // (t is not used after)
+        } else {
+          for (size_t j = 0; j < t.best.size(); ++j) t.best[j] += depth[j];
+        }
+        continue;
+      }
+      const int64_t open = t.best.back() - v.d;
+      t.best.pop_back();  // (grows with the level: the larger what a sequence has anyway)
+      v.closed = (int32_t)(std::lower_bound(t.best.begin(), t.best.end(), open) - t.best.begin());
+      if (todo.size() > 1)
+        for (size_t j = 0; j < t.best.size(); ++j) todo[todo.size() - 2].best[j] += std::max(t.best[j], open);
+      depth.pop_back();
+      todo.pop_back();
+    }
+    std::vector<std::pair<int32_t, int32_t>> down(1, {0, 0});  // a node, and the lowest chosen one above it
+    while (!down.empty()) {
+      const auto [x, above] = down.back();
+      down.pop_back();
+      const int32_t mine = x && tree[above].level < tree[x].closed ? x : above;
+      for (int32_t kid : tree[x].kids) {
+        if (kid >= 0) down.push_back({kid, mine});
+        else tree[mine].members.push_back(by[~kid]);
+      }
+    }
+    int32_t n = 0, at = 0;
+    std::vector<uint8_t> in(n_seq, 0);
+    for (size_t x = 1; x < tree.size(); ++x) {
+      const int64_t m = (int64_t)tree[x].members.size();
+      if (m < 2 || (m - 1) * tree[x].d * p->page < least) continue;
+      start[n] = at;
+      shared[n++] = (int32_t)tree[x].d;
+      for (int32_t i : tree[x].members) {
+        order[at++] = i;
+        in[i] = 1;
+      }
+    }
+    start[n] = at;
+    for (int32_t i = 0; i < n_seq; ++i)
+      if (!in[i]) order[at++] = i;
+    *n_group = n;
+    return KMOE_OK;
+  });
+}
+
 int kmoe_pages_compact(kmoe_pages *p, int32_t *src, int32_t *dst, int64_t cap, int64_t *n) {
   if (!p) return KMOE_E_INVALID;
   if (cap < 0 || !n || (cap > 0 && (!src || !dst))) return pfail(p, KMOE_E_INVALID, "compact: bad size or null pointer");

@@ -20,9 +20,10 @@ GGUF or KGUF reader hands its tensors over unchanged:
 Layers with routed experts go through kmoe_moe_ffn and its HBM expert tier;
 the rest through the decoder ops of include/kmoe.h. A single-token decode
 step reads its position from a device counter, so it is captured once as a
-HIP graph and replayed for every later token (greedy decoding keeps the
-sampled token on the device too). PagedDecoder runs many sequences together
-over a paged key-value cache.
+HIP graph and replayed for every later token (decoding keeps the sampled
+token on the device too, the largest logit's or one drawn by given random
+numbers). PagedDecoder runs many sequences together over a paged key-value
+cache, with the pages that they share read once or a choice of pages read at all.
 """
 from __future__ import annotations
 
@@ -118,8 +119,7 @@ class Decoder:
         self.cached = 0
         self.pos_dev = torch.zeros(1, dtype=torch.int32, device=dev)
         self.token_dev = torch.zeros(1, dtype=torch.int32, device=dev)
-        self.graph = None
-        self._graph_key = None  # what the graph was captured for (_key)
+        self._graphs = {}  # by kind of step: the graph, and what it was captured for (_key)
         self._graph_bufs = None
 
     def _make_cache(self):
@@ -258,66 +258,108 @@ class Decoder:
         """What a captured step depends on besides its buffers: the workspaces' addresses and the regime's kernels."""
         return self.ctx.workspace_generation(), self.ctx.regime()
 
-    def _decode_body(self):
+    def _captured(self, kind, body, rewind):
+        """The graph of a step: captured anew where a workspace that it points into was reallocated since (a longer prompt
+        chunk, another caller of the context), or the regime is another."""
+        graph, key = self._graphs.get(kind, (None, None))
+        if graph is not None and key == self._key():
+            return graph
+        torch = self.torch
+        body()  # at the same shapes: grows every workspace first
+        rewind()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        try:
+            with torch.cuda.graph(g):
+                self.ctx.set_stream(torch.cuda.current_stream())  # the capturing stream
+                body()
+        finally:
+            self.ctx.set_stream(torch.cuda.current_stream())
+        self._graphs[kind] = (g, self._key())
+        torch.cuda.synchronize()
+        return g
+
+    def _sampling(self, b, rows: int, u, n: int, **how):
+        """The settings of a sampled decode into buffers of b, and its random numbers [n, rows] on the device."""
+        torch = self.torch
+        u = torch.as_tensor(u, dtype=torch.float32)
+        if tuple(u.shape) != (n, rows) and (rows != 1 or tuple(u.shape) != (n,)):
+            raise ValueError(f"u: need [{n}, {rows}] random numbers, got {list(u.shape)}")
+        vals = {}
+        for name, v in how.items():
+            x = np.asarray(v, dtype=np.int64 if name == "top_k" else np.float64)
+            if x.shape not in ((), (rows,)):
+                raise ValueError(f"{name}: one value, or one for each of {rows} sequences")
+            x = np.broadcast_to(x, rows)
+            vals[name] = x.clip(-1, 2 ** 31 - 1).astype(np.int32) if name == "top_k" else x.astype(np.float32)
+        if "u" not in b:
+            b["u"] = torch.empty(rows, dtype=torch.float32, device=self.dev)
+            for name, x in vals.items():
+                b[name] = torch.empty(rows, dtype=torch.int32 if name == "top_k" else torch.float32, device=self.dev)
+        for name, x in vals.items():
+            b[name].copy_(torch.from_numpy(x.copy()))
+        return u.to(self.dev).reshape(n, rows).contiguous()
+
+    def _decode_body(self, sampled: bool):
+        b = self._graph_bufs
         ty, dims, t = self.embed
-        x = self.ctx.get_rows(ty, t, dims[1], dims[0], self.token_dev, out=self._graph_bufs["x"])
+        x = self.ctx.get_rows(ty, t, dims[1], dims[0], self.token_dev, out=b["x"])
         logits = self._stack(x, 1, 0, self.pos_dev)
-        self._graph_bufs["logits"] = logits
-        self.ctx.argmax(logits, out=self.token_dev, pos_dev=self.pos_dev, advance=1)
+        b["logits"] = logits
+        if sampled:
+            self.ctx.sample(logits.view(1, -1), b["u"], b["temperature"], b["top_k"], b["top_p"], b["min_p"],
+                            out=self.token_dev, pos_dev=self.pos_dev, advance=1)
+        else:
+            self.ctx.argmax(logits, out=self.token_dev, pos_dev=self.pos_dev, advance=1)
+
+    def _decode(self, first_token: int, n: int, use_graph: bool, how):
+        torch = self.torch
+        if self.cached + n > self.n_ctx:
+            raise ValueError("context full")
+        if self._graph_bufs is None:
+            self._graph_bufs = {"x": torch.empty((1, self.d), dtype=torch.float32, device=self.dev)}
+        u = None if how is None else self._sampling(self._graph_bufs, 1, n=n, **how)
+        self.pos_dev.fill_(self.cached)
+        self.token_dev.fill_(int(first_token))
+        out = torch.empty(n, dtype=torch.int32, device=self.dev)
+        step = lambda: self._decode_body(u is not None)  # noqa: E731
+        if use_graph:
+            pos, tok = self.pos_dev.clone(), self.token_dev.clone()
+            if u is not None:
+                self._graph_bufs["u"].copy_(u[0] if n else torch.zeros(1))
+
+            def rewind():
+                self.pos_dev.copy_(pos)
+                self.token_dev.copy_(tok)
+
+            step = self._captured("greedy" if u is None else "sampled", step, rewind).replay
+        for i in range(n):
+            if u is not None:
+                self._graph_bufs["u"].copy_(u[i])
+            step()
+            out[i:i + 1].copy_(self.token_dev)
+        self.cached += n
+        return out
 
     def decode_greedy(self, first_token: int, n: int, use_graph: bool = True):
         """Greedy decoding (sampler.rs:58-59): feed first_token, then each
         argmax, n steps; returns the n sampled ids. One step = one token
         through every layer, the head and argmax, all on the device; with
         use_graph the step is captured once and replayed."""
-        torch = self.torch
-        if self.cached + n > self.n_ctx:
-            raise ValueError("context full")
-        self.pos_dev.fill_(self.cached)
-        self.token_dev.fill_(int(first_token))
-        if self._graph_bufs is None:
-            self._graph_bufs = {"x": torch.empty((1, self.d), dtype=torch.float32, device=self.dev)}
-        out = torch.empty(n, dtype=torch.int32, device=self.dev)
-        if not use_graph:
-            for i in range(n):
-                self._decode_body()
-                out[i:i + 1].copy_(self.token_dev)
-            self.cached += n
-            return out
-        if self.graph is not None and self._key() != self._graph_key:
-            # a workspace the graph points into was reallocated since the capture
-            # (a longer prompt chunk, another caller of the context), or the regime
-            # is another: capture again
-            self.graph = None
-        if self.graph is None:
-            # warm-up call at the same shapes grows every workspace first
-            pos, tok = self.pos_dev.clone(), self.token_dev.clone()
-            self._decode_body()
-            self.pos_dev.copy_(pos)
-            self.token_dev.copy_(tok)
-            torch.cuda.synchronize()
-            g = torch.cuda.CUDAGraph()
-            try:
-                with torch.cuda.graph(g):
-                    self.ctx.set_stream(torch.cuda.current_stream())  # the capturing stream
-                    self._decode_body()
-            finally:
-                self.ctx.set_stream(torch.cuda.current_stream())
-            self.graph = g
-            self._graph_key = self._key()
-            torch.cuda.synchronize()
-        for i in range(n):
-            self.graph.replay()
-            out[i:i + 1].copy_(self.token_dev)
-        self.cached += n
-        return out
+        return self._decode(first_token, n, use_graph, None)
+
+    def decode_sample(self, first_token: int, n: int, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                      use_graph: bool = True):
+        """decode_greedy with the tokens drawn by Context.sample: u holds n random numbers in [0, 1), the caller's; the
+        settings are single numbers, read when the steps run."""
+        return self._decode(first_token, n, use_graph, dict(u=u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p))
 
     def close(self):
         for L in self.layers:
             if "moe" in L:
                 self.ctx.layer_destroy(L["moe"])
         self.layers = []
-        self.graph = None
+        self._graphs = {}
 
 
 class PagedDecoder(Decoder):
@@ -331,10 +373,20 @@ class PagedDecoder(Decoder):
     (hp["n_batch"] rows of forward, as many greedy steps as a page has positions)
     takes its pages before it runs. head_dim 64 or 128; a sequence has at most
     hp["n_ctx"] positions, a call at most 4096 sequences, and hp["n_batch"] rows at
-    a time of a forward call go through the layers."""
+    a time of a forward call go through the layers.
+
+    With share_prefixes the pages that several of a call's sequences hold in common
+    (forks of a prompt) are read once for all of them (Pages.groups finds them). With
+    select > 0 the attention of decode steps, and of forward calls with one token for each
+    sequence, goes over that many pages for each kv head: a row's own, the first
+    select_first and those whose bounds promise the largest scores; other calls go over
+    all. Neither goes with a window, nor with the other."""
+
+    SHARE_LEAST = 512  # positions read again (members less one, times those in common) from which a group is made
 
     def __init__(self, ctx: Context, hp: dict, tensors: dict, n_pages: int, page: int = 64, kv_type: int = F16,
-                 window: int = 0, n_sink: int = 0, layer_base: int = 1000):
+                 window: int = 0, n_sink: int = 0, layer_base: int = 1000, share_prefixes: bool = False, select: int = 0,
+                 select_first: int = 1):
         if hp["head_dim"] not in (64, 128):
             raise ValueError(f"head_dim {hp['head_dim']}: the paged cache has heads of 64 or 128")
         if kv_type not in (F16, Q8_0):
@@ -343,6 +395,11 @@ class PagedDecoder(Decoder):
             raise ValueError("window and n_sink: not negative, and n_sink with a window only")
         if page not in (32, 64, 128, 256):
             raise ValueError(f"page {page}: 32, 64, 128 or 256 positions")
+        if select < 0 or (select and not 0 <= select_first < select):
+            raise ValueError("select and select_first: not negative, and fewer first pages than selected ones")
+        if (share_prefixes or select) and window or (share_prefixes and select):
+            raise ValueError("share_prefixes, select and window: one of them at most")
+        self.share_prefixes, self.select, self.select_first = share_prefixes, select, select_first
         self.account = Pages(n_pages, page)
         self.kv = PagedKV(kv_type, hp["n_head_kv"], hp["head_dim"], page)
         self.n_pages, self.window, self.n_sink = n_pages, window, n_sink
@@ -353,6 +410,10 @@ class PagedDecoder(Decoder):
     def _make_cache(self):
         self.pages = self.torch.zeros((self.n_layer, self.n_pages, self.kv.page_bytes), dtype=self.torch.uint8,
                                       device=self.dev)
+        self.bounds = None
+        if self.select:
+            self.bounds = self.torch.zeros((self.n_layer, self.n_pages, self.nkv, 2, self.hd), dtype=self.torch.float16,
+                                           device=self.dev)
 
     # ---------------------------------------------------------- sequences
     def length(self, seq: int) -> int:
@@ -376,6 +437,9 @@ class PagedDecoder(Decoder):
         """Moves used pages to the front of the cache, at most `most`; how many were moved."""
         src, dst = self.account.compact(most)
         self._copy(list(zip(src.tolist(), dst.tolist())))
+        if self.bounds is not None and len(src):
+            s, d = (self.torch.from_numpy(x.astype(np.int64)).to(self.dev) for x in (src, dst))
+            self.bounds[:, d] = self.bounds[:, s]
         return len(src)
 
     def _copy(self, pairs):
@@ -433,9 +497,21 @@ class PagedDecoder(Decoder):
                 (account or self.account).trim(s, self.window, max(self.n_sink, had[s] or 0) if had else self.n_sink)
 
     # -------------------------------------------------------------- steps
-    def _paged_layer(self, L, pages, batch, x, f_prev):
-        """_layer for the rows of a batch; `pages`: the layer's."""
-        ctx, nh, nkv, hd, S = self.ctx, self.nh, self.nkv, self.hd, batch.s_rows
+    def _attend(self, l: int, batch, q):
+        """The batch's attention over layer l's pages, in the form that the batch asks for."""
+        ctx, pages = self.ctx, self.pages[l]
+        if self.select:
+            ctx.paged_bounds(self.kv, pages, batch, self.bounds[l])
+            if batch.steps:
+                return ctx.paged_attention_selected(self.kv, pages, self.bounds[l], batch, q, self.nh, self.select,
+                                                    self.select_first)
+        if getattr(batch, "groups", None) is not None:
+            return ctx.paged_attention_shared(self.kv, pages, batch, batch.groups, q, self.nh)
+        return ctx.paged_attention(self.kv, pages, batch, q, self.nh, self.window, self.n_sink)
+
+    def _paged_layer(self, l: int, batch, x, f_prev):
+        """_layer for the rows of a batch."""
+        ctx, nh, nkv, hd, S, L = self.ctx, self.nh, self.nkv, self.hd, batch.s_rows, self.layers[l]
         kvw, nq = nkv * hd, nh * hd
         if "wqkv" in L:
             ty, dims, t = L["wqkv"]
@@ -453,15 +529,14 @@ class PagedDecoder(Decoder):
             ctx.rmsnorm(q, L["q_norm"], self.eps, out=q)
         if "k_norm" in L:
             ctx.rmsnorm(k, L["k_norm"], self.eps, out=k)
-        qr = ctx.paged_rope_kv_store(self.kv, pages, batch, q, k, v, nh, self.rd, self.inv_freq, self.neox)
-        o = ctx.paged_attention(self.kv, pages, batch, qr, nh, self.window, self.n_sink)
-        return self._ffn(L, x, self._mm(L["wo"], o), S)
+        qr = ctx.paged_rope_kv_store(self.kv, self.pages[l], batch, q, k, v, nh, self.rd, self.inv_freq, self.neox)
+        return self._ffn(L, x, self._mm(L["wo"], self._attend(l, batch, qr)), S)
 
     def _rows(self, x, batch):
         """All layers over the batch's rows: (x, f), whose sum is the residual stream."""
         f = None
-        for L, pages in zip(self.layers, self.pages):
-            f = self._paged_layer(L, pages, batch, x, f)
+        for l in range(self.n_layer):
+            f = self._paged_layer(l, batch, x, f)
         return x, f
 
     def _logits(self, x, f):
@@ -477,6 +552,14 @@ class PagedDecoder(Decoder):
         d = self.torch.from_numpy(np.concatenate([ends, starts, table.reshape(-1)]).astype(np.int32)).to(self.dev)
         rs = None if max(counts) == 1 else d[n:2 * n + 1]
         return self.ctx.paged_batch(d[2 * n + 1:].view(n, cols), d[:n], rs, int(starts[-1]))
+
+    def _groups(self, seqs, rows: int):
+        """The order that puts sequences with pages in common beside each other, with where their groups begin and what
+        they share; None where nothing is worth sharing (or the call's rows are too many for it)."""
+        if not self.share_prefixes or len(seqs) < 2 or rows * self.nh > 1 << 21:
+            return None
+        order, start, shared = self.account.groups(seqs, self.SHARE_LEAST)
+        return (order.tolist(), start, shared) if len(shared) else None
 
     def _parts(self, rows: dict):
         """The rows in parts of n_batch: lists of (sequence, first token, end), a sequence at most once in each."""
@@ -499,7 +582,7 @@ class PagedDecoder(Decoder):
         for s, ts in rows.items():
             if not ts or min(ts) < 0 or max(ts) >= self.n_vocab:
                 raise ValueError(f"sequence {s}: need at least one token, each below {self.n_vocab}")
-        parts = self._parts(rows)
+        parts, steps = self._parts(rows), all(len(ts) == 1 for ts in rows.values())
         had, by_parts = self._reserve({s: len(ts) for s, ts in rows.items()}, [{s: j - i for s, i, j in p} for p in parts])
         try:
             logits = []
@@ -507,12 +590,20 @@ class PagedDecoder(Decoder):
                 if by_parts:
                     self._append({s: j - i for s, i, j in part})
                 ty, dims, t = self.embed
+                groups, done = self._groups([p[0] for p in part], sum(j - i for _, i, j in part)), [p[0] for p in part if p[2] == len(rows[p[0]])]
+                if groups:
+                    part = [part[i] for i in groups[0]]
                 x = self.ctx.get_rows(ty, t, dims[1], dims[0], [tk for s, i, j in part for tk in rows[s][i:j]])
                 counts = [j - i for _, i, j in part]
-                x, f = self._rows(x, self._batch([p[0] for p in part], [(had[s] or 0) + j for s, _, j in part], counts))
-                last = [e - 1 for e, (s, _, j) in zip(np.cumsum(counts).tolist(), part) if j == len(rows[s])]
+                batch = self._batch([p[0] for p in part], [(had[s] or 0) + j for s, _, j in part], counts)
+                batch.steps = steps
+                if groups:
+                    batch.groups = self.ctx.paged_groups(*(self.torch.from_numpy(g.copy()).to(self.dev) for g in groups[1:]))
+                x, f = self._rows(x, batch)
+                end = dict(zip([p[0] for p in part], np.cumsum(counts).tolist()))
+                last = [end[s] - 1 for s in done]
                 if last:
-                    if len(last) < len(x):
+                    if last != list(range(len(x))):
                         x, f = (self.ctx.get_rows(F32, y, len(y), self.d, last) for y in (x, f))
                     logits.append(self._logits(x, f))
                 if by_parts:
@@ -524,18 +615,34 @@ class PagedDecoder(Decoder):
         self._trim(rows)
         return logits
 
-    # ------------------------------------------------------ greedy decode
-    def _decode_rows(self, b):
+    # ------------------------------------------------------ decode steps
+    def _decode_rows(self, b, sampled: bool, shared: bool):
         ty, dims, t = self.embed
         x = self.ctx.get_rows(ty, t, dims[1], dims[0], b["tok"], out=b["x"])
+        b["batch"].groups = b["groups"] if shared else None
         b["logits"] = self._logits(*self._rows(x, b["batch"]))
+        if sampled:
+            self.ctx.sample(b["logits"], b["u"], b["temperature"], b["top_k"], b["top_p"], b["min_p"], out=b["tok"],
+                            pos_dev=b["len"], advance=1)
+            return
         for i in range(len(b["logits"])):
             self.ctx.argmax(b["logits"][i], out=b["tok"][i:i + 1], pos_dev=b["len"][i:i + 1], advance=1)
 
-    def decode_greedy(self, first: dict, n: int, use_graph: bool = True):
-        """Greedy decoding of several sequences together: feeds first {sequence: token}, then each one's argmax,
-        n steps; returns the sampled ids [n, len(first)]. With use_graph a step is captured once per number of
-        sequences and replayed: lengths, tokens and page tables are read on the device."""
+    def _buffers(self, n: int):
+        """The buffers of steps of n sequences, which the graphs hold."""
+        b, torch = self._graph_bufs, self.torch
+        if b is None or self._graph_n != n:
+            i32 = dict(dtype=torch.int32, device=self.dev)
+            b = {"x": torch.empty((n, self.d), dtype=torch.float32, device=self.dev), "tok": torch.empty(n, **i32),
+                 "len": torch.empty(n, **i32), "table": torch.empty((n, self.cols), **i32),
+                 "start": torch.empty(n // 2 + 2, **i32), "shared": torch.empty(n // 2 + 1, **i32)}
+            b["batch"] = self.ctx.paged_batch(b["table"], b["len"])
+            b["batch"].steps = True
+            b["groups"] = self.ctx.paged_groups(b["start"], b["shared"])
+            self._graph_bufs, self._graph_n, self._graphs = b, n, {}
+        return b
+
+    def _decode(self, first: dict, n: int, use_graph: bool, how):
         torch, seqs = self.torch, [int(s) for s in first]
         if n < 1:
             raise ValueError("n: at least one step")
@@ -547,53 +654,71 @@ class PagedDecoder(Decoder):
         try:
             if by_blocks:
                 self._append({s: blocks[0] for s in seqs})
-            b = self._graph_bufs
-            if b is None or self._graph_n != len(seqs):
-                i32 = dict(dtype=torch.int32, device=self.dev)
-                b = {"x": torch.empty((len(seqs), self.d), dtype=torch.float32, device=self.dev),
-                     "tok": torch.empty(len(seqs), **i32), "len": torch.empty(len(seqs), **i32),
-                     "table": torch.empty((len(seqs), self.cols), **i32)}
-                b["batch"] = self.ctx.paged_batch(b["table"], b["len"])
-                self._graph_bufs, self._graph_n, self.graph = b, len(seqs), None
-            at = torch.tensor([(had[s] or 0) + 1 for s in seqs], dtype=torch.int32)
-            tok = torch.tensor([int(t) for t in first.values()], dtype=torch.int32)
-            b["table"].copy_(torch.from_numpy(self.account.table(seqs, self.cols)[0]))
+            b = self._buffers(len(seqs))
+            u = None if how is None else self._sampling(b, len(seqs), n=n, **how)
+            groups = self._groups(seqs, len(seqs))
+            order = groups[0] if groups else list(range(len(seqs)))  # of the buffers' rows, among seqs
+            rows = [seqs[i] for i in order]
+            at = torch.tensor([(had[s] or 0) + 1 for s in rows], dtype=torch.int32)
+            tok = torch.tensor([int(first[s]) for s in rows], dtype=torch.int32)
+            b["table"].copy_(torch.from_numpy(self.account.table(rows, self.cols)[0]))
             b["len"].copy_(at)
             b["tok"].copy_(tok)
+            if groups:
+                start, shared = (np.zeros(len(b[x]), np.int32) for x in ("start", "shared"))
+                start[:], shared[:len(groups[2])] = groups[1][-1], groups[2]
+                start[:len(groups[1])] = groups[1]
+                b["start"].copy_(torch.from_numpy(start))
+                b["shared"].copy_(torch.from_numpy(shared))
+                if u is not None:
+                    to = torch.tensor(order, device=self.dev)
+                    u = u[:, to].contiguous()
+                    for x in ("temperature", "top_k", "top_p", "min_p"):
+                        b[x].copy_(b[x][to])
             out = torch.empty((n, len(seqs)), dtype=torch.int32, device=self.dev)
-            if use_graph and (self.graph is None or self._key() != self._graph_key):
-                self._decode_rows(b)  # grows every workspace first
-                b["len"].copy_(at)
-                b["tok"].copy_(tok)
-                torch.cuda.synchronize()
-                g = torch.cuda.CUDAGraph()
-                try:
-                    with torch.cuda.graph(g):
-                        self.ctx.set_stream(torch.cuda.current_stream())  # the capturing stream
-                        self._decode_rows(b)
-                finally:
-                    self.ctx.set_stream(torch.cuda.current_stream())
-                self.graph, self._graph_key = g, self._key()
-                torch.cuda.synchronize()
+            step = lambda: self._decode_rows(b, u is not None, bool(groups))  # noqa: E731
+            if use_graph:
+                if u is not None:
+                    b["u"].copy_(u[0])
+
+                def rewind():
+                    b["len"].copy_(at)
+                    b["tok"].copy_(tok)
+
+                step = self._captured(("greedy" if u is None else "sampled", bool(groups)), step, rewind).replay
             for i in range(n):
                 if by_blocks and i and i % page == 0:
                     self._trim(seqs, had)
                     self._append({s: blocks[i // page] for s in seqs})
                     b["table"].copy_(torch.from_numpy(self.account.table(seqs, self.cols)[0]))
-                if use_graph:
-                    self.graph.replay()
-                else:
-                    self._decode_rows(b)
+                if u is not None:
+                    b["u"].copy_(u[i])
+                step()
                 out[i].copy_(b["tok"])
+            if groups:
+                out = out[:, torch.tensor(np.argsort(order), device=self.dev)]
         except BaseException:
             self._back(had)
             raise
         self._trim(seqs)
         return out
 
+    def decode_greedy(self, first: dict, n: int, use_graph: bool = True):
+        """Greedy decoding of several sequences together: feeds first {sequence: token}, then each one's argmax,
+        n steps; returns the sampled ids [n, len(first)]. With use_graph a step is captured once per number of
+        sequences and replayed: lengths, tokens and page tables are read on the device."""
+        return self._decode({int(s): t for s, t in first.items()}, n, use_graph, None)
+
+    def decode_sample(self, first: dict, n: int, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, use_graph: bool = True):
+        """decode_greedy with the tokens drawn by Context.sample: u [n, len(first)] holds the caller's random numbers in
+        [0, 1); each setting is one number, or one per sequence in the order of first. A captured step reads them on the
+        device, too."""
+        return self._decode({int(s): t for s, t in first.items()}, n, use_graph,
+                            dict(u=u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p))
+
     def close(self):
         super().close()
-        self.pages = None
+        self.pages = self.bounds = None
         self.account.close()
 
 

@@ -127,6 +127,7 @@ SIGNATURES = {
     "kmoe_pages_drop": (C.c_int, [_P, _u32]),
     "kmoe_pages_length": (C.c_int, [_P, _u32, C.POINTER(_i64)]),
     "kmoe_pages_table": (C.c_int, [_P, _P, _i32, _i32, _P, _P]),
+    "kmoe_pages_groups": (C.c_int, [_P, _P, _i32, _i64, _P, _P, _P, C.POINTER(_i32)]),
     "kmoe_pages_compact": (C.c_int, [_P, _P, _P, _i64, C.POINTER(_i64)]),
     "kmoe_pages_usage": (C.c_int, [_P, C.POINTER(_i64), C.POINTER(_i64)]),
     "kmoe_measure": (C.c_int, [_P, _P]),
@@ -914,6 +915,15 @@ class Pages:
         self.check(self.lib.kmoe_pages_table(self.h, ids.ctypes.data, ids.size, table_cols, t.ctypes.data,
                                              n.ctypes.data))
         return t, n
+
+    def groups(self, seqs, least: int = 1):
+        """kmoe_pages_groups: (order, start, shared) of the groups among seqs that share `least` positions or more in all:
+        group i is seqs[order[start[i]:start[i + 1]]], with shared[i] pages in common."""
+        ids = np.array([self._seq(s) for s in seqs], np.uint32)
+        order, start, shared, n = np.empty(ids.size, np.int32), np.zeros(ids.size + 1, np.int32), np.empty(ids.size, np.int32), _i32()
+        self.check(self.lib.kmoe_pages_groups(self.h, ids.ctypes.data, ids.size, least, order.ctypes.data, start.ctypes.data,
+                                              shared.ctypes.data, C.byref(n)))
+        return order, start[:n.value + 1], shared[:n.value]
 
     def compact(self, most: int | None = None):
         """Moves used pages to the front (at most `most`): (src, dst) pages to copy."""
