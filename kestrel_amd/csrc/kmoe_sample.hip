@@ -18,6 +18,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "kmoe_device.h"
 #include "kmoe_launch.h"
 
@@ -28,16 +30,17 @@ typedef unsigned long long u64;
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kFix = 43;    // weights in units of 2^-43
 constexpr int kBins = 2048;
-constexpr u64 kOne = 1ull << kFix;
+constexpr int kTab = 256;
 constexpr int kGroup = 64, kChunk = 4096;  // elements of which k_sample_stats finds the largest, and the sum
 constexpr int kCand = 2048, kGroups = 1024;
+constexpr int kFew = 1024;  // elements of a bin that are compared one with another
 constexpr float kSpan = 24.0f;  // distances from the largest logit that the even bins tell apart, in units of T
 
-// Order of the logits as whole numbers: the larger the logit, the smaller its rank
-// (NaN as -inf, -0 as 0).
-__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x + 0.0f; }
+// NaN as -inf. Order of the logits as whole numbers: the larger the logit, the smaller
+// its rank (-0 as 0).
+__device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY); }
 __device__ __forceinline__ uint32_t rank_of(float x) {
-  const uint32_t b = __float_as_uint(x);
+  const uint32_t b = __float_as_uint(x + 0.0f);
   return ~(b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u));
 }
 __device__ __forceinline__ float of_rank(uint32_t r) {
@@ -47,10 +50,10 @@ __device__ __forceinline__ float of_rank(uint32_t r) {
 
 // What one row is drawn by.
 struct Row {
-  float max;     // largest logit
-  double inv_t;  // 1 / T
-  float scale;   // bins per unit of logit
-  double min_p;  // 0: all
+  double max;    // largest logit
+  double inv_t;  // 256 / (T log 2)
+  float top, scale;  // largest logit; bins per unit of logit
+  double min_w;  // min_p in units
   float u;
 };
 
@@ -66,72 +69,81 @@ struct Candidates {
   __device__ __forceinline__ float at(int i) const { return l[i]; }
 };
 
-// exp(x), -31 <= x <= 0: 2^(i / 64) from a table (LDS) times the exponential of what is
-// left, at most log(2) / 128, by its series: the sixth power's term is 2^-54.6.
-__device__ __forceinline__ double exp_of(double x, const double *tab) {
-  const double i = __builtin_rint(x * 92.332482616893656877);  // 64 / log 2
-  double r = fma(i, -0x1.62e42fefa3800p-7, x);                // log(2) / 64, its first 42 bits: exact times i
-  r = fma(i, -0x1.ef35793c76730p-51, r);
-  const int k = (int)i;
-  double y = fma(r, 1.0 / 120, 1.0 / 24);
-  y = fma(r, y, 1.0 / 6);
-  y = fma(r, y, 0.5);
-  y = fma(r, y, 1.0);
-  y = r * y;
-  const double t = tab[k & 63];
-  return ldexp(fma(t, y, t), k >> 6);
-}
-__device__ __forceinline__ double weight(const Row &r, float l, const double *tab) {
-  if (l == r.max) return 1.0;
-  const double x = ((double)l - (double)r.max) * r.inv_t;
-  return x > -31.0 && l != -INFINITY ? exp_of(x, tab) : 0.0;  // (exp(-31) is under half a unit)
-}
-// To the nearest unit: 2^52 and a number below it have a last bit of 1.
-__device__ __forceinline__ u64 fixed(double w) {
-  return (u64)__double_as_longlong(w * 0x1p43 + 0x1p52) & ((1ull << 52) - 1);
+// 2^(i / 256)
+__device__ __forceinline__ void make_table(double *tab) {
+  if (threadIdx.x < kTab) tab[threadIdx.x] = exp2((double)threadIdx.x / kTab);
 }
 
-// Even bins by the distance from the largest logit (not descending where the logits descend).
+// A weight in units: z = 256 log2 of it is i + f, |f| <= 1/2, and 2^(z / 256) a power of two
+// times 2^((i mod 256) / 256) (LDS) times the exponential of f log(2) / 256 by its
+// series, whose fifth power's term is 2^-54.5. i comes out of z's sum with 1.5 2^52,
+// whose last bit is 1. The largest logit's weight is 2^43 exactly. Below 2^-44 (-31
+// nats: z = -11450) the weight rounds to no unit, whatever it is. A NaN is an infinite
+// largest logit's distance from itself.
+__device__ __forceinline__ double weight(const Row &r, float l, const double *tab) {
+  double z = ((double)l - r.max) * r.inv_t;
+  z = fmax(fmin(z, 0.0), -11450.0);
+  const double s = z + 0x1.8p52;
+  const int i = (int)(uint32_t)__double_as_longlong(s);
+  const double f = z - (s - 0x1.8p52);
+  double y = fma(f, 0x1.3b2ab6fba4e77p-39, 0x1.c6b08d704a0c0p-29);  // (log(2) / 256)^k / k!
+  y = fma(f, y, 0x1.ebfbdff82c58fp-19);
+  y = fma(f, y, 0x1.62e42fefa39efp-9);
+  y = f * y;
+  const double t = tab[i & (kTab - 1)];
+  const double u = __hiloint2double(__double2hiint(t) + (((i >> 8) + kFix) << 20), __double2loint(t));
+  return fma(u, y, u);
+}
+// To the nearest unit: 2^52 and a number below it have a last bit of 1.
+__device__ __forceinline__ u64 fixed(double w) { return (u64)__double_as_longlong(w + 0x1p52) & ((1ull << 52) - 1); }
+
+// Even bins by the distance from the largest logit (not descending where the logits
+// descend); an infinite largest one's own distance is a NaN: bin 0.
 __device__ __forceinline__ int bin_of(const Row &r, float l) {
-  if (l == r.max) return 0;
-  return (int)fminf((r.max - l) * r.scale, (float)(kBins - 1));
+  return (int)__builtin_amdgcn_fmed3f((r.top - l) * r.scale, 0.0f, (float)(kBins - 1));
 }
 
 struct Shared {
-  double tab[64];
+  double tab[kTab];
   u64 mass[kBins];
   uint32_t count[kBins];
   u64 red[kWaves];
   uint32_t redi[kWaves];
   float redf[kWaves];
-  u64 before;
-  int at;
+  u64 before, above;
+  int at, n;
+  // elements of one bin
+  uint32_t rank[64];
+  u64 w[64];
   // candidates, and the groups that they are in with how many candidates each has
   float cand[kCand];
   int index[kCand];
   uint16_t group[kGroups], in_group[kGroups];
 };
 
-__device__ __forceinline__ u64 shfl_up64(u64 x, int d) {
-  const uint32_t lo = __shfl_up((uint32_t)x, d), hi = __shfl_up((uint32_t)(x >> 32), d);
-  return (u64)hi << 32 | lo;
+// Inclusive scan over a wave: within rows of 16 lanes, then row 0's and 2's totals onto
+// rows 1 and 3, then lane 31's onto the upper half.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_add(u64 x) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xf, false);
+  return x + ((u64)hi << 32 | lo);
 }
-__device__ __forceinline__ u64 wave_scan(u64 x) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const u64 y = shfl_up64(x, d);
-    if (lane >= d) x += y;
-  }
-  return x;
+__device__ __forceinline__ u64 wave_scan(u64 x) {
+  x = dpp_add<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);  // row_bcast 15, 31
+  return dpp_add<0x143, 0xc>(x);
 }
 // Exclusive scan over the work-group's threads, and the total.
 __device__ __forceinline__ u64 block_scan(u64 x, u64 &total, Shared &sh) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const u64 in = wave_scan(x);
-  __syncthreads();  // (the last call's sums are read)
+  lds_barrier();  // (the last call's sums are read)
   if (lane == 63) sh.red[wave] = in;
-  __syncthreads();
+  lds_barrier();
   u64 before = in - x;
   total = 0;
 #pragma unroll
@@ -156,7 +168,7 @@ __device__ __forceinline__ int crossing(const T *hist, u64 target, u64 &before, 
     sh.at = 2 * t + second;
     sh.before = x + (second ? a : 0);
   }
-  __syncthreads();
+  lds_barrier();
   before = sh.before;
   return sh.at;
 }
@@ -181,42 +193,6 @@ __device__ __forceinline__ void clear(T *h) {
   for (int i = threadIdx.x; i < kBins; i += kThreads) h[i] = 0;
 }
 
-// A beginning of the order: ranks below `rank`, and the first `ties` of those equal to it.
-struct Cut {
-  uint32_t rank;
-  u64 ties;
-};
-
-// Where the running sum over the elements of an even bin whose rank is below `limit`
-// reaches target (1 .. their sum): the value's rank, and what is left of the target
-// there. MASS: sums of weights, otherwise numbers of elements. Digit by digit.
-template <bool MASS, class S>
-__device__ __forceinline__ Cut cut_in_bin(const Row &r, const S &src, int bin, uint32_t limit, u64 target, Shared &sh) {
-  uint32_t found = 0;
-#pragma unroll 1
-  for (int d = 0; d < 3; ++d) {  // 11, 11 and 10 bits
-    const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, top = d == 0 ? 32 : d == 1 ? 21 : 10;
-    __syncthreads();
-    if (MASS) clear(sh.mass);
-    else clear(sh.count);
-    __syncthreads();
-    each(src, [&](int, float l) {
-      if (bin_of(r, l) != bin) return;
-      const uint32_t k = rank_of(l);
-      if (k >= limit || (d && k >> top != found >> top)) return;
-      const int b = (k >> shift) & (d == 2 ? 1023 : 2047);
-      if (MASS) atomicAdd(&sh.mass[b], fixed(weight(r, l, sh.tab)));
-      else atomicAdd(&sh.count[b], 1u);
-    });
-    __syncthreads();
-    u64 before;
-    const int b = MASS ? crossing(sh.mass, target, before, sh) : crossing(sh.count, target, before, sh);
-    target -= before;
-    found |= (uint32_t)b << shift;
-  }
-  return Cut{found, target};
-}
-
 // Sum of f(i, l) over the elements, to every thread.
 template <class S, class F>
 __device__ __forceinline__ u64 sum_of(const S &src, Shared &sh, F &&f) {
@@ -226,45 +202,153 @@ __device__ __forceinline__ u64 sum_of(const S &src, Shared &sh, F &&f) {
   return total;
 }
 
+// A beginning of the order: values above v, and the first `ties` of those equal to it.
+struct Cut {
+  float v;
+  u64 ties;
+};
+
+// Where the running sum over the elements of an even bin whose rank is below `limit`
+// reaches target (1 .. their sum): the value, what is left of the target there, and
+// (above) the weight of the bin's elements before it. MASS: sums of weights, otherwise
+// numbers of elements. Digit by digit of the rank; the even bins' sums of that kind are
+// used up.
+template <bool MASS, class S>
+__device__ __forceinline__ Cut cut_by_digits(const Row &r, const S &src, int bin, uint32_t limit, u64 target, u64 &above,
+                                             Shared &sh) {
+  uint32_t found = 0;
+#pragma unroll 1
+  for (int d = 0; d < 3; ++d) {  // 11, 11 and 10 bits
+    const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, top = d == 0 ? 32 : d == 1 ? 21 : 10;
+    lds_barrier();
+    if (MASS) clear(sh.mass);
+    else clear(sh.count);
+    lds_barrier();
+    each(src, [&](int, float l) {
+      if (bin_of(r, l) != bin) return;
+      const uint32_t k = rank_of(l);
+      if (k >= limit || (d && k >> top != found >> top)) return;
+      const int b = (k >> shift) & (d == 2 ? 1023 : 2047);
+      if (MASS) atomicAdd(&sh.mass[b], fixed(weight(r, l, sh.tab)));
+      else atomicAdd(&sh.count[b], 1u);
+    });
+    lds_barrier();
+    u64 before;
+    const int b = MASS ? crossing(sh.mass, target, before, sh) : crossing(sh.count, target, before, sh);
+    target -= before;
+    found |= (uint32_t)b << shift;
+  }
+  if (!MASS)
+    above = sum_of(src, sh, [&](int, float l) {
+      return bin_of(r, l) == bin && rank_of(l) < found ? fixed(weight(r, l, sh.tab)) : 0;
+    });
+  return Cut{of_rank(found), target};
+}
+
+// The same by the number of the bin's elements (`few` of them): up to 64 are compared with each
+// other (`held`: the counts stay), more of a long row are gathered first.
+template <bool MASS, class S>
+__device__ __forceinline__ Cut cut_in_bin(const Row &r, const S &src, int bin, int few, uint32_t limit, u64 target,
+                                          u64 &above, bool &held, Shared &sh) {
+  const int t = threadIdx.x;
+  if (few > 64) {
+    held = false;
+    if constexpr (std::is_same<S, Logits>::value) {
+      if (few <= kCand) {
+        lds_barrier();
+        if (t == 0) sh.n = 0;
+        lds_barrier();
+        each(src, [&](int, float l) {
+          if (bin_of(r, l) == bin) sh.cand[atomicAdd(&sh.n, 1)] = l;
+        });
+        lds_barrier();
+        return cut_by_digits<MASS>(r, Candidates{sh.cand, sh.n}, bin, limit, target, above, sh);
+      }
+    }
+    return cut_by_digits<MASS>(r, src, bin, limit, target, above, sh);
+  }
+  lds_barrier();
+  if (t == 0) sh.n = 0;
+  lds_barrier();
+  each(src, [&](int, float l) {
+    if (bin_of(r, l) != bin) return;
+    const uint32_t k = rank_of(l);
+    if (k >= limit) return;
+    const int i = atomicAdd(&sh.n, 1);
+    sh.rank[i] = k;
+    sh.w[i] = fixed(weight(r, l, sh.tab));
+  });
+  lds_barrier();
+  const int n = sh.n;
+  if (t < n) {
+    const uint32_t k = sh.rank[t];
+    u64 wb = 0, wt = 0;
+    uint32_t nb = 0, nt = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const uint32_t y = sh.rank[j];
+      const u64 w = sh.w[j];
+      wb += y < k ? w : 0;
+      wt += y == k ? w : 0;
+      nb += y < k;
+      nt += y == k;
+    }
+    const u64 before = MASS ? wb : nb, here_ = MASS ? wt : nt;
+    if (before < target && before + here_ >= target) {  // (equal ones write the same)
+      sh.at = (int)k;
+      sh.before = before;
+      sh.above = wb;
+    }
+  }
+  lds_barrier();
+  above = sh.above;
+  return Cut{of_rank((uint32_t)sh.at), target - sh.before};
+}
+
+// The first whole number that is p times x or more, 1 .. x's own.
+__device__ __forceinline__ u64 part_of(float p, u64 x) {
+  const double y = (double)p * (double)x;
+  u64 n = (u64)y;
+  n += (double)n < y;
+  return n > 1 ? n : 1;
+}
+
 // The cut by top_k (src.n or more: none) and top_p (1 or more: none) among the elements. all_: the
 // whole row's sum where the elements are not all that top_p counts, or 0.
 template <class S>
 __device__ __forceinline__ Cut find_cut(const Row &r, const S &src, int k, float p, u64 all_, Shared &sh) {
   const int t = threadIdx.x;
-  Cut cut{0xffffffffu, ~0ull};
+  Cut cut{-INFINITY, ~0ull};
   if (k >= src.n && p >= 1.0f) return cut;
-  __syncthreads();
+  lds_barrier();
   clear(sh.mass);
   clear(sh.count);
-  __syncthreads();
+  lds_barrier();
   each(src, [&](int, float l) {
     const int b = bin_of(r, l);
     atomicAdd(&sh.count[b], 1u);
-    const u64 w = p < 1.0f ? fixed(weight(r, l, sh.tab)) : 0;
-    if (w) atomicAdd(&sh.mass[b], w);
+    if (p < 1.0f) {
+      const u64 w = fixed(weight(r, l, sh.tab));
+      if (w) atomicAdd(&sh.mass[b], w);
+    }
   });
-  __syncthreads();
+  lds_barrier();
   // k falls into bin kb; m_bins: the sum of the bins before it, m_above: of all elements
   // before the k-th's value
   u64 n_before = 0, m_bins = 0, w_tie = 0;
   int kb = kBins;
   if (k < src.n) kb = crossing(sh.count, (u64)k, n_before, sh);
-  block_scan((2 * t < kb ? sh.mass[2 * t] : 0) + (2 * t + 1 < kb ? sh.mass[2 * t + 1] : 0), m_bins, sh);
-  u64 m_above = m_bins, all = m_bins;
+  if (p < 1.0f) block_scan((2 * t < kb ? sh.mass[2 * t] : 0) + (2 * t + 1 < kb ? sh.mass[2 * t + 1] : 0), m_bins, sh);
+  u64 m_above = m_bins, all = m_bins, above;
+  bool held = true;
   if (kb < kBins) {
-    cut = cut_in_bin<false>(r, src, kb, 0xffffffffu, (u64)k - n_before, sh);  // (the masses stay)
+    cut = cut_in_bin<false>(r, src, kb, (int)sh.count[kb], 0xffffffffu, (u64)k - n_before, above, held, sh);
     if (p >= 1.0f) return cut;
-    w_tie = fixed(weight(r, of_rank(cut.rank), sh.tab));
-    m_above += sum_of(src, sh, [&](int, float l) {
-      return bin_of(r, l) == kb && rank_of(l) < cut.rank ? fixed(weight(r, l, sh.tab)) : 0;
-    });
+    w_tie = fixed(weight(r, cut.v, sh.tab));
+    m_above += above;
     all = m_above + cut.ties * w_tie;
   }
-  const u64 whole = all_ ? all_ : all;
-  const double x = (double)p * (double)whole;
-  u64 target = (u64)x;
-  target += (double)target < x;
-  target = target > 1 ? target : 1;
+  u64 target = part_of(p, all_ ? all_ : all);
   if (target > all) {
     if (all_) return cut;  // further down than the elements go
     target = all;
@@ -275,13 +359,13 @@ __device__ __forceinline__ Cut find_cut(const Row &r, const S &src, int k, float
   }
   u64 before = m_bins;
   int b = kb;
-  uint32_t limit = cut.rank;
+  uint32_t limit = rank_of(cut.v);
   if (target <= m_bins) {
     b = crossing(sh.mass, target, before, sh);
     limit = 0xffffffffu;
   }
-  cut = cut_in_bin<true>(r, src, b, limit, target - before, sh);
-  w_tie = fixed(weight(r, of_rank(cut.rank), sh.tab));
+  cut = cut_in_bin<true>(r, src, b, held ? (int)sh.count[b] : src.n, limit, target - before, above, held, sh);
+  w_tie = fixed(weight(r, cut.v, sh.tab));
   cut.ties = (cut.ties + w_tie - 1) / w_tie;
   return cut;
 }
@@ -296,9 +380,9 @@ __device__ __forceinline__ int draw(const Row &r, const S &src, const Cut &cut, 
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   auto kept = [&](float l) -> u64 {
     const double x = weight(r, l, sh.tab);
-    return x >= r.min_p ? fixed(x) : 0;
+    return x >= r.min_w ? fixed(x) : 0;
   };
-  const u64 w_tie = kept(of_rank(cut.rank));
+  const u64 w_tie = kept(cut.v);
   u64 ties = cut.ties;
   bool first = true;
   auto begin = [&](u64 total) {
@@ -312,21 +396,29 @@ __device__ __forceinline__ int draw(const Row &r, const S &src, const Cut &cut, 
     const int b = a + part < start + len ? a + part : start + len;
     u64 s = 0;
     uint32_t c = 0;
-#pragma unroll 4
-    for (int i = a + lane; i < b; i += 64) {
-      const float l = src.at(i);
-      const uint32_t k = rank_of(l);
-      if (k < cut.rank) s += kept(l);
-      c += k == cut.rank;
+    constexpr int U = 8;
+    int i = a + lane;
+    auto add = [&](float l) {
+      const u64 x = kept(l);
+      s += l > cut.v ? x : 0;
+      c += l == cut.v;
+    };
+    for (; i + (U - 1) * 64 < b; i += U * 64) {
+      float x[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) x[j] = src.at(i + j * 64);
+#pragma unroll
+      for (int j = 0; j < U; ++j) add(x[j]);
     }
+    for (; i < b; i += 64) add(src.at(i));
     s = wave_scan(s);
     c = (uint32_t)group_sum_i<64>((int)c);
-    __syncthreads();
+    lds_barrier();
     if (lane == 63) {
       sh.red[wave] = s;
       sh.redi[wave] = c;
     }
-    __syncthreads();
+    lds_barrier();
     auto of_part = [&](int i, u64 left) { return sh.red[i] + (sh.redi[i] < left ? sh.redi[i] : left) * w_tie; };
     if (first) {
       u64 left = ties, total = 0;
@@ -337,23 +429,22 @@ __device__ __forceinline__ int draw(const Row &r, const S &src, const Cut &cut, 
       if (!total) return -1;
       begin(total);
     }
-    int i = 0;
-    for (; i < kWaves - 1; ++i) {
-      const u64 m = of_part(i, ties);
+    int k = 0;
+    for (; k < kWaves - 1; ++k) {
+      const u64 m = of_part(k, ties);
       if (goal < m) break;
       goal -= m;
-      ties -= sh.redi[i] < ties ? sh.redi[i] : ties;
+      ties -= sh.redi[k] < ties ? sh.redi[k] : ties;
     }
     const int end = start + len;
-    start += i * part;
+    start += k * part;
     len = start + part < end ? part : end - start;
   }
-  const float l = t < len ? src.at(start + t) : 0.0f;
-  const uint32_t k = rank_of(l);
-  const bool tie = t < len && k == cut.rank;
-  u64 total;
-  const u64 nth = block_scan(tie, total, sh);
-  const u64 m = t < len && (k < cut.rank || (tie && nth < ties)) ? kept(l) : 0;
+  const float l = t < len ? src.at(start + t) : -INFINITY;
+  const bool tie = t < len && l == cut.v;
+  u64 total, nth = 0;
+  if (ties < kThreads) nth = block_scan(tie, total, sh);
+  const u64 m = t < len && (l > cut.v || (tie && nth < ties)) ? kept(l) : 0;
   const u64 x = block_scan(m, total, sh);
   if (first) {
     if (!total) return -1;
@@ -363,7 +454,7 @@ __device__ __forceinline__ int draw(const Row &r, const S &src, const Cut &cut, 
     sh.at = start + t;
     sh.before = m;
   }
-  __syncthreads();
+  lds_barrier();
   w = sh.before;
   return sh.at;
 }
@@ -383,6 +474,16 @@ struct Settings {
     min_p = min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f;
     greedy = !(temp > 0.0f) || k == 1 || p <= 0.0f;
   }
+  __device__ __forceinline__ Row row(float top, float u) const {
+    Row r;
+    r.top = top;
+    r.max = top;
+    r.inv_t = fmax(369.32993046757463 / (double)temp, 1e-300);  // (T = inf: all finite logits weigh the same)
+    r.scale = fminf(fmaxf((float)(kBins / kSpan / (double)temp), 1.0e-37f), 3.0e38f);
+    r.min_w = (double)min_p * 0x1p43;
+    r.u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
+    return r;
+  }
   // whether the sum of all weights is asked for
   __device__ __forceinline__ bool sums(const SampleArgs &a) const { return !greedy && k >= (int)a.n && (p < 1.0f || min_p == 0.0f); }
 };
@@ -392,7 +493,7 @@ typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 // Per chunk of kChunk logits, the largest, the sum of the weights by that one (kFix
 // units) where it is asked for, and the largest of every kGroup.
 __global__ void __launch_bounds__(256) k_sample_stats(SampleArgs a, int64_t row0, SampleStats st) {
-  __shared__ double tab[64];
+  __shared__ double tab[kTab];
   __shared__ float red[4];
   __shared__ u64 redu[4];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = blockIdx.x;
@@ -401,7 +502,7 @@ __global__ void __launch_bounds__(256) k_sample_stats(SampleArgs a, int64_t row0
   const int n = (int)a.n, base = c * kChunk;
   const Settings s(a, row);
   const bool sums = s.sums(a);
-  if (sums && t < 64) tab[t] = exp2((double)t / 64);
+  if (sums) make_table(tab);
   float x[4][4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -425,21 +526,18 @@ __global__ void __launch_bounds__(256) k_sample_stats(SampleArgs a, int64_t row0
   }
   m = group_max<64>(m);
   if (lane == 0) red[wave] = m;
-  __syncthreads();
+  lds_barrier();
   m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   u64 sum = 0;
   if (sums) {
-    Row r;
-    r.max = m;
-    r.inv_t = 1.0 / (double)s.temp;
+    const Row r = s.row(m, 0.0f);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (base + j * 1024 + 4 * t + e < n) sum += fixed(weight(r, x[j][e], tab));
+      for (int e = 0; e < 4; ++e) sum += fixed(weight(r, x[j][e], tab));  // (-inf, past the row's end, weighs nothing)
     sum = wave_scan(sum);
     if (lane == 63) redu[wave] = sum;
-    __syncthreads();
+    lds_barrier();
     sum = redu[0] + redu[1] + redu[2] + redu[3];
   }
   if (t == 0) {
@@ -450,13 +548,13 @@ __global__ void __launch_bounds__(256) k_sample_stats(SampleArgs a, int64_t row0
 
 // The first element of [start, end) that is l.
 __device__ __forceinline__ int first_equal(const Logits &src, int start, int end, float l, Shared &sh) {
-  __syncthreads();
+  lds_barrier();
   if (threadIdx.x == 0) sh.at = end;
-  __syncthreads();
+  lds_barrier();
   int first = end;
   for (int i = start + threadIdx.x; i < end && first == end; i += kThreads) first = src.at(i) == l ? i : end;
   if (first < end) atomicMin(&sh.at, first);
-  __syncthreads();
+  lds_barrier();
   return sh.at;
 }
 
@@ -475,8 +573,9 @@ __device__ __forceinline__ int gather(const Row &r, const Logits &src, const flo
     n += (int)total;
   }
   if (n > kGroups) return -1;
-  __syncthreads();
-  auto load = [&](int i, float (&x)[4]) {
+  lds_barrier();
+  float x[4];  // of the last group that was looked at
+  auto load = [&](int i) {
     const int at = sh.group[i] * kGroup + 4 * l16;
     uint32_t in = 0;
 #pragma unroll
@@ -486,21 +585,21 @@ __device__ __forceinline__ int gather(const Row &r, const Logits &src, const flo
     }
     return in;
   };
+  uint32_t in = 0;
   for (int i = t >> 4; i < n; i += kThreads / 16) {
-    float x[4];
-    const int m = group_sum_i<16>(__builtin_popcount(load(i, x)));
+    in = load(i);
+    const int m = group_sum_i<16>(__builtin_popcount(in));
     if (l16 == 0) sh.in_group[i] = (uint16_t)m;
   }
-  __syncthreads();
+  lds_barrier();
   u64 total;
   const uint32_t mine = t < n ? sh.in_group[t] : 0;
   const int at = (int)block_scan(mine, total, sh);
   if (total > kCand) return -1;
   if (t < n) sh.in_group[t] = (uint16_t)at;
-  __syncthreads();
+  lds_barrier();
   for (int i = t >> 4; i < n; i += kThreads / 16) {
-    float x[4];
-    const uint32_t in = load(i, x);
+    if (n > kThreads / 16) in = load(i);
     int before = __builtin_popcount(in);
 #pragma unroll
     for (int d = 1; d < 16; d <<= 1) {
@@ -515,7 +614,7 @@ __device__ __forceinline__ int gather(const Row &r, const Logits &src, const flo
         sh.index[to++] = sh.group[i] * kGroup + 4 * l16 + e;
       }
   }
-  __syncthreads();
+  lds_barrier();
   return (int)total;
 }
 
@@ -524,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t ro
   __shared__ Shared sh;
   const int t = threadIdx.x;
   const int64_t row = row0 + blockIdx.x;
-  if (t < 64) sh.tab[t] = exp2((double)t / 64);
+  make_table(sh.tab);
   const Logits src{a.logits + row * a.stride, (int)a.n};
   const Settings s(a, row);
   const float *cm = st.chunk_max + (int64_t)blockIdx.x * chunks;
@@ -537,15 +636,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t ro
   }
   m = group_max<64>(m);
   if ((t & 63) == 0) sh.redf[t >> 6] = m;
-  __syncthreads();
+  lds_barrier();
   for (int i = 0; i < kWaves; ++i) m = fmaxf(m, sh.redf[i]);
-  Row r;
-  r.max = m;
-  r.u = a.u[row];
-  r.u = r.u > 0.0f ? fminf(r.u, 1.0f) : 0.0f;
-  r.min_p = s.min_p;
-  r.inv_t = 1.0 / (double)s.temp;
-  r.scale = fminf((float)(kBins / kSpan * r.inv_t), 3.0e38f);
+  const Row r = s.row(m, a.u[row]);
   int id = 0;
   float prob = 0.0f;
   if (m == -INFINITY) {  // nothing to draw from
@@ -553,9 +646,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t ro
     int start = 0, end = src.n;
     if (chunks) {
       if (t == 0) sh.at = chunks;
-      __syncthreads();
+      lds_barrier();
       if (t < chunks && cm[t] == m) atomicMin(&sh.at, t);
-      __syncthreads();
+      lds_barrier();
       start = sh.at * kChunk;
       end = start + kChunk < end ? start + kChunk : end;
     }
@@ -565,10 +658,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t ro
     // the chunks' sums by the row's largest
     u64 sum = 0, w = 0, mine = 0, before = 0;
     if (chunks && s.sums(a)) {
-      if (t < chunks) {
-        Row q = r;
-        mine = (u64)__builtin_rint((double)st.chunk_sum[(int64_t)blockIdx.x * chunks + t] * weight(q, cm[t], sh.tab));
-      }
+      if (t < chunks)
+        mine = (u64)__builtin_rint((double)st.chunk_sum[(int64_t)blockIdx.x * chunks + t] * 0x1p-43 * weight(r, cm[t], sh.tab));
       before = block_scan(mine, sum, sh);
     }
     int at = -1;
@@ -579,12 +670,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t ro
         sh.at = t;
         sh.before = before;
       }
-      __syncthreads();
+      lds_barrier();
       const int start = sh.at * kChunk, end = start + kChunk < src.n ? start + kChunk : src.n;
       goal -= sh.before;
       const float cl = cm[sh.at];
-      __syncthreads();
-      at = draw(r, src, Cut{0xffffffffu, ~0ull}, start, end - start, goal, sum, w, sum, sh);
+      lds_barrier();
+      at = draw(r, src, Cut{-INFINITY, ~0ull}, start, end - start, goal, sum, w, sum, sh);
       id = at >= 0 ? at : first_equal(src, start, end, cl, sh);  // (a chunk of many weights of under half a unit)
       w = at >= 0 ? w : 1;
       at = 0;
@@ -596,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t ro
       int b0 = kBins;
       clear(sh.mass);
       clear(sh.count);
-      __syncthreads();
+      lds_barrier();
       for (int g = t; g < n_group; g += kThreads) {
         const float x = gm[g];
         if (x == -INFINITY) continue;
@@ -604,22 +695,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t ro
         if (s.k < src.n) atomicAdd(&sh.count[b], 1u);
         else if (s.p < 1.0f) atomicAdd(&sh.mass[b], fixed(weight(r, x, sh.tab)));
       }
-      __syncthreads();
+      lds_barrier();
       u64 total, none;
       if (s.k < src.n) {
         block_scan((u64)sh.count[2 * t] + sh.count[2 * t + 1], total, sh);
         if ((u64)s.k <= total) b0 = crossing(sh.count, (u64)s.k, none, sh);
       } else if (s.p < 1.0f) {
-        const double x = (double)s.p * (double)sum;
-        u64 target = (u64)x;
-        target += (double)target < x;
-        target = target > 1 ? target : 1;
+        const u64 target = part_of(s.p, sum);
         block_scan(sh.mass[2 * t] + sh.mass[2 * t + 1], total, sh);
         if (target <= total) b0 = crossing(sh.mass, target, none, sh);
       }
-      if (r.min_p > 0.0 && (s.k >= src.n || s.p >= 1.0f)) {
+      if (s.min_p > 0.0f && (s.k >= src.n || s.p >= 1.0f)) {
         // (where top_p counts among the top_k all of those are needed)
-        const float x = (float)(-log(r.min_p) * (double)s.temp) * r.scale + 1.0f;
+        const float x = (float)(-log((double)s.min_p) * (double)s.temp) * r.scale + 1.0f;
         b0 = x < (float)b0 ? (int)x : b0;
       }
       if (b0 < kBins - 1) {
