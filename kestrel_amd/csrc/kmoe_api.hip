@@ -192,8 +192,8 @@ struct kmoe_ctx {
   hipStream_t stream = nullptr;
   std::string err;
   int regime = KMOE_REGIME_AVX2;
-  // device, zero between calls: kCounterWords completion counters, then the paged attention's
-  // and its choice of pages'
+  // device, zero between calls: kCounterWords completion counters, then the paged attention's,
+  // its choice of pages' and sampling's
   uint32_t *counters = nullptr;
   uint64_t vram_limit = 0;
   uint64_t vram_reserved = 0;
@@ -853,7 +853,7 @@ int kmoe_create(int device, kmoe_ctx **out) {
   }
   c->stream = c->own;
   // completion counters of multi-work-group kernels; zero between calls
-  const size_t cw = ((size_t)kCounterWords + paged_counters() + select_counters()) * 4;
+  const size_t cw = ((size_t)kCounterWords + paged_counters() + select_counters() + sample_counters()) * 4;
   if (hipMalloc((void **)&c->counters, cw) != hipSuccess || hipMemset(c->counters, 0, cw) != hipSuccess) {
     (void)hipStreamDestroy(c->own);
     delete c;
@@ -2560,7 +2560,7 @@ int kmoe_sample(kmoe_ctx *c, const float *logits, int64_t s_rows, int64_t n, int
   uint8_t *ws = nullptr;
   const int rc = kept_ws(c, c->sample, sample_ws_bytes(), "sampling", &ws);
   if (rc) return rc;
-  LAUNCH(c, "sample", launch_sample(c->stream, a, ws));
+  LAUNCH(c, "sample", launch_sample(c->stream, a, ws, c->counters + kCounterWords + paged_counters() + select_counters()));
   return KMOE_OK;
 }
 

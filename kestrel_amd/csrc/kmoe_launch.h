@@ -463,13 +463,18 @@ struct SampleArgs {
   float *prob;
   int32_t *pos, advance;
 };
-// What k_sample_stats finds of a row's chunks, for as many rows as the workspace holds.
+// What k_sample_stats finds of a row's chunks, for as many rows as the workspace holds,
+// and what the work-groups that share a row hand over: sums by bins of their parts, and
+// who has arrived (zero between calls).
 struct SampleStats {
   unsigned long long *chunk_sum;
-  float *chunk_max, *group_max;
+  float *chunk_max, *chunk_min, *chunk_low, *group_max;  // largest, least, lowest of the groups' largest; the groups' largest
+  unsigned long long *part_sum;
+  uint32_t *counters;
 };
 size_t sample_ws_bytes();
-hipError_t launch_sample(hipStream_t st, const SampleArgs &a, uint8_t *ws);
+int sample_counters();
+hipError_t launch_sample(hipStream_t st, const SampleArgs &a, uint8_t *ws, uint32_t *counters);
 hipError_t launch_argmax(hipStream_t st, const float *l, int64_t n, uint32_t *out, int32_t *pos_dev,
                          int32_t advance);
 hipError_t launch_pos_advance(hipStream_t st, int32_t *pos_dev, int32_t by);

@@ -34,7 +34,11 @@ constexpr int kTab = 256;
 constexpr int kGroup = 64, kChunk = 4096;  // elements of which k_sample_stats finds the largest, and the sum
 constexpr int kCand = 2048, kGroups = 1024;
 constexpr int kFew = 1024;  // elements of a bin that are compared one with another
-constexpr float kSpan = 24.0f;  // distances from the largest logit that the even bins tell apart, in units of T
+constexpr int kParts = 8;   // work-groups that share a row at most
+// Distances from the largest logit that the even bins tell apart: to the lowest that is binned,
+// at most this (a mask's -10^9 is none of the others' business) and 24 T, where
+// weights are what counts 24 T.
+constexpr float kSpan = 64.0f, kSpanT = 24.0f;
 
 // NaN as -inf. Order of the logits as whole numbers: the larger the logit, the smaller
 // its rank (-0 as 0).
@@ -109,7 +113,8 @@ struct Shared {
   uint32_t count[kBins];
   u64 red[kWaves];
   uint32_t redi[kWaves];
-  float redf[kWaves];
+  float redf[3][kWaves];
+  u64 part[kParts];
   u64 before, above;
   int at, n;
   // elements of one bin
@@ -479,10 +484,13 @@ struct Settings {
     r.top = top;
     r.max = top;
     r.inv_t = fmax(369.32993046757463 / (double)temp, 1e-300);  // (T = inf: all finite logits weigh the same)
-    r.scale = fminf(fmaxf((float)(kBins / kSpan / (double)temp), 1.0e-37f), 3.0e38f);
     r.min_w = (double)min_p * 0x1p43;
     r.u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
     return r;
+  }
+  // Bins per unit of logit; low: the lowest one.
+  __device__ __forceinline__ float scale(float top, float low, bool weights) const {
+    return fminf(fmaxf((kBins - 1) / fminf(top - low, (weights ? 0.0f : kSpan) + kSpanT * temp), 1.0e-37f), 3.0e38f);
   }
   // whether the sum of all weights is asked for
   __device__ __forceinline__ bool sums(const SampleArgs &a) const { return !greedy && k >= (int)a.n && (p < 1.0f || min_p == 0.0f); }
@@ -494,7 +502,7 @@ typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 // units) where it is asked for, and the largest of every kGroup.
 __global__ void __launch_bounds__(256) k_sample_stats(SampleArgs a, int64_t row0, SampleStats st) {
   __shared__ double tab[kTab];
-  __shared__ float red[4];
+  __shared__ float red[12];
   __shared__ u64 redu[4];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = blockIdx.x;
   const int64_t row = row0 + blockIdx.y;
@@ -517,17 +525,28 @@ __global__ void __launch_bounds__(256) k_sample_stats(SampleArgs a, int64_t row0
     }
   }
   float *gm = st.group_max + ((int64_t)blockIdx.y * gridDim.x + c) * (kChunk / kGroup);
-  float m = -INFINITY;
+  auto finite = [](float y) { return y == -INFINITY ? INFINITY : y; };  // (-inf is none of the lowest)
+  float m = -INFINITY, low = INFINITY, least = INFINITY;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
+    least = fminf(least, fminf(fminf(finite(x[j][0]), finite(x[j][1])), fminf(finite(x[j][2]), finite(x[j][3]))));
     const float g = group_max<16>(fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])));
     if ((lane & 15) == 0) gm[j * 16 + (t >> 4)] = g;
     m = fmaxf(m, g);
+    low = fminf(low, finite(g));
   }
   m = group_max<64>(m);
-  if (lane == 0) red[wave] = m;
+  low = -group_max<64>(-low);
+  least = -group_max<64>(-least);
+  if (lane == 0) {
+    red[wave] = m;
+    red[4 + wave] = low;
+    red[8 + wave] = least;
+  }
   lds_barrier();
   m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  low = fminf(fminf(red[4], red[5]), fminf(red[6], red[7]));
+  least = fminf(fminf(red[8], red[9]), fminf(red[10], red[11]));
   u64 sum = 0;
   if (sums) {
     const Row r = s.row(m, 0.0f);
@@ -542,6 +561,8 @@ __global__ void __launch_bounds__(256) k_sample_stats(SampleArgs a, int64_t row0
   }
   if (t == 0) {
     st.chunk_max[(int64_t)blockIdx.y * gridDim.x + c] = m;
+    st.chunk_low[(int64_t)blockIdx.y * gridDim.x + c] = low;
+    st.chunk_min[(int64_t)blockIdx.y * gridDim.x + c] = least;
     st.chunk_sum[(int64_t)blockIdx.y * gridDim.x + c] = sum;
   }
 }
@@ -618,30 +639,157 @@ __device__ __forceinline__ int gather(const Row &r, const Logits &src, const flo
   return (int)total;
 }
 
-// chunks: 0 without k_sample_stats before it.
+// A row of which more is kept than fits the candidates, without top_k: `parts` work-groups
+// share it. Each sums the weights of its part by bins; the last to arrive finds the cut
+// among the elements of the bin that the target falls into, and by the parts' sums the
+// part that the drawn token is in, so that only that one is gone through. Returns the token, -1 where
+// another work-group ends the row.
+__device__ __forceinline__ int draw_flat(const Row &r, const Logits &src, float p, const SampleStats &st, int parts, u64 &w,
+                                         u64 &sum, Shared &sh) {
+  const int t = threadIdx.x, len = (src.n + parts - 1) / parts, mine = blockIdx.y;
+  auto part = [&](int i) {
+    const int a = i * len < src.n ? i * len : src.n;
+    return Logits{src.l + a, src.n - a < len ? src.n - a : len};
+  };
+  lds_barrier();
+  clear(sh.mass);
+  lds_barrier();
+  each(part(mine), [&](int, float l) {
+    const u64 x = fixed(weight(r, l, sh.tab));
+    if (x) atomicAdd(&sh.mass[bin_of(r, l)], x);
+  });
+  lds_barrier();
+  u64 *all = st.part_sum + (int64_t)blockIdx.x * parts * kBins;
+  if (parts > 1) {
+    // (agent-scope accesses go past the XCDs' caches, and each wave has waited for its
+    // stores before the counter's add: no release besides)
+    for (int i = t; i < kBins; i += kThreads)
+      __hip_atomic_store(all + mine * kBins + i, sh.mass[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (t == 0) sh.n = (int)__hip_atomic_fetch_add(st.counters + blockIdx.x, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (sh.n != parts - 1) return -1;
+    if (t == 0) __hip_atomic_store(st.counters + blockIdx.x, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int i = t; i < kBins; i += kThreads) {
+      u64 x[kParts], s = 0;
+#pragma unroll
+      for (int k = 0; k < kParts; ++k)
+        x[k] = k < parts ? __hip_atomic_load(all + k * kBins + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+#pragma unroll
+      for (int k = 0; k < kParts; ++k) s += x[k];
+      sh.mass[i] = s;
+    }
+    lds_barrier();
+  }
+  u64 total, before;
+  block_scan(sh.mass[2 * t] + sh.mass[2 * t + 1], total, sh);
+  u64 target = part_of(p, total);
+  target = target < total ? target : total;
+  const int b = crossing(sh.mass, target, before, sh);
+  // the bin's elements, with their places
+  if (t == 0) sh.n = 0;
+  lds_barrier();
+  each(src, [&](int i, float l) {
+    if (bin_of(r, l) != b) return;
+    const int k = atomicAdd(&sh.n, 1);
+    if (k < kCand) {
+      sh.cand[k] = l;
+      sh.index[k] = i;
+    }
+  });
+  lds_barrier();
+  const int n = sh.n;
+  u64 none;
+  bool held = true;
+  Cut cut;
+  if (n > kCand) {
+    cut = cut_by_digits<true>(r, src, b, 0xffffffffu, target - before, none, sh);
+  } else {
+    const Candidates in{sh.cand, n};
+    cut = cut_in_bin<true>(r, in, b, n, 0xffffffffu, target - before, none, held, sh);
+  }
+  const double wt = weight(r, cut.v, sh.tab);
+  const u64 w_tie = fixed(wt);
+  cut.ties = (cut.ties + w_tie - 1) / w_tie;
+  // the parts' sums, where all of the kept weigh min_p and none of the equal ones is left out
+  u64 equal = 0;
+  if (n <= kCand && parts > 1) {
+    if (t < parts) sh.part[t] = 0;
+    lds_barrier();
+    uint32_t c = 0;
+    for (int i = t; i < n; i += kThreads) {
+      const float l = sh.cand[i];
+      c += l == cut.v;
+      if (l >= cut.v) atomicAdd(&sh.part[sh.index[i] / len], fixed(weight(r, l, sh.tab)));
+    }
+    block_scan(c, equal, sh);
+  }
+  if (n > kCand || parts == 1 || wt < r.min_w || equal > cut.ties) return draw(r, src, cut, 0, src.n, 0, 0, w, sum, sh);
+  for (int k = 0; k < parts; ++k) {
+    u64 s = 0, m;
+    for (int i = t; i < b; i += kThreads) s += __hip_atomic_load(all + k * kBins + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    block_scan(s, m, sh);
+    if (t == 0) sh.part[k] += m;
+  }
+  lds_barrier();
+  sum = 0;
+  for (int k = 0; k < parts; ++k) sum += sh.part[k];
+  u64 goal = (u64)((double)r.u * (double)sum);
+  goal = goal < sum ? goal : sum - 1;
+  int k = 0;
+  for (; k < parts - 1 && goal >= sh.part[k]; ++k) goal -= sh.part[k];
+  const Logits in = part(k);
+  lds_barrier();
+  return k * len + draw(r, in, Cut{cut.v, ~0ull}, 0, in.n, goal, sum, w, sum, sh);
+}
+
+// chunks: 0 without k_sample_stats before it. Grid: (rows, work-groups that share one).
 __global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t row0, SampleStats st, int chunks) {
   __shared__ Shared sh;
   const int t = threadIdx.x;
   const int64_t row = row0 + blockIdx.x;
+  const Settings s(a, row);
+  const bool flat = !s.greedy && s.k >= (int)a.n && s.p < 1.0f;  // (the others are one work-group's)
+  if (blockIdx.y && !flat) return;
   make_table(sh.tab);
   const Logits src{a.logits + row * a.stride, (int)a.n};
-  const Settings s(a, row);
   const float *cm = st.chunk_max + (int64_t)blockIdx.x * chunks;
-  // the largest logit
-  float m = -INFINITY;
+  // the largest logit, the least and the lowest of the groups' largest (without groups: the least again)
+  float m = -INFINITY, least = INFINITY, low = INFINITY;
   if (chunks) {
-    for (int i = t; i < chunks; i += kThreads) m = fmaxf(m, cm[i]);
+    const int64_t at = (int64_t)blockIdx.x * chunks;
+    for (int i = t; i < chunks; i += kThreads) {
+      m = fmaxf(m, cm[i]);
+      least = fminf(least, st.chunk_min[at + i]);
+      low = fminf(low, st.chunk_low[at + i]);
+    }
   } else {
-    each(src, [&](int, float l) { m = fmaxf(m, l); });
+    each(src, [&](int, float l) {
+      m = fmaxf(m, l);
+      least = fminf(least, l == -INFINITY ? INFINITY : l);
+    });
   }
   m = group_max<64>(m);
-  if ((t & 63) == 0) sh.redf[t >> 6] = m;
+  least = -group_max<64>(-least);
+  low = -group_max<64>(-low);
+  if ((t & 63) == 0) {
+    sh.redf[0][t >> 6] = m;
+    sh.redf[1][t >> 6] = least;
+    sh.redf[2][t >> 6] = low;
+  }
   lds_barrier();
-  for (int i = 0; i < kWaves; ++i) m = fmaxf(m, sh.redf[i]);
-  const Row r = s.row(m, a.u[row]);
+  for (int i = 0; i < kWaves; ++i) {
+    m = fmaxf(m, sh.redf[0][i]);
+    least = fminf(least, sh.redf[1][i]);
+    low = fminf(low, sh.redf[2][i]);
+  }
+  Row r = s.row(m, a.u[row]);
+  r.scale = s.scale(m, low, false);
   int id = 0;
   float prob = 0.0f;
   if (m == -INFINITY) {  // nothing to draw from
+    if (blockIdx.y) return;
   } else if (s.greedy) {
     int start = 0, end = src.n;
     if (chunks) {
@@ -673,10 +821,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t ro
       lds_barrier();
       const int start = sh.at * kChunk, end = start + kChunk < src.n ? start + kChunk : src.n;
       goal -= sh.before;
-      const float cl = cm[sh.at];
+      const float top = cm[sh.at];
       lds_barrier();
       at = draw(r, src, Cut{-INFINITY, ~0ull}, start, end - start, goal, sum, w, sum, sh);
-      id = at >= 0 ? at : first_equal(src, start, end, cl, sh);  // (a chunk of many weights of under half a unit)
+      id = at >= 0 ? at : first_equal(src, start, end, top, sh);  // (a chunk of many weights of under half a unit)
       w = at >= 0 ? w : 1;
       at = 0;
     } else if (chunks) {
@@ -685,8 +833,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t ro
       const float *gm = st.group_max + (int64_t)blockIdx.x * chunks * (kChunk / kGroup);
       const int n_group = (src.n + kGroup - 1) / kGroup;
       int b0 = kBins;
-      clear(sh.mass);
-      clear(sh.count);
+      lds_barrier();
+      if (s.k < src.n) clear(sh.count);
+      else clear(sh.mass);
       lds_barrier();
       for (int g = t; g < n_group; g += kThreads) {
         const float x = gm[g];
@@ -713,6 +862,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t ro
       if (b0 < kBins - 1) {
         const int n = gather(r, src, gm, n_group, b0, sh);
         if (n >= 0) {
+          if (blockIdx.y) return;
           const Candidates cand{sh.cand, n};
           Row f = r;
           f.scale = r.scale * ((float)kBins / (float)(b0 + 1));  // (their bins, finer)
@@ -723,8 +873,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t ro
       }
     }
     if (at < 0) {
-      const Cut cut = find_cut(r, src, s.k, s.p, 0, sh);
-      id = draw(r, src, cut, 0, src.n, 0, 0, w, sum, sh);
+      r.scale = s.scale(m, least, flat);
+      if (flat) {
+        id = draw_flat(r, src, s.p, st, (int)gridDim.y, w, sum, sh);
+        if (id < 0) return;
+      } else {
+        const Cut cut = find_cut(r, src, s.k, s.p, 0, sh);
+        id = draw(r, src, cut, 0, src.n, 0, 0, w, sum, sh);
+      }
     }
     prob = (float)((double)w / (double)sum);
   }
@@ -736,23 +892,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t ro
 }
 
 constexpr int64_t kFewTokens = 8192;  // a work-group reads so many as quickly as another launch comes
+constexpr int kShareRows = 256;       // rows times the work-groups that share one
 
 }  // namespace
 
-size_t sample_ws_bytes() { return (size_t)16 << 20; }
+constexpr size_t kStatBytes = (size_t)16 << 20;
+size_t sample_ws_bytes() { return kStatBytes + (size_t)kShareRows * kBins * 8; }
+int sample_counters() { return kShareRows; }
 
-hipError_t launch_sample(hipStream_t st, const SampleArgs &a, uint8_t *ws) {
+hipError_t launch_sample(hipStream_t st, const SampleArgs &a, uint8_t *ws, uint32_t *counters) {
   if (a.n <= kFewTokens) {
     KMOE_LAUNCH(k_sample, dim3((unsigned)a.rows), dim3(kThreads), 0, st, a, (int64_t)0, SampleStats{}, 0);
     return hipGetLastError();
   }
   const int chunks = (int)((a.n + kChunk - 1) / kChunk);
-  const int64_t each = (int64_t)chunks * (12 + 4 * (kChunk / kGroup)), most = (int64_t)sample_ws_bytes() / each;
+  const int64_t each = (int64_t)chunks * (20 + 4 * (kChunk / kGroup)), most = (int64_t)kStatBytes / each;
   for (int64_t row = 0; row < a.rows; row += most) {
     const int64_t n = a.rows - row < most ? a.rows - row : most;
-    const SampleStats s{(unsigned long long *)ws, (float *)(ws + 8 * most * chunks), (float *)(ws + 12 * most * chunks)};
+    // the chip's work-groups among few rows
+    const int parts = !a.top_p ? 1 : (int)(kShareRows / n < 1 ? 1 : kShareRows / n < kParts ? kShareRows / n : kParts);
+    auto at = [&](int64_t bytes) { return (float *)(ws + bytes * most * chunks); };
+    const SampleStats s{(unsigned long long *)ws, at(8), at(12), at(16), at(20), (unsigned long long *)(ws + kStatBytes), counters};
     KMOE_LAUNCH(k_sample_stats, dim3((unsigned)chunks, (unsigned)n), dim3(256), 0, st, a, row, s);
-    KMOE_LAUNCH(k_sample, dim3((unsigned)n), dim3(kThreads), 0, st, a, row, s, chunks);
+    KMOE_LAUNCH(k_sample, dim3((unsigned)n, (unsigned)parts), dim3(kThreads), 0, st, a, row, s, chunks);
   }
   return hipGetLastError();
 }
