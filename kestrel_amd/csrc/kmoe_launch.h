@@ -463,13 +463,16 @@ struct SampleArgs {
   float *prob;
   int32_t *pos, advance;
 };
-// What k_sample_stats finds of a row's chunks, for as many rows as the workspace holds,
-// and what the work-groups that share a row hand over: sums by bins of their parts, and
-// who has arrived (zero between calls).
+// What the kernels of a call leave for the next one, for as many rows as the workspace
+// holds: of a row's chunks the sum, the largest and the lowest of the groups' largest;
+// those; and of rows that work-groups share, sums by bins of their parts, what is known
+// of the row, the elements of a bin, and who has arrived (zero between calls).
 struct SampleStats {
   unsigned long long *chunk_sum;
-  float *chunk_max, *chunk_min, *chunk_low, *group_max;  // largest, least, lowest of the groups' largest; the groups' largest
+  float *chunk_max, *chunk_low, *group_max;
   unsigned long long *part_sum;
+  struct SampleRow *rows;
+  unsigned long long *in_bin;
   uint32_t *counters;
 };
 size_t sample_ws_bytes();

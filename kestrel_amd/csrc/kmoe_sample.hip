@@ -27,22 +27,30 @@ namespace kmoe {
 namespace {
 
 typedef unsigned long long u64;
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
+// Threads of a work-group: with 1024, every step between two barriers is issued four
+// times per SIMD, and most steps of a row are short (1 row of 32000: 16 us, 256 threads TODO).
+constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kFix = 43;    // weights in units of 2^-43
-constexpr int kBins = 2048;
+constexpr int kBins = 1024, kBinsEach = kBins / kThreads;
 constexpr int kTab = 256;
 constexpr int kGroup = 64, kChunk = 4096;  // elements of which k_sample_stats finds the largest, and the sum
 constexpr int kCand = 2048, kGroups = 1024;
 constexpr int kFew = 1024;  // elements of a bin that are compared one with another
-constexpr int kParts = 8;   // work-groups that share a row at most
+constexpr int kParts = 16;  // work-groups that share a row at most
+constexpr int kSegment = 1024;  // elements of which a draw knows the sum
 // Distances from the largest logit that the even bins tell apart: to the lowest that is binned,
 // at most this (a mask's -10^9 is none of the others' business) and 24 T, where
 // weights are what counts 24 T.
 constexpr float kSpan = 64.0f, kSpanT = 24.0f;
 
+// The larger of two that are no signalling NaNs (fmaxf quiets its operands first).
+__device__ __forceinline__ float max2(float a, float b) {
+  asm("v_max_f32 %0, %1, %2" : "=v"(a) : "v"(a), "v"(b));
+  return a;
+}
 // NaN as -inf. Order of the logits as whole numbers: the larger the logit, the smaller
 // its rank (-0 as 0).
-__device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY); }
+__device__ __forceinline__ float clean(float x) { return x == x ? x : -INFINITY; }
 __device__ __forceinline__ uint32_t rank_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.0f);
   return ~(b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u));
@@ -62,6 +70,7 @@ struct Row {
 };
 
 // Elements of a row: of the logits themselves, or candidates in LDS, in the order of their index.
+typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 struct Logits {
   const float *l;
   int n;
@@ -75,7 +84,8 @@ struct Candidates {
 
 // 2^(i / 256)
 __device__ __forceinline__ void make_table(double *tab) {
-  if (threadIdx.x < kTab) tab[threadIdx.x] = exp2((double)threadIdx.x / kTab);
+  static_assert(kTab == kThreads, "one entry a thread");
+  tab[threadIdx.x] = exp2((double)threadIdx.x / kTab);
 }
 
 // A weight in units: z = 256 log2 of it is i + f, |f| <= 1/2, and 2^(z / 256) a power of two
@@ -113,9 +123,9 @@ struct Shared {
   uint32_t count[kBins];
   u64 red[kWaves];
   uint32_t redi[kWaves];
-  float redf[3][kWaves];
+  float redf[2][kWaves];
   u64 part[kParts];
-  u64 before, above;
+  u64 before, above, ties;
   int at, n;
   // elements of one bin
   uint32_t rank[64];
@@ -160,42 +170,77 @@ __device__ __forceinline__ u64 block_scan(u64 x, u64 &total, Shared &sh) {
   return before;
 }
 
-// The first bin at which the running sum of hist reaches `target` (1 .. the total), and
-// the sum before it.
-template <class T>
+// The first of EACH * kThreads bins at which the running sum of hist reaches `target` (1 .. the
+// total), and the sum before it.
+template <int EACH, class T>
 __device__ __forceinline__ int crossing(const T *hist, u64 target, u64 &before, Shared &sh) {
   const int t = threadIdx.x;
-  const u64 a = hist[2 * t], b = hist[2 * t + 1];
-  u64 total;
-  const u64 x = block_scan(a + b, total, sh);
-  if (x < target && x + a + b >= target) {
-    const bool second = x + a < target;
-    sh.at = 2 * t + second;
-    sh.before = x + (second ? a : 0);
+  u64 x[EACH], s = 0, total;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) s += x[e] = hist[EACH * t + e];
+  u64 y = block_scan(s, total, sh);
+  if (y < target && y + s >= target) {
+    int e = 0;
+#pragma unroll
+    for (int k = 0; k < EACH - 1; ++k)
+      if (e == k && y + x[k] < target) {
+        y += x[k];
+        ++e;
+      }
+    sh.at = EACH * t + e;
+    sh.before = y;
   }
   lds_barrier();
   before = sh.before;
   return sh.at;
 }
+template <class T>
+__device__ __forceinline__ int crossing(const T *hist, u64 target, u64 &before, Shared &sh) {
+  return crossing<kBinsEach>(hist, target, before, sh);
+}
+// The sum of all bins below `end`.
+template <class T>
+__device__ __forceinline__ u64 sum_below(const T *hist, int end, Shared &sh) {
+  const int t = threadIdx.x;
+  u64 s = 0, total;
+#pragma unroll
+  for (int e = 0; e < kBinsEach; ++e) s += kBinsEach * t + e < end ? hist[kBinsEach * t + e] : 0;
+  block_scan(s, total, sh);
+  return total;
+}
 
-// f(i, l) for every element i, a work-group together.
-template <class S, class F>
-__device__ __forceinline__ void each(const S &src, F &&f) {
+// f(i, l) for every element i, a work-group together; loads of a row wait for each other
+// as little as the registers allow (32 elements a thread: a flat row's bin 15 -> 7 us).
+template <class F>
+__device__ __forceinline__ void each(const Candidates &src, F &&f) {
+  for (int i = threadIdx.x; i < src.n; i += kThreads) f(i, src.at(i));
+}
+template <class F>
+__device__ __forceinline__ void each(const Logits &src, F &&f) {
   constexpr int U = 8;
-  int i = threadIdx.x;
-  for (; i + (U - 1) * kThreads < src.n; i += U * kThreads) {
-    float x[U];
+  const int n4 = src.n & ~3;
+  for (int i0 = 4 * threadIdx.x; i0 < n4; i0 += 4 * U * kThreads) {
+    f32x4a4 x[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) x[j] = src.at(i + j * kThreads);
+    for (int j = 0; j < U; ++j) {
+      const int i = i0 + 4 * j * kThreads;
+      x[j] = *(const f32x4a4 *)(src.l + (i < n4 ? i : i0));
+    }
 #pragma unroll
-    for (int j = 0; j < U; ++j) f(i + j * kThreads, x[j]);
+    for (int j = 0; j < U; ++j) {
+      const int i = i0 + 4 * j * kThreads;
+      if (i >= n4) break;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f(i + e, clean(x[j][e]));
+    }
   }
-  for (; i < src.n; i += kThreads) f(i, src.at(i));
+  if ((int)threadIdx.x < src.n - n4) f(n4 + threadIdx.x, src.at(n4 + threadIdx.x));
 }
 
 template <class T>
 __device__ __forceinline__ void clear(T *h) {
-  for (int i = threadIdx.x; i < kBins; i += kThreads) h[i] = 0;
+#pragma unroll
+  for (int e = 0; e < kBinsEach; ++e) h[kThreads * e + threadIdx.x] = 0;
 }
 
 // Sum of f(i, l) over the elements, to every thread.
@@ -223,23 +268,22 @@ __device__ __forceinline__ Cut cut_by_digits(const Row &r, const S &src, int bin
                                              Shared &sh) {
   uint32_t found = 0;
 #pragma unroll 1
-  for (int d = 0; d < 3; ++d) {  // 11, 11 and 10 bits
-    const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, top = d == 0 ? 32 : d == 1 ? 21 : 10;
+  for (int shift = 24; shift >= 0; shift -= 8) {
     lds_barrier();
-    if (MASS) clear(sh.mass);
-    else clear(sh.count);
+    if (MASS) sh.mass[threadIdx.x] = 0;
+    else sh.count[threadIdx.x] = 0;
     lds_barrier();
     each(src, [&](int, float l) {
       if (bin_of(r, l) != bin) return;
       const uint32_t k = rank_of(l);
-      if (k >= limit || (d && k >> top != found >> top)) return;
-      const int b = (k >> shift) & (d == 2 ? 1023 : 2047);
+      if (k >= limit || (shift < 24 && (k ^ found) >> (shift + 8))) return;
+      const int b = (k >> shift) & 255;
       if (MASS) atomicAdd(&sh.mass[b], fixed(weight(r, l, sh.tab)));
       else atomicAdd(&sh.count[b], 1u);
     });
     lds_barrier();
     u64 before;
-    const int b = MASS ? crossing(sh.mass, target, before, sh) : crossing(sh.count, target, before, sh);
+    const int b = MASS ? crossing<1>(sh.mass, target, before, sh) : crossing<1>(sh.count, target, before, sh);
     target -= before;
     found |= (uint32_t)b << shift;
   }
@@ -322,7 +366,6 @@ __device__ __forceinline__ u64 part_of(float p, u64 x) {
 // whole row's sum where the elements are not all that top_p counts, or 0.
 template <class S>
 __device__ __forceinline__ Cut find_cut(const Row &r, const S &src, int k, float p, u64 all_, Shared &sh) {
-  const int t = threadIdx.x;
   Cut cut{-INFINITY, ~0ull};
   if (k >= src.n && p >= 1.0f) return cut;
   lds_barrier();
@@ -343,7 +386,7 @@ __device__ __forceinline__ Cut find_cut(const Row &r, const S &src, int k, float
   u64 n_before = 0, m_bins = 0, w_tie = 0;
   int kb = kBins;
   if (k < src.n) kb = crossing(sh.count, (u64)k, n_before, sh);
-  if (p < 1.0f) block_scan((2 * t < kb ? sh.mass[2 * t] : 0) + (2 * t + 1 < kb ? sh.mass[2 * t + 1] : 0), m_bins, sh);
+  if (p < 1.0f) m_bins = sum_below(sh.mass, kb, sh);
   u64 m_above = m_bins, all = m_bins, above;
   bool held = true;
   if (kb < kBins) {
@@ -375,94 +418,148 @@ __device__ __forceinline__ Cut find_cut(const Row &r, const S &src, int k, float
   return cut;
 }
 
-// The first kept element from `start` on at which the running sum passes u times the
-// sum, or `goal` where `whole` is given (the sum of a row of which src is a part): the
-// range is cut into 16 parts by sums of its waves until it has an element per thread.
-// Returns its weight and the sum; -1 where all weights are 0.
+// The first kept element at which the running sum passes u times the sum, or `goal` where `whole`
+// is given (the sum of a row of which src is a part). More elements than kSegment: by
+// the sums of segments first, a wave each. Returns its weight and the sum; -1 where all
+// weights are 0.
 template <class S>
-__device__ __forceinline__ int draw(const Row &r, const S &src, const Cut &cut, int start, int len, u64 goal, u64 whole,
-                                    u64 &w, u64 &sum, Shared &sh) {
+__device__ __forceinline__ int draw(const Row &r, const S &src, const Cut &cut, u64 goal, u64 whole, u64 &w, u64 &sum,
+                                    Shared &sh) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   auto kept = [&](float l) -> u64 {
     const double x = weight(r, l, sh.tab);
     return x >= r.min_w ? fixed(x) : 0;
   };
   const u64 w_tie = kept(cut.v);
-  u64 ties = cut.ties;
-  bool first = true;
-  auto begin = [&](u64 total) {
+  const bool limited = cut.ties < (u64)src.n;  // some of those equal to v may be left out
+  int start = 0, len = src.n;
+  u64 ties = cut.ties, total;
+  auto begin = [&]() {
     sum = whole ? whole : total;
     if (!whole) goal = (u64)((double)r.u * (double)sum);
     goal = goal < total ? goal : total - 1;  // (a part's sum, as the row's was formed, may be some units off)
-    first = false;
   };
-  while (len > kThreads) {
-    const int part = (len + kThreads - 1) / kThreads * 64, a = start + wave * part;
-    const int b = a + part < start + len ? a + part : start + len;
-    u64 s = 0;
-    uint32_t c = 0;
-    constexpr int U = 8;
-    int i = a + lane;
-    auto add = [&](float l) {
-      const u64 x = kept(l);
-      s += l > cut.v ? x : 0;
-      c += l == cut.v;
-    };
-    for (; i + (U - 1) * 64 < b; i += U * 64) {
-      float x[U];
-#pragma unroll
-      for (int j = 0; j < U; ++j) x[j] = src.at(i + j * 64);
-#pragma unroll
-      for (int j = 0; j < U; ++j) add(x[j]);
-    }
-    for (; i < b; i += 64) add(src.at(i));
-    s = wave_scan(s);
-    c = (uint32_t)group_sum_i<64>((int)c);
+  if (len > kSegment) {
+    const int n = (len + kSegment - 1) / kSegment;
     lds_barrier();
-    if (lane == 63) {
-      sh.red[wave] = s;
-      sh.redi[wave] = c;
-    }
-    lds_barrier();
-    auto of_part = [&](int i, u64 left) { return sh.red[i] + (sh.redi[i] < left ? sh.redi[i] : left) * w_tie; };
-    if (first) {
-      u64 left = ties, total = 0;
-      for (int i = 0; i < kWaves; ++i) {
-        total += of_part(i, left);
-        left -= sh.redi[i] < left ? sh.redi[i] : left;
+    for (int k = wave; k < n; k += kWaves) {
+      const int a = k * kSegment + lane, b = k * kSegment + kSegment < len ? k * kSegment + kSegment : len;
+      u64 s = 0;
+      uint32_t c = 0;
+      float x[kSegment / 64];
+#pragma unroll
+      for (int j = 0; j < kSegment / 64; ++j) x[j] = src.at(a + j * 64 < b ? a + j * 64 : b - 1);
+#pragma unroll
+      for (int j = 0; j < kSegment / 64; ++j) {
+        const u64 y = kept(x[j]);
+        const bool in = a + j * 64 < b;
+        s += in && (limited ? x[j] > cut.v : x[j] >= cut.v) ? y : 0;
+        c += in && x[j] == cut.v;
       }
-      if (!total) return -1;
-      begin(total);
+      s = wave_scan(s);
+      if (limited) c = (uint32_t)group_sum_i<64>((int)c);
+      if (lane == 63) {
+        sh.mass[k] = s;
+        if (limited) sh.count[k] = c;
+      }
     }
-    int k = 0;
-    for (; k < kWaves - 1; ++k) {
-      const u64 m = of_part(k, ties);
-      if (goal < m) break;
-      goal -= m;
-      ties -= sh.redi[k] < ties ? sh.redi[k] : ties;
+    lds_barrier();
+    u64 s[kBinsEach], all = 0, mine = 0, held = 0;
+#pragma unroll
+    for (int e = 0; e < kBinsEach; ++e) s[e] = kBinsEach * t + e < n ? sh.mass[kBinsEach * t + e] : 0;
+    if (limited) {  // how many of the equal ones each segment keeps
+      uint32_t c[kBinsEach];
+      u64 x = 0;
+#pragma unroll
+      for (int e = 0; e < kBinsEach; ++e) x += c[e] = kBinsEach * t + e < n ? sh.count[kBinsEach * t + e] : 0;
+      held = block_scan(x, total, sh);
+      u64 before = held;
+#pragma unroll
+      for (int e = 0; e < kBinsEach; ++e) {
+        const u64 left = ties > before ? ties - before : 0;
+        s[e] += (c[e] < left ? c[e] : left) * w_tie;
+        before += c[e];
+      }
     }
-    const int end = start + len;
-    start += k * part;
-    len = start + part < end ? part : end - start;
-  }
-  const float l = t < len ? src.at(start + t) : -INFINITY;
-  const bool tie = t < len && l == cut.v;
-  u64 total, nth = 0;
-  if (ties < kThreads) nth = block_scan(tie, total, sh);
-  const u64 m = t < len && (l > cut.v || (tie && nth < ties)) ? kept(l) : 0;
-  const u64 x = block_scan(m, total, sh);
-  if (first) {
+#pragma unroll
+    for (int e = 0; e < kBinsEach; ++e) mine += s[e];
+    all = block_scan(mine, total, sh);
     if (!total) return -1;
-    begin(total);
+    begin();
+    if (all <= goal && goal < all + mine) {
+      int e = 0;
+#pragma unroll
+      for (int k = 0; k < kBinsEach - 1; ++k)
+        if (e == k && all + s[k] <= goal) {
+          all += s[k];
+          if (limited) held += sh.count[kBinsEach * t + k];
+          ++e;
+        }
+      sh.at = kBinsEach * t + e;
+      sh.before = all;
+      sh.ties = held;
+    }
+    lds_barrier();
+    start = sh.at * kSegment;
+    len = start + kSegment < len ? kSegment : len - start;
+    goal -= sh.before;
+    ties = limited ? (ties > sh.ties ? ties - sh.ties : 0) : ties;
+    lds_barrier();
   }
-  if (x <= goal && goal < x + m) {
-    sh.at = start + t;
-    sh.before = m;
+  // EACH elements a thread
+  constexpr int EACH = kSegment / kThreads;
+  float l[EACH];
+  u64 m[EACH], x = 0, nth = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) l[e] = EACH * t + e < len ? src.at(start + EACH * t + e) : -INFINITY;
+  if (limited) {
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) x += EACH * t + e < len && l[e] == cut.v;
+    nth = block_scan(x, total, sh);
+    x = 0;
+  }
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const bool in = EACH * t + e < len, tie = in && l[e] == cut.v;
+    x += m[e] = in && (l[e] > cut.v || (tie && (!limited || nth < ties))) ? kept(l[e]) : 0;
+    nth += tie;
+  }
+  u64 at = block_scan(x, total, sh);
+  if (src.n <= kSegment) {
+    if (!total) return -1;
+    begin();
+  }
+  if (at <= goal && goal < at + x) {
+    int e = 0;
+#pragma unroll
+    for (int k = 0; k < EACH - 1; ++k)
+      if (e == k && at + m[k] <= goal) {
+        at += m[k];
+        ++e;
+      }
+    u64 v = 0;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) v = e == k ? m[k] : v;
+    sh.at = start + EACH * t + e;
+    sh.before = v;
   }
   lds_barrier();
   w = sh.before;
   return sh.at;
 }
+
+}  // namespace
+
+// A row that work-groups share: its cut lies in `bin`, where target is left of what is
+// looked for.
+struct SampleRow {
+  float top, scale;
+  int shared, bin;  // shared: work-groups, 0: the row is done
+  unsigned long long target;
+  unsigned long long part[kParts];  // the parts' sums before the bin
+};
+
+namespace {
 
 // A row's settings, as they are used.
 struct Settings {
@@ -496,13 +593,11 @@ struct Settings {
   __device__ __forceinline__ bool sums(const SampleArgs &a) const { return !greedy && k >= (int)a.n && (p < 1.0f || min_p == 0.0f); }
 };
 
-typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
-
 // Per chunk of kChunk logits, the largest, the sum of the weights by that one (kFix
 // units) where it is asked for, and the largest of every kGroup.
 __global__ void __launch_bounds__(256) k_sample_stats(SampleArgs a, int64_t row0, SampleStats st) {
   __shared__ double tab[kTab];
-  __shared__ float red[12];
+  __shared__ float red[8];
   __shared__ u64 redu[4];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = blockIdx.x;
   const int64_t row = row0 + blockIdx.y;
@@ -525,28 +620,27 @@ __global__ void __launch_bounds__(256) k_sample_stats(SampleArgs a, int64_t row0
     }
   }
   float *gm = st.group_max + ((int64_t)blockIdx.y * gridDim.x + c) * (kChunk / kGroup);
-  auto finite = [](float y) { return y == -INFINITY ? INFINITY : y; };  // (-inf is none of the lowest)
-  float m = -INFINITY, low = INFINITY, least = INFINITY;
+  float m = -INFINITY, low = INFINITY;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    least = fminf(least, fminf(fminf(finite(x[j][0]), finite(x[j][1])), fminf(finite(x[j][2]), finite(x[j][3]))));
-    const float g = group_max<16>(fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])));
+    float g = max2(max2(x[j][0], x[j][1]), max2(x[j][2], x[j][3]));
+    g = max2(g, dpp_f<kDppXor1>(g));
+    g = max2(g, dpp_f<kDppXor2>(g));
+    g = max2(g, dpp_f<kDppHalfMirror>(g));
+    g = max2(g, dpp_f<kDppMirror>(g));
     if ((lane & 15) == 0) gm[j * 16 + (t >> 4)] = g;
-    m = fmaxf(m, g);
-    low = fminf(low, finite(g));
+    m = max2(m, g);
+    low = fminf(low, g == -INFINITY ? INFINITY : g);
   }
   m = group_max<64>(m);
   low = -group_max<64>(-low);
-  least = -group_max<64>(-least);
   if (lane == 0) {
     red[wave] = m;
     red[4 + wave] = low;
-    red[8 + wave] = least;
   }
   lds_barrier();
   m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   low = fminf(fminf(red[4], red[5]), fminf(red[6], red[7]));
-  least = fminf(fminf(red[8], red[9]), fminf(red[10], red[11]));
   u64 sum = 0;
   if (sums) {
     const Row r = s.row(m, 0.0f);
@@ -562,7 +656,6 @@ __global__ void __launch_bounds__(256) k_sample_stats(SampleArgs a, int64_t row0
   if (t == 0) {
     st.chunk_max[(int64_t)blockIdx.y * gridDim.x + c] = m;
     st.chunk_low[(int64_t)blockIdx.y * gridDim.x + c] = low;
-    st.chunk_min[(int64_t)blockIdx.y * gridDim.x + c] = least;
     st.chunk_sum[(int64_t)blockIdx.y * gridDim.x + c] = sum;
   }
 }
@@ -573,24 +666,48 @@ __device__ __forceinline__ int first_equal(const Logits &src, int start, int end
   if (threadIdx.x == 0) sh.at = end;
   lds_barrier();
   int first = end;
-  for (int i = start + threadIdx.x; i < end && first == end; i += kThreads) first = src.at(i) == l ? i : end;
+  for (int i = start + threadIdx.x; i < end && first == end; i += 4 * kThreads) {
+    float x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = src.at(i + j * kThreads < end ? i + j * kThreads : i);
+#pragma unroll
+    for (int j = 3; j >= 0; --j) first = x[j] == l && i + j * kThreads < end ? i + j * kThreads : first;
+  }
   if (first < end) atomicMin(&sh.at, first);
   lds_barrier();
   return sh.at;
 }
 
+// The largest of a thread's four groups from g on (16-byte aligned).
+__device__ __forceinline__ f32x4a4 groups_at(const float *gm, int n_group, int g) {
+  f32x4a4 x = *(const f32x4a4 *)(gm + (g < n_group ? g : 0));  // (a chunk's groups, beyond the row's too, are all written)
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = g + e < n_group ? x[e] : -INFINITY;
+  return x;
+}
+
 // The elements whose even bin is at most b0, in sh.cand and sh.index, in their order;
-// -1 where they are too many. A group's largest says whether it has any.
-__device__ __forceinline__ int gather(const Row &r, const Logits &src, const float *gm, int n_group, int b0, Shared &sh) {
+// -1 where they are too many. A group's largest says whether it has any; g4: those of
+// the thread's first groups.
+__device__ __forceinline__ int gather(const Row &r, const Logits &src, const float *gm, f32x4a4 g4, int n_group, int b0,
+                                      Shared &sh) {
   const int t = threadIdx.x, l16 = t & 15;
   int n = 0;
-  for (int g0 = 0; g0 < n_group; g0 += kThreads) {
-    const int g = g0 + t;
-    const float x = g < n_group ? gm[g] : -INFINITY;
-    const bool in = x != -INFINITY && bin_of(r, x) <= b0;
+  for (int g0 = 0; g0 < n_group; g0 += 4 * kThreads) {
+    const int g = g0 + 4 * t;
+    if (g0) g4 = groups_at(gm, n_group, g);
+    uint32_t in = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (g4[e] != -INFINITY && bin_of(r, g4[e]) <= b0) in |= 1u << e;
     u64 total;
-    const int at = n + (int)block_scan(in, total, sh);
-    if (in && at < kGroups) sh.group[at] = (uint16_t)g;
+    int at = n + (int)block_scan(__builtin_popcount(in), total, sh);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (in >> e & 1) {
+        if (at < kGroups) sh.group[at] = (uint16_t)(g + e);
+        ++at;
+      }
     n += (int)total;
   }
   if (n > kGroups) return -1;
@@ -614,10 +731,17 @@ __device__ __forceinline__ int gather(const Row &r, const Logits &src, const flo
   }
   lds_barrier();
   u64 total;
-  const uint32_t mine = t < n ? sh.in_group[t] : 0;
-  const int at = (int)block_scan(mine, total, sh);
+  constexpr int EACH = kGroups / kThreads;
+  int c[EACH], mine = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) mine += c[e] = EACH * t + e < n ? sh.in_group[EACH * t + e] : 0;
+  int at = (int)block_scan(mine, total, sh);
   if (total > kCand) return -1;
-  if (t < n) sh.in_group[t] = (uint16_t)at;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    if (EACH * t + e < n) sh.in_group[EACH * t + e] = (uint16_t)at;
+    at += c[e];
+  }
   lds_barrier();
   for (int i = t >> 4; i < n; i += kThreads / 16) {
     if (n > kThreads / 16) in = load(i);
@@ -639,83 +763,157 @@ __device__ __forceinline__ int gather(const Row &r, const Logits &src, const flo
   return (int)total;
 }
 
-// A row of which more is kept than fits the candidates, without top_k: `parts` work-groups
-// share it. Each sums the weights of its part by bins; the last to arrive finds the cut
-// among the elements of the bin that the target falls into, and by the parts' sums the
-// part that the drawn token is in, so that only that one is gone through. Returns the token, -1 where
-// another work-group ends the row.
-__device__ __forceinline__ int draw_flat(const Row &r, const Logits &src, float p, const SampleStats &st, int parts, u64 &w,
-                                         u64 &sum, Shared &sh) {
-  const int t = threadIdx.x, len = (src.n + parts - 1) / parts, mine = blockIdx.y;
-  auto part = [&](int i) {
-    const int a = i * len < src.n ? i * len : src.n;
-    return Logits{src.l + a, src.n - a < len ? src.n - a : len};
-  };
+// A row of which more is kept than fits the candidates, without top_k, is shared by work-groups,
+// a part each. k_sample sums the weights of the parts by bins; the last work-group to
+// arrive finds the bin that the target falls into. k_sample_shared gathers that bin's
+// elements; the last to arrive finds the cut among them, and by the parts' sums the part
+// that the drawn token is in, so that only that one is gone through.
+__device__ __forceinline__ int part_len(int n, int parts) { return (n + parts - 1) / parts; }
+__device__ __forceinline__ Logits part_at(const Logits &src, int len, int i) {
+  const int a = i * len < src.n ? i * len : src.n;
+  return Logits{src.l + a, src.n - a < len ? src.n - a : len};
+}
+
+// Whether this work-group is the last of `parts` to arrive. What is handed over is
+// written and read by agent-scope accesses, which go past the XCDs' caches, and each
+// wave has waited for its stores before the counter's add: no release besides.
+__device__ __forceinline__ bool last_of(uint32_t *counter, int parts, Shared &sh) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sh.n = (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (sh.n == parts - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  return sh.n == parts - 1;
+}
+
+__device__ __forceinline__ void share(const Row &r, const Logits &src, float p, const SampleStats &st, int parts, Shared &sh) {
+  const int t = threadIdx.x, mine = blockIdx.y;
   lds_barrier();
   clear(sh.mass);
   lds_barrier();
-  each(part(mine), [&](int, float l) {
+  each(part_at(src, part_len(src.n, parts), mine), [&](int, float l) {
     const u64 x = fixed(weight(r, l, sh.tab));
     if (x) atomicAdd(&sh.mass[bin_of(r, l)], x);
   });
   lds_barrier();
   u64 *all = st.part_sum + (int64_t)blockIdx.x * parts * kBins;
-  if (parts > 1) {
-    // (agent-scope accesses go past the XCDs' caches, and each wave has waited for its
-    // stores before the counter's add: no release besides)
-    for (int i = t; i < kBins; i += kThreads)
-      __hip_atomic_store(all + mine * kBins + i, sh.mass[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (t == 0) sh.n = (int)__hip_atomic_fetch_add(st.counters + blockIdx.x, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if (sh.n != parts - 1) return -1;
-    if (t == 0) __hip_atomic_store(st.counters + blockIdx.x, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int i = t; i < kBins; i += kThreads) {
-      u64 x[kParts], s = 0;
 #pragma unroll
-      for (int k = 0; k < kParts; ++k)
-        x[k] = k < parts ? __hip_atomic_load(all + k * kBins + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+  for (int e = 0; e < kBinsEach; ++e)
+    __hip_atomic_store(all + mine * kBins + e * kThreads + t, sh.mass[e * kThreads + t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (!last_of(st.counters + 2 * blockIdx.x, parts, sh)) return;
+  auto load = [&](int k, int e) {
+    return k < parts ? __hip_atomic_load(all + k * kBins + e * kThreads + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+  };
+  u64 s[kBinsEach] = {};
+  for (int k0 = 0; k0 < parts; k0 += 4) {
+    u64 x[4][kBinsEach];
 #pragma unroll
-      for (int k = 0; k < kParts; ++k) s += x[k];
-      sh.mass[i] = s;
-    }
-    lds_barrier();
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < kBinsEach; ++e) x[k][e] = load(k0 + k, e);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < kBinsEach; ++e) s[e] += x[k][e];
   }
-  u64 total, before;
-  block_scan(sh.mass[2 * t] + sh.mass[2 * t + 1], total, sh);
-  u64 target = part_of(p, total);
+#pragma unroll
+  for (int e = 0; e < kBinsEach; ++e) sh.mass[e * kThreads + t] = s[e];
+  lds_barrier();
+  const u64 total = sum_below(sh.mass, kBins, sh);
+  u64 target = part_of(p, total), before;
   target = target < total ? target : total;
   const int b = crossing(sh.mass, target, before, sh);
-  // the bin's elements, with their places
+  if (t < kParts) sh.part[t] = 0;
+  lds_barrier();
+  for (int k0 = 0; k0 < parts; k0 += 4) {
+    u64 x[4] = {};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < kBinsEach; ++e) {
+        const u64 y = load(k0 + k, e);
+        x[k] += e * kThreads + t < b ? y : 0;
+      }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      x[k] = wave_scan(x[k]);
+      if ((t & 63) == 63 && k0 + k < parts) atomicAdd(&sh.part[k0 + k], x[k]);
+    }
+  }
+  lds_barrier();
+  SampleRow *row = st.rows + blockIdx.x;
+  if (t < parts) row->part[t] = sh.part[t];
+  if (t == 0) {
+    row->top = r.top;
+    row->scale = r.scale;
+    row->shared = parts;
+    row->bin = b;
+    row->target = target - before;
+  }
+}
+
+__device__ __forceinline__ void answer(const SampleArgs &a, int64_t row, int id, float prob) {
+  a.out[row] = (uint32_t)id;
+  if (a.prob) a.prob[row] = prob;
+  if (a.pos) a.pos[row] += a.advance;
+}
+
+// Grid: (rows, parts).
+__global__ void __launch_bounds__(kThreads) k_sample_shared(SampleArgs a, int64_t row0, SampleStats st) {
+  const SampleRow *have = st.rows + blockIdx.x;
+  const int parts = have->shared;
+  if (parts == 0) return;
+  __shared__ Shared sh;
+  const int t = threadIdx.x;
+  const int64_t row = row0 + blockIdx.x;
+  make_table(sh.tab);
   if (t == 0) sh.n = 0;
   lds_barrier();
-  each(src, [&](int i, float l) {
+  const Logits src{a.logits + row * a.stride, (int)a.n};
+  Row r = Settings(a, row).row(have->top, a.u[row]);
+  r.scale = have->scale;
+  const int len = part_len(src.n, parts), mine = blockIdx.y, b = have->bin;
+  each(part_at(src, len, mine), [&](int i, float l) {
     if (bin_of(r, l) != b) return;
     const int k = atomicAdd(&sh.n, 1);
     if (k < kCand) {
       sh.cand[k] = l;
-      sh.index[k] = i;
+      sh.index[k] = mine * len + i;
     }
   });
   lds_barrier();
-  const int n = sh.n;
-  u64 none;
-  bool held = true;
-  Cut cut;
-  if (n > kCand) {
-    cut = cut_by_digits<true>(r, src, b, 0xffffffffu, target - before, none, sh);
-  } else {
-    const Candidates in{sh.cand, n};
-    cut = cut_in_bin<true>(r, in, b, n, 0xffffffffu, target - before, none, held, sh);
+  uint32_t *const counter = st.counters + 2 * blockIdx.x;
+  u64 *list = st.in_bin + (int64_t)blockIdx.x * kCand;
+  const int own = sh.n;
+  if (t == 0) sh.at = (int)__hip_atomic_fetch_add(counter + 1, (uint32_t)own, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  lds_barrier();
+  const int at = sh.at;
+  for (int i = t; i < own && i < kCand && at + i < kCand; i += kThreads)
+    __hip_atomic_store(list + at + i, (u64)(uint32_t)sh.index[i] << 32 | __float_as_uint(sh.cand[i]), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+  if (!last_of(counter, parts, sh)) return;
+  const int n = (int)__hip_atomic_load(counter + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int i = t; i < n && i < kCand; i += kThreads) {
+    const u64 x = __hip_atomic_load(list + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    sh.cand[i] = __uint_as_float((uint32_t)x);
+    sh.index[i] = (int)(x >> 32);
   }
+  __syncthreads();
+  if (t == 0) __hip_atomic_store(counter + 1, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  u64 none, w, sum;
+  bool held = true;
+  Cut cut = n > kCand ? cut_by_digits<true>(r, src, b, 0xffffffffu, have->target, none, sh)
+                      : cut_in_bin<true>(r, Candidates{sh.cand, n}, b, n, 0xffffffffu, have->target, none, held, sh);
   const double wt = weight(r, cut.v, sh.tab);
   const u64 w_tie = fixed(wt);
   cut.ties = (cut.ties + w_tie - 1) / w_tie;
   // the parts' sums, where all of the kept weigh min_p and none of the equal ones is left out
   u64 equal = 0;
-  if (n <= kCand && parts > 1) {
-    if (t < parts) sh.part[t] = 0;
+  if (n <= kCand) {
+    lds_barrier();
+    if (t < parts) sh.part[t] = have->part[t];
     lds_barrier();
     uint32_t c = 0;
     for (int i = t; i < n; i += kThreads) {
@@ -725,64 +923,62 @@ __device__ __forceinline__ int draw_flat(const Row &r, const Logits &src, float 
     }
     block_scan(c, equal, sh);
   }
-  if (n > kCand || parts == 1 || wt < r.min_w || equal > cut.ties) return draw(r, src, cut, 0, src.n, 0, 0, w, sum, sh);
-  for (int k = 0; k < parts; ++k) {
-    u64 s = 0, m;
-    for (int i = t; i < b; i += kThreads) s += __hip_atomic_load(all + k * kBins + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    block_scan(s, m, sh);
-    if (t == 0) sh.part[k] += m;
+  int id;
+  if (n > kCand || wt < r.min_w || equal > cut.ties) {
+    id = draw(r, src, cut, 0, 0, w, sum, sh);
+  } else {
+    sum = 0;
+    for (int k = 0; k < parts; ++k) sum += sh.part[k];
+    u64 goal = (u64)((double)r.u * (double)sum);
+    goal = goal < sum ? goal : sum - 1;
+    int k = 0;
+    for (; k < parts - 1 && goal >= sh.part[k]; ++k) goal -= sh.part[k];
+    id = k * len + draw(r, part_at(src, len, k), Cut{cut.v, ~0ull}, goal, sum, w, sum, sh);
   }
-  lds_barrier();
-  sum = 0;
-  for (int k = 0; k < parts; ++k) sum += sh.part[k];
-  u64 goal = (u64)((double)r.u * (double)sum);
-  goal = goal < sum ? goal : sum - 1;
-  int k = 0;
-  for (; k < parts - 1 && goal >= sh.part[k]; ++k) goal -= sh.part[k];
-  const Logits in = part(k);
-  lds_barrier();
-  return k * len + draw(r, in, Cut{cut.v, ~0ull}, 0, in.n, goal, sum, w, sum, sh);
+  if (t == 0) answer(a, row, id, (float)((double)w / (double)sum));
 }
 
-// chunks: 0 without k_sample_stats before it. Grid: (rows, work-groups that share one).
-__global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t row0, SampleStats st, int chunks) {
+// chunks: 0 without k_sample_stats before it. Grid: (rows, work-groups that may share one).
+__global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, int64_t row0, SampleStats st, int chunks) {
   __shared__ Shared sh;
   const int t = threadIdx.x;
   const int64_t row = row0 + blockIdx.x;
   const Settings s(a, row);
-  const bool flat = !s.greedy && s.k >= (int)a.n && s.p < 1.0f;  // (the others are one work-group's)
+  const bool flat = gridDim.y > 1 && !s.greedy && s.k >= (int)a.n && s.p < 1.0f;  // (the others are one work-group's)
   if (blockIdx.y && !flat) return;
   make_table(sh.tab);
   const Logits src{a.logits + row * a.stride, (int)a.n};
-  const float *cm = st.chunk_max + (int64_t)blockIdx.x * chunks;
-  // the largest logit, the least and the lowest of the groups' largest (without groups: the least again)
-  float m = -INFINITY, least = INFINITY, low = INFINITY;
+  // the largest logit, and the lowest of the groups' largest (without groups: of all)
+  float m = -INFINITY, low = INFINITY;
+  const int64_t c0 = (int64_t)blockIdx.x * chunks;
+  const float *cm = st.chunk_max + c0, *gm = st.group_max + c0 * (kChunk / kGroup);
+  const int n_group = (src.n + kGroup - 1) / kGroup;
+  f32x4a4 g4{0};
+  u64 chunk_sum = 0;  // (at most kThreads chunks: one a thread)
+  float chunk_max = -INFINITY;
   if (chunks) {
-    const int64_t at = (int64_t)blockIdx.x * chunks;
-    for (int i = t; i < chunks; i += kThreads) {
-      m = fmaxf(m, cm[i]);
-      least = fminf(least, st.chunk_min[at + i]);
-      low = fminf(low, st.chunk_low[at + i]);
+    g4 = groups_at(gm, n_group, 4 * t);
+    if (t < chunks) {
+      chunk_max = m = cm[t];
+      low = st.chunk_low[c0 + t];
+      chunk_sum = st.chunk_sum[c0 + t];
     }
   } else {
     each(src, [&](int, float l) {
       m = fmaxf(m, l);
-      least = fminf(least, l == -INFINITY ? INFINITY : l);
+      low = fminf(low, l == -INFINITY ? INFINITY : l);
     });
   }
   m = group_max<64>(m);
-  least = -group_max<64>(-least);
   low = -group_max<64>(-low);
   if ((t & 63) == 0) {
     sh.redf[0][t >> 6] = m;
-    sh.redf[1][t >> 6] = least;
-    sh.redf[2][t >> 6] = low;
+    sh.redf[1][t >> 6] = low;
   }
   lds_barrier();
   for (int i = 0; i < kWaves; ++i) {
     m = fmaxf(m, sh.redf[0][i]);
-    least = fminf(least, sh.redf[1][i]);
-    low = fminf(low, sh.redf[2][i]);
+    low = fminf(low, sh.redf[1][i]);
   }
   Row r = s.row(m, a.u[row]);
   r.scale = s.scale(m, low, false);
@@ -795,7 +991,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t ro
     if (chunks) {
       if (t == 0) sh.at = chunks;
       lds_barrier();
-      if (t < chunks && cm[t] == m) atomicMin(&sh.at, t);
+      if (t < chunks && chunk_max == m) atomicMin(&sh.at, t);
       lds_barrier();
       start = sh.at * kChunk;
       end = start + kChunk < end ? start + kChunk : end;
@@ -807,7 +1003,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t ro
     u64 sum = 0, w = 0, mine = 0, before = 0;
     if (chunks && s.sums(a)) {
       if (t < chunks)
-        mine = (u64)__builtin_rint((double)st.chunk_sum[(int64_t)blockIdx.x * chunks + t] * 0x1p-43 * weight(r, cm[t], sh.tab));
+        mine = (u64)__builtin_rint((double)chunk_sum * 0x1p-43 * weight(r, chunk_max, sh.tab));
       before = block_scan(mine, sum, sh);
     }
     int at = -1;
@@ -823,35 +1019,36 @@ __global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t ro
       goal -= sh.before;
       const float top = cm[sh.at];
       lds_barrier();
-      at = draw(r, src, Cut{-INFINITY, ~0ull}, start, end - start, goal, sum, w, sum, sh);
-      id = at >= 0 ? at : first_equal(src, start, end, top, sh);  // (a chunk of many weights of under half a unit)
+      at = draw(r, Logits{src.l + start, end - start}, Cut{-INFINITY, ~0ull}, goal, sum, w, sum, sh);
+      id = at >= 0 ? start + at : first_equal(src, start, end, top, sh);  // (a chunk of many weights of under half a unit)
       w = at >= 0 ? w : 1;
       at = 0;
     } else if (chunks) {
       // a bin that holds the last kept token, or one after it, by the groups' largest: as
       // many of them as tokens are kept, or of as much weight
-      const float *gm = st.group_max + (int64_t)blockIdx.x * chunks * (kChunk / kGroup);
-      const int n_group = (src.n + kGroup - 1) / kGroup;
       int b0 = kBins;
       lds_barrier();
       if (s.k < src.n) clear(sh.count);
       else clear(sh.mass);
       lds_barrier();
-      for (int g = t; g < n_group; g += kThreads) {
-        const float x = gm[g];
-        if (x == -INFINITY) continue;
-        const int b = bin_of(r, x);
-        if (s.k < src.n) atomicAdd(&sh.count[b], 1u);
-        else if (s.p < 1.0f) atomicAdd(&sh.mass[b], fixed(weight(r, x, sh.tab)));
+      for (int g = 4 * t; g < n_group; g += 4 * kThreads) {
+        const f32x4a4 y = g < 4 * kThreads ? g4 : groups_at(gm, n_group, g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (y[e] == -INFINITY) continue;
+          const int b = bin_of(r, y[e]);
+          if (s.k < src.n) atomicAdd(&sh.count[b], 1u);
+          else if (s.p < 1.0f) atomicAdd(&sh.mass[b], fixed(weight(r, y[e], sh.tab)));
+        }
       }
       lds_barrier();
       u64 total, none;
       if (s.k < src.n) {
-        block_scan((u64)sh.count[2 * t] + sh.count[2 * t + 1], total, sh);
+        total = sum_below(sh.count, kBins, sh);
         if ((u64)s.k <= total) b0 = crossing(sh.count, (u64)s.k, none, sh);
       } else if (s.p < 1.0f) {
         const u64 target = part_of(s.p, sum);
-        block_scan(sh.mass[2 * t] + sh.mass[2 * t + 1], total, sh);
+        total = sum_below(sh.mass, kBins, sh);
         if (target <= total) b0 = crossing(sh.mass, target, none, sh);
       }
       if (s.min_p > 0.0f && (s.k >= src.n || s.p >= 1.0f)) {
@@ -860,44 +1057,44 @@ __global__ void __launch_bounds__(kThreads, 1) k_sample(SampleArgs a, int64_t ro
         b0 = x < (float)b0 ? (int)x : b0;
       }
       if (b0 < kBins - 1) {
-        const int n = gather(r, src, gm, n_group, b0, sh);
+        const int n = gather(r, src, gm, g4, n_group, b0, sh);
         if (n >= 0) {
           if (blockIdx.y) return;
           const Candidates cand{sh.cand, n};
           Row f = r;
           f.scale = r.scale * ((float)kBins / (float)(b0 + 1));  // (their bins, finer)
           const Cut cut = find_cut(f, cand, s.k, s.p, s.k < src.n ? 0 : sum, sh);
-          at = draw(f, cand, cut, 0, n, 0, 0, w, sum, sh);
+          at = draw(f, cand, cut, 0, 0, w, sum, sh);
           id = sh.index[at];
         }
       }
     }
     if (at < 0) {
-      r.scale = s.scale(m, least, flat);
+      // (elements lie about as far below the groups' largest as those lie apart, twice or three times)
+      r.scale = s.scale(m, chunks ? m - 4.0f * (m - low) - 1.0f : low, s.k >= src.n);
       if (flat) {
-        id = draw_flat(r, src, s.p, st, (int)gridDim.y, w, sum, sh);
-        if (id < 0) return;
-      } else {
-        const Cut cut = find_cut(r, src, s.k, s.p, 0, sh);
-        id = draw(r, src, cut, 0, src.n, 0, 0, w, sum, sh);
+        share(r, src, s.p, st, (int)gridDim.y, sh);
+        return;
       }
+      const Cut cut = find_cut(r, src, s.k, s.p, 0, sh);
+      id = draw(r, src, cut, 0, 0, w, sum, sh);
     }
     prob = (float)((double)w / (double)sum);
   }
   if (t == 0) {
-    a.out[row] = (uint32_t)id;
-    if (a.prob) a.prob[row] = prob;
-    if (a.pos) a.pos[row] += a.advance;
+    answer(a, row, id, prob);
+    if (gridDim.y > 1) st.rows[blockIdx.x].shared = 0;
   }
 }
 
 constexpr int64_t kFewTokens = 8192;  // a work-group reads so many as quickly as another launch comes
-constexpr int kShareRows = 256;       // rows times the work-groups that share one
+constexpr int kShareRows = 512;       // rows times the work-groups that share one
+constexpr size_t kStatBytes = (size_t)16 << 20, kSumBytes = (size_t)kShareRows * kBins * 8,
+                 kListBytes = (size_t)kShareRows / 2 * kCand * 8, kRowBytes = kShareRows / 2 * sizeof(SampleRow);
 
 }  // namespace
 
-constexpr size_t kStatBytes = (size_t)16 << 20;
-size_t sample_ws_bytes() { return kStatBytes + (size_t)kShareRows * kBins * 8; }
+size_t sample_ws_bytes() { return kStatBytes + kSumBytes + kListBytes + kRowBytes; }
 int sample_counters() { return kShareRows; }
 
 hipError_t launch_sample(hipStream_t st, const SampleArgs &a, uint8_t *ws, uint32_t *counters) {
@@ -906,15 +1103,20 @@ hipError_t launch_sample(hipStream_t st, const SampleArgs &a, uint8_t *ws, uint3
     return hipGetLastError();
   }
   const int chunks = (int)((a.n + kChunk - 1) / kChunk);
-  const int64_t each = (int64_t)chunks * (20 + 4 * (kChunk / kGroup)), most = (int64_t)kStatBytes / each;
+  const int64_t each = (int64_t)chunks * (16 + 4 * (kChunk / kGroup)), most = (int64_t)kStatBytes / each;
   for (int64_t row = 0; row < a.rows; row += most) {
     const int64_t n = a.rows - row < most ? a.rows - row : most;
-    // the chip's work-groups among few rows
-    const int parts = !a.top_p ? 1 : (int)(kShareRows / n < 1 ? 1 : kShareRows / n < kParts ? kShareRows / n : kParts);
+    // the chip's work-groups among few rows that top_p may leave much of
+    int parts = a.top_p && n <= kShareRows / 2 ? (int)(kShareRows / n) : 1;
+    parts = parts < kParts ? parts : kParts;
+    parts = parts < chunks ? parts : chunks;
     auto at = [&](int64_t bytes) { return (float *)(ws + bytes * most * chunks); };
-    const SampleStats s{(unsigned long long *)ws, at(8), at(12), at(16), at(20), (unsigned long long *)(ws + kStatBytes), counters};
+    uint8_t *const sums = ws + kStatBytes, *const list = sums + kSumBytes;
+    const SampleStats s{(unsigned long long *)ws,   at(8), at(12), at(16), (unsigned long long *)sums, (SampleRow *)(list + kListBytes),
+                        (unsigned long long *)list, counters};
     KMOE_LAUNCH(k_sample_stats, dim3((unsigned)chunks, (unsigned)n), dim3(256), 0, st, a, row, s);
     KMOE_LAUNCH(k_sample, dim3((unsigned)n, (unsigned)parts), dim3(kThreads), 0, st, a, row, s, chunks);
+    if (parts > 1) KMOE_LAUNCH(k_sample_shared, dim3((unsigned)n, (unsigned)parts), dim3(kThreads), 0, st, a, row, s);
   }
   return hipGetLastError();
 }
