@@ -489,7 +489,7 @@ int kmoe_argmax(kmoe_ctx *ctx, const float *logits_dev, int64_t n, uint32_t *out
  * tokens, prob (may be NULL) the probabilities they were drawn with among the kept. When
  * pos_dev [s_rows] is non-NULL, each is advanced by `advance` afterwards. out, prob and
  * pos must not overlap each other or the inputs. At most 2^20 rows. The context keeps a
- * workspace of 25 MB for it, as kmoe_paged_attention keeps one, with the same rules for
+ * workspace of 30 MB for it, as kmoe_paged_attention keeps one, with the same rules for
  * streams, captures and the VRAM budget. */
 #define KMOE_SAMPLE_MAX 1048576
 typedef struct {

@@ -34,7 +34,7 @@ constexpr int kFix = 43;    // weights in units of 2^-43
 constexpr int kBins = 1024, kBinsEach = kBins / kThreads;
 constexpr int kTab = 256;
 constexpr int kGroup = 64, kChunk = 4096;  // elements of which k_sample_stats finds the largest, and the sum
-constexpr int kCand = 2048, kGroups = 1024;
+constexpr int kCand = 4096, kGroups = 1024;
 constexpr int kFew = 1024;  // elements of a bin that are compared one with another
 constexpr int kParts = 16;  // work-groups that share a row at most
 constexpr int kSegment = 1024;  // elements of which a draw knows the sum
@@ -294,37 +294,17 @@ __device__ __forceinline__ Cut cut_by_digits(const Row &r, const S &src, int bin
   return Cut{of_rank(found), target};
 }
 
-// The same by the number of the bin's elements (`few` of them): up to 64 are compared with each
-// other (`held`: the counts stay), more of a long row are gathered first.
-template <bool MASS, class S>
-__device__ __forceinline__ Cut cut_in_bin(const Row &r, const S &src, int bin, int few, uint32_t limit, u64 target,
-                                          u64 &above, bool &held, Shared &sh) {
+// The same among at most 64 elements, those that in() names: each is compared with all.
+template <bool MASS, class S, class F>
+__device__ __forceinline__ Cut cut_of_few(const Row &r, const S &src, F &&in, u64 target, u64 &above, Shared &sh) {
   const int t = threadIdx.x;
-  if (few > 64) {
-    held = false;
-    if constexpr (std::is_same<S, Logits>::value) {
-      if (few <= kCand) {
-        lds_barrier();
-        if (t == 0) sh.n = 0;
-        lds_barrier();
-        each(src, [&](int, float l) {
-          if (bin_of(r, l) == bin) sh.cand[atomicAdd(&sh.n, 1)] = l;
-        });
-        lds_barrier();
-        return cut_by_digits<MASS>(r, Candidates{sh.cand, sh.n}, bin, limit, target, above, sh);
-      }
-    }
-    return cut_by_digits<MASS>(r, src, bin, limit, target, above, sh);
-  }
   lds_barrier();
   if (t == 0) sh.n = 0;
   lds_barrier();
   each(src, [&](int, float l) {
-    if (bin_of(r, l) != bin) return;
-    const uint32_t k = rank_of(l);
-    if (k >= limit) return;
+    if (!in(l)) return;
     const int i = atomicAdd(&sh.n, 1);
-    sh.rank[i] = k;
+    sh.rank[i] = rank_of(l);
     sh.w[i] = fixed(weight(r, l, sh.tab));
   });
   lds_barrier();
@@ -352,6 +332,53 @@ __device__ __forceinline__ Cut cut_in_bin(const Row &r, const S &src, int bin, i
   lds_barrier();
   above = sh.above;
   return Cut{of_rank((uint32_t)sh.at), target - sh.before};
+}
+
+// The same by the number of the bin's elements (`few` of them): up to 64 are compared with each
+// other (`held`: the counts stay), more of a long row are gathered first.
+template <bool MASS, bool FINER = true, class S>
+__device__ __forceinline__ Cut cut_in_bin(const Row &r, const S &src, int bin, int few, uint32_t limit, u64 target,
+                                          u64 &above, bool &held, Shared &sh) {
+  const int t = threadIdx.x;
+  if (few > 64) {
+    held = false;
+    if constexpr (std::is_same<S, Logits>::value) {
+      if (few <= kCand) {
+        lds_barrier();
+        if (t == 0) sh.n = 0;
+        lds_barrier();
+        each(src, [&](int, float l) {
+          if (bin_of(r, l) == bin) sh.cand[atomicAdd(&sh.n, 1)] = l;
+        });
+        lds_barrier();
+        return cut_by_digits<MASS>(r, Candidates{sh.cand, sh.n}, bin, limit, target, above, sh);
+      }
+    }
+    if constexpr (FINER && MASS && std::is_same<S, Candidates>::value) {
+      // finer bins of what lies in this one (the others' elements fall in the first and the
+      // last, which the cut is not looked for among)
+      Row f = r;
+      f.top = r.top - (float)bin / r.scale;
+      f.scale = r.scale * kBins;
+      auto in = [&](float l) { return bin_of(r, l) == bin && rank_of(l) < limit; };
+      lds_barrier();
+      clear(sh.mass);
+      clear(sh.count);
+      lds_barrier();
+      each(src, [&](int, float l) {
+        if (!in(l)) return;
+        const int b = bin_of(f, l);
+        atomicAdd(&sh.mass[b], fixed(weight(r, l, sh.tab)));
+        atomicAdd(&sh.count[b], 1u);
+      });
+      lds_barrier();
+      u64 before;
+      const int b = crossing(sh.mass, target, before, sh);
+      if (sh.count[b] <= 64) return cut_of_few<true>(r, src, [&](float l) { return in(l) && bin_of(f, l) == b; }, target - before, above, sh);
+    }
+    return cut_by_digits<MASS>(r, src, bin, limit, target, above, sh);
+  }
+  return cut_of_few<MASS>(r, src, [&](float l) { return bin_of(r, l) == bin && rank_of(l) < limit; }, target, above, sh);
 }
 
 // The first whole number that is p times x or more, 1 .. x's own.
@@ -442,13 +469,20 @@ __device__ __forceinline__ int draw(const Row &r, const S &src, const Cut &cut, 
   if (len > kSegment) {
     const int n = (len + kSegment - 1) / kSegment;
     lds_barrier();
+    float x[kSegment / 64], next[kSegment / 64];
+    auto load = [&](int k) {
+      const int a = k * kSegment + lane;
+#pragma unroll
+      for (int j = 0; j < kSegment / 64; ++j) next[j] = src.l[a + j * 64 < len ? a + j * 64 : len - 1];
+    };
+    load(wave);
     for (int k = wave; k < n; k += kWaves) {
       const int a = k * kSegment + lane, b = k * kSegment + kSegment < len ? k * kSegment + kSegment : len;
       u64 s = 0;
       uint32_t c = 0;
-      float x[kSegment / 64];
 #pragma unroll
-      for (int j = 0; j < kSegment / 64; ++j) x[j] = src.at(a + j * 64 < b ? a + j * 64 : b - 1);
+      for (int j = 0; j < kSegment / 64; ++j) x[j] = clean(next[j]);
+      if (k + kWaves < n) load(k + kWaves);
 #pragma unroll
       for (int j = 0; j < kSegment / 64; ++j) {
         const u64 y = kept(x[j]);
@@ -551,12 +585,12 @@ __device__ __forceinline__ int draw(const Row &r, const S &src, const Cut &cut, 
 }  // namespace
 
 // A row that work-groups share: its cut lies in `bin`, where target is left of what is
-// looked for.
+// looked for; the parts' sums before it.
 struct SampleRow {
   float top, scale;
   int shared, bin;  // shared: work-groups, 0: the row is done
   unsigned long long target;
-  unsigned long long part[kParts];  // the parts' sums before the bin
+  unsigned long long part[kParts];
 };
 
 namespace {
@@ -712,22 +746,34 @@ __device__ __forceinline__ int gather(const Row &r, const Logits &src, const flo
   }
   if (n > kGroups) return -1;
   lds_barrier();
-  float x[4];  // of the last group that was looked at
-  auto load = [&](int i) {
-    const int at = sh.group[i] * kGroup + 4 * l16;
-    uint32_t in = 0;
+  // a row of 16 lanes per group, four groups at a time; of up to 64 groups the elements stay
+  // in registers
+  constexpr int U = 4, ROWS = kThreads / 16;
+  float x[U][4];
+  uint32_t in[U];
+  auto load = [&](int i0) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[e] = at + e < src.n ? src.at(at + e) : -INFINITY;
-      if (x[e] != -INFINITY && bin_of(r, x[e]) <= b0) in |= 1u << e;
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * ROWS, at = i < n ? sh.group[i] * kGroup + 4 * l16 : src.n;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[u][e] = src.l[at + e < src.n ? at + e : src.n - 1];
+      in[u] = at + 4 <= src.n ? 15 : at < src.n ? (1u << (src.n - at)) - 1 : 0;
     }
-    return in;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[u][e] = clean(x[u][e]);
+        if (x[u][e] == -INFINITY || bin_of(r, x[u][e]) > b0) in[u] &= ~(1u << e);
+      }
   };
-  uint32_t in = 0;
-  for (int i = t >> 4; i < n; i += kThreads / 16) {
-    in = load(i);
-    const int m = group_sum_i<16>(__builtin_popcount(in));
-    if (l16 == 0) sh.in_group[i] = (uint16_t)m;
+  for (int i0 = t >> 4; i0 < n; i0 += U * ROWS) {
+    load(i0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int m = group_sum_i<16>(__builtin_popcount(in[u]));
+      if (l16 == 0 && i0 + u * ROWS < n) sh.in_group[i0 + u * ROWS] = (uint16_t)m;
+    }
   }
   lds_barrier();
   u64 total;
@@ -743,21 +789,26 @@ __device__ __forceinline__ int gather(const Row &r, const Logits &src, const flo
     at += c[e];
   }
   lds_barrier();
-  for (int i = t >> 4; i < n; i += kThreads / 16) {
-    if (n > kThreads / 16) in = load(i);
-    int before = __builtin_popcount(in);
+  for (int i0 = t >> 4; i0 < n; i0 += U * ROWS) {
+    if (n > U * ROWS) load(i0);
 #pragma unroll
-    for (int d = 1; d < 16; d <<= 1) {
-      const int y = __shfl_up(before, d, 16);
-      if (l16 >= d) before += y;
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * ROWS;
+      const int own = __builtin_popcount(in[u]);
+      int before = own;  // inclusive, over the row of lanes
+      before += __builtin_amdgcn_update_dpp(0, before, 0x111, 0xf, 0xf, false);
+      before += __builtin_amdgcn_update_dpp(0, before, 0x112, 0xf, 0xf, false);
+      before += __builtin_amdgcn_update_dpp(0, before, 0x114, 0xf, 0xf, false);
+      before += __builtin_amdgcn_update_dpp(0, before, 0x118, 0xf, 0xf, false);
+      if (i >= n || !own) continue;
+      int to = sh.in_group[i] + before - own;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (in[u] & (1u << e)) {
+          sh.cand[to] = x[u][e];
+          sh.index[to++] = sh.group[i] * kGroup + 4 * l16 + e;
+        }
     }
-    int to = sh.in_group[i] + before - __builtin_popcount(in);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (in & (1u << e)) {
-        sh.cand[to] = x[e];
-        sh.index[to++] = sh.group[i] * kGroup + 4 * l16 + e;
-      }
   }
   lds_barrier();
   return (int)total;
@@ -803,18 +854,16 @@ __device__ __forceinline__ void share(const Row &r, const Logits &src, float p, 
   for (int e = 0; e < kBinsEach; ++e)
     __hip_atomic_store(all + mine * kBins + e * kThreads + t, sh.mass[e * kThreads + t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   if (!last_of(st.counters + 2 * blockIdx.x, parts, sh)) return;
-  auto load = [&](int k, int e) {
-    return k < parts ? __hip_atomic_load(all + k * kBins + e * kThreads + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
-  };
   u64 s[kBinsEach] = {};
-  for (int k0 = 0; k0 < parts; k0 += 4) {
-    u64 x[4][kBinsEach];
+  for (int k0 = 0; k0 < parts; k0 += 8) {
+    u64 x[8][kBinsEach];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < 8; ++k)
 #pragma unroll
-      for (int e = 0; e < kBinsEach; ++e) x[k][e] = load(k0 + k, e);
+      for (int e = 0; e < kBinsEach; ++e)
+        x[k][e] = k0 + k < parts ? __hip_atomic_load(all + (k0 + k) * kBins + e * kThreads + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < 8; ++k)
 #pragma unroll
       for (int e = 0; e < kBinsEach; ++e) s[e] += x[k][e];
   }
@@ -825,33 +874,44 @@ __device__ __forceinline__ void share(const Row &r, const Logits &src, float p, 
   u64 target = part_of(p, total), before;
   target = target < total ? target : total;
   const int b = crossing(sh.mass, target, before, sh);
-  if (t < kParts) sh.part[t] = 0;
-  lds_barrier();
-  for (int k0 = 0; k0 < parts; k0 += 4) {
-    u64 x[4] = {};
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int e = 0; e < kBinsEach; ++e) {
-        const u64 y = load(k0 + k, e);
-        x[k] += e * kThreads + t < b ? y : 0;
-      }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      x[k] = wave_scan(x[k]);
-      if ((t & 63) == 63 && k0 + k < parts) atomicAdd(&sh.part[k0 + k], x[k]);
-    }
-  }
-  lds_barrier();
-  SampleRow *row = st.rows + blockIdx.x;
-  if (t < parts) row->part[t] = sh.part[t];
   if (t == 0) {
+    SampleRow *row = st.rows + blockIdx.x;
     row->top = r.top;
     row->scale = r.scale;
     row->shared = parts;
     row->bin = b;
     row->target = target - before;
   }
+}
+
+// The part that the drawn token is in by the parts' sums (sh.part), what is left of the
+// goal there, and the sum.
+__device__ __forceinline__ int part_drawn(const Row &r, int parts, u64 &goal, u64 &sum, const Shared &sh) {
+  sum = 0;
+  for (int k = 0; k < parts; ++k) sum += sh.part[k];
+  goal = (u64)((double)r.u * (double)sum);
+  goal = goal < sum ? goal : sum - 1;
+  int k = 0;
+  for (; k < parts - 1 && goal >= sh.part[k]; ++k) goal -= sh.part[k];
+  return k;
+}
+
+// The same with min_p alone, which needs no cut: the last work-group to arrive draws. -1 in the others.
+__device__ __forceinline__ int draw_shared(const Row &r, const Logits &src, const SampleStats &st, int parts, u64 &w, u64 &sum,
+                                           Shared &sh) {
+  const int t = threadIdx.x, len = part_len(src.n, parts);
+  const u64 own = sum_of(part_at(src, len, blockIdx.y), sh, [&](int, float l) {
+    const double x = weight(r, l, sh.tab);
+    return x >= r.min_w ? fixed(x) : 0;
+  });
+  u64 *all = st.part_sum + (int64_t)blockIdx.x * parts * kBins;
+  if (t == 0) __hip_atomic_store(all + blockIdx.y, own, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (!last_of(st.counters + 2 * blockIdx.x, parts, sh)) return -1;
+  if (t < parts) sh.part[t] = __hip_atomic_load(all + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  lds_barrier();
+  u64 goal;
+  const int k = part_drawn(r, parts, goal, sum, sh);
+  return k * len + draw(r, part_at(src, len, k), Cut{-INFINITY, ~0ull}, goal, sum, w, sum, sh);
 }
 
 __device__ __forceinline__ void answer(const SampleArgs &a, int64_t row, int id, float prob) {
@@ -884,7 +944,17 @@ __global__ void __launch_bounds__(kThreads) k_sample_shared(SampleArgs a, int64_
     }
   });
   lds_barrier();
+  // the part's sum before the bin
+  u64 *all = st.part_sum + ((int64_t)blockIdx.x * parts + mine) * kBins, s = 0, below;
+#pragma unroll
+  for (int e = 0; e < kBinsEach; ++e) {
+    const u64 x = __hip_atomic_load(all + e * kThreads + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s += e * kThreads + t < b ? x : 0;
+  }
+  block_scan(s, below, sh);
   uint32_t *const counter = st.counters + 2 * blockIdx.x;
+  unsigned long long *const part = st.rows[blockIdx.x].part;
+  if (t == 0) __hip_atomic_store(part + mine, below, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   u64 *list = st.in_bin + (int64_t)blockIdx.x * kCand;
   const int own = sh.n;
   if (t == 0) sh.at = (int)__hip_atomic_fetch_add(counter + 1, (uint32_t)own, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -913,7 +983,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_shared(SampleArgs a, int64_
   u64 equal = 0;
   if (n <= kCand) {
     lds_barrier();
-    if (t < parts) sh.part[t] = have->part[t];
+    if (t < parts) sh.part[t] = __hip_atomic_load(part + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     lds_barrier();
     uint32_t c = 0;
     for (int i = t; i < n; i += kThreads) {
@@ -927,12 +997,8 @@ __global__ void __launch_bounds__(kThreads) k_sample_shared(SampleArgs a, int64_
   if (n > kCand || wt < r.min_w || equal > cut.ties) {
     id = draw(r, src, cut, 0, 0, w, sum, sh);
   } else {
-    sum = 0;
-    for (int k = 0; k < parts; ++k) sum += sh.part[k];
-    u64 goal = (u64)((double)r.u * (double)sum);
-    goal = goal < sum ? goal : sum - 1;
-    int k = 0;
-    for (; k < parts - 1 && goal >= sh.part[k]; ++k) goal -= sh.part[k];
+    u64 goal;
+    const int k = part_drawn(r, parts, goal, sum, sh);
     id = k * len + draw(r, part_at(src, len, k), Cut{cut.v, ~0ull}, goal, sum, w, sum, sh);
   }
   if (t == 0) answer(a, row, id, (float)((double)w / (double)sum));
@@ -944,7 +1010,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, int64_t row0,
   const int t = threadIdx.x;
   const int64_t row = row0 + blockIdx.x;
   const Settings s(a, row);
-  const bool flat = gridDim.y > 1 && !s.greedy && s.k >= (int)a.n && s.p < 1.0f;  // (the others are one work-group's)
+  const bool flat = gridDim.y > 1 && !s.greedy && s.k >= (int)a.n && (s.p < 1.0f || s.min_p > 0.0f);  // (the others are one work-group's)
   if (blockIdx.y && !flat) return;
   make_table(sh.tab);
   const Logits src{a.logits + row * a.stride, (int)a.n};
@@ -1072,12 +1138,17 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, int64_t row0,
     if (at < 0) {
       // (elements lie about as far below the groups' largest as those lie apart, twice or three times)
       r.scale = s.scale(m, chunks ? m - 4.0f * (m - low) - 1.0f : low, s.k >= src.n);
-      if (flat) {
+      if (flat && s.p < 1.0f) {
         share(r, src, s.p, st, (int)gridDim.y, sh);
         return;
       }
-      const Cut cut = find_cut(r, src, s.k, s.p, 0, sh);
-      id = draw(r, src, cut, 0, 0, w, sum, sh);
+      if (flat) {
+        id = draw_shared(r, src, st, (int)gridDim.y, w, sum, sh);
+        if (id < 0) return;
+      } else {
+        const Cut cut = find_cut(r, src, s.k, s.p, 0, sh);
+        id = draw(r, src, cut, 0, 0, w, sum, sh);
+      }
     }
     prob = (float)((double)w / (double)sum);
   }
@@ -1088,7 +1159,10 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, int64_t row0,
 }
 
 constexpr int64_t kFewTokens = 8192;  // a work-group reads so many as quickly as another launch comes
-constexpr int kShareRows = 512;       // rows times the work-groups that share one
+// Rows times the work-groups that share one, and the tokens from which rows are shared: it takes
+// another launch (4 us), whether a row turns out to be kept for the most part or not.
+constexpr int kShareRows = 512;
+constexpr int64_t kShareTokens = 65536;
 constexpr size_t kStatBytes = (size_t)16 << 20, kSumBytes = (size_t)kShareRows * kBins * 8,
                  kListBytes = (size_t)kShareRows / 2 * kCand * 8, kRowBytes = kShareRows / 2 * sizeof(SampleRow);
 
@@ -1107,16 +1181,15 @@ hipError_t launch_sample(hipStream_t st, const SampleArgs &a, uint8_t *ws, uint3
   for (int64_t row = 0; row < a.rows; row += most) {
     const int64_t n = a.rows - row < most ? a.rows - row : most;
     // the chip's work-groups among few rows that top_p may leave much of
-    int parts = a.top_p && n <= kShareRows / 2 ? (int)(kShareRows / n) : 1;
+    int parts = (a.top_p || a.min_p) && a.n >= kShareTokens && n <= kShareRows / 2 ? (int)(kShareRows / n) : 1;
     parts = parts < kParts ? parts : kParts;
-    parts = parts < chunks ? parts : chunks;
     auto at = [&](int64_t bytes) { return (float *)(ws + bytes * most * chunks); };
     uint8_t *const sums = ws + kStatBytes, *const list = sums + kSumBytes;
     const SampleStats s{(unsigned long long *)ws,   at(8), at(12), at(16), (unsigned long long *)sums, (SampleRow *)(list + kListBytes),
                         (unsigned long long *)list, counters};
     KMOE_LAUNCH(k_sample_stats, dim3((unsigned)chunks, (unsigned)n), dim3(256), 0, st, a, row, s);
     KMOE_LAUNCH(k_sample, dim3((unsigned)n, (unsigned)parts), dim3(kThreads), 0, st, a, row, s, chunks);
-    if (parts > 1) KMOE_LAUNCH(k_sample_shared, dim3((unsigned)n, (unsigned)parts), dim3(kThreads), 0, st, a, row, s);
+    if (parts > 1 && a.top_p) KMOE_LAUNCH(k_sample_shared, dim3((unsigned)n, (unsigned)parts), dim3(kThreads), 0, st, a, row, s);
   }
   return hipGetLastError();
 }

@@ -277,3 +277,17 @@ def test_more_rows_than_the_workspace_holds(ctx):
     got = ctx.sample(x, u, top_k=k)
     for i in list(range(20550, 20570)) + [0, S - 1]:
         assert got[i].item() == _reference(x[i].cpu().numpy(), u[i].item(), k=30)[0]
+
+
+@pytest.mark.parametrize("S", [1, 3, 17, 40, 200, 256, 257])
+def test_rows_that_work_groups_share(ctx, S):
+    """Rows of which much is kept beside others, at every number of work-groups that share one."""
+    rng = np.random.default_rng(S)
+    n = 70001
+    x = (rng.standard_normal((S, n)) * rng.choice([0.3, 1, 2, 5], (S, 1))).astype(np.float32)
+    x[::3, 7] += 25.0  # (and rows that are not flat)
+    x[1::5] = np.round(x[1::5] * 4) / 4  # equal logits at every cut
+    x[2::7, ::2] = -np.inf
+    for how in (dict(p=rng.choice([0.3, 0.9, 0.999], S), temp=rng.choice([0.7, 1.0, 2.0], S)), dict(m=rng.choice([0.0, 1e-4, 0.01], S), temp=1.5),
+                dict(p=rng.choice([0.6, 0.95, 1.0], S), m=rng.choice([0.0, 1e-3, 0.05], S), k=rng.choice([0, 0, 20, 5000], S))):
+        _check(ctx, x, rng.random(S).astype(np.float32), **how)
