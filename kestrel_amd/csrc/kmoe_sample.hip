@@ -33,7 +33,7 @@ constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kFix = 43;    // weights in units of 2^-43
 constexpr int kBins = 1024, kBinsEach = kBins / kThreads;
 constexpr int kTab = 256;
-constexpr int kGroup = 64, kChunk = 4096;  // elements of which k_sample_stats finds the largest, and the sum
+constexpr int kGroup = 64, kChunk = 1024;  // elements of which k_sample_stats finds the largest, and the sum
 constexpr int kCand = 4096, kGroups = 1024;
 constexpr int kFew = 1024;  // elements of a bin that are compared one with another
 constexpr int kParts = 16;  // work-groups that share a row at most
@@ -94,9 +94,12 @@ __device__ __forceinline__ void make_table(double *tab) {
 // whose last bit is 1. The largest logit's weight is 2^43 exactly. Below 2^-44 (-31
 // nats: z = -11450) the weight rounds to no unit, whatever it is. A NaN is an infinite
 // largest logit's distance from itself.
+// MAY_BE_INF: the largest logit may be infinite.
+template <bool MAY_BE_INF = true>
 __device__ __forceinline__ double weight(const Row &r, float l, const double *tab) {
   double z = ((double)l - r.max) * r.inv_t;
-  z = fmax(fmin(z, 0.0), -11450.0);
+  if constexpr (MAY_BE_INF) z = fmin(z, 0.0);
+  z = fmax(z, -11450.0);
   const double s = z + 0x1.8p52;
   const int i = (int)(uint32_t)__double_as_longlong(s);
   const double f = z - (s - 0x1.8p52);
@@ -595,6 +598,9 @@ struct SampleRow {
 
 namespace {
 
+// Chunks of a row in the workspace: whole fours.
+__host__ __device__ __forceinline__ int chunk_stride(int chunks) { return (chunks + 3) & ~3; }
+
 // A row's settings, as they are used.
 struct Settings {
   float temp, p, min_p;
@@ -628,69 +634,87 @@ struct Settings {
 };
 
 // Per chunk of kChunk logits, the largest, the sum of the weights by that one (kFix
-// units) where it is asked for, and the largest of every kGroup.
-__global__ void __launch_bounds__(256) k_sample_stats(SampleArgs a, int64_t row0, SampleStats st) {
+// units) where it is asked for, and the largest of every kGroup. A wave takes `each`
+// chunks one after the other, the next one's loads on their way meanwhile, and waits for
+// no other wave. Bound by the vector units where sums are asked for (20 instructions a weight,
+// 14 of them in 64 bits), otherwise by the loads.
+__global__ void __launch_bounds__(256) k_sample_stats(SampleArgs a, int64_t row0, SampleStats st, int chunks, int each) {
+  constexpr int U = kChunk / 256;
   __shared__ double tab[kTab];
-  __shared__ float red[8];
-  __shared__ u64 redu[4];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = blockIdx.x;
+  const int t = threadIdx.x, lane = t & 63, c0 = (blockIdx.x * 4 + (t >> 6)) * each;
+  const int c1 = c0 + each < chunks ? c0 + each : chunks;
   const int64_t row = row0 + blockIdx.y;
   const float *l = a.logits + row * a.stride;
-  const int n = (int)a.n, base = c * kChunk;
-  const Settings s(a, row);
-  const bool sums = s.sums(a);
-  if (sums) make_table(tab);
-  float x[4][4];
+  const int n = (int)a.n;
+  float next[U][4];
+  auto load = [&](int c) {
+    const int base = c * kChunk + 4 * lane;
+    if (c * kChunk + kChunk <= n) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int i = base + j * 1024 + 4 * t;
-    if (i + 4 <= n) {
-      const f32x4a4 y = *(const f32x4a4 *)(l + i);
+      for (int j = 0; j < U; ++j) {
+        const f32x4a4 y = *(const f32x4a4 *)(l + base + j * 256);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[j][e] = clean(y[e]);
+        for (int e = 0; e < 4; ++e) next[j][e] = y[e];
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[j][e] = i + e < n ? clean(l[i + e]) : -INFINITY;
+      for (int j = 0; j < U; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) next[j][e] = base + j * 256 + e < n ? l[base + j * 256 + e] : -INFINITY;
     }
-  }
-  float *gm = st.group_max + ((int64_t)blockIdx.y * gridDim.x + c) * (kChunk / kGroup);
-  float m = -INFINITY, low = INFINITY;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float g = max2(max2(x[j][0], x[j][1]), max2(x[j][2], x[j][3]));
-    g = max2(g, dpp_f<kDppXor1>(g));
-    g = max2(g, dpp_f<kDppXor2>(g));
-    g = max2(g, dpp_f<kDppHalfMirror>(g));
-    g = max2(g, dpp_f<kDppMirror>(g));
-    if ((lane & 15) == 0) gm[j * 16 + (t >> 4)] = g;
-    m = max2(m, g);
-    low = fminf(low, g == -INFINITY ? INFINITY : g);
-  }
-  m = group_max<64>(m);
-  low = -group_max<64>(-low);
-  if (lane == 0) {
-    red[wave] = m;
-    red[4 + wave] = low;
-  }
-  lds_barrier();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  low = fminf(fminf(red[4], red[5]), fminf(red[6], red[7]));
-  u64 sum = 0;
+  };
+  if (c0 < c1) load(c0);
+  const Settings s(a, row);
+  const bool sums = s.sums(a);
   if (sums) {
-    const Row r = s.row(m, 0.0f);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum += fixed(weight(r, x[j][e], tab));  // (-inf, past the row's end, weighs nothing)
-    sum = wave_scan(sum);
-    if (lane == 63) redu[wave] = sum;
+    make_table(tab);
     lds_barrier();
-    sum = redu[0] + redu[1] + redu[2] + redu[3];
   }
-  if (t == 0) {
-    st.chunk_max[(int64_t)blockIdx.y * gridDim.x + c] = m;
-    st.chunk_low[(int64_t)blockIdx.y * gridDim.x + c] = low;
-    st.chunk_sum[(int64_t)blockIdx.y * gridDim.x + c] = sum;
+  for (int c = c0; c < c1; ++c) {
+    float x[U][4];
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[j][e] = clean(next[j][e]);
+    if (c + 1 < c1) load(c + 1);
+    const int64_t at = (int64_t)blockIdx.y * chunk_stride(chunks) + c;
+    float *gm = st.group_max + at * (kChunk / kGroup);
+    float m = -INFINITY, low = INFINITY;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      float g = max2(max2(x[j][0], x[j][1]), max2(x[j][2], x[j][3]));
+      g = max2(g, dpp_f<kDppXor1>(g));
+      g = max2(g, dpp_f<kDppXor2>(g));
+      g = max2(g, dpp_f<kDppHalfMirror>(g));
+      g = max2(g, dpp_f<kDppMirror>(g));
+      if ((lane & 15) == 0) gm[j * 4 + (lane >> 4)] = g;
+      m = max2(m, g);
+      low = fminf(low, g == -INFINITY ? INFINITY : g);
+    }
+    m = max2(m, __shfl_xor(m, 16));
+    m = max2(m, __shfl_xor(m, 32));
+    low = fminf(low, __shfl_xor(low, 16));
+    low = fminf(low, __shfl_xor(low, 32));
+    u64 sum = 0;
+    if (sums) {
+      const Row r = s.row(m, 0.0f);
+      auto add = [&](auto inf_) {
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)  // (-inf, past the row's end, weighs nothing)
+            sum += (u64)__double_as_longlong(weight<decltype(inf_)::value>(r, x[j][e], tab) + 0x1p52);
+        sum -= (u64)(4 * U) * 0x4330000000000000ull;  // (the sum's exponents, see fixed())
+      };
+      if (m == INFINITY) add(std::true_type());
+      else add(std::false_type());
+      sum = wave_scan(sum);
+    }
+    if (lane == 63) {
+      st.chunk_max[at] = m;
+      st.chunk_low[at] = low;
+      st.chunk_sum[at] = sum;
+    }
   }
 }
 
@@ -1016,18 +1040,28 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, int64_t row0,
   const Logits src{a.logits + row * a.stride, (int)a.n};
   // the largest logit, and the lowest of the groups' largest (without groups: of all)
   float m = -INFINITY, low = INFINITY;
-  const int64_t c0 = (int64_t)blockIdx.x * chunks;
-  const float *cm = st.chunk_max + c0, *gm = st.group_max + c0 * (kChunk / kGroup);
+  const int64_t c0 = (int64_t)blockIdx.x * chunk_stride(chunks);
+  const float *gm = st.group_max + c0 * (kChunk / kGroup);
   const int n_group = (src.n + kGroup - 1) / kGroup;
   f32x4a4 g4{0};
-  u64 chunk_sum = 0;  // (at most kThreads chunks: one a thread)
-  float chunk_max = -INFINITY;
+  constexpr int CE = 4;  // chunks a thread, at most KMOE_SAMPLE_MAX / kChunk in all
+  u64 chunk_sum[CE] = {};
+  float chunk_max[CE];
+#pragma unroll
+  for (int e = 0; e < CE; ++e) chunk_max[e] = -INFINITY;
   if (chunks) {
     g4 = groups_at(gm, n_group, 4 * t);
-    if (t < chunks) {
-      chunk_max = m = cm[t];
-      low = st.chunk_low[c0 + t];
-      chunk_sum = st.chunk_sum[c0 + t];
+    if (CE * t < chunks) {
+#pragma unroll
+      for (int e = 0; e < CE; ++e) {  // (whole fours are there, those past the row's are not looked at)
+        const bool in = CE * t + e < chunks;
+        const float x = st.chunk_max[c0 + CE * t + e], y = st.chunk_low[c0 + CE * t + e];
+        const u64 z = st.chunk_sum[c0 + CE * t + e];
+        chunk_max[e] = in ? x : -INFINITY;
+        chunk_sum[e] = in ? z : 0;
+        m = fmaxf(m, chunk_max[e]);
+        low = fminf(low, in ? y : INFINITY);
+      }
     }
   } else {
     each(src, [&](int, float l) {
@@ -1057,7 +1091,9 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, int64_t row0,
     if (chunks) {
       if (t == 0) sh.at = chunks;
       lds_barrier();
-      if (t < chunks && chunk_max == m) atomicMin(&sh.at, t);
+#pragma unroll
+      for (int e = 0; e < CE; ++e)
+        if (chunk_max[e] == m) atomicMin(&sh.at, CE * t + e);
       lds_barrier();
       start = sh.at * kChunk;
       end = start + kChunk < end ? start + kChunk : end;
@@ -1068,8 +1104,11 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, int64_t row0,
     // the chunks' sums by the row's largest
     u64 sum = 0, w = 0, mine = 0, before = 0;
     if (chunks && s.sums(a)) {
-      if (t < chunks)
-        mine = (u64)__builtin_rint((double)chunk_sum * 0x1p-43 * weight(r, chunk_max, sh.tab));
+#pragma unroll
+      for (int e = 0; e < CE; ++e) {
+        chunk_sum[e] = (u64)__builtin_rint((double)chunk_sum[e] * 0x1p-43 * weight(r, chunk_max[e], sh.tab));
+        mine += chunk_sum[e];
+      }
       before = block_scan(mine, sum, sh);
     }
     int at = -1;
@@ -1077,13 +1116,24 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, int64_t row0,
       u64 goal = (u64)((double)r.u * (double)sum);
       goal = goal < sum ? goal : sum - 1;
       if (before <= goal && goal < before + mine) {
-        sh.at = t;
+        int e = 0;
+#pragma unroll
+        for (int k = 0; k < CE - 1; ++k)
+          if (e == k && before + chunk_sum[k] <= goal) {
+            before += chunk_sum[k];
+            ++e;
+          }
+        float x = chunk_max[0];
+#pragma unroll
+        for (int k = 1; k < CE; ++k) x = e == k ? chunk_max[k] : x;
+        sh.at = CE * t + e;
         sh.before = before;
+        sh.redf[0][0] = x;
       }
       lds_barrier();
       const int start = sh.at * kChunk, end = start + kChunk < src.n ? start + kChunk : src.n;
       goal -= sh.before;
-      const float top = cm[sh.at];
+      const float top = sh.redf[0][0];
       lds_barrier();
       at = draw(r, Logits{src.l + start, end - start}, Cut{-INFINITY, ~0ull}, goal, sum, w, sum, sh);
       id = at >= 0 ? start + at : first_equal(src, start, end, top, sh);  // (a chunk of many weights of under half a unit)
@@ -1176,18 +1226,21 @@ hipError_t launch_sample(hipStream_t st, const SampleArgs &a, uint8_t *ws, uint3
     KMOE_LAUNCH(k_sample, dim3((unsigned)a.rows), dim3(kThreads), 0, st, a, (int64_t)0, SampleStats{}, 0);
     return hipGetLastError();
   }
-  const int chunks = (int)((a.n + kChunk - 1) / kChunk);
-  const int64_t each = (int64_t)chunks * (16 + 4 * (kChunk / kGroup)), most = (int64_t)kStatBytes / each;
+  const int chunks = (int)((a.n + kChunk - 1) / kChunk), stride = chunk_stride(chunks);
+  const int64_t bytes = (int64_t)stride * (16 + 4 * (kChunk / kGroup)), most = (int64_t)kStatBytes / bytes;
   for (int64_t row = 0; row < a.rows; row += most) {
     const int64_t n = a.rows - row < most ? a.rows - row : most;
     // the chip's work-groups among few rows that top_p may leave much of
     int parts = (a.top_p || a.min_p) && a.n >= kShareTokens && n <= kShareRows / 2 ? (int)(kShareRows / n) : 1;
     parts = parts < kParts ? parts : kParts;
-    auto at = [&](int64_t bytes) { return (float *)(ws + bytes * most * chunks); };
+    auto at = [&](int64_t x) { return (float *)(ws + x * most * stride); };
     uint8_t *const sums = ws + kStatBytes, *const list = sums + kSumBytes;
     const SampleStats s{(unsigned long long *)ws,   at(8), at(12), at(16), (unsigned long long *)sums, (SampleRow *)(list + kListBytes),
                         (unsigned long long *)list, counters};
-    KMOE_LAUNCH(k_sample_stats, dim3((unsigned)chunks, (unsigned)n), dim3(256), 0, st, a, row, s);
+    // chunks a wave: one where the waves do not fill the chip four times, at most eight
+    const int64_t fill = n * chunks / 4096;
+    const int each = fill < 1 ? 1 : fill < 8 ? (int)fill : 8;
+    KMOE_LAUNCH(k_sample_stats, dim3((unsigned)(chunks + 4 * each - 1) / (4 * each), (unsigned)n), dim3(256), 0, st, a, row, s, chunks, each);
     KMOE_LAUNCH(k_sample, dim3((unsigned)n, (unsigned)parts), dim3(kThreads), 0, st, a, row, s, chunks);
     if (parts > 1 && a.top_p) KMOE_LAUNCH(k_sample_shared, dim3((unsigned)n, (unsigned)parts), dim3(kThreads), 0, st, a, row, s);
   }

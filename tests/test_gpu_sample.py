@@ -267,7 +267,7 @@ def test_more_tokens_kept_than_fit_the_candidates(ctx, how):
 
 
 def test_more_rows_than_the_workspace_holds(ctx):
-    """The rows go by parts then: 16 MB hold 20560 rows of 3 chunks."""
+    """The rows go by parts then: 16 MB hold 17476 rows of 9 chunks."""
     import torch
 
     S, n = 20900, 8200
@@ -275,7 +275,7 @@ def test_more_rows_than_the_workspace_holds(ctx):
     u = torch.rand(S, device="cuda", generator=torch.Generator("cuda").manual_seed(2))
     k = torch.full((S,), 30, dtype=torch.int32, device="cuda")
     got = ctx.sample(x, u, top_k=k)
-    for i in list(range(20550, 20570)) + [0, S - 1]:
+    for i in list(range(17470, 17485)) + [0, S - 1]:
         assert got[i].item() == _reference(x[i].cpu().numpy(), u[i].item(), k=30)[0]
 
 
