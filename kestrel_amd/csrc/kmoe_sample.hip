@@ -28,13 +28,13 @@ namespace {
 
 typedef unsigned long long u64;
 // Threads of a work-group: with 1024, every step between two barriers is issued four
-// times per SIMD, and most steps of a row are short (1 row of 32000: 16 us, 256 threads TODO).
+// times per SIMD, and most steps of a row are short (256 rows without a cut: 12 us, with 256 7).
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kFix = 43;    // weights in units of 2^-43
 constexpr int kBins = 1024, kBinsEach = kBins / kThreads;
 constexpr int kTab = 256;
 constexpr int kGroup = 64, kChunk = 1024;  // elements of which k_sample_stats finds the largest, and the sum
-constexpr int kCand = 4096, kGroups = 1024;
+constexpr int kCand = 4096, kGroups = 1024, kFewGroups = 256;
 constexpr int kFew = 1024;  // elements of a bin that are compared one with another
 constexpr int kParts = 16;  // work-groups that share a row at most
 constexpr int kSegment = 1024;  // elements of which a draw knows the sum
@@ -136,7 +136,7 @@ struct Shared {
   // candidates, and the groups that they are in with how many candidates each has
   float cand[kCand];
   int index[kCand];
-  uint16_t group[kGroups], in_group[kGroups];
+  uint16_t group[kGroups], in_group[128];
 };
 
 // Inclusive scan over a wave: within rows of 16 lanes, then row 0's and 2's totals onto
@@ -744,12 +744,73 @@ __device__ __forceinline__ f32x4a4 groups_at(const float *gm, int n_group, int g
   return x;
 }
 
+// Candidates of sh.group's n groups, in their order, behind the first `have`; a row of 16
+// lanes per group, U of them at a time. Returns how many there are now (they end at kCand).
+template <int U>
+__device__ __forceinline__ int gather_groups(const Row &r, const Logits &src, int n, int b0, Shared &sh) {
+  constexpr int ROWS = kThreads / 16;
+  static_assert(U * ROWS <= 128, "two counts a lane");
+  const int t = threadIdx.x, l16 = t & 15, lane = t & 63;
+  int have = 0;
+  for (int i0 = 0; i0 < n && have <= kCand; i0 += U * ROWS) {
+    float x[U][4];
+    uint32_t in[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * ROWS + (t >> 4), at = i < n ? sh.group[i] * kGroup + 4 * l16 : src.n;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[u][e] = src.l[at + e < src.n ? at + e : src.n - 1];
+      in[u] = at + 4 <= src.n ? 15 : at < src.n ? (1u << (src.n - at)) - 1 : 0;
+    }
+    lds_barrier();  // (the last round's counts are read)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[u][e] = clean(x[u][e]);
+        if (x[u][e] == -INFINITY || bin_of(r, x[u][e]) > b0) in[u] &= ~(1u << e);
+      }
+      const int m = group_sum_i<16>(__builtin_popcount(in[u]));
+      if (l16 == 0) sh.in_group[u * ROWS + (t >> 4)] = (uint16_t)m;
+    }
+    lds_barrier();
+    // candidates before each of the round's groups, two a lane: every wave for itself
+    const u64 c0 = 2 * lane < U * ROWS ? sh.in_group[2 * lane] : 0, c1 = 2 * lane < U * ROWS ? sh.in_group[2 * lane + 1] : 0;
+    const int sum = (int)wave_scan(c0 + c1);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = u * ROWS + (t >> 4), own = __builtin_popcount(in[u]);
+      // up to the group's pair, without the pair's second where the group is the first
+      int to = have + __shfl(sum, k >> 1) - (k & 1 ? sh.in_group[k] : sh.in_group[k] + sh.in_group[k + 1]);
+      int before = own;  // inclusive, over the row of lanes
+      before += __builtin_amdgcn_update_dpp(0, before, 0x111, 0xf, 0xf, false);
+      before += __builtin_amdgcn_update_dpp(0, before, 0x112, 0xf, 0xf, false);
+      before += __builtin_amdgcn_update_dpp(0, before, 0x114, 0xf, 0xf, false);
+      before += __builtin_amdgcn_update_dpp(0, before, 0x118, 0xf, 0xf, false);
+      to += before - own;
+      const int first = i0 + k < n ? sh.group[i0 + k] * kGroup + 4 * l16 : 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (in[u] & (1u << e)) {
+          if (to < kCand) {
+            sh.cand[to] = x[u][e];
+            sh.index[to] = first + e;
+          }
+          ++to;
+        }
+    }
+    have += __shfl(sum, 63);
+  }
+  lds_barrier();
+  return have;
+}
+
 // The elements whose even bin is at most b0, in sh.cand and sh.index, in their order;
-// -1 where they are too many. A group's largest says whether it has any; g4: those of
-// the thread's first groups.
-__device__ __forceinline__ int gather(const Row &r, const Logits &src, const float *gm, f32x4a4 g4, int n_group, int b0,
+// -1 where they are too many, or lie in more than `most` groups. A group's largest
+// says whether it has any; g4: those of the thread's first groups.
+__device__ __forceinline__ int gather(const Row &r, const Logits &src, const float *gm, f32x4a4 g4, int n_group, int b0, int most,
                                       Shared &sh) {
-  const int t = threadIdx.x, l16 = t & 15;
+  const int t = threadIdx.x;
   int n = 0;
   for (int g0 = 0; g0 < n_group; g0 += 4 * kThreads) {
     const int g = g0 + 4 * t;
@@ -768,74 +829,10 @@ __device__ __forceinline__ int gather(const Row &r, const Logits &src, const flo
       }
     n += (int)total;
   }
-  if (n > kGroups) return -1;
+  if (n > most) return -1;
   lds_barrier();
-  // a row of 16 lanes per group, four groups at a time; of up to 64 groups the elements stay
-  // in registers
-  constexpr int U = 4, ROWS = kThreads / 16;
-  float x[U][4];
-  uint32_t in[U];
-  auto load = [&](int i0) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * ROWS, at = i < n ? sh.group[i] * kGroup + 4 * l16 : src.n;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[u][e] = src.l[at + e < src.n ? at + e : src.n - 1];
-      in[u] = at + 4 <= src.n ? 15 : at < src.n ? (1u << (src.n - at)) - 1 : 0;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[u][e] = clean(x[u][e]);
-        if (x[u][e] == -INFINITY || bin_of(r, x[u][e]) > b0) in[u] &= ~(1u << e);
-      }
-  };
-  for (int i0 = t >> 4; i0 < n; i0 += U * ROWS) {
-    load(i0);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int m = group_sum_i<16>(__builtin_popcount(in[u]));
-      if (l16 == 0 && i0 + u * ROWS < n) sh.in_group[i0 + u * ROWS] = (uint16_t)m;
-    }
-  }
-  lds_barrier();
-  u64 total;
-  constexpr int EACH = kGroups / kThreads;
-  int c[EACH], mine = 0;
-#pragma unroll
-  for (int e = 0; e < EACH; ++e) mine += c[e] = EACH * t + e < n ? sh.in_group[EACH * t + e] : 0;
-  int at = (int)block_scan(mine, total, sh);
-  if (total > kCand) return -1;
-#pragma unroll
-  for (int e = 0; e < EACH; ++e) {
-    if (EACH * t + e < n) sh.in_group[EACH * t + e] = (uint16_t)at;
-    at += c[e];
-  }
-  lds_barrier();
-  for (int i0 = t >> 4; i0 < n; i0 += U * ROWS) {
-    if (n > U * ROWS) load(i0);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * ROWS;
-      const int own = __builtin_popcount(in[u]);
-      int before = own;  // inclusive, over the row of lanes
-      before += __builtin_amdgcn_update_dpp(0, before, 0x111, 0xf, 0xf, false);
-      before += __builtin_amdgcn_update_dpp(0, before, 0x112, 0xf, 0xf, false);
-      before += __builtin_amdgcn_update_dpp(0, before, 0x114, 0xf, 0xf, false);
-      before += __builtin_amdgcn_update_dpp(0, before, 0x118, 0xf, 0xf, false);
-      if (i >= n || !own) continue;
-      int to = sh.in_group[i] + before - own;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (in[u] & (1u << e)) {
-          sh.cand[to] = x[u][e];
-          sh.index[to++] = sh.group[i] * kGroup + 4 * l16 + e;
-        }
-    }
-  }
-  lds_barrier();
-  return (int)total;
+  n = n <= 64 ? gather_groups<4>(r, src, n, b0, sh) : gather_groups<8>(r, src, n, b0, sh);
+  return n <= kCand ? n : -1;
 }
 
 // A row of which more is kept than fits the candidates, without top_k, is shared by work-groups,
@@ -863,51 +860,6 @@ __device__ __forceinline__ bool last_of(uint32_t *counter, int parts, Shared &sh
   return sh.n == parts - 1;
 }
 
-__device__ __forceinline__ void share(const Row &r, const Logits &src, float p, const SampleStats &st, int parts, Shared &sh) {
-  const int t = threadIdx.x, mine = blockIdx.y;
-  lds_barrier();
-  clear(sh.mass);
-  lds_barrier();
-  each(part_at(src, part_len(src.n, parts), mine), [&](int, float l) {
-    const u64 x = fixed(weight(r, l, sh.tab));
-    if (x) atomicAdd(&sh.mass[bin_of(r, l)], x);
-  });
-  lds_barrier();
-  u64 *all = st.part_sum + (int64_t)blockIdx.x * parts * kBins;
-#pragma unroll
-  for (int e = 0; e < kBinsEach; ++e)
-    __hip_atomic_store(all + mine * kBins + e * kThreads + t, sh.mass[e * kThreads + t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  if (!last_of(st.counters + 2 * blockIdx.x, parts, sh)) return;
-  u64 s[kBinsEach] = {};
-  for (int k0 = 0; k0 < parts; k0 += 8) {
-    u64 x[8][kBinsEach];
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-#pragma unroll
-      for (int e = 0; e < kBinsEach; ++e)
-        x[k][e] = k0 + k < parts ? __hip_atomic_load(all + (k0 + k) * kBins + e * kThreads + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-#pragma unroll
-      for (int e = 0; e < kBinsEach; ++e) s[e] += x[k][e];
-  }
-#pragma unroll
-  for (int e = 0; e < kBinsEach; ++e) sh.mass[e * kThreads + t] = s[e];
-  lds_barrier();
-  const u64 total = sum_below(sh.mass, kBins, sh);
-  u64 target = part_of(p, total), before;
-  target = target < total ? target : total;
-  const int b = crossing(sh.mass, target, before, sh);
-  if (t == 0) {
-    SampleRow *row = st.rows + blockIdx.x;
-    row->top = r.top;
-    row->scale = r.scale;
-    row->shared = parts;
-    row->bin = b;
-    row->target = target - before;
-  }
-}
-
 // The part that the drawn token is in by the parts' sums (sh.part), what is left of the
 // goal there, and the sum.
 __device__ __forceinline__ int part_drawn(const Row &r, int parts, u64 &goal, u64 &sum, const Shared &sh) {
@@ -920,22 +872,80 @@ __device__ __forceinline__ int part_drawn(const Row &r, int parts, u64 &goal, u6
   return k;
 }
 
-// The same with min_p alone, which needs no cut: the last work-group to arrive draws. -1 in the others.
-__device__ __forceinline__ int draw_shared(const Row &r, const Logits &src, const SampleStats &st, int parts, u64 &w, u64 &sum,
-                                           Shared &sh) {
-  const int t = threadIdx.x, len = part_len(src.n, parts);
-  const u64 own = sum_of(part_at(src, len, blockIdx.y), sh, [&](int, float l) {
-    const double x = weight(r, l, sh.tab);
-    return x >= r.min_w ? fixed(x) : 0;
-  });
-  u64 *all = st.part_sum + (int64_t)blockIdx.x * parts * kBins;
-  if (t == 0) __hip_atomic_store(all + blockIdx.y, own, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  if (!last_of(st.counters + 2 * blockIdx.x, parts, sh)) return -1;
-  if (t < parts) sh.part[t] = __hip_atomic_load(all + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// k_sample's share of that. With min_p what weighs that much is summed, too: where it is less
+// than top_p asks for (or top_p asks for nothing) it is what is kept, and the last work-group to arrive
+// draws. Returns the token then, otherwise -1.
+__device__ __forceinline__ int share(const Row &r, const Logits &src, float p, const SampleStats &st, int parts, u64 &w, u64 &sum,
+                                     Shared &sh) {
+  const int t = threadIdx.x, mine = blockIdx.y, len = part_len(src.n, parts);
+  const bool bins = p < 1.0f, least = r.min_w > 0.0;
   lds_barrier();
-  u64 goal;
-  const int k = part_drawn(r, parts, goal, sum, sh);
-  return k * len + draw(r, part_at(src, len, k), Cut{-INFINITY, ~0ull}, goal, sum, w, sum, sh);
+  clear(sh.mass);
+  lds_barrier();
+  u64 heavy = 0;
+  each(part_at(src, len, mine), [&](int, float l) {
+    const double y = weight(r, l, sh.tab);
+    const u64 x = fixed(y);
+    if (least) heavy += y >= r.min_w ? x : 0;
+    if (bins && x) atomicAdd(&sh.mass[bin_of(r, l)], x);
+  });
+  SampleRow *row = st.rows + blockIdx.x;
+  if (least) {
+    u64 total;
+    block_scan(heavy, total, sh);
+    if (t == 0) __hip_atomic_store(row->part + mine, total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  lds_barrier();
+  u64 *all = st.part_sum + (int64_t)blockIdx.x * parts * kBins;
+  if (bins)
+#pragma unroll
+    for (int e = 0; e < kBinsEach; ++e)
+      __hip_atomic_store(all + mine * kBins + e * kThreads + t, sh.mass[e * kThreads + t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (!last_of(st.counters + 2 * blockIdx.x, parts, sh)) return -1;
+  u64 all_heavy = ~0ull;
+  if (least) {
+    if (t < parts) sh.part[t] = __hip_atomic_load(row->part + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    lds_barrier();
+    all_heavy = 0;
+    for (int k = 0; k < parts; ++k) all_heavy += sh.part[k];
+  }
+  u64 target = ~0ull, before = 0;
+  int b = 0;
+  if (bins) {
+    u64 s[kBinsEach] = {};
+    for (int k0 = 0; k0 < parts; k0 += 8) {
+      u64 x[8][kBinsEach];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int e = 0; e < kBinsEach; ++e)
+          x[k][e] = k0 + k < parts ? __hip_atomic_load(all + (k0 + k) * kBins + e * kThreads + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int e = 0; e < kBinsEach; ++e) s[e] += x[k][e];
+    }
+#pragma unroll
+    for (int e = 0; e < kBinsEach; ++e) sh.mass[e * kThreads + t] = s[e];
+    lds_barrier();
+    const u64 total = sum_below(sh.mass, kBins, sh);
+    target = part_of(p, total);
+    target = target < total ? target : total;
+    b = crossing(sh.mass, target, before, sh);
+  }
+  if (all_heavy < target) {
+    u64 goal;
+    const int k = part_drawn(r, parts, goal, sum, sh);
+    return k * len + draw(r, part_at(src, len, k), Cut{-INFINITY, ~0ull}, goal, sum, w, sum, sh);
+  }
+  if (t == 0) {
+    row->top = r.top;
+    row->scale = r.scale;
+    row->shared = parts;
+    row->bin = b;
+    row->target = target - before;
+  }
+  return -1;
 }
 
 __device__ __forceinline__ void answer(const SampleArgs &a, int64_t row, int id, float prob) {
@@ -1000,10 +1010,9 @@ __global__ void __launch_bounds__(kThreads) k_sample_shared(SampleArgs a, int64_
   bool held = true;
   Cut cut = n > kCand ? cut_by_digits<true>(r, src, b, 0xffffffffu, have->target, none, sh)
                       : cut_in_bin<true>(r, Candidates{sh.cand, n}, b, n, 0xffffffffu, have->target, none, held, sh);
-  const double wt = weight(r, cut.v, sh.tab);
-  const u64 w_tie = fixed(wt);
+  const u64 w_tie = fixed(weight(r, cut.v, sh.tab));
   cut.ties = (cut.ties + w_tie - 1) / w_tie;
-  // the parts' sums, where all of the kept weigh min_p and none of the equal ones is left out
+  // the parts' sums, where none of the equal ones is left out (all of the kept weigh min_p)
   u64 equal = 0;
   if (n <= kCand) {
     lds_barrier();
@@ -1018,7 +1027,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_shared(SampleArgs a, int64_
     block_scan(c, equal, sh);
   }
   int id;
-  if (n > kCand || wt < r.min_w || equal > cut.ties) {
+  if (n > kCand || equal > cut.ties) {
     id = draw(r, src, cut, 0, 0, w, sum, sh);
   } else {
     u64 goal;
@@ -1173,7 +1182,9 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, int64_t row0,
         b0 = x < (float)b0 ? (int)x : b0;
       }
       if (b0 < kBins - 1) {
-        const int n = gather(r, src, gm, g4, n_group, b0, sh);
+        // (a row that may be shared is, rather than going through more groups than this: 256
+        // took 6 us, 1000 20)
+        const int n = gather(r, src, gm, g4, n_group, b0, flat ? kFewGroups : kGroups, sh);
         if (n >= 0) {
           if (blockIdx.y) return;
           const Candidates cand{sh.cand, n};
@@ -1188,12 +1199,8 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, int64_t row0,
     if (at < 0) {
       // (elements lie about as far below the groups' largest as those lie apart, twice or three times)
       r.scale = s.scale(m, chunks ? m - 4.0f * (m - low) - 1.0f : low, s.k >= src.n);
-      if (flat && s.p < 1.0f) {
-        share(r, src, s.p, st, (int)gridDim.y, sh);
-        return;
-      }
       if (flat) {
-        id = draw_shared(r, src, st, (int)gridDim.y, w, sum, sh);
+        id = share(r, src, s.p, st, (int)gridDim.y, w, sum, sh);
         if (id < 0) return;
       } else {
         const Cut cut = find_cut(r, src, s.k, s.p, 0, sh);
