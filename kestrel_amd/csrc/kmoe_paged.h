@@ -127,7 +127,7 @@ struct SelectArgs {
   const uint16_t *bounds;
   const float *q;
   int n_head, group, n_select, n_first;
-  unsigned long long *scores;
+  uint64_t *scores;
   int32_t *table, *len, *row_start;
   uint32_t *counters;
 };

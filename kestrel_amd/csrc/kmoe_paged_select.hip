@@ -19,12 +19,14 @@
 #include "kmoe_launch.h"
 #include "kmoe_device.h"
 #include "kmoe_paged.h"
+#include "kmoe_scan.h"
 
 namespace kmoe {
 namespace {
 
-typedef unsigned long long u64;
+typedef uint64_t u64;
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 // ------------------------------------------------------------------- bounds
 
@@ -130,8 +132,9 @@ __global__ void __launch_bounds__(256) k_paged_bounds(PagedArgs a, int n_unit, u
 
 // ---------------------------------------------------------------- selection
 
-constexpr int kPart = 512;    // pages that a work-group scores
+constexpr int kPart = 512;    // pages that a work-group scores at most
 constexpr int kBins = 1024;
+constexpr int kHeld = 4096;   // columns whose ranks are chosen among in LDS
 
 // Order of the scores as whole numbers, the best ones smallest; NaN before all.
 __device__ __forceinline__ u64 rank_of(double x) {
@@ -140,22 +143,12 @@ __device__ __forceinline__ u64 rank_of(double x) {
 }
 constexpr u64 kNoPage = ~0ull;  // (the rank of no score: -inf's is 0xffefff..)
 
-__device__ __forceinline__ double sum_lanes(double x, int width) {
-  for (int d = 1; d < width; d <<= 1) x += __shfl_xor(x, d);
-  return x;
-}
-
 __device__ __forceinline__ int block_scan(int x, int &total, int *red) {  // exclusive, 256 threads
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int in = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(in, d);
-    if (lane >= d) in += y;
-  }
-  __syncthreads();
+  const int in = wave_scan_i(x);
+  lds_barrier();
   if (lane == 63) red[wave] = in;
-  __syncthreads();
+  lds_barrier();
   int before = in - x;
   total = 0;
 #pragma unroll
@@ -166,27 +159,193 @@ __device__ __forceinline__ int block_scan(int x, int &total, int *red) {  // exc
   return before;
 }
 
-struct Ranks {
+// Ranks of a row's columns, in LDS or as other work-groups handed them over.
+struct Held {
+  const u64 *p;  // (LDS)
+  int n;
+  __device__ __forceinline__ u64 at(int i) const { return p[i]; }
+};
+struct Handed {
   const u64 *p;
-  bool local;  // in LDS, or handed over by other work-groups
-  __device__ __forceinline__ u64 at(int i) const {
-    return local ? p[i] : __hip_atomic_load(p + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  int n;
+  __device__ __forceinline__ u64 at(int i) const { return __hip_atomic_load(p + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+};
+// f(c, rank) for all of them, a work-group together, eight a thread on their way at a time.
+template <class R, class F>
+__device__ __forceinline__ void each(const R &r, F &&f) {
+  constexpr int U = 8;
+  for (int c = threadIdx.x; c < r.n; c += 256 * U) {
+    u64 k[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) k[u] = r.at(c + 256 * u < r.n ? c + 256 * u : c);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c + 256 * u < r.n) f(c + 256 * u, k[u]);
   }
+}
+
+struct Choice {
+  u64 ext[2][4], few[64];
+  int count[kBins], red[4], found[2], n_few;
 };
 
-// A work-group: kPart pages of one row and kv head; the last one of a row to arrive
-// chooses. Grid: (parts, rows by kv heads).
+// The best `want` of the columns, into `to` in their order; how many there are. Among those
+// whose rank lies in [lo, hi], the bin of the want-th is found by steps of a power of
+// two, and taken as the next range: ten bits a time, of 64 at most, until it holds few.
+template <class R>
+__device__ __forceinline__ int choose(const R &r, int want, const int32_t *tab, int n_kv, int g, int32_t *to, Choice &sh) {
+  const int t = threadIdx.x, lane = t & 63;
+  int have = 0, total;
+  u64 lo = 0, hi = kNoPage - 1;
+  u64 cut = kNoPage - 1;  // ranks up to it are taken, of those equal to it `ties`
+  int ties = INT32_MAX;
+  for (bool begun = false;; begun = true) {
+    u64 mn = kNoPage, mx = 0;
+    each(r, [&](int, u64 k) {
+      have += k != kNoPage;
+      const bool in = k >= lo && k <= hi;
+      mn = in && k < mn ? k : mn;
+      mx = in && k > mx ? k : mx;
+    });
+    wave_range(mn, mx);
+    if (!begun) {
+      block_scan(have, total, sh.red);
+      if (total <= want) break;  // all of them
+      if (want <= 0) return 0;
+    }
+    lds_barrier();
+    if (lane == 63) {
+      sh.ext[0][t >> 6] = mn;
+      sh.ext[1][t >> 6] = mx;
+    }
+#pragma unroll
+    for (int e = 0; e < kBins / 256; ++e) sh.count[256 * e + t] = 0;
+    if (t == 0) sh.n_few = 0;
+    lds_barrier();
+    mn = sh.ext[0][0];
+    mx = sh.ext[1][0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      mn = sh.ext[0][w] < mn ? sh.ext[0][w] : mn;
+      mx = sh.ext[1][w] > mx ? sh.ext[1][w] : mx;
+    }
+    if (mn == mx) {  // equal ones: the first by column
+      cut = mn;
+      ties = want;
+      break;
+    }
+    const int bits = 64 - __clzll((long long)(mx - mn)), shift = bits > 10 ? bits - 10 : 0;
+    each(r, [&](int, u64 k) {
+      if (k >= mn && k <= mx) atomicAdd(&sh.count[(k - mn) >> shift], 1);
+    });
+    lds_barrier();
+    int x[4], sum = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum += x[e] = sh.count[4 * t + e];
+    int before = block_scan(sum, total, sh.red);
+    if (before < want && before + sum >= want) {
+      int e = 0;
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        if (e == k && before + x[k] < want) {
+          before += x[k];
+          ++e;
+        }
+      sh.found[0] = 4 * t + e;
+      sh.found[1] = before;
+    }
+    lds_barrier();
+    lo = mn + ((u64)sh.found[0] << shift);
+    hi = mx - lo > (1ull << shift) - 1 ? lo + ((1ull << shift) - 1) : mx;
+    want -= sh.found[1];
+    if (shift == 0) {
+      cut = lo;
+      ties = want;
+      break;
+    }
+    if (sh.count[sh.found[0]] <= 64) {  // each with all of them
+      each(r, [&](int, u64 k) {
+        if (k >= lo && k <= hi) sh.few[atomicAdd(&sh.n_few, 1)] = k;
+      });
+      lds_barrier();
+      const int m = sh.n_few;
+      if (t < m) {
+        const u64 k = sh.few[t];
+        int nb = 0, nt = 0;
+#pragma unroll 4
+        for (int j = 0; j < m; ++j) {
+          nb += sh.few[j] < k;
+          nt += sh.few[j] == k;
+        }
+        if (nb < want && nb + nt >= want) {  // (equal ones write the same)
+          sh.ext[0][0] = k;
+          sh.found[0] = want - nb;
+        }
+      }
+      lds_barrier();
+      cut = sh.ext[0][0];
+      ties = sh.found[0];
+      break;
+    }
+  }
+  // eight columns a thread
+  constexpr int E = 8;
+  int at = 0;
+  for (int c = 0; c < r.n; c += 256 * E) {
+    const int j = c + E * t;
+    u64 k[E];
+    int id[E], tied = 0, under = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      k[e] = j + e < r.n ? r.at(j + e) : kNoPage;
+      id[e] = j + e < r.n ? tab[j + e] : 0;
+      tied += k[e] == cut;
+      under += k[e] < cut;
+    }
+    int nt = 0, m, before = 0;
+    if (ties != INT32_MAX) before = block_scan(tied, nt, sh.red);
+    auto left = [&](int x) { return ties > x ? ties - x : 0; };
+    int x = at + block_scan(under + (tied < left(before) ? tied : left(before)), m, sh.red);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const bool tie = k[e] == cut;
+      if (k[e] < cut || (tie && before < ties)) to[x++] = id[e] * n_kv + g;
+      before += tie;
+    }
+    at += m;
+    ties = ties == INT32_MAX ? ties : left(nt);
+  }
+  return at;
+}
+
+// A work-group: `part` pages of one row and kv head; the last one of a row to arrive
+// chooses. Grid: (parts, rows by kv heads). Bound by latencies: the row's place, its q, the
+// pages' numbers, their bounds and what is handed over wait for each other.
 template <int HD>
-__global__ void __launch_bounds__(256) k_paged_select(SelectArgs s, int64_t i0) {
-  constexpr int LP = HD / 8;  // lanes that share a page
-  __shared__ u64 key[kPart];
-  __shared__ int count[kBins];
-  __shared__ u64 ext[2][4];
-  __shared__ int red[4], last, found[2];
+__global__ void __launch_bounds__(256) k_paged_select(SelectArgs s, int64_t i0, int part) {
+  constexpr int LP = HD / 8, PAGES = 256 / LP;  // lanes that share a page, pages of a round
+  __shared__ u64 key[kHeld];
+  __shared__ int ids[kPart];
+  __shared__ Choice sh;
+  __shared__ int last;
   const PagedArgs &a = s.a;
   const int t = threadIdx.x, lane = t & 63;
   const int64_t i = i0 + blockIdx.y, row = i / a.n_kv;
   const int g = (int)(i - row * a.n_kv);
+  // its heads' q, on its way first
+  const int l = lane % LP;
+  const float *q = s.q + (row * s.n_head + (int64_t)g * s.group) * HD + 8 * l;
+  constexpr int HU = 4;
+  f32x4a4 y[HU][2];
+  auto load_q = [&](int h0) {
+#pragma unroll
+    for (int h = 0; h < HU; ++h) {
+      const float *p = q + (int64_t)(h0 + h < s.group ? h0 + h : 0) * HD;
+      y[h][0] = *(const f32x4a4 *)p;
+      y[h][1] = *(const f32x4a4 *)(p + 4);
+    }
+  };
+  load_q(0);
   // the row's sequence and position
   int b = 0;
   int64_t r0, n;
@@ -218,144 +377,76 @@ __global__ void __launch_bounds__(256) k_paged_select(SelectArgs s, int64_t i0) 
     return;
   }
   const int mine = (int)((end - 1) / a.page);  // the row's own column
-  const int parts = mine / kPart + 1;
+  const int parts = mine / part + 1;
   if ((int)blockIdx.x >= parts) return;
-  const int c0 = blockIdx.x * kPart, c1 = c0 + kPart < mine ? c0 + kPart : mine;  // to score: columns before its own
+  const int c0 = blockIdx.x * part, nc = c0 + part < mine ? part : mine - c0;  // to score: columns before its own
   const int32_t *tab = a.table + (int64_t)b * a.table_cols;
   auto page = [&](int c) {
     const int32_t id = tab[c];
     return id >= 0 && id < a.n_pages ? id : -1;
   };
-  const int own = page(mine) >= 0, first = s.n_first < mine ? s.n_first : mine;
-  // its heads' positive and negative parts, summed
-  const int l = lane % LP;
+  const int own_id = page(mine), own = own_id >= 0, first = s.n_first < mine ? s.n_first : mine;
+  for (int c = t; c < part; c += 256) ids[c] = c < nc ? page(c0 + c) : -1;
+  // the heads' positive and negative parts, summed
   double qp[8], qn[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) qp[e] = qn[e] = 0.0;
-  const float *q = s.q + (row * s.n_head + (int64_t)g * s.group) * HD + 8 * l;
-  for (int h = 0; h < s.group; ++h) {
+  for (int h0 = 0; h0 < s.group; h0 += HU) {
+    if (h0) load_q(h0);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const double x = q[(int64_t)h * HD + e];
-      qp[e] += x > 0.0 ? x : x != x ? x : 0.0;
-      qn[e] += x < 0.0 ? x : 0.0;
-    }
-  }
-  for (int c = c0 + t / LP; c < c0 + kPart; c += 256 / LP) {
-    u64 k = kNoPage;
-    if (c < c1) {  // (uniform among the lanes of a page)
-      const int id = page(c);
-      if (id >= 0) {
-        const uint16_t *bd = s.bounds + ((int64_t)id * a.n_kv + g) * 2 * HD + 8 * l;
-        const h8 lo = *(const h8 *)bd, hi = *(const h8 *)(bd + HD);
-        double x = 0.0;
+    for (int h = 0; h < HU; ++h) {
+      if (h0 + h >= s.group) break;
+      const float v[8] = {y[h][0][0], y[h][0][1], y[h][0][2], y[h][0][3], y[h][1][0], y[h][1][1], y[h][1][2], y[h][1][3]};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x = fma((double)(float)lo[e], qn[e], fma((double)(float)hi[e], qp[e], x));
-        k = c < first ? 0 : rank_of(sum_lanes(x, LP));
+      for (int e = 0; e < 8; ++e) {
+        const double x = v[e];
+        qp[e] += x > 0.0 ? x : x != x ? x : 0.0;
+        qn[e] += x < 0.0 ? x : 0.0;
       }
     }
-    if (l == 0) key[c - c0] = k;
   }
-  __syncthreads();
-  Ranks r{key, true};
+  lds_barrier();
+  constexpr int U = 4;
+  for (int c = t / LP; c < nc; c += U * PAGES) {
+    h8 lo[U], hi[U];
+    int id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      id[u] = c + u * PAGES < nc ? ids[c + u * PAGES] : -1;
+      const uint16_t *bd = s.bounds + ((int64_t)(id[u] < 0 ? 0 : id[u]) * a.n_kv + g) * 2 * HD + 8 * l;
+      lo[u] = *(const h8 *)bd;
+      hi[u] = *(const h8 *)(bd + HD);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      double x = 0.0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x = fma((double)(float)lo[u][e], qn[e], fma((double)(float)hi[u][e], qp[e], x));
+      const u64 k = c0 + c + u * PAGES < first ? 0 : rank_of(group_sum_d<LP>(x));
+      if (l == 0 && c + u * PAGES < nc) key[c + u * PAGES] = id[u] < 0 ? kNoPage : k;
+    }
+  }
+  lds_barrier();
+  bool held = true;
+  u64 *all = s.scores + (int64_t)blockIdx.y * a.table_cols;
   if (parts > 1) {
-    u64 *all = s.scores + (int64_t)blockIdx.y * a.table_cols;
-    for (int c = c0 + t; c < c1; c += 256) __hip_atomic_store(all + c, key[c - c0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int c = t; c < nc; c += 256) __hip_atomic_store(all + c0 + c, key[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (t == 0) last = __hip_atomic_fetch_add(s.counters + blockIdx.y, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)parts - 1;
     __syncthreads();
     if (!last) return;
     if (t == 0) __hip_atomic_store(s.counters + blockIdx.y, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    r = Ranks{all, false};
-  }
-  // The best `want` of the columns before its own. Among those whose rank lies in [lo,
-  // hi], the bin of the want-th is found by steps of a power of two, and taken as the
-  // next range: ten bits a time, of 64 at most.
-  int want = s.n_select - own, have = 0;
-  for (int c = t; c < mine; c += 256) have += r.at(c) != kNoPage;
-  int total;
-  block_scan(have, total, red);
-  u64 cut = kNoPage - 1;  // ranks up to it are taken, of those equal to it `ties`
-  int ties = INT32_MAX;
-  if (want <= 0) {  // its own page alone
-    cut = 0;
-    ties = 0;
-  } else if (total > want) {
-    u64 lo = 0, hi = kNoPage - 1;
-    for (;;) {
-      u64 mn = kNoPage, mx = 0;
-      for (int c = t; c < mine; c += 256) {
-        const u64 k = r.at(c);
-        if (k < lo || k > hi) continue;
-        mn = k < mn ? k : mn;
-        mx = k > mx ? k : mx;
-      }
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const u64 y = __shfl_xor(mn, d), z = __shfl_xor(mx, d);
-        mn = y < mn ? y : mn;
-        mx = z > mx ? z : mx;
-      }
-      __syncthreads();
-      if (lane == 0) {
-        ext[0][t >> 6] = mn;
-        ext[1][t >> 6] = mx;
-      }
-      for (int c = t; c < kBins; c += 256) count[c] = 0;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        mn = ext[0][w] < mn ? ext[0][w] : mn;
-        mx = ext[1][w] > mx ? ext[1][w] : mx;
-      }
-      if (mn == mx) {  // equal ones: the first by column
-        cut = mn;
-        ties = want;
-        break;
-      }
-      const int shift = 64 - __clzll((long long)(mx - mn)) > 10 ? 64 - __clzll((long long)(mx - mn)) - 10 : 0;
-      for (int c = t; c < mine; c += 256) {
-        const u64 k = r.at(c);
-        if (k >= mn && k <= mx) atomicAdd(&count[(k - mn) >> shift], 1);
-      }
-      __syncthreads();
-      int x[4], sum = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum += x[e] = count[4 * t + e];
-      int before = block_scan(sum, total, red);
-      if (before < want && before + sum >= want) {
-        int e = 0;
-        for (; before + x[e] < want; ++e) before += x[e];
-        found[0] = 4 * t + e;
-        found[1] = before;
-      }
-      __syncthreads();
-      lo = mn + ((u64)found[0] << shift);
-      hi = mx - lo > (1ull << shift) - 1 ? lo + ((1ull << shift) - 1) : mx;
-      want -= found[1];
-      if (shift == 0) {
-        cut = lo;
-        ties = want;
-        break;
-      }
+    held = mine <= kHeld;
+    if (held) {
+      each(Handed{all, mine}, [&](int c, u64 k) { key[c] = k; });
+      lds_barrier();
     }
   }
-  // the chosen ones in the order of their columns, then its own
-  int at = 0;
-  for (int c = 0; c < mine; c += 256) {
-    const u64 k = c + t < mine ? r.at(c + t) : kNoPage;
-    int nt = 0, m, before = 0;
-    const bool tie = k == cut;
-    if (ties != INT32_MAX) before = block_scan(tie, nt, red);
-    const bool take = k < cut || (tie && before < ties);
-    const int x = at + block_scan(take, m, red);
-    if (take) to[x] = tab[c + t] * a.n_kv + g;
-    at += m;
-    ties = ties == INT32_MAX ? ties : ties - nt;
-  }
+  const int want = s.n_select - own;
+  const int at = held ? choose(Held{key, mine}, want, tab, a.n_kv, g, to, sh) : choose(Handed{all, mine}, want, tab, a.n_kv, g, to, sh);
   if (t == 0) {
-    if (own) to[at] = tab[mine] * a.n_kv + g;
+    if (own) to[at] = own_id * a.n_kv + g;
     s.len[blockIdx.y] = (int32_t)(at * (int64_t)a.page + (own ? end - (int64_t)mine * a.page : 0));
   }
 }
@@ -385,14 +476,16 @@ hipError_t launch_paged_attention_selected(hipStream_t st, const PagedArgs &a, c
   const int group = n_head / a.n_kv, n_sel = n_select < a.table_cols ? n_select : a.table_cols;
   const int64_t units = a.s_rows * a.n_kv;
   const int64_t most = std::min(std::min(kRowsAtOnce, kScores / a.table_cols), kChosen / n_sel);
-  SelectArgs s{a, bounds, q, n_head, group, n_sel, n_first, (unsigned long long *)ws, (int32_t *)(ws + kScores * 8), nullptr, nullptr, select_counters};
+  SelectArgs s{a, bounds, q, n_head, group, n_sel, n_first, (uint64_t *)ws, (int32_t *)(ws + kScores * 8), nullptr, nullptr, select_counters};
   s.len = s.table + kChosen;
   s.row_start = s.len + kRowsAtOnce;
   for (int64_t i = 0; i < units; i += most) {
     const int n = (int)std::min(most, units - i);
-    const dim3 grid((unsigned)((a.table_cols + kPart - 1) / kPart), (unsigned)n);
-    if (a.hd == 64) KMOE_LAUNCH(k_paged_select<64>, grid, dim3(256), 0, st, s, i);
-    else KMOE_LAUNCH(k_paged_select<128>, grid, dim3(256), 0, st, s, i);
+    // few rows: more work-groups a row (1 row of 8 kv heads, 2047 pages: TODO)
+    const int each = (int64_t)n * ((a.table_cols + kPart - 1) / kPart) < 512 ? kPart / 4 : kPart;
+    const dim3 grid((unsigned)((a.table_cols + each - 1) / each), (unsigned)n);
+    if (a.hd == 64) KMOE_LAUNCH(k_paged_select<64>, grid, dim3(256), 0, st, s, i, each);
+    else KMOE_LAUNCH(k_paged_select<128>, grid, dim3(256), 0, st, s, i, each);
     PagedArgs p = a;
     p.n_kv = 1;
     p.n_pages = a.n_pages * a.n_kv;

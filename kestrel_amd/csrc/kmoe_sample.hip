@@ -22,6 +22,7 @@
 
 #include "kmoe_device.h"
 #include "kmoe_launch.h"
+#include "kmoe_scan.h"
 
 namespace kmoe {
 namespace {
@@ -139,22 +140,6 @@ struct Shared {
   uint16_t group[kGroups], in_group[128];
 };
 
-// Inclusive scan over a wave: within rows of 16 lanes, then row 0's and 2's totals onto
-// rows 1 and 3, then lane 31's onto the upper half.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ u64 dpp_add(u64 x) {
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xf, false);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xf, false);
-  return x + ((u64)hi << 32 | lo);
-}
-__device__ __forceinline__ u64 wave_scan(u64 x) {
-  x = dpp_add<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
-  x = dpp_add<0x112, 0xf>(x);
-  x = dpp_add<0x114, 0xf>(x);
-  x = dpp_add<0x118, 0xf>(x);
-  x = dpp_add<0x142, 0xa>(x);  // row_bcast 15, 31
-  return dpp_add<0x143, 0xc>(x);
-}
 // Exclusive scan over the work-group's threads, and the total.
 __device__ __forceinline__ u64 block_scan(u64 x, u64 &total, Shared &sh) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
