@@ -94,6 +94,10 @@ __device__ __forceinline__ uint8_t *paged_block(const PagedArgs &a, int64_t bloc
   return a.pages + (id * a.n_kv + g) * block_bytes;
 }
 
+// The same without a window for sequences of one row that read each other's pages: they stay in
+// the caches.
+hipError_t launch_paged_attention_again(hipStream_t st, const PagedArgs &a, const float *q, int n_head, float *out,
+                                        float *part, uint32_t *counters);
 // Sequences with pages in common (kmoe_paged_groups): group i holds sequences start[i] ..
 // start[i + 1] - 1 and the first pages[i] columns of its first one's table. skip: tiles
 // of 32 positions that a sequence leaves to its group; ml: maximum and sum of the weights

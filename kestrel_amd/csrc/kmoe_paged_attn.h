@@ -229,8 +229,8 @@ __device__ __forceinline__ Span span_of(int64_t pos_lo, int64_t pos_hi, int64_t 
 
 // What a launch works: whole sequences; what the sequences of each group have in common
 // (kShared: a group counts as a sequence, all its rows see all of it); or what is left of
-// the sequences then (kOwn).
-enum { kWhole = 0, kShared = 1, kOwn = 2 };
+// the sequences then (kOwn); or whole sequences that have pages in common (kAgain).
+enum { kWhole = 0, kShared = 1, kOwn = 2, kAgain = 3 };
 
 // Rows of group i together, its first sequence, and its positions in common.
 __device__ __forceinline__ void group_rows(const PagedArgs &a, const SharedArgs &s, int i, int &b0, int64_t &r0, int64_t &n,

@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
     // the block of a tile's page (page 0 stands in for one that does not exist)
     auto block = [&](int id) { return a.pages + ((int64_t)id * a.n_kv + g) * bb; };
     auto exists = [&](int id) { return id >= 0 && id < a.n_pages; };
-    Frags<T, HD, C == 1> fr;
+    Frags<T, HD, C == 1 && MODE != kAgain> fr;
     int v = s_.at + wave;
     int id = page_of(v), id_next = page_of(v + 4);  // pages of the wave's tile and of its next one
     if (v < v_last) {
@@ -683,6 +683,11 @@ hipError_t launch_paged_attention(hipStream_t st, const PagedArgs &a, const floa
                                   int64_t n_sink, float *out, float *part, uint32_t *counters) {
   const int w = window >= INT32_MAX ? 0 : (int)window, sink = (int)(n_sink < (1 << 30) ? n_sink : (1 << 30));
   return launch_mode<kWhole>(st, a, SharedArgs{}, q, n_head, w, sink, out, part, counters);
+}
+
+hipError_t launch_paged_attention_again(hipStream_t st, const PagedArgs &a, const float *q, int n_head, float *out,
+                                        float *part, uint32_t *counters) {
+  return launch_mode<kAgain>(st, a, SharedArgs{}, q, n_head, 0, 0, out, part, counters);
 }
 
 hipError_t launch_paged_attention_shared(hipStream_t st, const PagedArgs &a, const SharedArgs &sa, const float *q,

@@ -496,7 +496,9 @@ hipError_t launch_paged_attention_selected(hipStream_t st, const PagedArgs &a, c
     p.seq_len = s.len;
     p.table = s.table;
     const int64_t at = i * group * a.hd;
-    const hipError_t e = launch_paged_attention(st, p, q + at, group, 0, 0, out + at, part, counters);
+    // rows of a chunk choose many of the same pages
+    const hipError_t e = a.row_start ? launch_paged_attention_again(st, p, q + at, group, out + at, part, counters)
+                                     : launch_paged_attention(st, p, q + at, group, 0, 0, out + at, part, counters);
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
