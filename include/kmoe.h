@@ -637,8 +637,8 @@ int kmoe_paged_bounds(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *pa
  * n_first < n_select), all that there are where they are fewer. A page without an entry
  * in the table is not chosen. A NaN score counts as the best. No score of a position
  * passes its page's, summed over the heads; pages whose keys lie apart from the query's direction are not read. With
- * n_select >= table_cols it is kmoe_paged_attention itself. table_cols up to 2^20 and
- * n_pages * n_kv up to 2^31 - 1 (KMOE_E_UNSUPPORTED past them). Besides that call's workspace it keeps one of
+ * n_select >= table_cols it is kmoe_paged_attention itself. table_cols up to 2^20,
+ * table_cols * n_kv up to 2^22 and n_pages * n_kv up to 2^31 - 1 (KMOE_E_UNSUPPORTED past them). Besides that call's workspace it keeps one of
  * 50 MB, with the same rules. */
 int kmoe_paged_attention_selected(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *pages_dev,
                                   const uint16_t *bounds_dev, const kmoe_paged_batch *batch, const float *q_dev,

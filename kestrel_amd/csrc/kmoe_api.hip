@@ -2724,7 +2724,7 @@ int kmoe_paged_attention_shared(kmoe_ctx *c, const kmoe_paged_desc *d, const voi
   rc = kept_ws(c, c->paged, paged_part_floats() * sizeof(float), "paged attention partials", &part);
   if (!rc) rc = kept_ws(c, c->shared, kSharedHeads * 8 + KMOE_PAGED_MAX_SEQ * 4, "shared parts of rows", &ml);
   if (rc) return rc;
-  const SharedArgs sa{groups->start_dev, groups->pages_dev, groups->n_group, (int32_t *)(ml + kSharedHeads * 8), (float *)ml};
+  const SharedArgs sa{groups->start_dev, groups->pages_dev, groups->n_group, 0, (int32_t *)(ml + kSharedHeads * 8), (float *)ml};
   LAUNCH(c, "paged_attention_shared", launch_paged_attention_shared(c->stream, a, sa, q, n_head, out, (float *)part,
                                                                     c->counters + kCounterWords));
   return KMOE_OK;
@@ -2755,8 +2755,8 @@ int kmoe_paged_attention_selected(kmoe_ctx *c, const kmoe_paged_desc *d, const v
   if (rc) return rc;
   if (n_first < 0 || n_select <= n_first)
     return fail(c, KMOE_E_INVALID, "%d pages with the first %d among them (need 0 <= n_first < n_select)", n_select, n_first);
-  if (a.table_cols > select_max_cols() || a.n_pages * a.n_kv > INT32_MAX)
-    return fail(c, KMOE_E_UNSUPPORTED, "%d columns, %lld pages of %d kv heads (at most 2^20, and 2^31 - 1 together)",
+  if (!select_fits(a.table_cols, a.n_kv) || a.n_pages * a.n_kv > INT32_MAX)
+    return fail(c, KMOE_E_UNSUPPORTED, "%d columns, %lld pages of %d kv heads (at most 2^20 columns, 2^22 by kv heads, 2^31 - 1 pages by kv heads)",
                 a.table_cols, (long long)a.n_pages, a.n_kv);
   rc = check_paged_q(c, a, q, n_head, out);
   if (rc || a.s_rows == 0) return rc;

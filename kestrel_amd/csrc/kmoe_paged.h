@@ -94,9 +94,10 @@ __device__ __forceinline__ uint8_t *paged_block(const PagedArgs &a, int64_t bloc
   return a.pages + (id * a.n_kv + g) * block_bytes;
 }
 
-// The same without a window for sequences of one row that read each other's pages: they stay in
-// the caches.
-hipError_t launch_paged_attention_again(hipStream_t st, const PagedArgs &a, const float *q, int n_head, float *out,
+// The same without a window for sequences of one row that read each other's pages, which stay in
+// the caches: sequence b is row b % rows * (n_seq / rows) + b / rows of q and out, and
+// its row is left as it is where its length is negative.
+hipError_t launch_paged_attention_again(hipStream_t st, const PagedArgs &a, int rows, const float *q, int n_head, float *out,
                                         float *part, uint32_t *counters);
 // Sequences with pages in common (kmoe_paged_groups): group i holds sequences start[i] ..
 // start[i + 1] - 1 and the first pages[i] columns of its first one's table. skip: tiles
@@ -105,6 +106,7 @@ hipError_t launch_paged_attention_again(hipStream_t st, const PagedArgs &a, cons
 struct SharedArgs {
   const int32_t *start, *pages;
   int n_group;
+  int rows;  // launch_paged_attention_again's
   int32_t *skip;
   float *ml;
 };
@@ -124,18 +126,19 @@ hipError_t launch_paged_attention(hipStream_t st, const PagedArgs &a, const floa
 
 // A choice of pages (kmoe_paged_attention_selected), for some of the rows by kv heads at a
 // time: scores holds the ranks of pages that several work-groups score, counters (zero
-// between calls) who has arrived, table, len and row_start the batch that is left, a
-// sequence of one row per row and kv head.
+// between calls) who has arrived, table and len the batch that is left, a
+// sequence of one row per row and kv head (len -1: not a row of any sequence).
 struct SelectArgs {
   PagedArgs a;
   const uint16_t *bounds;
   const float *q;
   int n_head, group, n_select, n_first;
+  int rows;  // of the launch; sequence b is row b % rows, kv head b / rows where rows share pages, otherwise the other way round
   uint64_t *scores;
-  int32_t *table, *len, *row_start;
+  int32_t *table, *len;
   uint32_t *counters;
 };
-int64_t select_max_cols();
+bool select_fits(int64_t table_cols, int n_kv);
 int select_counters();
 size_t select_ws_bytes();
 hipError_t launch_paged_bounds(hipStream_t st, const PagedArgs &a, uint16_t *bounds);

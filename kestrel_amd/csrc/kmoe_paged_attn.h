@@ -336,6 +336,7 @@ __device__ void make_plan(const PagedArgs &a, const SharedArgs &sa, int n_seq, i
     } else {
       paged_rows(a, b, r0, n);
       len = a.seq_len[b] > 0 ? a.seq_len[b] : 0;  // (a length below the rows leaves them nothing)
+      if constexpr (MODE == kAgain) n = a.seq_len[b] >= 0;
       if constexpr (MODE == kOwn) {
         skip = sa.skip[b];
         lens[n_seq + b] = skip;
@@ -467,6 +468,9 @@ struct Cursor {
         s.b = __builtin_amdgcn_readfirstlane(s.b);
         s.r0 = __builtin_amdgcn_readfirstlane((int)r0);
         s.n = __builtin_amdgcn_readfirstlane((int)n);
+      } else if constexpr (MODE == kAgain) {
+        s.r0 = b % sa.rows * (n_seq / sa.rows) + b / sa.rows;
+        s.n = 1;  // (one without a row takes no place in the line)
       } else if (a.row_start) {
         const const_i32 rs = (const_i32)(uintptr_t)a.row_start + b;
         s.r0 = rs[0] < 0 ? 0 : rs[0];

@@ -685,9 +685,11 @@ hipError_t launch_paged_attention(hipStream_t st, const PagedArgs &a, const floa
   return launch_mode<kWhole>(st, a, SharedArgs{}, q, n_head, w, sink, out, part, counters);
 }
 
-hipError_t launch_paged_attention_again(hipStream_t st, const PagedArgs &a, const float *q, int n_head, float *out,
+hipError_t launch_paged_attention_again(hipStream_t st, const PagedArgs &a, int rows, const float *q, int n_head, float *out,
                                         float *part, uint32_t *counters) {
-  return launch_mode<kAgain>(st, a, SharedArgs{}, q, n_head, 0, 0, out, part, counters);
+  SharedArgs sa{};
+  sa.rows = rows;
+  return launch_mode<kAgain>(st, a, sa, q, n_head, 0, 0, out, part, counters);
 }
 
 hipError_t launch_paged_attention_shared(hipStream_t st, const PagedArgs &a, const SharedArgs &sa, const float *q,

@@ -322,7 +322,7 @@ __device__ __forceinline__ int choose(const R &r, int want, const int32_t *tab, 
 // chooses. Grid: (parts, rows by kv heads). Bound by latencies: the row's place, its q, the
 // pages' numbers, their bounds and what is handed over wait for each other.
 template <int HD>
-__global__ void __launch_bounds__(256) k_paged_select(SelectArgs s, int64_t i0, int part) {
+__global__ void __launch_bounds__(256) k_paged_select(SelectArgs s, int64_t row0, int part) {
   constexpr int LP = HD / 8, PAGES = 256 / LP;  // lanes that share a page, pages of a round
   __shared__ u64 key[kHeld];
   __shared__ int ids[kPart];
@@ -330,8 +330,8 @@ __global__ void __launch_bounds__(256) k_paged_select(SelectArgs s, int64_t i0, 
   __shared__ int last;
   const PagedArgs &a = s.a;
   const int t = threadIdx.x, lane = t & 63;
-  const int64_t i = i0 + blockIdx.y, row = i / a.n_kv;
-  const int g = (int)(i - row * a.n_kv);
+  const int at_row = a.row_start ? blockIdx.y % s.rows : blockIdx.y / a.n_kv, g = a.row_start ? blockIdx.y / s.rows : blockIdx.y % a.n_kv;
+  const int64_t row = row0 + at_row;
   // its heads' q, on its way first
   const int l = lane % LP;
   const float *q = s.q + (row * s.n_head + (int64_t)g * s.group) * HD + 8 * l;
@@ -360,20 +360,19 @@ __global__ void __launch_bounds__(256) k_paged_select(SelectArgs s, int64_t i0, 
   }
   paged_rows(a, b, r0, n);
   const bool in = row >= r0 && row < r0 + n;
-  if (a.row_start && blockIdx.x == 0 && t == 0) {  // rows that no sequence has lie before the first and behind the last
-    int64_t lo, hi, m;
-    paged_rows(a, 0, lo, m);
-    paged_rows(a, a.n_seq - 1, hi, m);
-    hi += m;
-    auto clip = [&](int64_t r) { return r < lo * a.n_kv ? lo * a.n_kv : r > hi * a.n_kv ? hi * a.n_kv : r; };
-    s.row_start[blockIdx.y] = (int32_t)(clip(i) - i0);
-    if (blockIdx.y == gridDim.y - 1) s.row_start[gridDim.y] = (int32_t)(clip(i + 1) - i0);
-  }
   const int64_t cap = (int64_t)a.table_cols * a.page, pos = in ? (int64_t)a.seq_len[b] - n + row - r0 : -1;
   const int64_t end = pos + 1 < cap ? pos + 1 : cap;
   int32_t *to = s.table + (int64_t)blockIdx.y * s.n_select;
   if (end <= 0) {
-    if (blockIdx.x == 0 && t == 0) s.len[blockIdx.y] = 0;
+    if (blockIdx.x == 0 && t == 0) {  // rows that no sequence has lie before the first and behind the last
+      int64_t lo = 0, hi = 0, m;
+      if (!in) {
+        paged_rows(a, 0, lo, m);
+        paged_rows(a, a.n_seq - 1, hi, m);
+        hi += m;
+      }
+      s.len[blockIdx.y] = in || (row >= lo && row < hi) ? 0 : -1;
+    }
     return;
   }
   const int mine = (int)((end - 1) / a.page);  // the row's own column
@@ -451,15 +450,16 @@ __global__ void __launch_bounds__(256) k_paged_select(SelectArgs s, int64_t i0, 
   }
 }
 
-constexpr int64_t kRowsAtOnce = 1024;             // rows by kv heads of a launch
-constexpr int64_t kScores = (int64_t)1 << 22;     // of a launch
-constexpr int64_t kChosen = (int64_t)1 << 22;
+// Rows by kv heads of a launch (the attention's plan of more takes LDS that work-groups then
+// lack), or one row's where it has more kv heads.
+constexpr int64_t kRowsAtOnce = 1024, kMostHeads = 4096;
+constexpr int64_t kScores = (int64_t)1 << 22;  // ranks, and chosen pages, of a launch
 
 }  // namespace
 
-int64_t select_max_cols() { return (int64_t)1 << 20; }
-int select_counters() { return (int)kRowsAtOnce; }
-size_t select_ws_bytes() { return kScores * 8 + kChosen * 4 + (2 * kRowsAtOnce + 1) * 4; }
+bool select_fits(int64_t table_cols, int n_kv) { return table_cols <= (int64_t)1 << 20 && table_cols * n_kv <= kScores; }
+int select_counters() { return (int)kMostHeads; }
+size_t select_ws_bytes() { return kScores * 8 + kScores * 4 + kMostHeads * 4; }
 
 hipError_t launch_paged_bounds(hipStream_t st, const PagedArgs &a, uint16_t *bounds) {
   const int64_t n = a.row_start ? a.s_rows / a.page + 2 * (int64_t)a.n_seq : a.n_seq;
@@ -474,14 +474,15 @@ hipError_t launch_paged_attention_selected(hipStream_t st, const PagedArgs &a, c
                                            int n_head, int n_select, int n_first, float *out, float *part,
                                            uint32_t *counters, uint8_t *ws, uint32_t *select_counters) {
   const int group = n_head / a.n_kv, n_sel = n_select < a.table_cols ? n_select : a.table_cols;
-  const int64_t units = a.s_rows * a.n_kv;
-  const int64_t most = std::min(std::min(kRowsAtOnce, kScores / a.table_cols), kChosen / n_sel);
-  SelectArgs s{a, bounds, q, n_head, group, n_sel, n_first, (uint64_t *)ws, (int32_t *)(ws + kScores * 8), nullptr, nullptr, select_counters};
-  s.len = s.table + kChosen;
-  s.row_start = s.len + kRowsAtOnce;
-  for (int64_t i = 0; i < units; i += most) {
-    const int n = (int)std::min(most, units - i);
-    // few rows: more work-groups a row (1 row of 8 kv heads, 2047 pages: TODO)
+  // rows of a launch: as many launches as are needed, the rows in equal parts
+  const int64_t most = std::max<int64_t>(1, std::min(kRowsAtOnce, kScores / a.table_cols) / a.n_kv);
+  const int64_t launches = (a.s_rows + most - 1) / most, rows = (a.s_rows + launches - 1) / launches;
+  SelectArgs s{a, bounds, q, n_head, group, n_sel, n_first, 0, (uint64_t *)ws, (int32_t *)(ws + kScores * 8), nullptr, select_counters};
+  s.len = s.table + kScores;
+  for (int64_t i = 0; i < a.s_rows; i += rows) {
+    s.rows = (int)std::min(rows, a.s_rows - i);
+    const int n = s.rows * a.n_kv;
+    // few rows: more work-groups a row (1 row of 8 kv heads, 2047 pages: 24 us with 512 pages each, 17 with 128)
     const int each = (int64_t)n * ((a.table_cols + kPart - 1) / kPart) < 512 ? kPart / 4 : kPart;
     const dim3 grid((unsigned)((a.table_cols + each - 1) / each), (unsigned)n);
     if (a.hd == 64) KMOE_LAUNCH(k_paged_select<64>, grid, dim3(256), 0, st, s, i, each);
@@ -492,12 +493,12 @@ hipError_t launch_paged_attention_selected(hipStream_t st, const PagedArgs &a, c
     p.n_seq = n;
     p.table_cols = n_sel;
     p.s_rows = n;
-    p.row_start = a.row_start ? s.row_start : nullptr;
+    p.row_start = nullptr;
     p.seq_len = s.len;
     p.table = s.table;
-    const int64_t at = i * group * a.hd;
-    // rows of a chunk choose many of the same pages
-    const hipError_t e = a.row_start ? launch_paged_attention_again(st, p, q + at, group, out + at, part, counters)
+    const int64_t at = i * n_head * a.hd;
+    // rows of a chunk choose many of the same pages: kv head by kv head, kept in the caches
+    const hipError_t e = a.row_start ? launch_paged_attention_again(st, p, s.rows, q + at, group, out + at, part, counters)
                                      : launch_paged_attention(st, p, q + at, group, 0, 0, out + at, part, counters);
     if (e != hipSuccess) return e;
   }

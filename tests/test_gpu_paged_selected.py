@@ -182,6 +182,15 @@ def test_more_rows_than_a_launch_takes(ctx):  # noqa: F811
     _check(c, 4, 4, 1, [330, 0, 170])
 
 
+def test_more_kv_heads_than_rows_of_a_launch(ctx):  # noqa: F811
+    """One row, and one chunk, of 1500 kv heads; contexts that two work-groups score."""
+    c = Cache(ctx, F16, 1500, 64, 32, [32 * 4 + 3, 32 * 5], 6)
+    _check(c, 1500, 2, 0)
+    _check(c, 1500, 3, 1, [2, 1])
+    c = Cache(ctx, F16, 300, 64, 32, [32 * 130 + 3], 7)
+    _check(c, 300, 4, 1)
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("n_select", [2, 40, 700])
 def test_contexts_that_several_work_groups_score(ctx, t, n_select):  # noqa: F811
@@ -411,6 +420,16 @@ def test_refusals(ctx):  # noqa: F811
     with pytest.raises(KmoeError) as e:
         call(n_head=34, q=torch.zeros((2, 34 * 64), device="cuda"))
     assert e.value.status == -2
+    many = PagedKV(F16, 8, 64, 32)
+    p8, b8 = torch.zeros((1, many.page_bytes), dtype=torch.uint8, device="cuda"), torch.zeros((1, 8, 2, 64), dtype=torch.float16, device="cuda")
+    for cols, ok in (((1 << 19) + 1, False), (1 << 19, True)):  # 2^22 columns by kv heads
+        b = ctx.paged_batch(torch.full((1, cols), -1, dtype=torch.int32, device="cuda"), _dev([1 << 24], np.int32))
+        if ok:
+            assert not ctx.paged_attention_selected(many, p8, b8, b, torch.ones((1, 512), device="cuda"), 8, 3).any()
+        else:
+            with pytest.raises(KmoeError) as e:
+                ctx.paged_attention_selected(many, p8, b8, b, torch.ones((1, 512), device="cuda"), 8, 3)
+            assert e.value.status == -2
     wide = ctx.paged_batch(torch.zeros((1, (1 << 20) + 1), dtype=torch.int32, device="cuda"), _dev([1], np.int32))
     with pytest.raises(KmoeError) as e:
         call(batch=wide, q=q[:1].contiguous())
