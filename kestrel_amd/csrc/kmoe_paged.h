@@ -133,7 +133,7 @@ struct SelectArgs {
   const uint16_t *bounds;
   const float *q;
   int n_head, group, n_select, n_first;
-  int rows;  // of the launch; sequence b is row b % rows, kv head b / rows where rows share pages, otherwise the other way round
+  int rows;  // of a launch of the attention; its sequence b is row b % rows, kv head b / rows where rows share pages, otherwise the other way round
   uint64_t *scores;
   int32_t *table, *len;
   uint32_t *counters;

@@ -319,7 +319,7 @@ __device__ __forceinline__ int choose(const R &r, int want, const int32_t *tab, 
 }
 
 // A work-group: `part` pages of one row and kv head; the last one of a row to arrive
-// chooses. Grid: (parts, rows by kv heads). Bound by latencies: the row's place, its q, the
+// chooses. Grid: (parts, rows by kv heads), for several launches of the attention. Bound by latencies: the row's place, its q, the
 // pages' numbers, their bounds and what is handed over wait for each other.
 template <int HD>
 __global__ void __launch_bounds__(256) k_paged_select(SelectArgs s, int64_t row0, int part) {
@@ -330,7 +330,13 @@ __global__ void __launch_bounds__(256) k_paged_select(SelectArgs s, int64_t row0
   __shared__ int last;
   const PagedArgs &a = s.a;
   const int t = threadIdx.x, lane = t & 63;
-  const int at_row = a.row_start ? blockIdx.y % s.rows : blockIdx.y / a.n_kv, g = a.row_start ? blockIdx.y / s.rows : blockIdx.y % a.n_kv;
+  int at_row = blockIdx.y / a.n_kv, g = blockIdx.y % a.n_kv;
+  if (a.row_start) {  // kv head by kv head within a launch of the attention
+    const int first = at_row / s.rows * s.rows, left = gridDim.y / a.n_kv - first, rows = left < s.rows ? left : s.rows;
+    const int x = blockIdx.y - first * a.n_kv;
+    g = x / rows;
+    at_row = first + x % rows;
+  }
   const int64_t row = row0 + at_row;
   // its heads' q, on its way first
   const int l = lane % LP;
@@ -450,8 +456,8 @@ __global__ void __launch_bounds__(256) k_paged_select(SelectArgs s, int64_t row0
   }
 }
 
-// Rows by kv heads of a launch (the attention's plan of more takes LDS that work-groups then
-// lack), or one row's where it has more kv heads.
+// Rows by kv heads of a launch of the attention (its plan of more takes LDS that work-groups
+// then lack) and of the choice's, or one row's where it has more kv heads.
 constexpr int64_t kRowsAtOnce = 1024, kMostHeads = 4096;
 constexpr int64_t kScores = (int64_t)1 << 22;  // ranks, and chosen pages, of a launch
 
@@ -474,19 +480,26 @@ hipError_t launch_paged_attention_selected(hipStream_t st, const PagedArgs &a, c
                                            int n_head, int n_select, int n_first, float *out, float *part,
                                            uint32_t *counters, uint8_t *ws, uint32_t *select_counters) {
   const int group = n_head / a.n_kv, n_sel = n_select < a.table_cols ? n_select : a.table_cols;
-  // rows of a launch: as many launches as are needed, the rows in equal parts
-  const int64_t most = std::max<int64_t>(1, std::min(kRowsAtOnce, kScores / a.table_cols) / a.n_kv);
+  // rows of a launch of the attention: as many launches as are needed, the rows in equal parts;
+  // a launch of the choice is for as many of those as its workspace holds (300 rows of 4 kv
+  // heads, 250 pages: TODO us, two of 22 for an attention's launch each)
+  const int64_t fit = std::min(kMostHeads, kScores / a.table_cols) / a.n_kv;
+  const int64_t most = std::max<int64_t>(1, std::min(kRowsAtOnce / a.n_kv, fit));
   const int64_t launches = (a.s_rows + most - 1) / most, rows = (a.s_rows + launches - 1) / launches;
-  SelectArgs s{a, bounds, q, n_head, group, n_sel, n_first, 0, (uint64_t *)ws, (int32_t *)(ws + kScores * 8), nullptr, select_counters};
+  const int64_t at_once = std::max<int64_t>(1, fit / rows) * rows;
+  SelectArgs s{a, bounds, q, n_head, group, n_sel, n_first, (int)rows, (uint64_t *)ws, (int32_t *)(ws + kScores * 8), nullptr, select_counters};
   s.len = s.table + kScores;
   for (int64_t i = 0; i < a.s_rows; i += rows) {
-    s.rows = (int)std::min(rows, a.s_rows - i);
-    const int n = s.rows * a.n_kv;
-    // few rows: more work-groups a row (1 row of 8 kv heads, 2047 pages: 24 us with 512 pages each, 17 with 128)
-    const int each = (int64_t)n * ((a.table_cols + kPart - 1) / kPart) < 512 ? kPart / 4 : kPart;
-    const dim3 grid((unsigned)((a.table_cols + each - 1) / each), (unsigned)n);
-    if (a.hd == 64) KMOE_LAUNCH(k_paged_select<64>, grid, dim3(256), 0, st, s, i, each);
-    else KMOE_LAUNCH(k_paged_select<128>, grid, dim3(256), 0, st, s, i, each);
+    const int n_rows = (int)std::min(rows, a.s_rows - i), n = n_rows * a.n_kv;
+    const int64_t before = i % at_once * a.n_kv;
+    if (before == 0) {
+      const int64_t heads = std::min(at_once, a.s_rows - i) * a.n_kv;
+      // few rows: more work-groups a row (1 row of 8 kv heads, 2047 pages: 24 us with 512 pages each, 17 with 128)
+      const int each = heads * ((a.table_cols + kPart - 1) / kPart) < 512 ? kPart / 4 : kPart;
+      const dim3 grid((unsigned)((a.table_cols + each - 1) / each), (unsigned)heads);
+      if (a.hd == 64) KMOE_LAUNCH(k_paged_select<64>, grid, dim3(256), 0, st, s, i, each);
+      else KMOE_LAUNCH(k_paged_select<128>, grid, dim3(256), 0, st, s, i, each);
+    }
     PagedArgs p = a;
     p.n_kv = 1;
     p.n_pages = a.n_pages * a.n_kv;
@@ -494,11 +507,11 @@ hipError_t launch_paged_attention_selected(hipStream_t st, const PagedArgs &a, c
     p.table_cols = n_sel;
     p.s_rows = n;
     p.row_start = nullptr;
-    p.seq_len = s.len;
-    p.table = s.table;
+    p.seq_len = s.len + before;
+    p.table = s.table + before * n_sel;
     const int64_t at = i * n_head * a.hd;
     // rows of a chunk choose many of the same pages: kv head by kv head, kept in the caches
-    const hipError_t e = a.row_start ? launch_paged_attention_again(st, p, s.rows, q + at, group, out + at, part, counters)
+    const hipError_t e = a.row_start ? launch_paged_attention_again(st, p, n_rows, q + at, group, out + at, part, counters)
                                      : launch_paged_attention(st, p, q + at, group, 0, 0, out + at, part, counters);
     if (e != hipSuccess) return e;
   }
