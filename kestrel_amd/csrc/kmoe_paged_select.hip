@@ -482,7 +482,7 @@ hipError_t launch_paged_attention_selected(hipStream_t st, const PagedArgs &a, c
   const int group = n_head / a.n_kv, n_sel = n_select < a.table_cols ? n_select : a.table_cols;
   // rows of a launch of the attention: as many launches as are needed, the rows in equal parts;
   // a launch of the choice is for as many of those as its workspace holds (300 rows of 4 kv
-  // heads, 250 pages: TODO us, two of 22 for an attention's launch each)
+  // heads, 250 pages: 32 us, two of 22 for an attention's launch each)
   const int64_t fit = std::min(kMostHeads, kScores / a.table_cols) / a.n_kv;
   const int64_t most = std::max<int64_t>(1, std::min(kRowsAtOnce / a.n_kv, fit));
   const int64_t launches = (a.s_rows + most - 1) / most, rows = (a.s_rows + launches - 1) / launches;
