@@ -237,7 +237,7 @@ __device__ __forceinline__ void group_rows(const PagedArgs &a, const SharedArgs 
                                            int64_t &len) {
   int lo = s.start[i], hi = s.start[i + 1];
   lo = lo < 0 ? 0 : lo;
-  hi = hi > a.n_seq ? a.n_seq : hi;
+  hi = hi < 0 ? 0 : hi < a.n_seq ? hi : a.n_seq;
   int32_t pages = s.pages[i];
   pages = pages < 0 ? 0 : pages < a.table_cols ? pages : a.table_cols;
   len = (int64_t)pages * a.page;

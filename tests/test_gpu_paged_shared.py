@@ -2,6 +2,7 @@
 itself: groups of all kinds beside sequences of their own, single rows and chunks,
 pages that are missing, values that are not finite, captured calls, refusals."""
 import ctypes as C
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
@@ -102,6 +103,48 @@ def test_entries_past_the_batch_or_the_table_are_cut_off(ctx, start, pages):  # 
     lens = [70, 80, 90, 100]
     c = _shared(ctx, F16, 2, 64, 32, lens, [0, 2, 4], [2, 0], 7)
     _check(c, 4, start, pages)
+
+
+@pytest.mark.parametrize("start,pages", [([0, 3, -2 ** 31], [2, 1]), ([3, -2 ** 31], [2]), ([2 ** 31 - 1, -2 ** 31], [1]), ([3, 1], [2])])
+def test_a_group_that_ends_before_it_begins_is_none(ctx, start, pages):  # noqa: F811
+    c = _shared(ctx, F16, 2, 64, 32, [70, 80, 90, 100], [0, 3], [2], 7)
+    _check(c, 4, start, pages)
+
+
+@pytest.mark.parametrize("nh,nkv,hd,most", [(4, 2, 64, 1), (4, 2, 128, 1), (16, 1, 64, 3), (16, 1, 128, 3)])
+def test_as_many_sequences_as_a_call_takes(ctx, nh, nkv, hd, most):  # noqa: F811
+    """4096 sequences, in groups of every size up to 60 with one or two pages of 32 in common."""
+    rng = np.random.default_rng(hd + most)
+    lens = rng.integers(most, 110, 4096).tolist()
+    rows = None if most == 1 else rng.integers(1, most + 1, 4096).tolist()
+    if rows:
+        lens = [max(n, r) for n, r in zip(lens, rows)]
+    start = np.unique(np.concatenate([[0, 4096], np.cumsum(rng.integers(1, 61, 200))]).clip(0, 4096)).tolist()
+    pages = rng.integers(0, 3, len(start) - 1).tolist()
+    c = _shared(ctx, F16, nkv, hd, 32, lens, start, pages, 14)
+    S = 4096 if rows is None else sum(rows)
+    q = rng.standard_normal((S, nh, hd)).astype(np.float32)
+    got = _attend(c, q, nh, start, pages, rows).reshape(S, nh, hd)
+    assert np.isfinite(got).all()
+    pick = [0, 1, 255, 256, 257, 2048, 4094, 4095] + rng.integers(0, 4096, 60).tolist()
+    rs = np.concatenate([[0], np.cumsum([1] * 4096 if rows is None else rows)])
+    at = np.concatenate([np.arange(rs[b], rs[b + 1]) for b in pick])
+    sub = SimpleNamespace(kv=c.kv, lens=[lens[b] for b in pick], hk=[c.hk[b] for b in pick], hv=[c.hv[b] for b in pick])
+    ref, tol, _ = _reference(sub, q[at], None if rows is None else [rows[b] for b in pick], nh)
+    _close(got[at], ref, tol * (1 + 8 / 64))
+
+
+def test_as_many_groups_as_sequences(ctx):  # noqa: F811
+    """4096 groups, two thousand of them of two sequences, the others empty."""
+    lens, start = [40 + i % 50 for i in range(4096)], np.repeat(np.arange(0, 4097, 2), 2)[:4097].tolist()
+    pages = [1] * 4096
+    c = _shared(ctx, F16, 1, 64, 32, lens, start, pages, 15)
+    q = np.random.default_rng(5).standard_normal((4096, 2, 64)).astype(np.float32)
+    got = _attend(c, q, 2, start, pages).reshape(4096, 2, 64)
+    pick = list(range(0, 4096, 73))
+    sub = SimpleNamespace(kv=c.kv, lens=[lens[b] for b in pick], hk=[c.hk[b] for b in pick], hv=[c.hv[b] for b in pick])
+    ref, tol, _ = _reference(sub, q[pick], None, 2)
+    _close(got[pick], ref, tol * (1 + 8 / 64))
 
 
 @pytest.mark.parametrize("t", TYPES)
