@@ -625,8 +625,9 @@ int kmoe_paged_attention_shared(kmoe_ctx *ctx, const kmoe_paged_desc *desc, cons
  * included; KMOE_Q8_0: quant * scale, rounded to the nearest f16 and kept finite). So a call
  * after every store keeps them up to date; they are formed anew from the page each
  * time, and do not depend on what was there. A NaN key is passed over. A page without an
- * entry in the table, and the others, are left as they were. Copies of pages need
- * copies of their bounds. */
+ * entry in the table, and the others, are left as they were; of a page that rows of two
+ * sequences of the batch lie on, either one's bounds stay. Copies of pages need copies of
+ * their bounds. bounds must not overlap the pages. */
 int kmoe_paged_bounds(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *pages_dev, const kmoe_paged_batch *batch,
                       uint16_t *bounds_dev);
 /* kmoe_paged_attention (without a window) over some of the pages, chosen for each row
@@ -635,11 +636,11 @@ int kmoe_paged_bounds(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *pa
  *   sum over the kv head's heads, sum over dims d of max(q_d lo_d, q_d hi_d)
  * by the pages' bounds, in 64 bits, equal ones by position; n_select pages in all (0 <=
  * n_first < n_select), all that there are where they are fewer. A page without an entry
- * in the table is not chosen. A NaN score counts as the best. No score of a position
- * passes its page's, summed over the heads; pages whose keys lie apart from the query's direction are not read. With
- * n_select >= table_cols it is kmoe_paged_attention itself. table_cols up to 2^20,
- * table_cols * n_kv up to 2^22 and n_pages * n_kv up to 2^31 - 1 (KMOE_E_UNSUPPORTED past them). Besides that call's workspace it keeps one of
- * 50 MB, with the same rules. */
+ * in the table is not chosen. A NaN score counts as the best. No position's scores, summed
+ * over the heads, pass its page's (but for the rounding of KMOE_Q8_0's bounds). With
+ * n_select >= table_cols it is kmoe_paged_attention itself. table_cols up to 2^20, table_cols * n_kv
+ * up to 2^22 and n_pages * n_kv up to 2^31 - 1 (KMOE_E_UNSUPPORTED past them). Besides that
+ * call's workspace it keeps one of 50 MB, with the same rules. */
 int kmoe_paged_attention_selected(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *pages_dev,
                                   const uint16_t *bounds_dev, const kmoe_paged_batch *batch, const float *q_dev,
                                   int32_t n_head, int32_t n_select, int32_t n_first, float *out_dev);
@@ -691,12 +692,13 @@ int kmoe_pages_length(const kmoe_pages *p, uint32_t seq, int64_t *n);
  * pages) and their lengths, host memory. */
 int kmoe_pages_table(kmoe_pages *p, const uint32_t *seqs, int32_t n_seq, int32_t table_cols, int32_t *table,
                      int32_t *seq_len);
-/* Groups for kmoe_paged_attention_shared among n_seq sequences, each named once: sequences
- * whose first pages are the same ones, so chosen that as few positions as can be are read more than once.
- * order [n_seq] receives the sequences' indexes, the groups' members one behind the other and the
- * sequences that are in none behind them; group i holds order[start[i]] .. order[start[i + 1] - 1]
- * (start [n_seq + 1]) and shares shared[i] pages (shared [n_seq]); *n_group groups. A
- * group is made where (members - 1) * shared positions come to `least` or more. */
+/* Groups for kmoe_paged_attention_shared among n_seq sequences (at most KMOE_PAGED_MAX_SEQ),
+ * each named once: sequences whose first pages are the same ones, so chosen that as few
+ * positions as can be are read more than once. order [n_seq] receives the sequences'
+ * indexes, the groups' members one behind the other and the sequences that are in none behind
+ * them; group i holds order[start[i]] .. order[start[i + 1] - 1] (start [n_seq + 1]) and
+ * shares shared[i] pages (shared [n_seq]); *n_group groups. A group is made where
+ * (members - 1) * shared positions come to `least` or more. */
 int kmoe_pages_groups(kmoe_pages *p, const uint32_t *seqs, int32_t n_seq, int64_t least, int32_t *order, int32_t *start,
                       int32_t *shared, int32_t *n_group);
 /* Moves the used pages to the front, the highest first, at most cap of them:

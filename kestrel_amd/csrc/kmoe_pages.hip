@@ -313,6 +313,7 @@ int kmoe_pages_groups(kmoe_pages *p, const uint32_t *seqs, int32_t n_seq, int64_
   if (!p) return KMOE_E_INVALID;
   if (n_seq < 0 || least < 0 || !n_group || !start || (n_seq > 0 && (!seqs || !order || !shared)))
     return pfail(p, KMOE_E_INVALID, "groups: bad size or null pointer");
+  if (n_seq > KMOE_PAGED_MAX_SEQ) return pfail(p, KMOE_E_INVALID, "groups: %d sequences (at most %d)", n_seq, KMOE_PAGED_MAX_SEQ);
   return guarded(p, [&]() -> int {
     std::vector<const Seq *> s(n_seq);
     std::vector<int32_t> by(n_seq);  // sequences with a common beginning lie beside each other

@@ -131,3 +131,14 @@ def test_refusals():
         bad[i] = None
         assert f(*bad) == -1
     assert f(p.h, None, -1, 1, None, x.ctypes.data, None, C.byref(n)) == -1
+
+
+def test_as_many_sequences_as_a_batch_takes():
+    p = kmoe.Pages(10, PAGE)
+    p.append(0, 2 * PAGE)
+    for i in range(1, 4097):
+        p.fork(0, i, 2 * PAGE)
+    order, start, shared = p.groups(range(4096))
+    assert start.tolist() == [0, 4096] and shared.tolist() == [2] and sorted(order.tolist()) == list(range(4096))
+    with pytest.raises(kmoe.KmoeError, match="at most 4096"):
+        p.groups(range(4097))
