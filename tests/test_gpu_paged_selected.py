@@ -182,6 +182,13 @@ def test_more_rows_than_a_launch_takes(ctx):  # noqa: F811
     _check(c, 4, 4, 1, [330, 0, 170])
 
 
+@pytest.mark.parametrize("lens,rows,extra", [([900, 60, 500], [800, 0, 300], 0), ([600, 40], [170, 1], 1 << 14), ([40 + i % 60 for i in range(1100)], None, 0)])
+def test_more_rows_than_a_choice_takes(ctx, lens, rows, extra):  # noqa: F811
+    """Over 4096 rows by kv heads, or 2^22 by the table's columns: several launches of the choice, too."""
+    c = Cache(ctx, F16, 4, 64, 32, lens, 8, extra_cols=extra)
+    _check(c, 4, 3, 1, rows)
+
+
 def test_more_kv_heads_than_rows_of_a_launch(ctx):  # noqa: F811
     """One row, and one chunk, of 1500 kv heads; contexts that two work-groups score."""
     c = Cache(ctx, F16, 1500, 64, 32, [32 * 4 + 3, 32 * 5], 6)
