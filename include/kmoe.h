@@ -609,11 +609,14 @@ int kmoe_paged_attention(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void 
  * result is kmoe_paged_attention's up to the last bits: a row's shared part and its own
  * are formed apart, in f32, and joined by their maxima and sums; rows that come out not finite
  * are formed again over their own table as there. s_rows * n_head is at most 2^21
- * (KMOE_E_UNSUPPORTED past it). Besides that call's workspace it keeps one of 17 MB, with the
- * same rules. */
+ * (KMOE_E_UNSUPPORTED past it). Forming the parts apart takes some microseconds: groups that
+ * would save less (few members or positions, rows that fill the matrix tiles anyway) are worked
+ * sequence by sequence, unless `always` is set. Besides that call's workspace it keeps one
+ * of 17 MB, with the same rules. */
 typedef struct {
   int32_t n_group; /* 0 .. KMOE_PAGED_MAX_SEQ */
   const int32_t *start_dev, *pages_dev;
+  int32_t always;
 } kmoe_paged_groups;
 int kmoe_paged_attention_shared(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *pages_dev,
                                 const kmoe_paged_batch *batch, const kmoe_paged_groups *groups, const float *q_dev,

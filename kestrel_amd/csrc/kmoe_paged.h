@@ -109,6 +109,10 @@ struct SharedArgs {
   int rows;  // launch_paged_attention_again's
   int32_t *skip;
   float *ml;
+  // whether a group is worth it, and all of them together: columns of a column tile when
+  // sequences are worked whole and when groups are; weight that is to be saved (0: always worth it)
+  int cols_whole, cols;
+  int64_t least;
 };
 
 hipError_t launch_paged_store(hipStream_t st, const PagedArgs &a, const float *q, int64_t q_stride, const float *k,
@@ -147,7 +151,7 @@ hipError_t launch_paged_attention_selected(hipStream_t st, const PagedArgs &a, c
                                            uint32_t *counters, uint8_t *ws, uint32_t *select_counters);
 // Rows by heads that ml holds.
 constexpr int64_t kSharedHeads = (int64_t)1 << 21;
-hipError_t launch_paged_attention_shared(hipStream_t st, const PagedArgs &a, const SharedArgs &sa, const float *q,
+hipError_t launch_paged_attention_shared(hipStream_t st, const PagedArgs &a, SharedArgs sa, bool always, const float *q,
                                          int n_head, float *out, float *part, uint32_t *counters);
 
 }  // namespace kmoe

@@ -232,9 +232,16 @@ __device__ __forceinline__ Span span_of(int64_t pos_lo, int64_t pos_hi, int64_t 
 // the sequences then (kOwn); or whole sequences that have pages in common (kAgain).
 enum { kWhole = 0, kShared = 1, kOwn = 2, kAgain = 3 };
 
-// Rows of group i together, its first sequence, and its positions in common.
-__device__ __forceinline__ void group_rows(const PagedArgs &a, const SharedArgs &s, int i, int &b0, int64_t &r0, int64_t &n,
-                                           int64_t &len) {
+// What a tile of 32 positions and 16, or 32, columns takes, one with the other (heads of 128,
+// F16: 0.65 ns a call's whole work, and 1.4).
+constexpr int kWeight16 = 5, kWeight32 = 11;
+__host__ __device__ __forceinline__ int tile_weight(int cols) { return cols == 16 ? kWeight16 : kWeight32; }
+
+// Rows of group i together, its first sequence, its positions in common, and the weight that
+// it saves per tile of those and kv head. Where that is not positive (rows that fill the
+// column tiles anyway), or there is but one sequence, nothing is in common.
+__device__ __forceinline__ int64_t group_rows(const PagedArgs &a, const SharedArgs &s, int i, int group, int &b0, int64_t &r0,
+                                              int64_t &n, int64_t &len) {
   int lo = s.start[i], hi = s.start[i + 1];
   lo = lo < 0 ? 0 : lo;
   hi = hi < 0 ? 0 : hi < a.n_seq ? hi : a.n_seq;
@@ -243,11 +250,17 @@ __device__ __forceinline__ void group_rows(const PagedArgs &a, const SharedArgs 
   len = (int64_t)pages * a.page;
   b0 = lo;
   r0 = n = 0;
-  if (hi - lo <= 1 || !pages) return;  // (one sequence alone has nothing in common)
+  if (hi - lo <= 1 || !pages) return 0;
   int64_t r1, m;
   paged_rows(a, lo, r0, n);
   paged_rows(a, hi - 1, r1, m);
   n = r1 + m > r0 ? r1 + m - r0 : 0;
+  if (!s.least) return 0;
+  auto tiles = [&](int cols) { return (n * group + cols - 1) / cols; };
+  const int64_t seqs = hi - lo < n ? hi - lo : n, full = tiles(s.cols_whole);  // (a sequence has a column tile at least)
+  const int64_t saved = (seqs > full ? seqs : full) * tile_weight(s.cols_whole) - tiles(s.cols) * tile_weight(s.cols);
+  if (saved <= 0) n = 0;
+  return saved > 0 ? saved : 0;
 }
 
 // How a call's work is shared out. A column tile is COLS columns: the sequence's
@@ -322,17 +335,18 @@ __device__ __forceinline__ int64_t scan(int64_t x, int64_t &total, int64_t *red)
 }
 
 // start[b] (b <= n, the sequences or groups): the line's tiles before sequence b; lens[b]: its length, kOwn:
-// lens[n + b]: the tiles of it that its group works.
+// lens[n + b]: the tiles of it that its group works. kShared: nothing at all where too little is saved.
 template <class SH, int MODE>
 __device__ void make_plan(const PagedArgs &a, const SharedArgs &sa, int n_seq, int group, int64_t cap, int window, int sink,
                           int64_t *start, int32_t *lens, int64_t *red) {
   const int per = (n_seq + 255) / 256, b0 = threadIdx.x * per;
+  int64_t saved = 0;
   auto space = [&](int b) -> int64_t {
     int64_t r0, n, len;
     int skip = 0;
     if constexpr (MODE == kShared) {
       int first;
-      group_rows(a, sa, b, first, r0, n, len);
+      saved += group_rows(a, sa, b, group, first, r0, n, len) * a.n_kv * (len / kTile);
     } else {
       paged_rows(a, b, r0, n);
       len = a.seq_len[b] > 0 ? a.seq_len[b] : 0;  // (a length below the rows leaves them nothing)
@@ -347,7 +361,8 @@ __device__ void make_plan(const PagedArgs &a, const SharedArgs &sa, int n_seq, i
     return (int64_t)s.units * a.n_kv * s.per;
   };
   if (n_seq == 1) {  // (no scan: 37 positions 9.3 -> 8.6 us)
-    const int64_t x = space(0);
+    int64_t x = space(0);
+    if (MODE == kShared && saved < sa.least) x = 0;
     if (threadIdx.x == 0) {
       start[0] = 0;
       start[1] = x;
@@ -358,6 +373,14 @@ __device__ void make_plan(const PagedArgs &a, const SharedArgs &sa, int n_seq, i
   int64_t sum = 0, total;
   for (int b = b0; b < b0 + per && b < n_seq; ++b) sum += space(b);
   int64_t at = scan(sum, total, red);
+  if constexpr (MODE == kShared) {
+    if (sa.least) {
+      int64_t all;
+      __syncthreads();  // (the first scan's sums are read)
+      scan(saved, all, red);
+      if (all < sa.least) total = 0;
+    }
+  }
   if (per == 1) {
     if (b0 < n_seq) start[b0] = at;
   } else {
@@ -464,7 +487,7 @@ struct Cursor {
       s.skip = 0;
       if constexpr (MODE == kShared) {
         int64_t r0, n, len;
-        group_rows(a, sa, b, s.b, r0, n, len);
+        group_rows(a, sa, b, group, s.b, r0, n, len);
         s.b = __builtin_amdgcn_readfirstlane(s.b);
         s.r0 = __builtin_amdgcn_readfirstlane((int)r0);
         s.n = __builtin_amdgcn_readfirstlane((int)n);

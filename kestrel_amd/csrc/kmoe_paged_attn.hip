@@ -101,8 +101,9 @@ constexpr int paged_occ(int hd, int c) { return hd == 64 ? (c == 1 ? 4 : 3) : (c
 template <int HD, int COLS>
 using Work = Shares<COLS, 4, (HD == 64 && COLS == 16 ? 12 : 8), 8, 24>;
 
-// sa.skip: what a sequence's group works of it, where all its rows lie behind that.
-__device__ void find_skip(const PagedArgs &a, const SharedArgs &sa) {
+// sa.skip: what a sequence's group works of it (any: whether groups work anything), where all its
+// rows lie behind that.
+__device__ void find_skip(const PagedArgs &a, const SharedArgs &sa, int group, bool any) {
   for (int b = threadIdx.x; b < a.n_seq; b += 256) {
     int lo = 0;  // the last group that starts at or before b
     for (int hi = sa.n_group; hi - lo > 1;) {
@@ -112,9 +113,9 @@ __device__ void find_skip(const PagedArgs &a, const SharedArgs &sa) {
     }
     int b0;
     int64_t r0, n, len, at, m;
-    group_rows(a, sa, lo, b0, r0, n, len);
+    group_rows(a, sa, lo, group, b0, r0, n, len);
     paged_rows(a, b, at, m);
-    const bool in = sa.start[lo] <= b && b < sa.start[lo + 1] && m > 0 && at >= r0 && at + m <= r0 + n;
+    const bool in = any && sa.start[lo] <= b && b < sa.start[lo + 1] && m > 0 && at >= r0 && at + m <= r0 + n;
     sa.skip[b] = in && (int64_t)a.seq_len[b] - m >= len ? (int)(len / kTile) : 0;
   }
 }
@@ -158,10 +159,10 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
   const int group = nh / a.n_kv, magic = 65536 / group + 1;  // x / group = x * magic >> 16 for x < 4096
   const int64_t bb = paged_block_bytes(T, a.page, HD);
   const int pshift = __builtin_ctz(a.page);
-  if constexpr (MODE == kShared)
-    if (blockIdx.x == gridDim.x - 1) find_skip(a, sa);
   Cursor<Work<HD, COLS>, MODE> cur(a, sa, nh, window, sink, start,
                                    (int32_t *)(start + (MODE == kShared ? sa.n_group : a.n_seq) + 1), red);
+  if constexpr (MODE == kShared)
+    if (blockIdx.x == gridDim.x - 1) find_skip(a, sa, group, start[sa.n_group] > 0);
   const int64_t cap = cur.cap;
 
   // wave 3 finds the next segment while this one's first loads are on their way (all
@@ -643,16 +644,19 @@ size_t paged_part_floats() {
 }
 int paged_counters() { return paged_grid(64, 1); }
 
+// 16 columns per tile where sequences have few rows: at 32 columns each 36 us with
+// 16, 23 with 32 (16 sequences of 2000 positions, Q8_0, heads of 64); decode steps
+// of 8 heads would leave three quarters of 32 idle
+static int columns(const PagedArgs &a, int group, int n_seq) { return a.s_rows * group <= (int64_t)24 * n_seq ? 16 : 32; }
+
 // sa: of a launch over groups, or over what they leave (MODE).
 template <int MODE>
 static hipError_t launch_mode(hipStream_t st, const PagedArgs &a, const SharedArgs &sa, const float *q, int n_head, int w,
                               int sink, float *out, float *part, uint32_t *counters) {
   const int group = n_head / a.n_kv, n_seq = MODE == kShared ? sa.n_group : a.n_seq;
-  // 16 columns per tile where sequences have few rows: at 32 columns each 36 us with
-  // 16, 23 with 32 (16 sequences of 2000 positions, Q8_0, heads of 64); decode steps
-  // of 8 heads would leave three quarters of 32 idle
-  const bool one = a.s_rows * group <= (int64_t)24 * n_seq;
-  const int cols = one ? 16 : 32, full = paged_grid(a.hd, one ? 1 : 2);
+  const int cols = columns(a, group, n_seq);
+  const bool one = cols == 16;
+  const int full = paged_grid(a.hd, one ? 1 : 2);
   // no more work-groups than the longest sequences that the table allows would fill
   const int64_t units = (a.s_rows * group / cols + n_seq) * a.n_kv;
   const int cost = one && a.hd == 64 ? Work<64, 16>::cost : Work<128, 16>::cost;
@@ -692,8 +696,26 @@ hipError_t launch_paged_attention_again(hipStream_t st, const PagedArgs &a, int 
   return launch_mode<kAgain>(st, a, sa, q, n_head, 0, 0, out, part, counters);
 }
 
-hipError_t launch_paged_attention_shared(hipStream_t st, const PagedArgs &a, const SharedArgs &sa, const float *q,
+// Two launches and two parts of every row cost 12 us that must be saved: 10000 tiles of 16 columns
+// TODO measured. Where not even sequences that share all of the table would save as much,
+// the batch is worked whole at once.
+constexpr int64_t kLeastSaved = 10000 * kWeight16;
+
+hipError_t launch_paged_attention_shared(hipStream_t st, const PagedArgs &a, SharedArgs sa, bool always, const float *q,
                                          int n_head, float *out, float *part, uint32_t *counters) {
+  const int group = n_head / a.n_kv;
+  sa.cols_whole = columns(a, group, a.n_seq);
+  sa.cols = columns(a, group, sa.n_group);
+  sa.least = always ? 0 : kLeastSaved;
+  if (!always) {
+    // per sequence, a column tile against its rows' part of one; per row that fills its column
+    // tiles, one part against the other; a column tile's rest per group
+    const int ww = tile_weight(sa.cols_whole), ws = tile_weight(sa.cols), n_seq = a.n_seq, n_group = std::min(sa.n_group, a.n_seq);
+    const int64_t few = (int64_t)n_seq * std::max(0, ww * sa.cols - ws * group) / sa.cols;
+    const int64_t many = a.s_rows * group * std::max(0, ww * sa.cols - ws * sa.cols_whole) / (sa.cols * sa.cols_whole) + (int64_t)n_group * ww;
+    if (std::max(few, many) * a.n_kv * ((int64_t)a.table_cols * a.page / kTile) < sa.least)
+      return launch_paged_attention(st, a, q, n_head, 0, 0, out, part, counters);
+  }
   const hipError_t e = launch_mode<kShared>(st, a, sa, q, n_head, 0, 0, out, part, counters);
   return e == hipSuccess ? launch_mode<kOwn>(st, a, sa, q, n_head, 0, 0, out, part, counters) : e;
 }

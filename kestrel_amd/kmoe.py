@@ -174,7 +174,7 @@ class PagedBatch(C.Structure):
 class PagedGroups(C.Structure):
     """kmoe_paged_groups (include/kmoe.h), with the tensors it points into."""
 
-    _fields_ = [("n_group", _i32), ("start", _P), ("pages", _P)]
+    _fields_ = [("n_group", _i32), ("start", _P), ("pages", _P), ("always", _i32)]
 
 
 @dataclass(frozen=True)
@@ -478,13 +478,14 @@ class Context:
                                                  n_head, window, n_sink, _ptr(out)))
         return out
 
-    def paged_groups(self, start, pages) -> PagedGroups:
+    def paged_groups(self, start, pages, always: bool = False) -> PagedGroups:
         """kmoe_paged_groups: sequences start[i] .. start[i + 1] - 1 of a batch share the first pages[i] pages; int32 on
-        the device (start [n + 1], pages [n]), read when a call's kernels run. The struct keeps them alive."""
+        the device (start [n + 1], pages [n]), read when a call's kernels run. The struct keeps them alive. always: read
+        them once even where reading them again would be quicker."""
         i32, n = self.torch.int32, pages.numel()
         self._need("pages", pages, i32, 1, n)
         self._need("start", start, i32, 1, n + 1)
-        g = PagedGroups(n, _ptr(start), _ptr(pages) or None)
+        g = PagedGroups(n, _ptr(start), _ptr(pages) or None, always)
         g.keep = (start, pages)
         return g
 

@@ -32,7 +32,7 @@ def _shared(ctx, t, nkv, hd, page, lens, start, pages, seed, **kw):  # noqa: F81
 def _attend(c, q, nh, start, pages, rows=None, out=None, batch=None):
     import torch
 
-    g = c.ctx.paged_groups(_dev(start, np.int32), _dev(pages, np.int32))
+    g = c.ctx.paged_groups(_dev(start, np.int32), _dev(pages, np.int32), always=True)
     o = c.ctx.paged_attention_shared(c.kv, c.pages, batch or c.batch(rows), g, _dev(q.reshape(len(q), -1)), nh, out=out)
     torch.cuda.synchronize()
     return o.cpu().numpy()
@@ -227,7 +227,7 @@ def test_captured_calls_follow_the_arrays(ctx):  # noqa: F811
     table, lens = torch.full((4, cols), -1, dtype=torch.int32, device="cuda"), torch.ones(4, dtype=torch.int32, device="cuda")
     start, shared = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
     dq, out = _dev(q.reshape(4, -1)), torch.empty((4, 1024), device="cuda")
-    batch, groups = ctx.paged_batch(table, lens), ctx.paged_groups(start, shared)
+    batch, groups = ctx.paged_batch(table, lens), ctx.paged_groups(start, shared, always=True)
     ctx.paged_attention_shared(cs[0].kv, pages, batch, groups, dq, 8, out=out)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
@@ -257,7 +257,7 @@ def test_streams_take_turns(ctx):  # noqa: F811
 
     lens, start, pages = [2000 + i for i in range(8)], [0, 8], [60]
     c = _shared(ctx, F16, 2, 128, 32, lens, start, pages, 12)
-    g, q = ctx.paged_groups(_dev(start, np.int32), _dev(pages, np.int32)), _dev(np.random.default_rng(4).standard_normal((2, 8, 1024)))
+    g, q = ctx.paged_groups(_dev(start, np.int32), _dev(pages, np.int32), always=True), _dev(np.random.default_rng(4).standard_normal((2, 8, 1024)))
     qs, b = [x.float().contiguous() for x in q], c.batch()
     want = [ctx.paged_attention_shared(c.kv, c.pages, b, g, x, 8).clone() for x in qs]
     torch.cuda.synchronize()
