@@ -2722,16 +2722,11 @@ int kmoe_paged_attention_shared(kmoe_ctx *c, const kmoe_paged_desc *d, const voi
   DeviceGuard g(c->device);
   uint8_t *part = nullptr, *ml = nullptr;
   rc = kept_ws(c, c->paged, paged_part_floats() * sizeof(float), "paged attention partials", &part);
-  if (!rc) rc = kept_ws(c, c->shared, kSharedHeads * 8 + KMOE_PAGED_MAX_SEQ * 4, "shared parts of rows", &ml);
+  if (!rc) rc = kept_ws(c, c->shared, shared_ws_bytes(), "shared parts of rows", &ml);
   if (rc) return rc;
-  SharedArgs sa{};
-  sa.start = groups->start_dev;
-  sa.pages = groups->pages_dev;
-  sa.n_group = groups->n_group;
-  sa.skip = (int32_t *)(ml + kSharedHeads * 8);
-  sa.ml = (float *)ml;
-  LAUNCH(c, "paged_attention_shared", launch_paged_attention_shared(c->stream, a, sa, groups->always != 0, q, n_head, out,
-                                                                    (float *)part, c->counters + kCounterWords));
+  LAUNCH(c, "paged_attention_shared",
+         launch_paged_attention_shared(c->stream, a, groups->start_dev, groups->pages_dev, groups->n_group, groups->always != 0,
+                                       q, n_head, out, (float *)part, c->counters + kCounterWords, ml));
   return KMOE_OK;
 }
 

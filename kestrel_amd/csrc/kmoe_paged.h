@@ -100,18 +100,20 @@ __device__ __forceinline__ uint8_t *paged_block(const PagedArgs &a, int64_t bloc
 hipError_t launch_paged_attention_again(hipStream_t st, const PagedArgs &a, int rows, const float *q, int n_head, float *out,
                                         float *part, uint32_t *counters);
 // Sequences with pages in common (kmoe_paged_groups): group i holds sequences start[i] ..
-// start[i + 1] - 1 and the first pages[i] columns of its first one's table. skip: tiles
-// of 32 positions that a sequence leaves to its group; ml: maximum and sum of the weights
-// of what the group's positions give a row's head, whose weighted mean stands in out.
+// start[i + 1] - 1 and the first pages[i] columns of its first one's table. ml: maximum and
+// sum of the weights of what the group's positions give a row's head, whose weighted mean
+// stands in out; plan, lens: how what is left is shared out, for the launch that works it.
 struct SharedArgs {
   const int32_t *start, *pages;
   int n_group;
   int rows;  // launch_paged_attention_again's
-  int32_t *skip;
   float *ml;
-  // whether a group is worth it, and all of them together: columns of a column tile when
-  // sequences are worked whole and when groups are; weight that is to be saved (0: always worth it)
-  int cols_whole, cols;
+  int64_t *plan;
+  int32_t *lens;
+  // whether a group is worth it, and all of them together: columns of a column tile (log 2)
+  // when sequences are worked whole and when groups are; weight that is to be saved (0: always
+  // worth it)
+  int log_whole, log_cols;
   int64_t least;
 };
 
@@ -149,9 +151,11 @@ hipError_t launch_paged_bounds(hipStream_t st, const PagedArgs &a, uint16_t *bou
 hipError_t launch_paged_attention_selected(hipStream_t st, const PagedArgs &a, const uint16_t *bounds, const float *q,
                                            int n_head, int n_select, int n_first, float *out, float *part,
                                            uint32_t *counters, uint8_t *ws, uint32_t *select_counters);
-// Rows by heads that ml holds.
+// Rows by heads that ml holds, for kmoe_paged_attention_shared.
 constexpr int64_t kSharedHeads = (int64_t)1 << 21;
-hipError_t launch_paged_attention_shared(hipStream_t st, const PagedArgs &a, SharedArgs sa, bool always, const float *q,
-                                         int n_head, float *out, float *part, uint32_t *counters);
+size_t shared_ws_bytes();
+hipError_t launch_paged_attention_shared(hipStream_t st, const PagedArgs &a, const int32_t *start, const int32_t *pages,
+                                         int n_group, bool always, const float *q, int n_head, float *out, float *part,
+                                         uint32_t *counters, uint8_t *ws);
 
 }  // namespace kmoe

@@ -231,11 +231,13 @@ __device__ __forceinline__ Span span_of(int64_t pos_lo, int64_t pos_hi, int64_t 
 // (kShared: a group counts as a sequence, all its rows see all of it); or what is left of
 // the sequences then (kOwn); or whole sequences that have pages in common (kAgain).
 enum { kWhole = 0, kShared = 1, kOwn = 2, kAgain = 3 };
+constexpr int kPlanners = 8;  // work-groups of kShared that work no tiles (one plans kOwn's): the others stay whole eights
 
-// What a tile of 32 positions and 16, or 32, columns takes, one with the other (heads of 128,
-// F16: 0.65 ns a call's whole work, and 1.4).
+// What a tile of 32 positions takes with 16 columns, and with 32, one against the other: the whole
+// chip's time by the number of tiles, each kind as many at once as its registers allow (heads of
+// 128, F16, 40000 of 16: 0.65 ns; 20000 of 32: 1.4).
 constexpr int kWeight16 = 5, kWeight32 = 11;
-__host__ __device__ __forceinline__ int tile_weight(int cols) { return cols == 16 ? kWeight16 : kWeight32; }
+__host__ __device__ __forceinline__ int tile_weight(int log_cols) { return log_cols == 4 ? kWeight16 : kWeight32; }
 
 // Rows of group i together, its first sequence, its positions in common, and the weight that
 // it saves per tile of those and kv head. Where that is not positive (rows that fill the
@@ -256,9 +258,9 @@ __device__ __forceinline__ int64_t group_rows(const PagedArgs &a, const SharedAr
   paged_rows(a, hi - 1, r1, m);
   n = r1 + m > r0 ? r1 + m - r0 : 0;
   if (!s.least) return 0;
-  auto tiles = [&](int cols) { return (n * group + cols - 1) / cols; };
-  const int64_t seqs = hi - lo < n ? hi - lo : n, full = tiles(s.cols_whole);  // (a sequence has a column tile at least)
-  const int64_t saved = (seqs > full ? seqs : full) * tile_weight(s.cols_whole) - tiles(s.cols) * tile_weight(s.cols);
+  auto tiles = [&](int log) { return ((int)n * group + (1 << log) - 1) >> log; };
+  const int seqs = hi - lo < (int)n ? hi - lo : (int)n, full = tiles(s.log_whole);  // (a sequence has a column tile at least)
+  const int saved = (seqs > full ? seqs : full) * tile_weight(s.log_whole) - tiles(s.log_cols) * tile_weight(s.log_cols);
   if (saved <= 0) n = 0;
   return saved > 0 ? saved : 0;
 }
@@ -334,11 +336,28 @@ __device__ __forceinline__ int64_t scan(int64_t x, int64_t &total, int64_t *red)
   return x;
 }
 
+// The tiles that sequence b's group works of it, where all its rows lie behind that.
+__device__ __forceinline__ int skip_of(const PagedArgs &a, const SharedArgs &sa, int group, int b) {
+  int lo = 0;  // the last group that starts at or before b
+  for (int hi = sa.n_group; hi - lo > 1;) {
+    const int mid = (lo + hi) >> 1;
+    if (sa.start[mid] <= b) lo = mid;
+    else hi = mid;
+  }
+  int b0;
+  int64_t r0, n, len, at, m;
+  group_rows(a, sa, lo, group, b0, r0, n, len);
+  paged_rows(a, b, at, m);
+  const bool in = sa.start[lo] <= b && b < sa.start[lo + 1] && m > 0 && at >= r0 && at + m <= r0 + n;
+  return in && (int64_t)a.seq_len[b] - m >= len ? (int)(len / kTile) : 0;
+}
+
 // start[b] (b <= n, the sequences or groups): the line's tiles before sequence b; lens[b]: its length, kOwn:
-// lens[n + b]: the tiles of it that its group works. kShared: nothing at all where too little is saved.
+// lens[n + b]: the tiles of it that its group works (any: whether groups work anything).
+// kShared: nothing at all where too little is saved.
 template <class SH, int MODE>
 __device__ void make_plan(const PagedArgs &a, const SharedArgs &sa, int n_seq, int group, int64_t cap, int window, int sink,
-                          int64_t *start, int32_t *lens, int64_t *red) {
+                          int64_t *start, int32_t *lens, int64_t *red, bool any = true) {
   const int per = (n_seq + 255) / 256, b0 = threadIdx.x * per;
   int64_t saved = 0;
   auto space = [&](int b) -> int64_t {
@@ -352,7 +371,7 @@ __device__ void make_plan(const PagedArgs &a, const SharedArgs &sa, int n_seq, i
       len = a.seq_len[b] > 0 ? a.seq_len[b] : 0;  // (a length below the rows leaves them nothing)
       if constexpr (MODE == kAgain) n = a.seq_len[b] >= 0;
       if constexpr (MODE == kOwn) {
-        skip = sa.skip[b];
+        skip = any ? skip_of(a, sa, group, b) : 0;
         lens[n_seq + b] = skip;
       }
     }
@@ -434,7 +453,7 @@ struct Cursor {
   const SharedArgs &sa;
   const int64_t *start;
   const int32_t *lens;
-  int n_seq, group, window, sink, rank, b;
+  int n_seq, group, window, sink, wgs, rank, b;
   int64_t cap, share, x0, x1, x;
 
   // This work-group's stretch; neighbours in the line share an XCD's L2.
@@ -442,10 +461,23 @@ struct Cursor {
                                     int64_t *start_, int32_t *lens_, int64_t *red)
       : a(a_), sa(sa_), start(start_), lens(lens_), n_seq(MODE == kShared ? sa_.n_group : a_.n_seq), group(nh / a_.n_kv),
         window(window_), sink(sink_), cap((int64_t)a_.table_cols * a_.page) {
-    make_plan<SH, MODE>(a, sa, n_seq, group, cap, window, sink, start_, lens_, red);
+    if constexpr (MODE == kOwn) {  // (a work-group of the launch before has made the plan: 64 rows behind 6000 positions 61 -> 57 us)
+      for (int b = threadIdx.x; b < n_seq; b += 256) {
+        const int64_t at = sa.plan[b];
+        const int32_t len = sa.lens[b], skip = sa.lens[n_seq + b];
+        start_[b] = at;
+        lens_[b] = len;
+        lens_[n_seq + b] = skip;
+      }
+      if (threadIdx.x == 0) start_[n_seq] = sa.plan[n_seq];
+      __syncthreads();
+    } else {
+      make_plan<SH, MODE>(a, sa, n_seq, group, cap, window, sink, start_, lens_, red);
+    }
     const int64_t total = uniform64(start[n_seq]);
-    rank = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
-    share = div64(total + gridDim.x - 1, gridDim.x);
+    wgs = (int)gridDim.x - (MODE == kShared ? kPlanners : 0);
+    rank = (int)(blockIdx.x & 7) * (wgs >> 3) + (int)(blockIdx.x >> 3);
+    share = div64(total + wgs - 1, wgs);
     share = share < SH::least ? SH::least : share < 4 * SH::STEP ? SH::up((int)share) : share;
     // One sequence: whole units where they fill the work-groups about as well, a join
     // and the segments besides cost more than these tiles (1777 rows, 16 heads: 64 ->
@@ -461,8 +493,8 @@ struct Cursor {
         const int parts = p.per / SH::least;
         if (parts) share = SH::up((p.per + parts - 1) / parts);
       } else {
-        const int64_t each = div64(units + gridDim.x - 1, gridDim.x) * p.per;
-        if (2 * units >= gridDim.x && each <= share + SH::whole) share = each;
+        const int64_t each = div64(units + wgs - 1, wgs) * p.per;
+        if (2 * units >= wgs && each <= share + SH::whole) share = each;
       }
     }
     x0 = rank * share;

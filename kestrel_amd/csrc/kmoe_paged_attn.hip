@@ -101,25 +101,6 @@ constexpr int paged_occ(int hd, int c) { return hd == 64 ? (c == 1 ? 4 : 3) : (c
 template <int HD, int COLS>
 using Work = Shares<COLS, 4, (HD == 64 && COLS == 16 ? 12 : 8), 8, 24>;
 
-// sa.skip: what a sequence's group works of it (any: whether groups work anything), where all its
-// rows lie behind that.
-__device__ void find_skip(const PagedArgs &a, const SharedArgs &sa, int group, bool any) {
-  for (int b = threadIdx.x; b < a.n_seq; b += 256) {
-    int lo = 0;  // the last group that starts at or before b
-    for (int hi = sa.n_group; hi - lo > 1;) {
-      const int mid = (lo + hi) >> 1;
-      if (sa.start[mid] <= b) lo = mid;
-      else hi = mid;
-    }
-    int b0;
-    int64_t r0, n, len, at, m;
-    group_rows(a, sa, lo, group, b0, r0, n, len);
-    paged_rows(a, b, at, m);
-    const bool in = any && sa.start[lo] <= b && b < sa.start[lo + 1] && m > 0 && at >= r0 && at + m <= r0 + n;
-    sa.skip[b] = in && (int64_t)a.seq_len[b] - m >= len ? (int)(len / kTile) : 0;
-  }
-}
-
 // Work-group: four waves, one segment of a column tile at a time; wave w takes
 // its tiles w, w + 4, ... (32 positions each) with its own running softmax, and
 // the waves are merged through LDS.
@@ -159,10 +140,16 @@ __global__ void __launch_bounds__(256, paged_occ(HD, C))
   const int group = nh / a.n_kv, magic = 65536 / group + 1;  // x / group = x * magic >> 16 for x < 4096
   const int64_t bb = paged_block_bytes(T, a.page, HD);
   const int pshift = __builtin_ctz(a.page);
+  if (MODE == kShared && blockIdx.x >= gridDim.x - kPlanners + 1) return;
   Cursor<Work<HD, COLS>, MODE> cur(a, sa, nh, window, sink, start,
                                    (int32_t *)(start + (MODE == kShared ? sa.n_group : a.n_seq) + 1), red);
   if constexpr (MODE == kShared)
-    if (blockIdx.x == gridDim.x - 1) find_skip(a, sa, group, start[sa.n_group] > 0);
+    if (blockIdx.x == gridDim.x - kPlanners) {
+      const bool any = start[sa.n_group] > 0;
+      if (sa.log_whole == 4) make_plan<Work<HD, 16>, kOwn>(a, sa, a.n_seq, group, cur.cap, 0, 0, sa.plan, sa.lens, red, any);
+      else make_plan<Work<HD, 32>, kOwn>(a, sa, a.n_seq, group, cur.cap, 0, 0, sa.plan, sa.lens, red, any);
+      return;
+    }
   const int64_t cap = cur.cap;
 
   // wave 3 finds the next segment while this one's first loads are on their way (all
@@ -647,21 +634,21 @@ int paged_counters() { return paged_grid(64, 1); }
 // 16 columns per tile where sequences have few rows: at 32 columns each 36 us with
 // 16, 23 with 32 (16 sequences of 2000 positions, Q8_0, heads of 64); decode steps
 // of 8 heads would leave three quarters of 32 idle
-static int columns(const PagedArgs &a, int group, int n_seq) { return a.s_rows * group <= (int64_t)24 * n_seq ? 16 : 32; }
+static int log_columns(const PagedArgs &a, int group, int n_seq) { return a.s_rows * group <= (int64_t)24 * n_seq ? 4 : 5; }
 
 // sa: of a launch over groups, or over what they leave (MODE).
 template <int MODE>
 static hipError_t launch_mode(hipStream_t st, const PagedArgs &a, const SharedArgs &sa, const float *q, int n_head, int w,
                               int sink, float *out, float *part, uint32_t *counters) {
   const int group = n_head / a.n_kv, n_seq = MODE == kShared ? sa.n_group : a.n_seq;
-  const int cols = columns(a, group, n_seq);
+  const int cols = 1 << log_columns(a, group, n_seq);
   const bool one = cols == 16;
   const int full = paged_grid(a.hd, one ? 1 : 2);
   // no more work-groups than the longest sequences that the table allows would fill
   const int64_t units = (a.s_rows * group / cols + n_seq) * a.n_kv;
   const int cost = one && a.hd == 64 ? Work<64, 16>::cost : Work<128, 16>::cost;
   const int64_t most = units * (((int64_t)a.table_cols * a.page / kTile + cost) / Work<64, 16>::least + 2);
-  const unsigned grid = (unsigned)std::min<int64_t>(full, (most + 7) / 8 * 8);
+  const unsigned grid = (unsigned)std::min<int64_t>(full, (most + 7) / 8 * 8 + (MODE == kShared ? kPlanners : 0));
   const size_t lds = (size_t)(n_seq + 1) * 8 + (size_t)n_seq * (MODE == kOwn ? 8 : 4);
   float *ml = part + (size_t)2 * full * cols * a.hd;
 #define KMOE_PAGED(T, H, C) \
@@ -696,24 +683,39 @@ hipError_t launch_paged_attention_again(hipStream_t st, const PagedArgs &a, int 
   return launch_mode<kAgain>(st, a, sa, q, n_head, 0, 0, out, part, counters);
 }
 
-// Two launches and two parts of every row cost 12 us that must be saved: 10000 tiles of 16 columns
-// TODO measured. Where not even sequences that share all of the table would save as much,
-// the batch is worked whole at once.
-constexpr int64_t kLeastSaved = 10000 * kWeight16;
+// Two launches and two parts of every row take 8 .. 12 us more: as much as 10000 tiles of 16 columns
+// of 128 dims, or 20000 of 64, that are not worked. (8 .. 64 sequences behind what they share, F16,
+// heads of 128, whole | shared: 6000 tiles saved 24 .. 31 | 27 .. 43 us, 12000 32 .. 50 | 32 .. 46, 24000
+// 60 .. 85 | 36 .. 45; heads of 64, Q8_0: 14000 24 .. 26 | 28 .. 29, 28000 33 .. 36 | 29 .. 37, 56000
+// 53 | 35 .. 39.) Where not even sequences that have all of the table in common would save as
+// much, the batch is worked whole at once. The launch that finds out what is saved takes 5 us
+// of that (288 rows, 18000 tiles of 64 saved: whole 53, found out to be whole 57, shared 52).
+static int64_t tiles_saved(int64_t tiles, int hd) { return tiles * kWeight16 * (128 / hd); }
+constexpr int64_t kWorthLaunch = 10000, kWorthSharing = 7000;
 
-hipError_t launch_paged_attention_shared(hipStream_t st, const PagedArgs &a, SharedArgs sa, bool always, const float *q,
-                                         int n_head, float *out, float *part, uint32_t *counters) {
+size_t shared_ws_bytes() { return kSharedHeads * 8 + (4096 + 1) * 8 + 2 * 4096 * 4; }
+
+hipError_t launch_paged_attention_shared(hipStream_t st, const PagedArgs &a, const int32_t *start, const int32_t *pages,
+                                         int n_group, bool always, const float *q, int n_head, float *out, float *part,
+                                         uint32_t *counters, uint8_t *ws) {
   const int group = n_head / a.n_kv;
-  sa.cols_whole = columns(a, group, a.n_seq);
-  sa.cols = columns(a, group, sa.n_group);
-  sa.least = always ? 0 : kLeastSaved;
+  SharedArgs sa{};
+  sa.start = start;
+  sa.pages = pages;
+  sa.n_group = n_group;
+  sa.ml = (float *)ws;
+  sa.plan = (int64_t *)(ws + kSharedHeads * 8);
+  sa.lens = (int32_t *)(sa.plan + 4096 + 1);
+  sa.log_whole = log_columns(a, group, a.n_seq);
+  sa.log_cols = log_columns(a, group, n_group);
+  sa.least = always ? 0 : tiles_saved(kWorthSharing, a.hd);
   if (!always) {
     // per sequence, a column tile against its rows' part of one; per row that fills its column
     // tiles, one part against the other; a column tile's rest per group
-    const int ww = tile_weight(sa.cols_whole), ws = tile_weight(sa.cols), n_seq = a.n_seq, n_group = std::min(sa.n_group, a.n_seq);
-    const int64_t few = (int64_t)n_seq * std::max(0, ww * sa.cols - ws * group) / sa.cols;
-    const int64_t many = a.s_rows * group * std::max(0, ww * sa.cols - ws * sa.cols_whole) / (sa.cols * sa.cols_whole) + (int64_t)n_group * ww;
-    if (std::max(few, many) * a.n_kv * ((int64_t)a.table_cols * a.page / kTile) < sa.least)
+    const int cw = 1 << sa.log_whole, cs = 1 << sa.log_cols, ww = tile_weight(sa.log_whole), ws_ = tile_weight(sa.log_cols);
+    const int64_t few = (int64_t)a.n_seq * std::max(0, ww * cs - ws_ * group) / cs;
+    const int64_t many = a.s_rows * group * std::max(0, ww * cs - ws_ * cw) / (cs * cw) + (int64_t)std::min(n_group, a.n_seq) * ww;
+    if (std::max(few, many) * a.n_kv * ((int64_t)a.table_cols * a.page / kTile) < tiles_saved(kWorthLaunch, a.hd))
       return launch_paged_attention(st, a, q, n_head, 0, 0, out, part, counters);
   }
   const hipError_t e = launch_mode<kShared>(st, a, sa, q, n_head, 0, 0, out, part, counters);

@@ -382,7 +382,10 @@ class PagedDecoder(Decoder):
     select_first and those whose bounds promise the largest scores; other calls go over
     all. Neither goes with a window, nor with the other."""
 
-    SHARE_LEAST = 512  # positions read again (members less one, times those in common) from which a group is made
+    # positions by kv heads and dims that would be read again (members less one, times those in common) from which a
+    # group is made, with up to four heads a kv head: the 8 .. 12 us a layer that reading them once takes more (measured
+    # for 32 heads over 8 of 128: 45000 positions; 16 over 4: 100000; 16 over 8 of 64, Q8_0: 110000; 32 over 4: 190000)
+    SHARE_LEAST = 45000 * 8 * 128
 
     def __init__(self, ctx: Context, hp: dict, tensors: dict, n_pages: int, page: int = 64, kv_type: int = F16,
                  window: int = 0, n_sink: int = 0, layer_base: int = 1000, share_prefixes: bool = False, select: int = 0,
@@ -558,7 +561,7 @@ class PagedDecoder(Decoder):
         they share; None where nothing is worth sharing (or the call's rows are too many for it)."""
         if not self.share_prefixes or len(seqs) < 2 or rows * self.nh > 1 << 21:
             return None
-        order, start, shared = self.account.groups(seqs, self.SHARE_LEAST)
+        order, start, shared = self.account.groups(seqs, self.SHARE_LEAST * max(4, self.nh // self.nkv) // (4 * self.nkv * self.hd))
         return (order.tolist(), start, shared) if len(shared) else None
 
     def _parts(self, rows: dict):
@@ -598,7 +601,8 @@ class PagedDecoder(Decoder):
                 batch = self._batch([p[0] for p in part], [(had[s] or 0) + j for s, _, j in part], counts)
                 batch.steps = steps
                 if groups:
-                    batch.groups = self.ctx.paged_groups(*(self.torch.from_numpy(g.copy()).to(self.dev) for g in groups[1:]))
+                    batch.groups = self.ctx.paged_groups(*(self.torch.from_numpy(g.copy()).to(self.dev) for g in groups[1:]),
+                                                         always=True)
                 x, f = self._rows(x, batch)
                 end = dict(zip([p[0] for p in part], np.cumsum(counts).tolist()))
                 last = [end[s] - 1 for s in done]
@@ -638,7 +642,7 @@ class PagedDecoder(Decoder):
                  "start": torch.empty(n // 2 + 2, **i32), "shared": torch.empty(n // 2 + 1, **i32)}
             b["batch"] = self.ctx.paged_batch(b["table"], b["len"])
             b["batch"].steps = True
-            b["groups"] = self.ctx.paged_groups(b["start"], b["shared"])
+            b["groups"] = self.ctx.paged_groups(b["start"], b["shared"], always=True)
             self._graph_bufs, self._graph_n, self._graphs = b, n, {}
         return b
 

@@ -29,10 +29,10 @@ def _shared(ctx, t, nkv, hd, page, lens, start, pages, seed, **kw):  # noqa: F81
     return c
 
 
-def _attend(c, q, nh, start, pages, rows=None, out=None, batch=None):
+def _attend(c, q, nh, start, pages, rows=None, out=None, batch=None, always=True):
     import torch
 
-    g = c.ctx.paged_groups(_dev(start, np.int32), _dev(pages, np.int32), always=True)
+    g = c.ctx.paged_groups(_dev(start, np.int32), _dev(pages, np.int32), always=always)
     o = c.ctx.paged_attention_shared(c.kv, c.pages, batch or c.batch(rows), g, _dev(q.reshape(len(q), -1)), nh, out=out)
     torch.cuda.synchronize()
     return o.cpu().numpy()
@@ -200,6 +200,25 @@ def test_not_finite(ctx, t, what):  # noqa: F811
     assert np.array_equal(np.isnan(want), np.isnan(got)) and np.array_equal(np.isinf(want), np.isinf(got))
     f = np.isfinite(want)
     assert np.abs(want[f] - got[f]).max(initial=0) <= 2e-6 and np.isfinite(got[3]).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("hd,shared", [(128, 48), (64, 96)])
+def test_groups_are_read_once_where_that_saves_enough(ctx, t, hd, shared):  # noqa: F811
+    """Besides groups that are not worth it, and batches of them alone; without `always`."""
+    lens = [shared * 32 + 1 + i % 40 for i in range(48)] + [40, 50, 60, 1500]
+    for start, pages in (([0, 48, 51], [shared, 1]), ([48, 51], [1]), ([0, 2, 51], [1, 1]), ([0, 0, 48], [shared, shared])):
+        c = _shared(ctx, t, 8, hd, 32, lens, start, pages, 16)
+        q = np.random.default_rng(6).standard_normal((len(lens), 16, hd)).astype(np.float32)
+        g = _attend(c, q, 16, start, pages, always=False)
+        pick = [0, 1, 30, 47, 48, 50, 51]
+        sub = SimpleNamespace(kv=c.kv, lens=[lens[b] for b in pick], hk=[c.hk[b] for b in pick], hv=[c.hv[b] for b in pick])
+        ref, tol, _ = _reference(sub, q[pick], None, 16)
+        _close(g.reshape(q.shape)[pick], ref, tol * (1 + 8 / 64))
+        whole = ctx.paged_attention(c.kv, c.pages, c.batch(), _dev(q.reshape(len(q), -1)), 16).cpu().numpy()
+        g = g.reshape(whole.shape)
+        # 47 rows of 8 kv heads save 16000 (heads of 64: 32000) tiles' work, the others next to nothing
+        assert np.array_equal(g, whole) == (pages[0] != shared and pages[-1] != shared)
 
 
 def test_rows_behind_the_last_sequence_and_given_outputs(ctx):  # noqa: F811
