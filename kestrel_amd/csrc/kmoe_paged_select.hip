@@ -61,7 +61,8 @@ __device__ __forceinline__ bool touched(const PagedArgs &a, int i, int &b, int64
 __device__ __forceinline__ float min16(float v) { return -group_max<16>(-v); }
 
 // One wave per page, kv head and 32 (Q8_0: 64) dims: its K tiles one by one, every
-// lane eight (sixteen) dims of one position of each.
+// lane eight (sixteen) dims of one position of each, as the store laid them: 16 contiguous bytes.
+// Bound by the launch (64 pages of 8 kv heads 5 us, of which a page's tiles take 1).
 template <int T>
 __global__ void __launch_bounds__(256) k_paged_bounds(PagedArgs a, int n_unit, uint16_t *__restrict__ bounds) {
   constexpr int DIMS = T == kPgF16 ? 32 : 64, E = T == kPgF16 ? 8 : 16;
@@ -319,8 +320,10 @@ __device__ __forceinline__ int choose(const R &r, int want, const int32_t *tab, 
 }
 
 // A work-group: `part` pages of one row and kv head; the last one of a row to arrive
-// chooses. Grid: (parts, rows by kv heads), for several launches of the attention. Bound by latencies: the row's place, its q, the
-// pages' numbers, their bounds and what is handed over wait for each other.
+// chooses. Grid: (parts, rows by kv heads), for several launches of the attention. Bound by
+// latencies where rows are few: the row's place, its q, the pages' numbers, their bounds and what
+// is handed over wait for each other (a row of 8 kv heads, 2047 pages: 16 us). Of many by the vector
+// units, half of it the scores' conversions and products in 64 bits (300 rows of 4, 250 pages: 32).
 template <int HD>
 __global__ void __launch_bounds__(256) k_paged_select(SelectArgs s, int64_t row0, int part) {
   constexpr int LP = HD / 8, PAGES = 256 / LP;  // lanes that share a page, pages of a round
