@@ -139,7 +139,9 @@ struct SelectArgs {
   const uint16_t *bounds;
   const float *q;
   int n_head, group, n_select, n_first;
-  int rows;  // of a launch of the attention; its sequence b is row b % rows, kv head b / rows where rows share pages, otherwise the other way round
+  // of a launch of the attention: its sequence b is row b % rows, kv head b / rows where rows share
+  // pages, otherwise the other way round
+  int rows;
   uint64_t *scores;
   int32_t *table, *len;
   uint32_t *counters;

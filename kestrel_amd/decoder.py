@@ -593,7 +593,8 @@ class PagedDecoder(Decoder):
                 if by_parts:
                     self._append({s: j - i for s, i, j in part})
                 ty, dims, t = self.embed
-                groups, done = self._groups([p[0] for p in part], sum(j - i for _, i, j in part)), [p[0] for p in part if p[2] == len(rows[p[0]])]
+                done = [s for s, _, j in part if j == len(rows[s])]
+                groups = self._groups([s for s, _, _ in part], sum(j - i for _, i, j in part))
                 if groups:
                     part = [part[i] for i in groups[0]]
                 x = self.ctx.get_rows(ty, t, dims[1], dims[0], [tk for s, i, j in part for tk in rows[s][i:j]])
@@ -601,8 +602,8 @@ class PagedDecoder(Decoder):
                 batch = self._batch([p[0] for p in part], [(had[s] or 0) + j for s, _, j in part], counts)
                 batch.steps = steps
                 if groups:
-                    batch.groups = self.ctx.paged_groups(*(self.torch.from_numpy(g.copy()).to(self.dev) for g in groups[1:]),
-                                                         always=True)
+                    start, shared = (self.torch.from_numpy(g.copy()).to(self.dev) for g in groups[1:])
+                    batch.groups = self.ctx.paged_groups(start, shared, always=steps)  # (chunks: the call decides)
                 x, f = self._rows(x, batch)
                 end = dict(zip([p[0] for p in part], np.cumsum(counts).tolist()))
                 last = [end[s] - 1 for s in done]
