@@ -21,6 +21,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "kmoe_paged_rows.h"
+
 namespace kmoe {
 
 constexpr int kPgF16 = 1, kPgQ8 = 8;  // ggml type ids
@@ -77,11 +79,9 @@ __device__ __forceinline__ void paged_rows(const PagedArgs &a, int b, int64_t &r
     n = b < a.s_rows ? 1 : 0;
     return;
   }
-  int64_t lo = a.row_start[b], hi = a.row_start[b + 1];
-  lo = lo < 0 ? 0 : lo;
-  hi = hi > a.s_rows ? a.s_rows : hi;
-  r0 = lo;
-  n = hi > lo ? hi - lo : 0;
+  const RowRange r = row_range(a.row_start[b], a.row_start[b + 1], a.s_rows);
+  r0 = r.r0;
+  n = r.n;
 }
 
 // Block of kv head g in the page of sequence b's position p, or null where the

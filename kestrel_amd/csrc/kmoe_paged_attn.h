@@ -253,10 +253,12 @@ __device__ __forceinline__ int64_t group_rows(const PagedArgs &a, const SharedAr
   b0 = lo;
   r0 = n = 0;
   if (hi - lo <= 1 || !pages) return 0;
-  int64_t r1, m;
-  paged_rows(a, lo, r0, n);
-  paged_rows(a, hi - 1, r1, m);
-  n = r1 + m > r0 ? r1 + m - r0 : 0;
+  RowRange first, last;
+  paged_rows(a, lo, first.r0, first.n);
+  paged_rows(a, hi - 1, last.r0, last.n);
+  const RowRange all = group_range(first, last);
+  r0 = all.r0;
+  n = all.n;
   if (!s.least) return 0;
   auto tiles = [&](int log) { return ((int)n * group + (1 << log) - 1) >> log; };
   const int seqs = hi - lo < (int)n ? hi - lo : (int)n, full = tiles(s.log_whole);  // (a sequence has a column tile at least)
