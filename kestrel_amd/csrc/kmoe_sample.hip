@@ -1103,7 +1103,10 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, int64_t row0,
     if (chunks && s.sums(a)) {
 #pragma unroll
       for (int e = 0; e < CE; ++e) {
-        chunk_sum[e] = (u64)__builtin_rint((double)chunk_sum[e] * 0x1p-43 * weight(r, chunk_max[e], sh.tab));
+        // (nothing where not even the largest weighs a unit: no token of it can be drawn. Where it
+        // does, so does the sum: both are rounded alike)
+        const double y = weight(r, chunk_max[e], sh.tab);
+        chunk_sum[e] = fixed(y) ? (u64)__builtin_rint((double)chunk_sum[e] * 0x1p-43 * y) : 0;
         mine += chunk_sum[e];
       }
       before = block_scan(mine, sum, sh);
@@ -1120,22 +1123,15 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, int64_t row0,
             before += chunk_sum[k];
             ++e;
           }
-        float x = chunk_max[0];
-#pragma unroll
-        for (int k = 1; k < CE; ++k) x = e == k ? chunk_max[k] : x;
         sh.at = CE * t + e;
         sh.before = before;
-        sh.redf[0][0] = x;
       }
       lds_barrier();
       const int start = sh.at * kChunk, end = start + kChunk < src.n ? start + kChunk : src.n;
       goal -= sh.before;
-      const float top = sh.redf[0][0];
       lds_barrier();
       at = draw(r, Logits{src.l + start, end - start}, Cut{-INFINITY, ~0ull}, goal, sum, w, sum, sh);
-      id = at >= 0 ? start + at : first_equal(src, start, end, top, sh);  // (a chunk of many weights of under half a unit)
-      w = at >= 0 ? w : 1;
-      at = 0;
+      id = start + at;
     } else if (chunks) {
       // a bin that holds the last kept token, or one after it, by the groups' largest: as
       // many of them as tokens are kept, or of as much weight
