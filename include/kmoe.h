@@ -484,8 +484,9 @@ int kmoe_argmax(kmoe_ctx *ctx, const float *logits_dev, int64_t n, uint32_t *out
  *   min_p        NULL, NaN, 0 or less: all; above 1 counts as 1
  * A NaN logit counts as -inf; if all are, the token is 0 and its probability 0. With
  * +inf logits only those are drawn. Weights are 64-bit floats, summed as multiples of
- * 2^-43 (a token of less than half of that is not drawn), so a row's token does not
- * depend on the other rows or on how the work is shared out. out [s_rows] receives the
+ * 2^-43: a sum is off by at most half of that for each of its tokens, and a token of less
+ * than half of that is not drawn. A row's token does not depend on the other rows or on
+ * how the work is shared out. out [s_rows] receives the
  * tokens, prob (may be NULL) the probabilities they were drawn with among the kept. When
  * pos_dev [s_rows] is non-NULL, each is advanced by `advance` afterwards. out, prob and
  * pos must not overlap each other or the inputs. At most 2^20 rows. The context keeps a

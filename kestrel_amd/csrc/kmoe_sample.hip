@@ -14,7 +14,9 @@
 // whole numbers do not depend on their order, so neither atomics nor the way a row
 // is shared out change a result. 2^20 weights of at most 1 fit 63 bits; what is
 // rounded off is 2^-44 of the largest weight each, at most 2^-24 of the sum (the
-// step of u) in all.
+// step of u) in all. The sum of a whole long row, which the draw without a cut and top_p
+// go by, is that of its chunks, each summed by its own largest logit before the row's is
+// known: rounded otherwise than the row's weights, but the same on every path of a row.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -378,7 +380,7 @@ __device__ __forceinline__ u64 part_of(float p, u64 x) {
 }
 
 // The cut by top_k (src.n or more: none) and top_p (1 or more: none) among the elements. all_: the
-// whole row's sum where the elements are not all that top_p counts, or 0.
+// whole row's sum by its chunks (0: the elements' own), which top_p is a part of; the elements need not be the whole row.
 template <class S>
 __device__ __forceinline__ Cut find_cut(const Row &r, const S &src, int k, float p, u64 all_, Shared &sh) {
   Cut cut{-INFINITY, ~0ull};
@@ -859,9 +861,9 @@ __device__ __forceinline__ int part_drawn(const Row &r, int parts, u64 &goal, u6
 
 // k_sample's share of that. With min_p what weighs that much is summed, too: where it is less
 // than top_p asks for (or top_p asks for nothing) it is what is kept, and the last work-group to arrive
-// draws. Returns the token then, otherwise -1.
-__device__ __forceinline__ int share(const Row &r, const Logits &src, float p, const SampleStats &st, int parts, u64 &w, u64 &sum,
-                                     Shared &sh) {
+// draws. Returns the token then, otherwise -1. all_: the row's sum, as the chunks' say.
+__device__ __forceinline__ int share(const Row &r, const Logits &src, float p, u64 all_, const SampleStats &st, int parts, u64 &w,
+                                     u64 &sum, Shared &sh) {
   const int t = threadIdx.x, mine = blockIdx.y, len = part_len(src.n, parts);
   const bool bins = p < 1.0f, least = r.min_w > 0.0;
   lds_barrier();
@@ -914,7 +916,7 @@ __device__ __forceinline__ int share(const Row &r, const Logits &src, float p, c
     for (int e = 0; e < kBinsEach; ++e) sh.mass[e * kThreads + t] = s[e];
     lds_barrier();
     const u64 total = sum_below(sh.mass, kBins, sh);
-    target = part_of(p, total);
+    target = part_of(p, all_);
     target = target < total ? target : total;
     b = crossing(sh.mass, target, before, sh);
   }
@@ -1184,10 +1186,10 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, int64_t row0,
       // (elements lie about as far below the groups' largest as those lie apart, twice or three times)
       r.scale = s.scale(m, chunks ? m - 4.0f * (m - low) - 1.0f : low, s.k >= src.n);
       if (flat) {
-        id = share(r, src, s.p, st, (int)gridDim.y, w, sum, sh);
+        id = share(r, src, s.p, sum, st, (int)gridDim.y, w, sum, sh);
         if (id < 0) return;
       } else {
-        const Cut cut = find_cut(r, src, s.k, s.p, 0, sh);
+        const Cut cut = find_cut(r, src, s.k, s.p, s.k < src.n ? 0 : sum, sh);
         id = draw(r, src, cut, 0, 0, w, sum, sh);
       }
     }
