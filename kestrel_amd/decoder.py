@@ -282,7 +282,9 @@ class Decoder:
     def _sampling(self, b, rows: int, u, n: int, **how):
         """The settings of a sampled decode into buffers of b, and its random numbers [n, rows] on the device."""
         torch = self.torch
-        u = torch.as_tensor(u, dtype=torch.float32)
+        u = torch.as_tensor(u, dtype=torch.float64)
+        # (below 1 stays below 1, from where on the last kept token is drawn, however little it weighs)
+        u = torch.where(u < 1, u.to(torch.float32).clamp(max=1 - 2.0 ** -24), u.to(torch.float32))
         if tuple(u.shape) != (n, rows) and (rows != 1 or tuple(u.shape) != (n,)):
             raise ValueError(f"u: need [{n}, {rows}] random numbers, got {list(u.shape)}")
         vals = {}
