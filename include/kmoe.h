@@ -697,12 +697,12 @@ int kmoe_pages_length(const kmoe_pages *p, uint32_t seq, int64_t *n);
 int kmoe_pages_table(kmoe_pages *p, const uint32_t *seqs, int32_t n_seq, int32_t table_cols, int32_t *table,
                      int32_t *seq_len);
 /* Groups for kmoe_paged_attention_shared among n_seq sequences (at most KMOE_PAGED_MAX_SEQ),
- * each named once: sequences whose first pages are the same ones, so chosen that as few
- * positions as can be are read more than once. order [n_seq] receives the sequences'
+ * each named once: sequences whose first pages are the same ones, (members - 1) * shared
+ * positions of which come to `least` or more. They are so chosen that few positions are read
+ * more than once, as few as can be where `least` is a page or less. order [n_seq] receives the sequences'
  * indexes, the groups' members one behind the other and the sequences that are in none behind
  * them; group i holds order[start[i]] .. order[start[i + 1] - 1] (start [n_seq + 1]) and
- * shares shared[i] pages (shared [n_seq]); *n_group groups. A group is made where
- * (members - 1) * shared positions come to `least` or more. */
+ * shares shared[i] pages (shared [n_seq]); *n_group groups. */
 int kmoe_pages_groups(kmoe_pages *p, const uint32_t *seqs, int32_t n_seq, int64_t least, int32_t *order, int32_t *start,
                       int32_t *shared, int32_t *n_group);
 /* Moves the used pages to the front, the highest first, at most cap of them:

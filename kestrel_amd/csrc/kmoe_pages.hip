@@ -359,18 +359,20 @@ int kmoe_pages_groups(kmoe_pages *p, const uint32_t *seqs, int32_t n_seq, int64_
     // Nodes chosen for groups: a sequence belongs to the lowest one above it. Together they
     // save the sum over the sequences of their node's d, less d once per node: the most
     // of that, by the level of the lowest chosen node above (0: none), from the leaves up.
-    // (An explicit stack: nodes may nest n_seq deep.)
+    // A node whose own sequences would save less than `least` is not chosen, so that they
+    // go to one above. (An explicit stack: nodes may nest n_seq deep.)
     struct Step {
       int32_t node;
       size_t kid;
-      std::vector<int64_t> best;  // by that level, its own among them
+      std::vector<int64_t> best;   // by that level, its own among them
+      std::vector<int32_t> count;  // sequences that belong to the node of that level then
     };
     std::vector<Step> todo;
     std::vector<int64_t> depth;
     auto enter = [&](int32_t x) {
       tree[x].level = (int32_t)depth.size();
       depth.push_back(tree[x].d);
-      todo.push_back(Step{x, 0, std::vector<int64_t>(depth.size(), 0)});
+      todo.push_back(Step{x, 0, std::vector<int64_t>(depth.size(), 0), std::vector<int32_t>(depth.size(), 0)});
     };
     enter(0);
     while (!todo.empty()) {
@@ -381,15 +383,21 @@ int kmoe_pages_groups(kmoe_pages *p, const uint32_t *seqs, int32_t n_seq, int64_
         if (kid >= 0) {
           enter(kid);  // (t is not used after)
         } else {
-          for (size_t j = 0; j < t.best.size(); ++j) t.best[j] += depth[j];
+          for (size_t j = 0; j < t.best.size(); ++j) t.best[j] += depth[j], ++t.count[j];
         }
         continue;
       }
       const int64_t open = t.best.back() - v.d;
+      const bool enough = (t.count.back() - 1) * v.d * p->page >= least;
       t.best.pop_back();  // (grows with the level: the larger what a sequence has anyway)
-      v.closed = (int32_t)(std::lower_bound(t.best.begin(), t.best.end(), open) - t.best.begin());
-      if (todo.size() > 1)
-        for (size_t j = 0; j < t.best.size(); ++j) todo[todo.size() - 2].best[j] += std::max(t.best[j], open);
+      v.closed = enough ? (int32_t)(std::lower_bound(t.best.begin(), t.best.end(), open) - t.best.begin()) : 0;
+      if (todo.size() > 1) {
+        Step &up = todo[todo.size() - 2];
+        for (int32_t j = 0; j < (int32_t)t.best.size(); ++j) {
+          up.best[j] += j < v.closed ? open : t.best[j];
+          up.count[j] += j < v.closed ? 0 : t.count[j];
+        }
+      }
       depth.pop_back();
       todo.pop_back();
     }
@@ -406,8 +414,7 @@ int kmoe_pages_groups(kmoe_pages *p, const uint32_t *seqs, int32_t n_seq, int64_
     int32_t n = 0, at = 0;
     std::vector<uint8_t> in(n_seq, 0);
     for (size_t x = 1; x < tree.size(); ++x) {
-      const int64_t m = (int64_t)tree[x].members.size();
-      if (m < 2 || (m - 1) * tree[x].d * p->page < least) continue;
+      if (tree[x].members.empty()) continue;
       start[n] = at;
       shared[n++] = (int32_t)tree[x].d;
       for (int32_t i : tree[x].members) {
