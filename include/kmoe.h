@@ -630,7 +630,7 @@ int kmoe_paged_attention_shared(kmoe_ctx *ctx, const kmoe_paged_desc *desc, cons
  * after every store keeps them up to date; they are formed anew from the page each
  * time, and do not depend on what was there. A NaN key is passed over. A page without an
  * entry in the table, and the others, are left as they were; of a page that rows of two
- * sequences of the batch lie on, either one's bounds stay. Copies of pages need copies of
+ * sequences of the batch lie on, each bound is either one's. Copies of pages need copies of
  * their bounds. bounds must not overlap the pages. */
 int kmoe_paged_bounds(kmoe_ctx *ctx, const kmoe_paged_desc *desc, const void *pages_dev, const kmoe_paged_batch *batch,
                       uint16_t *bounds_dev);

@@ -2538,7 +2538,7 @@ int kmoe_sample(kmoe_ctx *c, const float *logits, int64_t s_rows, int64_t n, int
                 const float *u, uint32_t *out, float *prob, int32_t *pos, int32_t advance) {
   if (!c) return KMOE_E_INVALID;
   if (n <= 0 || n > KMOE_SAMPLE_MAX) return fail(c, KMOE_E_INVALID, "%lld logits a row (1 .. %d)", (long long)n, KMOE_SAMPLE_MAX);
-  constexpr int64_t kMaxRows = (int64_t)1 << 20;  // (a work-group of 1024 per row stays a valid grid)
+  constexpr int64_t kMaxRows = (int64_t)1 << 20;  // (a work-group of 256 per row stays a valid grid; long rows go by parts)
   if (s_rows < 0 || s_rows > kMaxRows) return fail(c, KMOE_E_INVALID, "%lld rows (at most 2^20)", (long long)s_rows);
   if (stride < n || stride > INT64_MAX / 8 / kMaxRows)
     return fail(c, KMOE_E_INVALID, "rows of %lld floats %lld apart", (long long)n, (long long)stride);

@@ -451,7 +451,6 @@ hipError_t launch_rope_kv(hipStream_t st, const float *q, const float *k, const 
                           int neox, int64_t n_ctx, float *q_out, uint16_t *kc, uint16_t *vc);
 hipError_t launch_swiglu(hipStream_t st, const float *g, const float *u, int64_t n, float *out);
 hipError_t launch_add_rows(hipStream_t st, float *x, const float *b, int64_t rows, int64_t cols);
-// argmax of l[0..n) into out[0]; pos_dev (may be null) += advance afterwards.
 // ---- sampling (kmoe_sample.hip): kmoe_sample's arguments, checked by the caller
 struct SampleArgs {
   const float *logits;
@@ -478,6 +477,7 @@ struct SampleStats {
 size_t sample_ws_bytes();
 int sample_counters();
 hipError_t launch_sample(hipStream_t st, const SampleArgs &a, uint8_t *ws, uint32_t *counters);
+// argmax of l[0..n) into out[0]; pos_dev (may be null) += advance afterwards.
 hipError_t launch_argmax(hipStream_t st, const float *l, int64_t n, uint32_t *out, int32_t *pos_dev,
                          int32_t advance);
 hipError_t launch_pos_advance(hipStream_t st, int32_t *pos_dev, int32_t by);

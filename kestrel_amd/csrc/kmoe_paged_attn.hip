@@ -120,9 +120,9 @@ using Work = Shares<COLS, 4, (HD == 64 && COLS == 16 ? 12 : 8), 8, 24>;
 //
 // MODE (see kmoe_paged_attn.h): kShared leaves a row's mean over its group's positions in
 // out, with the maximum and sum of the weights in sa.ml; kOwn joins that with its own. 64
-// rows behind 6000 positions, 32 heads over 8, F16: 36 and 21 us, whole 218. kShared is bound
-// by what L2 hands out (every column tile of a group reads all of its positions) and
-// the latencies of a work-group's plan, first loads, merge and join; kOwn by the latter.
+// rows behind 6000 positions, 32 heads over 8, F16: 36 and 21 us, whole 224. Both are bound by the
+// latencies of a work-group's plan, first loads, merge and join: kShared's CUs work for 57% of
+// its cycles, and L2 hands out 195 MB in it (eight column tiles read the same 24 MB), 5 TB/s.
 // kAgain: loads go through the caches, as rows share pages (a chunk of 300 rows that choose
 // 24 pages each: 181 us past the caches, 142 through them, 122 kv head by kv head).
 template <int T, int HD, int C, int MODE>
@@ -692,7 +692,9 @@ hipError_t launch_paged_attention_again(hipStream_t st, const PagedArgs &a, int 
 // of 128 dims, or 20000 of 64, that are not worked. (8 .. 64 sequences behind what they share, F16,
 // heads of 128, whole | shared: 6000 tiles saved 24 .. 31 | 27 .. 43 us, 12000 32 .. 50 | 32 .. 46, 24000
 // 60 .. 85 | 36 .. 45; heads of 64, Q8_0: 14000 24 .. 26 | 28 .. 29, 28000 33 .. 36 | 29 .. 37, 56000
-// 53 | 35 .. 39.) Where not even sequences that have all of the table in common would save as
+// 53 | 35 .. 39. The limits are the same for the other types: heads of 64, F16, 29 | 27 just below and
+// 32 | 27 just above; heads of 128, Q8_0, 34 | 40 and 37 | 43 just above, where the whole form would be
+// the quicker one.) Where not even sequences that have all of the table in common would save as
 // much, the batch is worked whole at once. The launch that finds out what is saved takes 5 us
 // of that (288 rows, 18000 tiles of 64 saved: whole 53, found out to be whole 57, shared 52).
 static int64_t tiles_saved(int64_t tiles, int hd) { return tiles * kWeight16 * (128 / hd); }

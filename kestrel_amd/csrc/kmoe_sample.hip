@@ -623,8 +623,8 @@ struct Settings {
 // Per chunk of kChunk logits, the largest, the sum of the weights by that one (kFix
 // units) where it is asked for, and the largest of every kGroup. A wave takes `each`
 // chunks one after the other, the next one's loads on their way meanwhile, and waits for
-// no other wave. Bound by the vector units where sums are asked for (20 instructions a weight,
-// 14 of them in 64 bits: 256 rows of 151936 46 us, 3.4 TB/s), otherwise by the loads (30).
+// no other wave. Bound by the vector units where sums are asked for (32 instructions a logit, 20 of
+// them the weight's, 14 in 64 bits: 256 rows of 151936 46 us, 3.4 TB/s), otherwise by the loads (30).
 __global__ void __launch_bounds__(256) k_sample_stats(SampleArgs a, int64_t row0, SampleStats st, int chunks, int each) {
   constexpr int U = kChunk / 256;
   __shared__ double tab[kTab];

@@ -386,7 +386,9 @@ class PagedDecoder(Decoder):
 
     # positions by kv heads and dims that would be read again (members less one, times those in common) from which a
     # group is made, with up to four heads a kv head: the 8 .. 12 us a layer that reading them once takes more (measured
-    # for 32 heads over 8 of 128: 45000 positions; 16 over 4: 100000; 16 over 8 of 64, Q8_0: 110000; 32 over 4: 190000)
+    # for 32 heads over 8 of 128: 45000 positions; 16 over 4: 100000; 16 over 8 of 64, Q8_0: 110000; 32 over 4: 190000).
+    # Decode steps always read such groups' pages once, as what they share is known here; prompt chunks, whose rows fill the
+    # matrix tiles more or less, leave it to the call's own count of tiles.
     SHARE_LEAST = 45000 * 8 * 128
 
     def __init__(self, ctx: Context, hp: dict, tensors: dict, n_pages: int, page: int = 64, kv_type: int = F16,
