@@ -1130,7 +1130,8 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, int64_t row0,
       }
       lds_barrier();
       const int start = sh.at * kChunk, end = start + kChunk < src.n ? start + kChunk : src.n;
-      goal -= sh.before;
+      // (the chunk's sum may be less than those of its tokens, of which u = 1 finds the last)
+      goal = r.u < 1.0f ? goal - sh.before : ~0ull;
       lds_barrier();
       at = draw(r, Logits{src.l + start, end - start}, Cut{-INFINITY, ~0ull}, goal, sum, w, sum, sh);
       id = start + at;

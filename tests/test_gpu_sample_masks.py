@@ -34,3 +34,13 @@ def test_a_chunk_with_one_token_that_can_be_drawn(ctx, n):  # noqa: F811
     x[:, [5000, n - 700]] = -30.316
     ids = _check(ctx, x, U)
     assert ids.tolist() == [5000] * 4 + [n // 2] * 2 + [n - 700] * 2
+
+
+@pytest.mark.parametrize("n", [9000, 32000, 151936])
+def test_the_last_token_where_sums_are_rounded_down(ctx, n):  # noqa: F811
+    """The last tokens weigh 0.556 of 2^-43 each, which counts as 2^-43: u = 1 finds the last one all the same."""
+    x = np.full((U.size, n), -np.inf, np.float32)
+    x[:, n // 2] = 0.0
+    x[:, n - 300:n - 20] = -30.392
+    ids = _check(ctx, x, U)
+    assert ids.tolist() == [n // 2] * 6 + [n - 21] * 2
